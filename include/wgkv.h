@@ -609,6 +609,73 @@ int wgkv_rope_qkv_norm_ring_write(const void* q, int64_t q_sh, const void* k, in
                                   int32_t* ring_state, void* pool_k, void* pool_v, void* local_pre_key,
                                   const int32_t* global_lengths, int32_t* cache_seqlens, void* stream);
 
+/* ------------------------------------------------------------------------
+ * A paged cache held in 4 bits.  No counterpart in the reference, whose cache
+ * is bf16: these entry points stand beside wgkv_paged_decode_attn for caches
+ * that should take a third of its memory and bandwidth.
+ *
+ * k_cache/v_cache  u8 (num_pages, page_size/16, 10*D), contiguous, 16-byte
+ *                  aligned: tiles of 16 tokens of one head.  Groups of 32
+ *                  consecutive values of a row share a bf16 step s and middle
+ *                  m; a value with code c in 0..15 reads as m + s*(c - 7.5).
+ *                  With t = token % 16: keys hold 16-bit words (t, d/8, d%2)
+ *                  of the codes d%8 = d%2 + {0,2,4,6}, values words (t/4,
+ *                  d/(D/16), t%4/2, d%(D/16)/4, t%2) of four consecutive
+ *                  codes, lowest bits first; then, at byte 8*D, pairs (s, m)
+ *                  (t/4, d/32, t%4).
+ * block_table, lengths, D in {64,128}, page_size in {16,32,64}: as
+ * wgkv_paged_decode_attn.  dtype: 0 bf16, 1 fp32, 2 fp16.
+ *
+ * wgkv_kv4_append quantises the tokens of key/value (B, T, H, D; element
+ * strides, d contiguous; bases 16-byte aligned, strides whole 16 bytes) that
+ * g_mask (u8 (B, H, T), t contiguous; NULL: all) admits and writes them, in
+ * order, to positions lengths[b,h], ... of each head:
+ *   s = bf16((max - min) / 15), 0 below 2^-126;  m = bf16((max + min) / 2),
+ *   both rounded to fp32 first;
+ *   c = round((x - m)/s + 7.5) clamped to 0..15, ties to even; a group that
+ *   holds a NaN or an infinity gets s = m = NaN.
+ * new_lengths (B, H) receives the lengths after the call and may be lengths.
+ * Positions beyond max_pages*page_size and pages outside the pool are not
+ * written; *status (or NULL) is then raised to WGKV_ERR_CAPACITY.  B*H <=
+ * 65535.  Two launches for T > 64 (workspace as sized, else 0 bytes), else
+ * one.
+ *
+ * wgkv_kv4_read writes rows i < rows of each head to key/value (B, rows, H,
+ * D; shared element strides, aligned as above): position starts[b,h] + i
+ * (NULL: 0; negative starts count as 0), zeros from lengths[b,h] on and where
+ * the page is outside the pool.
+ *
+ * wgkv_kv4_decode_attn has wgkv_paged_decode_attn's contract over such a
+ * cache.
+ * ---------------------------------------------------------------------- */
+size_t wgkv_kv4_append_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t tokens);
+
+int wgkv_kv4_append(
+    const void* key, int64_t k_stride_b, int64_t k_stride_t, int64_t k_stride_h,
+    const void* value, int64_t v_stride_b, int64_t v_stride_t, int64_t v_stride_h, int32_t dtype,
+    const uint8_t* g_mask, int64_t gm_stride_b, int64_t gm_stride_h,
+    const int32_t* lengths, int64_t len_stride_b, int32_t* new_lengths, int64_t new_stride_b,
+    void* k_cache, void* v_cache, int64_t num_pages, int32_t page_size,
+    const int32_t* block_table, int64_t bt_stride_b, int64_t bt_stride_h, int32_t max_pages,
+    int32_t batch, int32_t tokens, int32_t num_kv_heads, int32_t head_dim,
+    int32_t* status, void* workspace, size_t workspace_bytes, void* stream);
+
+int wgkv_kv4_read(
+    const void* k_cache, const void* v_cache, int64_t num_pages, int32_t page_size,
+    const int32_t* block_table, int64_t bt_stride_b, int64_t bt_stride_h, int32_t max_pages,
+    const int32_t* lengths, int64_t len_stride_b, const int32_t* starts, int64_t start_stride_b,
+    void* key, void* value, int64_t out_stride_b, int64_t out_stride_t, int64_t out_stride_h, int32_t dtype,
+    int32_t batch, int32_t rows, int32_t num_kv_heads, int32_t head_dim, void* stream);
+
+int wgkv_kv4_decode_attn(
+    const void* q, int64_t q_stride_b, int64_t q_stride_h,
+    const void* k_cache, const void* v_cache, int64_t num_pages, int32_t page_size,
+    const int32_t* cache_seqlens, int64_t sl_stride_b,
+    const int32_t* block_table, int64_t bt_stride_b, int64_t bt_stride_h, int32_t max_pages,
+    void* out, int64_t out_stride_b, int64_t out_stride_h,
+    int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    float softmax_scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,584 @@
+"""The 4-bit cache's operators against the 64-bit oracle: appended bytes and
+read-back values bit for bit, attention within the bound that its roundings
+give (oracle.kv4.attend)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv4 as ok
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+I32 = torch.int32
+
+
+def table_for(tokens, P, gen, spare=0, extra=3):
+    """Page ids of heads with these token counts: a permutation of the pool
+    (``extra`` pages unused), -1 past the end; (B, H, width + spare)."""
+    B, H = tokens.shape
+    pages = (tokens + P - 1) // P
+    total, width = int(pages.sum()) + extra, max(1, int(pages.max())) + spare
+    perm = torch.randperm(total, generator=gen).to(I32)
+    bt = torch.full((B, H, width), -1, dtype=I32)
+    off = 0
+    for b in range(B):
+        for h in range(H):
+            n = int(pages[b, h])
+            bt[b, h, :n] = perm[off:off + n]
+            off += n
+    return bt, total
+
+
+def pool(total, P, D, fill=0xFF):
+    """Pools whose unwritten bytes read as NaN (0xFFFF is a bf16 NaN)."""
+    return [torch.full((total, P // 16, 10 * D), fill, dtype=torch.uint8) for _ in range(2)]
+
+
+def check_append(k, v, lens, mask, P, D, seed, caps=None, table=None, **kw):
+    """One append on the device and in the oracle: bytes, lengths, status."""
+    import wgkv
+    gen = torch.Generator().manual_seed(seed)
+    B, T, H, _ = k.shape
+    n_new = torch.full((B, H), T) if mask is None else mask.to(torch.bool).sum(2).cpu()
+    bt, total = table_for(lens.clamp(min=0) + n_new, P, gen)
+    if table is not None:
+        bt = table(bt, total)
+    if caps is not None:
+        bt = bt[..., :caps].contiguous()
+    kc, vc = pool(total, P, D)
+    dk, dv = kc.to(DEV), vc.to(DEV)
+    status = torch.zeros(1, dtype=I32, device=DEV)
+    print(f"[kv4 append] k={tuple(k.shape)} {k.dtype} P={P} pages={total} table={tuple(bt.shape)}", flush=True)
+    new = wgkv.kv4_append(k.to(DEV) if not k.is_cuda else k, v.to(DEV) if not v.is_cuda else v, dk, dv, bt.to(DEV),
+                          lens.to(DEV, I32), g_mask=None if mask is None else mask.to(DEV), status=status, **kw)
+    torch.cuda.synchronize()
+    okc, ovc = kc.numpy(), vc.numpy()
+    ref, lost = ok.append(k.double().cpu().numpy(), v.double().cpu().numpy(), okc, ovc, bt.numpy(), lens.numpy(),
+                          None if mask is None else mask.bool().cpu().numpy())
+    assert np.array_equal(new.cpu().numpy(), ref)
+    assert int(status) == (3 if lost else 0)
+    for got, want, what in ((dk, okc, "k"), (dv, ovc, "v")):
+        diff = got.cpu().numpy() != want
+        assert not diff.any(), f"{what}: {int(diff.sum())} bytes differ, first at {np.argwhere(diff)[0]}"
+    return dk, dv, bt, new
+
+
+def rows(gen, *shape, dtype=torch.bfloat16):
+    x = torch.randn(*shape, generator=gen) * (1 + 3 * (torch.arange(shape[-1]) % 29 == 3)) + 0.5
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("D,P", [(64, 16), (64, 64), (128, 16), (128, 32)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T,kind", [(1, "all"), (3, "all"), (70, "all"), (64, "mask"), (131, "mask"), (40, "none")])
+def test_append(D, P, dtype, T, kind):
+    gen = torch.Generator().manual_seed(T * D + P)
+    B, H = 2, 3
+    k, v = rows(gen, B, T, H, D, dtype=dtype), rows(gen, B, T, H, D, dtype=dtype)
+    lens = torch.tensor([[0, 1, 15], [16, 37, 130]], dtype=I32)
+    mask = None
+    if kind == "mask":
+        mask = torch.rand(B, H, T, generator=gen) < torch.tensor([0.05, 0.4, 0.97])[None, :, None]
+        mask[1, 0] = False
+    elif kind == "none":
+        mask = torch.zeros(B, H, T, dtype=torch.bool)
+    check_append(k, v, lens, mask, P, D, seed=1)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_append_over_segments(masked):
+    """Several counting segments, an odd row length (unaligned mask rows)."""
+    gen = torch.Generator().manual_seed(9)
+    B, T, H, D = 1, 8321, 2, 64
+    k, v = rows(gen, B, T, H, D), rows(gen, B, T, H, D)
+    mask = (torch.rand(B, H, T, generator=gen) < 0.08).to(torch.uint8) * 7 if masked else None
+    if not masked:
+        k, v = k[:, :4500], v[:, :4500]
+    check_append(k, v, torch.tensor([[5, 0]], dtype=I32), mask, 16, D, seed=2)
+
+
+@pytest.mark.parametrize("what", ["heads_first", "slice", "misaligned", "last_dim", "expanded", "mask_strided", "u8"])
+def test_append_layouts(what):
+    gen = torch.Generator().manual_seed(3)
+    B, T, H, D = 2, 37, 2, 64
+    k, v = rows(gen, B, T, H, D).to(DEV), rows(gen, B, T, H, D).to(DEV)
+    mask = (torch.rand(B, H, T, generator=gen) < 0.5).to(DEV)
+    if what == "heads_first":
+        k = k.transpose(1, 2).contiguous().transpose(1, 2)
+    elif what == "slice":
+        big = torch.zeros(B, T + 2, 3 * H, D, dtype=torch.bfloat16, device=DEV)
+        big[:, 1:-1, H:2 * H] = k
+        k = big[:, 1:-1, H:2 * H]
+    elif what == "misaligned":
+        big = torch.zeros(B, T, H, D + 3, dtype=torch.bfloat16, device=DEV)
+        big[..., 3:] = k
+        k = big[..., 3:]
+    elif what == "last_dim":
+        v = v.transpose(2, 3).contiguous().transpose(2, 3)
+    elif what == "expanded":
+        k, v = k[:, :, :1].expand(B, T, H, D), v[:1].expand(B, T, H, D)
+    elif what == "mask_strided":
+        mask = mask.transpose(1, 2).contiguous().transpose(1, 2)
+    else:
+        mask = mask.to(torch.uint8) * 200
+    check_append(k, v, torch.tensor([[0, 7], [18, 33]], dtype=I32), mask, 16, D, seed=4)
+
+
+def test_append_borders_between_codes():
+    """Values on and next to the borders between two codes fall on their
+    side: exact multiples of the step (ties go to the even code), and fp32
+    neighbours of them."""
+    D = 64
+    s, m = 0.25, 1.0
+    ticks = m + s * np.arange(-7, 8)                     # the 15 borders, range 14 s of 15 s
+    row = np.concatenate([[m - 7.5 * s, m + 7.5 * s], ticks, ticks])
+    x32 = row.astype(np.float32)
+    x32[2:17] = np.nextafter(x32[2:17], np.float32(np.inf))
+    x32[17:] = np.nextafter(x32[17:], np.float32(-np.inf))
+    for arr, dt in ((row, torch.bfloat16), (row, torch.float16), (x32, torch.float32)):
+        x = torch.from_numpy(np.tile(arr, 2)).to(dt).view(1, 1, 1, D)
+        assert np.array_equal(ok.quantise(x.double().numpy())[1].ravel(), [s, s])
+        check_append(x, -x, torch.zeros(1, 1, dtype=I32), None, 16, D, seed=5)
+    # a step whose fp32 rounding lies halfway between two bf16 values
+    x = torch.linspace(-2.0 ** -26, 15 * (1 + 2.0 ** -8), 32)
+    x[0], x[31] = -2.0 ** -26, 15 * (1 + 2.0 ** -8)
+    assert ok.quantise(x.double().numpy())[1].item() == 1.0
+    x = torch.cat([x, -x]).view(1, 1, 1, D)
+    check_append(x, -x, torch.zeros(1, 1, dtype=I32), None, 16, D, seed=5)
+    # tiny values beside large middles, and fp32 rows of wide dynamic range
+    gen = torch.Generator().manual_seed(6)
+    x = torch.randn(1, 50, 2, D, generator=gen) * torch.exp(8 * torch.randn(1, 50, 2, D, generator=gen))
+    check_append(x, x.flip(1), torch.zeros(1, 2, dtype=I32), None, 16, D, seed=5)
+
+
+def test_append_special_values():
+    D, T = 64, 12
+    gen = torch.Generator().manual_seed(8)
+    x = torch.randn(1, T, 1, D, generator=gen)
+    x[0, 0, 0, :32] = -2.5
+    x[0, 1, 0, 3] = float("inf")
+    x[0, 2, 0, 40] = float("nan")
+    x[0, 3, 0, :32] = torch.linspace(-3e38, 3e38, 32)
+    x[0, 4, 0, :32] = torch.linspace(0, 1e-40, 32)
+    x[0, 5, 0] = 0.0
+    x[0, 6, 0] = 3.4e38
+    x[0, 7, 0, :32] = 100 + torch.linspace(-0.01, 0.01, 32)
+    x[0, 8, 0, 5] = -float("inf")
+    x[0, 9, 0] = 2.0 ** -120 * torch.randn(D, generator=gen)
+    x[0, 10, 0, :32] = 3.38e38
+    for dt in (torch.float32, torch.bfloat16):
+        check_append(x.to(dt), -x.to(dt), torch.zeros(1, 1, dtype=I32), None, 16, D, seed=9)
+    mask = torch.isfinite(x).all(-1).transpose(1, 2)  # what the mask leaves out may hold anything
+    check_append(x, -x, torch.zeros(1, 1, dtype=I32), mask, 16, D, seed=9)
+
+
+def test_append_without_room():
+    """Tokens past the table and on pages outside the pool are dropped, the
+    status is raised, lengths stop at the capacity; nothing else is touched."""
+    gen = torch.Generator().manual_seed(10)
+    k, v = rows(gen, 2, 70, 2, 64), rows(gen, 2, 70, 2, 64)
+    lens = torch.tensor([[0, 30], [47, 500]], dtype=I32)
+    _, _, _, new = check_append(k, v, lens, None, 16, 64, seed=11, caps=4)
+    assert new.cpu().tolist() == [[64, 64], [64, 64]]
+
+    def holes(bt, total):
+        bt = bt.clone()
+        bt[0, 0, 1] = -1
+        bt[1, 0, 3] = total
+        bt[1, 1, 0] = 2 ** 31 - 1
+        return bt
+    check_append(k, v, torch.tensor([[0, 30], [47, -3]], dtype=I32), None, 16, 64, seed=12, table=holes)
+
+
+def test_append_nothing():
+    k = torch.zeros(2, 0, 2, 64, dtype=torch.bfloat16)
+    check_append(k, k.clone(), torch.tensor([[0, 5], [17, 2]], dtype=I32), None, 16, 64, seed=13)
+
+
+@pytest.mark.parametrize("T", [1, 64, 200])
+def test_append_writes_lengths_in_place(T):
+    import wgkv
+    gen = torch.Generator().manual_seed(T)
+    k, v = rows(gen, 2, T, 3, 64).to(DEV), rows(gen, 2, T, 3, 64).to(DEV)
+    lens = torch.tensor([[0, 3, 9], [33, 1, 16]], dtype=I32)
+    bt, total = table_for(lens + T, 16, gen)
+    a, b = [[t.to(DEV) for t in pool(total, 16, 64)] for _ in range(2)]
+    sl = lens.to(DEV)
+    new = wgkv.kv4_append(k, v, *a, bt.to(DEV), sl)
+    assert torch.equal(sl.cpu(), lens)
+    assert wgkv.kv4_append(k, v, *b, bt.to(DEV), sl, out=sl) is sl
+    assert torch.equal(sl, new) and torch.equal(new.cpu(), lens + T)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def random_cache(gen, lens, P, D, spare=0):
+    """A cache of random tokens written by the oracle's packer's rules (any
+    codes, steps and middles), bytes past the lengths reading as NaN."""
+    bt, total = table_for(lens, P, gen, spare)
+    kc, vc = (x.numpy() for x in pool(total, P, D))
+    rng = np.random.default_rng(int(torch.randint(1 << 30, (1,), generator=gen)))
+    for b in range(lens.shape[0]):
+        for h in range(lens.shape[1]):
+            for p in range(int(lens[b, h])):
+                pg = int(bt[b, h, p // P])
+                for cache, keys in ((kc, True), (vc, False)):
+                    ok.put(cache[pg, p % P // 16], p % 16, rng.integers(0, 16, D),
+                           ok.bf16(rng.uniform(0.05, 0.4, D // 32)), ok.bf16(rng.normal(size=D // 32) * 0.3), keys)
+    return kc, vc, bt
+
+
+def oracle_read(kc, vc, bt, lens, n, starts):
+    B, H = lens.shape
+    D = kc.shape[2] // 10
+    out = [np.zeros((B, n, H, D)), np.zeros((B, n, H, D))]
+    for b in range(B):
+        for h in range(H):
+            ln, st = int(lens[b, h]), max(int(starts[b, h]), 0)
+            for o, cache, keys in ((out[0], kc, True), (out[1], vc, False)):
+                x = ok.values(*ok.rows(cache, bt[b, h].numpy(), ln, keys)) if ln else np.zeros((0, D))
+                x = x[st:st + n]
+                o[b, :x.shape[0], h] = x
+    return [torch.from_numpy(o) for o in out]
+
+
+@pytest.mark.parametrize("D,P", [(64, 16), (64, 32), (128, 16), (128, 64)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_read(D, P, dtype):
+    import wgkv
+    gen = torch.Generator().manual_seed(D + P)
+    lens = torch.tensor([[0, 1, 15], [64, 37, 130]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, P, D)
+    dk, dv = torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV)
+    for n, starts in [(130, None), (1, None), (200, None), (3, [[0, 0, 14], [61, 37, 127]]), (40, [[7, -3, 1], [2, 30, 99]])]:
+        print(f"[kv4 read] D={D} P={P} {dtype} rows={n} starts={starts}", flush=True)
+        st = None if starts is None else torch.tensor(starts, dtype=I32)
+        got = wgkv.kv4_read(dk, dv, bt.to(DEV), lens.to(DEV), n, starts=None if st is None else st.to(DEV), dtype=dtype)
+        want = oracle_read(kc, vc, bt, lens, n, torch.zeros_like(lens) if st is None else st)
+        for g, w in zip(got, want):
+            assert g.dtype == dtype and torch.equal(g.cpu(), w.float().to(dtype))
+
+
+def test_read_out_tensors_and_bad_pages():
+    import wgkv
+    gen = torch.Generator().manual_seed(21)
+    lens = torch.tensor([[40, 70]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, 16, 64)
+    dk, dv, dl = torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV), lens.to(DEV)
+    ref = wgkv.kv4_read(dk, dv, bt.to(DEV), dl, 70)
+    heads_first = [torch.zeros(1, 2, 70, 64, dtype=torch.bfloat16, device=DEV).transpose(1, 2) for _ in range(2)]
+    odd = [torch.zeros(1, 70, 2, 67, dtype=torch.bfloat16, device=DEV)[..., 3:] for _ in range(2)]
+    mixed = [heads_first[0].clone(), torch.zeros(1, 70, 2, 64, dtype=torch.bfloat16, device=DEV)]
+    for out in (heads_first, odd, mixed):
+        got = wgkv.kv4_read(dk, dv, bt.to(DEV), dl, 70, out=out)
+        assert got[0] is out[0] and torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1])
+    bad = bt.clone()
+    bad[0, 0, 1], bad[0, 1, 4] = kc.shape[0], -7
+    got = wgkv.kv4_read(dk, dv, bad.to(DEV), dl, 70)
+    for g, r in zip(got, ref):
+        r = r.clone()
+        r[0, 16:32, 0] = 0
+        r[0, 64:, 1] = 0
+        assert torch.equal(g, r)
+    assert wgkv.kv4_read(dk, dv, bt.to(DEV), dl, 0)[0].shape == (1, 0, 2, 64)
+
+
+def check_attend(q, kc, vc, bt, lens, scale, **kw):
+    import wgkv
+    print(f"[kv4 attend] q={tuple(q.shape)} pool={kc.shape} lens={lens.flatten().tolist()[:8]}", flush=True)
+    got = wgkv.paged_decode_attn_kv4(q.to(DEV), torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV),
+                                     lens.to(DEV), bt.to(DEV), scale, **kw)
+    torch.cuda.synchronize()
+    want, bound = ok.attend(q[:, 0].double().numpy(), kc, vc, bt.numpy(), lens.numpy(), scale)
+    err = np.abs(got[:, 0].double().cpu().numpy() - want)
+    assert (err <= bound).all(), f"worst error / bound {np.nanmax(err / bound)}, nan {int(np.isnan(err).sum())}"
+    return got
+
+
+@pytest.mark.parametrize("D,P", [(64, 16), (64, 64), (128, 16), (128, 32)])
+@pytest.mark.parametrize("G", [1, 2, 3, 4, 5, 6, 7, 8])
+def test_attend_head_groups(D, P, G):
+    gen = torch.Generator().manual_seed(G * D + P)
+    lens = torch.tensor([[0, 1, 33], [16, 95, 128]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, P, D)
+    q = torch.randn(2, 1, 3 * G, D, generator=gen).to(torch.bfloat16)
+    check_attend(q, kc, vc, bt, lens, D ** -0.5)
+
+
+@pytest.mark.parametrize("n", [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 129, 255, 257, 511, 513])
+def test_attend_lengths(n):
+    gen = torch.Generator().manual_seed(n)
+    lens = torch.tensor([[n, max(0, n - 1)]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, 16, 64, spare=2)
+    q = torch.randn(1, 1, 8, 64, generator=gen).to(torch.bfloat16)
+    check_attend(q, kc, vc, bt, lens, 64 ** -0.5)
+
+
+def device_cache(lens, P, D, seed, total=None):
+    """A cache filled on the device by kv4_append; (kc, vc, table)."""
+    import wgkv
+    gen = torch.Generator().manual_seed(seed)
+    bt, n = table_for(lens, P, gen)
+    kc, vc = (t.to(DEV) for t in pool(n, P, D))
+    T = int(lens.max())
+    B, H = lens.shape
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    k, v = (torch.randn(B, T, H, D, generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    mask = torch.arange(T)[None, None] < lens[..., None]
+    new = wgkv.kv4_append(k, v, kc, vc, bt.to(DEV), torch.zeros_like(lens).to(DEV), g_mask=mask.to(DEV))
+    assert torch.equal(new.cpu(), lens)
+    return kc, vc, bt
+
+
+@pytest.mark.parametrize("B,H,G,D,lens", [
+    (1, 1, 4, 128, [4097]),
+    (1, 2, 8, 128, [3000, 17]),
+    (1, 1, 8, 64, [5003]),
+    (2, 20, 2, 64, "ragged"),       # 40 heads
+    (3, 30, 4, 128, "short"),       # 90 heads
+])
+def test_attend_split_over_workgroups(B, H, G, D, lens):
+    """Heads cut over many workgroups, among others of every length."""
+    gen = torch.Generator().manual_seed(B * H + D)
+    if lens == "ragged":
+        ln = torch.randint(0, 900, (B, H), generator=gen, dtype=I32)
+        ln[0, 3], ln[1, 7] = 0, 2600
+    elif lens == "short":
+        ln = torch.randint(0, 70, (B, H), generator=gen, dtype=I32)
+        ln[2, 29] = 1500
+    else:
+        ln = torch.tensor(lens, dtype=I32).view(B, H)
+    kc, vc, bt = device_cache(ln, 16, D, seed=B + H)
+    q = torch.randn(B, 1, H * G, D, generator=gen).to(torch.bfloat16)
+    check_attend(q, kc.cpu().numpy(), vc.cpu().numpy(), bt, ln, D ** -0.5)
+
+
+def test_attend_many_heads():
+    """2048 heads: the most the call takes; lengths 0 to 40."""
+    gen = torch.Generator().manual_seed(31)
+    ln = torch.randint(0, 41, (64, 32), generator=gen, dtype=I32)
+    kc, vc, bt = device_cache(ln, 16, 64, seed=32)
+    q = torch.randn(64, 1, 32, 64, generator=gen).to(torch.bfloat16)
+    check_attend(q, kc.cpu().numpy(), vc.cpu().numpy(), bt, ln, 0.125)
+
+
+@pytest.mark.parametrize("what", ["large_scores", "one_dominant", "zero_scale", "negative_scale", "equal"])
+def test_attend_scores(what):
+    gen = torch.Generator().manual_seed(41)
+    lens = torch.tensor([[200, 77]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, 16, 64)
+    q = torch.randn(1, 1, 4, 64, generator=gen)
+    scale = 0.125
+    if what == "large_scores":
+        q = q * 40
+    elif what == "one_dominant":
+        q = q * 0.01
+        c, s, m = ok.get(kc[int(bt[0, 0, 11]), 0], 5, 64, True)
+        q[0, 0, :2] = torch.from_numpy(ok.values(c, s, m)).float() * 30
+    elif what == "zero_scale":
+        scale = 0.0
+    elif what == "negative_scale":
+        scale = -0.7
+    else:
+        q = torch.zeros_like(q)
+    check_attend(q.to(torch.bfloat16), kc, vc, bt, lens, scale)
+
+
+def test_attend_nan_in_a_head_stays_there():
+    """A stored NaN makes its own head's output NaN and no other's."""
+    import wgkv
+    gen = torch.Generator().manual_seed(43)
+    lens = torch.tensor([[50, 50]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, 16, 64)
+    q = torch.randn(1, 1, 4, 64, generator=gen).to(torch.bfloat16)
+    ok.put(kc[int(bt[0, 1, 2]), 0], 3, np.zeros(64, np.int64), np.array([np.nan, 0.1]), np.array([np.nan, 0.0]), True)
+    got = wgkv.paged_decode_attn_kv4(q.to(DEV), torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV),
+                                     lens.to(DEV), bt.to(DEV), 0.125).cpu()
+    want, bound = ok.attend(q[:, 0].double().numpy(), kc, vc, bt.numpy(), torch.tensor([[50, 0]]).numpy(), 0.125)
+    assert (np.abs(got[0, 0, :2].double().numpy() - want[0, :2]) <= bound[0, :2]).all()
+    assert torch.isnan(got[0, 0, 2:]).all()
+
+
+def test_attend_clamps_lengths_and_pages():
+    gen = torch.Generator().manual_seed(44)
+    lens = torch.tensor([[64, 30, 16]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, 16, 64)
+    q = torch.randn(1, 1, 6, 64, generator=gen).to(torch.bfloat16)
+    for x in (kc, vc):  # the pages that clamped ids reach hold numbers
+        x[0] = x[int(bt[0, 0, 1])]
+        x[-1] = x[int(bt[0, 1, 0])]
+    bt = bt.clone()
+    bt[0, 0, 2], bt[0, 1, 0] = -5, 2 ** 31 - 1
+    check_attend(q, kc, vc, bt[..., :4], torch.tensor([[2 ** 31 - 1, 30, -9]], dtype=I32), 0.125)
+
+
+@pytest.mark.parametrize("what", ["q_slice", "q_misaligned", "out", "out_misaligned", "tables"])
+def test_attend_layouts(what):
+    import wgkv
+    gen = torch.Generator().manual_seed(45)
+    lens = torch.tensor([[64, 30], [7, 16]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, 16, 64)
+    dk, dv = torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV)
+    q = torch.randn(2, 1, 4, 64, generator=gen).to(torch.bfloat16).to(DEV)
+    sl, tb, out = lens.to(DEV), bt.to(DEV), None
+    ref = wgkv.paged_decode_attn_kv4(q, dk, dv, sl, tb, 0.125)
+    if what == "q_slice":
+        q = torch.cat([q, q, q], 2)[:, :, 4:8]
+    elif what == "q_misaligned":
+        q = torch.nn.functional.pad(q, (1, 2))[..., 1:-2]
+    elif what == "out":
+        out = torch.zeros(2, 1, 12, 64, dtype=torch.bfloat16, device=DEV)[:, :, 4:8]
+    elif what == "out_misaligned":
+        out = torch.zeros(2, 1, 4, 65, dtype=torch.bfloat16, device=DEV)[..., 1:]
+    else:
+        sl = sl.t().contiguous().t()
+        tb = torch.stack([tb, tb], -1)[..., 0]
+    got = wgkv.paged_decode_attn_kv4(q, dk, dv, sl, tb, 0.125, out=out)
+    assert torch.equal(got, ref) and (out is None or got is out)
+
+
+def test_pool_beyond_32_bits():
+    """Pages past 4 GiB of a pool, and single rows there."""
+    import wgkv
+    D, P, n = 128, 64, 900_000  # 4.6 GB each
+    kc, vc = (torch.empty(n, P // 16, 10 * D, dtype=torch.uint8, device=DEV) for _ in range(2))
+    gen = torch.Generator().manual_seed(51)
+    T = 100
+    k, v = rows(gen, 1, T, 1, D), rows(gen, 1, T, 1, D)
+    q = torch.randn(1, 1, 4, D, generator=gen).to(torch.bfloat16)
+    small = [x.numpy() for x in pool(2, P, D)]
+    ok.append(k.double().numpy(), v.double().numpy(), *small, np.array([[[0, 1]]]), np.zeros((1, 1), np.int64))
+    bt = torch.tensor([[[n - 1, n - 7]]], dtype=I32, device=DEV)
+    sl = wgkv.kv4_append(k.to(DEV), v.to(DEV), kc, vc, bt, torch.zeros(1, 1, dtype=I32, device=DEV))
+    assert torch.equal(kc[n - 1].cpu(), torch.from_numpy(small[0][0]))
+    want = oracle_read(*small, torch.tensor([[[0, 1]]]), torch.tensor([[T]]), T, torch.zeros(1, 1))
+    for g, w in zip(wgkv.kv4_read(kc, vc, bt, sl, T), want):
+        assert torch.equal(g.cpu(), w.to(torch.bfloat16))
+    got = wgkv.paged_decode_attn_kv4(q.to(DEV), kc, vc, sl, bt, D ** -0.5)
+    ref, bound = ok.attend(q[:, 0].double().numpy(), *small, np.array([[[0, 1]]]), np.array([[T]]), D ** -0.5)
+    assert (np.abs(got[:, 0].double().cpu().numpy() - ref) <= bound).all()
+
+
+def test_prompt_then_decode_steps():
+    """The operators as a decoder uses them: a gated prompt is appended, then
+    each step appends its token and attends; the cache read back at the end
+    is the oracle's."""
+    import wgkv
+    gen = torch.Generator().manual_seed(61)
+    B, H, G, D, P, S, steps = 2, 2, 4, 128, 16, 150, 5
+    k, v = rows(gen, B, S, H, D), rows(gen, B, S, H, D)
+    mask = torch.rand(B, H, S, generator=gen) < 0.4
+    mask[0, 1] = False
+    n = mask.sum(2) + steps
+    bt, total = table_for(n, P, gen)
+    kc, vc = (x.numpy() for x in pool(total, P, D))
+    dk, dv = torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV)
+    sl = torch.zeros(B, H, dtype=I32, device=DEV)
+    ref, _ = ok.append(k.double().numpy(), v.double().numpy(), kc, vc, bt.numpy(), np.zeros((B, H), np.int64), mask.numpy())
+    wgkv.kv4_append(k.to(DEV), v.to(DEV), dk, dv, bt.to(DEV), sl, g_mask=mask.to(DEV), out=sl)
+    for i in range(steps):
+        k1, v1 = rows(gen, B, 1, H, D), rows(gen, B, 1, H, D)
+        q = torch.randn(B, 1, H * G, D, generator=gen).to(torch.bfloat16)
+        ref, _ = ok.append(k1.double().numpy(), v1.double().numpy(), kc, vc, bt.numpy(), ref)
+        wgkv.kv4_append(k1.to(DEV), v1.to(DEV), dk, dv, bt.to(DEV), sl, out=sl)
+        got = wgkv.paged_decode_attn_kv4(q.to(DEV), dk, dv, sl, bt.to(DEV), D ** -0.5)
+        want, bound = ok.attend(q[:, 0].double().numpy(), kc, vc, bt.numpy(), ref, D ** -0.5)
+        assert (np.abs(got[:, 0].double().cpu().numpy() - want) <= bound).all(), i
+    assert np.array_equal(sl.cpu().numpy(), ref)
+    for g, w in zip(wgkv.kv4_read(dk, dv, bt.to(DEV), sl, int(n.max()), dtype=torch.float32),
+                    oracle_read(kc, vc, bt, torch.from_numpy(ref), int(n.max()), torch.zeros(B, H))):
+        assert torch.equal(g.cpu(), w.float())
+
+
+def test_captured_decode_step():
+    """Two captured steps (append, attend) replayed in turn with eager calls
+    between them: each replay continues the same caches."""
+    import wgkv
+    gen = torch.Generator().manual_seed(71)
+    B, H, G, D, P, S, steps = 1, 4, 4, 128, 16, 600, 6
+    lens = torch.tensor([[S, 30, 1, 257]], dtype=I32)
+    kc, vc, bt = device_cache(lens, P, D, seed=72)
+    width = int((lens.max() + 2 * steps + P - 1) // P)
+    total = kc.shape[0]
+    full = torch.full((B, H, width), -1, dtype=I32)
+    full[..., :bt.shape[2]] = bt
+    for h in range(H):  # pages for the steps to come
+        for j in range(width):
+            if full[0, h, j] < 0:
+                full[0, h, j] = total
+                total += 1
+    kc, vc = (torch.cat([x, torch.zeros(total - x.shape[0], *x.shape[1:], dtype=torch.uint8, device=DEV)]) for x in (kc, vc))
+    full = full.to(DEV)
+
+    def state():
+        return kc.clone(), vc.clone(), lens.to(DEV)
+    ins = [tuple(torch.randn(B, 1, n, D, generator=gen).to(torch.bfloat16).to(DEV) for n in (H, H, H * G))
+           for _ in range(2 * steps)]
+    ea, ga, gb = state(), state(), state()
+
+    def step(st, k1, v1, q):
+        wgkv.kv4_append(k1, v1, st[0], st[1], full, st[2], out=st[2])
+        return wgkv.paged_decode_attn_kv4(q, st[0], st[1], st[2], full, D ** -0.5)
+    stat = [[torch.zeros_like(t) for t in ins[0]] for _ in range(2)]
+    warm = state()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(warm, *ins[0])
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for st, x in ((ga, stat[0]), (gb, stat[1])):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(st, *x))
+        graphs.append(g)
+    for i in range(steps):
+        want = step(ea, *ins[i])
+        for g, x, o in zip(graphs, stat, outs):
+            for d, s in zip(x, ins[i]):
+                d.copy_(s)
+            g.replay()
+            assert torch.equal(o, want), i
+        torch.cuda.synchronize()
+    for st in (ga, gb):
+        assert all(torch.equal(x, y) for x, y in zip(st, ea))
+    # both graphs at once, on streams of their own
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for i in range(steps, 2 * steps):
+        want = step(ea, *ins[i])
+        for x in stat:
+            for d, s in zip(x, ins[i]):
+                d.copy_(s)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, (s1, s2)):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[0], want) and torch.equal(outs[1], want), i
+
+
+def test_calls_on_two_streams_at_once():
+    import wgkv
+    gen = torch.Generator().manual_seed(81)
+    ln = torch.randint(500, 3000, (2, 8), generator=gen, dtype=I32)
+    kc, vc, bt = device_cache(ln, 16, 128, seed=82)
+    sl, tb = ln.to(DEV), bt.to(DEV)
+    qs = [torch.randn(2, 1, 32, 128, generator=gen).to(torch.bfloat16).to(DEV) for _ in range(2)]
+    refs = [wgkv.paged_decode_attn_kv4(q, kc, vc, sl, tb, 0.09) for q in qs]
+    rk = wgkv.kv4_read(kc, vc, tb, sl, 600)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in qs]
+    outs = [[], []]
+    for i in range(20):
+        for j, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[j].append(wgkv.paged_decode_attn_kv4(qs[j], kc, vc, sl, tb, 0.09))
+                if i % 7 == 0:
+                    got = wgkv.kv4_read(kc, vc, tb, sl, 600)
+                    outs[j].append(got)
+    torch.cuda.synchronize()
+    for j in range(2):
+        for o in outs[j]:
+            if isinstance(o, tuple):
+                assert torch.equal(o[0], rk[0]) and torch.equal(o[1], rk[1])
+            else:
+                assert torch.equal(o, refs[j])

@@ -1,0 +1,145 @@
+"""The 4-bit cache, host only: the oracle's format against its definition,
+and the calls that are refused (argument checks run before any HIP call)."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv4 as ok
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("keys", [True, False])
+def test_oracle_tile_round_trip(D, keys):
+    """Every code, step and middle has its own place in a tile."""
+    rng = np.random.default_rng(D + keys)
+    places = set()
+    for t in range(16):
+        for d in range(D):
+            at, sh = ok.offsets(t, d, D, keys)
+            places.add((int(at), int(sh)))
+    assert places == {(a, s) for a in range(8 * D) for s in (0, 4)}
+    tile = np.full(10 * D, 0xA5, np.uint8)
+    c = rng.integers(0, 16, (16, D))
+    s, m = ok.bf16(rng.uniform(0, 2, (16, D // 32))), ok.bf16(rng.normal(size=(16, D // 32)))
+    for t in rng.permutation(16):
+        ok.put(tile, t, c[t], s[t], m[t], keys)
+    for t in range(16):
+        for got, want in zip(ok.get(tile, t, D, keys), (c[t], s[t], m[t])):
+            assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("mean", [0.0, 3.0, 1e4])
+def test_oracle_quantisation_error(mean):
+    """|value - x| <= s/2 and what the rounded m and s cost: half a bf16 step
+    (2^-8 relative) of m, and 7.5 s 2^-8 at the ends of the range."""
+    x = np.random.default_rng(1).normal(size=(200, 64)) + mean
+    c, s, m = ok.quantise(x)
+    sw, mw = np.repeat(s, 32, 1), np.repeat(m, 32, 1)
+    assert (np.abs(ok.values(c, s, m) - x) <= sw / 2 + np.abs(mw) * 2.0 ** -8 + 7.5 * sw * 2.0 ** -8 + 1e-12).all()
+
+
+def test_oracle_special_groups():
+    x = np.zeros((5, 64))
+    x[0, :32] = -2.5          # constant: reads exactly
+    x[1, 3] = np.inf
+    x[2, 40] = np.nan
+    x[3, :32] = np.linspace(-3e38, 3e38, 32)
+    x[4, :32] = np.linspace(0, 1e-40, 32)  # a step below 2^-126 is 0
+    v = ok.values(*ok.quantise(x))
+    assert (v[0, :32] == -2.5).all() and (v[0, 32:] == 0).all()
+    assert np.isnan(v[1, :32]).all() and (v[1, 32:] == 0).all()
+    assert (v[2, :32] == 0).all() and np.isnan(v[2, 32:]).all()
+    assert np.isfinite(v[3]).all() and np.abs(v[3, :32] - x[3, :32]).max() <= 6e38 / 30 * 1.02
+    assert (np.abs(v[4] - x[4]) <= 1e-40).all()
+
+
+def _args(B=2, T=3, H=2, D=64, P=16, blocks=4):
+    k = torch.zeros(B, T, H, D, dtype=torch.bfloat16)
+    kc = torch.zeros(8, P // 16, 10 * D, dtype=torch.uint8)
+    return (k, k.clone(), kc, kc.clone(), torch.zeros(B, H, blocks, dtype=torch.int32),
+            torch.zeros(B, H, dtype=torch.int32))
+
+
+def test_append_refusals():
+    import wgkv
+    k, v, kc, vc, bt, sl = _args()
+    for bad, err in [
+        ((k[0], v, kc, vc, bt, sl), AssertionError),
+        ((k, v[:, :2], kc, vc, bt, sl), AssertionError),
+        ((k.double(), v.double(), kc, vc, bt, sl), TypeError),
+        ((k, v.float(), kc, vc, bt, sl), TypeError),
+        ((k[..., :32], v[..., :32], kc, vc, bt, sl), AssertionError),
+        ((k, v, kc.int(), vc, bt, sl), TypeError),
+        ((k, v, kc, vc[:4], bt, sl), AssertionError),
+        ((k, v, kc[..., :320], vc[..., :320], bt, sl), AssertionError),
+        ((k, v, torch.cat([kc, kc])[::2], torch.cat([vc, vc])[::2], bt, sl), ValueError),
+        ((k, v, kc, vc, bt[:1], sl), AssertionError),
+        ((k, v, kc, vc, bt.long(), sl), TypeError),
+        ((k, v, kc, vc, bt, sl[:, :1]), AssertionError),
+        ((k, v, kc, vc, bt, sl.long()), TypeError),
+        ((k, v, kc, vc, bt, sl), ValueError),  # host tensors
+    ]:
+        with pytest.raises(err):
+            wgkv.kv4_append(*bad)
+    for kw, err in [(dict(g_mask=torch.ones(2, 3, 2)), AssertionError),
+                    (dict(out=torch.zeros(2, 2)), AssertionError),
+                    (dict(out=torch.zeros(2, 3, dtype=torch.int32)), AssertionError),
+                    (dict(status=torch.zeros(1)), TypeError)]:
+        with pytest.raises(err):
+            wgkv.kv4_append(k, v, kc, vc, bt, sl, **kw)
+
+
+def test_read_and_attention_refusals():
+    import wgkv
+    _, _, kc, vc, bt, sl = _args()
+    q = torch.zeros(2, 1, 4, 64, dtype=torch.bfloat16)
+    for bad, kw, err in [
+        ((kc, vc, bt, sl[0], 4), {}, AssertionError),
+        ((kc, vc, bt, sl, -1), {}, AssertionError),
+        ((kc, vc, bt, sl, 4), dict(dtype=torch.float64), TypeError),
+        ((kc, vc, bt, sl, 4), dict(starts=sl.long()), AssertionError),
+        ((kc, vc, bt, sl, 4), {}, ValueError),
+    ]:
+        with pytest.raises(err):
+            wgkv.kv4_read(*bad, **kw)
+    for bad, kw, err in [
+        ((q[:, 0], kc, vc, sl, bt), {}, AssertionError),
+        ((torch.zeros(2, 2, 4, 64, dtype=torch.bfloat16), kc, vc, sl, bt), {}, AssertionError),
+        ((q.float(), kc, vc, sl, bt), {}, TypeError),
+        ((q[:, :, :3], kc, vc, sl, bt), {}, AssertionError),
+        ((q, kc, vc, sl.long(), bt), {}, TypeError),
+        ((q, kc, vc, sl, bt), {}, ValueError),
+    ]:
+        with pytest.raises(err):
+            wgkv.paged_decode_attn_kv4(*bad, 0.125, **kw)
+    for args in [(4, 24, 64), (4, 16, 96)]:
+        with pytest.raises(ValueError):
+            wgkv.kv4_cache(*args, device="cpu")
+
+
+def test_c_entry_points_check_arguments_without_gpu():
+    from wgkv import _lib
+    L = _lib.lib()
+    x = 4096  # an aligned, never dereferenced address
+    assert L.wgkv_kv4_append_workspace_bytes(1, 8, 64) == 0
+    assert L.wgkv_kv4_append_workspace_bytes(2, 3, 65) == 4 * 6 * (1 + 1 + 2)
+
+    def append(key=x, sk=64, dtype=0, cache=x, pages=4, page=16, maxp=4, B=1, T=4, H=1, D=64, ws=None, n=0):
+        return L.wgkv_kv4_append(key, sk, sk, sk, x, sk, sk, sk, dtype, None, 0, 0, x, 1, x, 1, cache, x, pages, page,
+                                 x, 4, 4, maxp, B, T, H, D, None, ws, n, None)
+
+    for kw, want in [(dict(key=None), _lib.ERR_ARG), (dict(T=-1), _lib.ERR_ARG), (dict(B=0), _lib.ERR_ARG),
+                     (dict(maxp=0), _lib.ERR_ARG), (dict(pages=0), _lib.ERR_ARG),
+                     (dict(key=x + 2), _lib.ERR_UNSUPPORTED), (dict(sk=60), _lib.ERR_UNSUPPORTED),
+                     (dict(dtype=3), _lib.ERR_UNSUPPORTED), (dict(D=96), _lib.ERR_UNSUPPORTED),
+                     (dict(page=8), _lib.ERR_UNSUPPORTED), (dict(cache=x + 8), _lib.ERR_UNSUPPORTED),
+                     (dict(maxp=1 << 28), _lib.ERR_UNSUPPORTED), (dict(B=256, H=257), _lib.ERR_UNSUPPORTED),
+                     (dict(T=65), _lib.ERR_WORKSPACE), (dict(T=65, ws=x, n=8), _lib.ERR_WORKSPACE)]:
+        assert append(**kw) == want, kw
+
+    def read(out=x, so=64, rows=4, dtype=0, D=64):
+        return L.wgkv_kv4_read(x, x, 4, 16, x, 4, 4, 4, x, 1, None, 0, out, x, so, so, so, dtype, 1, rows, 1, D, None)
+
+    for kw, want in [(dict(out=None), _lib.ERR_ARG), (dict(rows=0), _lib.ERR_ARG), (dict(so=4), _lib.ERR_UNSUPPORTED),
+                     (dict(dtype=-1), _lib.ERR_UNSUPPORTED), (dict(D=32), _lib.ERR_UNSUPPORTED)]:
+        assert read(**kw) == want, kw
