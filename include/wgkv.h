@@ -646,7 +646,9 @@ int wgkv_rope_qkv_norm_ring_write(const void* q, int64_t q_sh, const void* k, in
  * the page is outside the pool.
  *
  * wgkv_kv4_decode_attn has wgkv_paged_decode_attn's contract over such a
- * cache.
+ * cache, in one launch.  Its workspace's first 8192 bytes (per-head arrival
+ * counters) must be zero before a call; every call leaves them zero.  Calls
+ * that share a workspace must be ordered.
  * ---------------------------------------------------------------------- */
 size_t wgkv_kv4_append_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t tokens);
 
@@ -667,6 +669,8 @@ int wgkv_kv4_read(
     void* key, void* value, int64_t out_stride_b, int64_t out_stride_t, int64_t out_stride_h, int32_t dtype,
     int32_t batch, int32_t rows, int32_t num_kv_heads, int32_t head_dim, void* stream);
 
+size_t wgkv_kv4_decode_workspace_bytes(int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim);
+
 int wgkv_kv4_decode_attn(
     const void* q, int64_t q_stride_b, int64_t q_stride_h,
     const void* k_cache, const void* v_cache, int64_t num_pages, int32_t page_size,
@@ -674,7 +678,7 @@ int wgkv_kv4_decode_attn(
     const int32_t* block_table, int64_t bt_stride_b, int64_t bt_stride_h, int32_t max_pages,
     void* out, int64_t out_stride_b, int64_t out_stride_h,
     int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-    float softmax_scale, void* stream);
+    float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -244,23 +244,6 @@ __device__ __forceinline__ float dot2_bf16(uint32_t a, uint32_t b, float c) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, a), __builtin_bit_cast(bf16x2_t, b), c, false);
 }
 
-// Device-coherent accesses to the split partials.  The stores write through
-// to the point of coherence of the whole device and the loads do not return
-// a line that another XCD's writes left stale in this XCD's L2 (agent-scope
-// relaxed atomics: sc1 on gfx950; buffer cache-policy bit 4 for the 16-byte
-// loads).  No L2 writeback or invalidation is needed then: release/acquire
-// fences at device scope write back and invalidate whole L2s, which also
-// drops the K lines the other workgroups of the XCD are reading.
-__device__ __forceinline__ void store_coherent(float* p, float v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float load_coherent(const float* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ f32x4_t load_coherent4(__amdgpu_buffer_rsrc_t r, int byte_off) {
-  return __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, byte_off, 0, 16));
-}
-
 template <int D, int G, int NW>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(waves_per_simd(G, NW), waves_per_simd(G, NW))))
 void decode_split_kernel(DecodeArgs a) {

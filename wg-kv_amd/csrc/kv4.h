@@ -46,7 +46,7 @@ struct Kv4Pages {
   int max_pages;
 };
 
-WGKV_DEVICE int64_t kv4_capacity(const Kv4Pages& p) { return (int64_t)p.max_pages * p.page_size; }
+__host__ __device__ inline int64_t kv4_capacity(const Kv4Pages& p) { return (int64_t)p.max_pages * p.page_size; }
 
 // First byte of tile `tile` (position / 16) of a head, or -1 where its page
 // is outside the pool.

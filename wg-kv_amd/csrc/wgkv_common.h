@@ -174,6 +174,23 @@ WGKV_DEVICE int count_flags(const uint8_t* m, int lo, int hi, int t, int n) {
   return c;
 }
 
+// Device-coherent accesses to the split partials.  The stores write through
+// to the point of coherence of the whole device and the loads do not return
+// a line that another XCD's writes left stale in this XCD's L2 (agent-scope
+// relaxed atomics: sc1 on gfx950; buffer cache-policy bit 4 for the 16-byte
+// loads).  No L2 writeback or invalidation is needed then: release/acquire
+// fences at device scope write back and invalidate whole L2s, which also
+// drops the K lines the other workgroups of the XCD are reading.
+WGKV_DEVICE void store_coherent(float* p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+WGKV_DEVICE float load_coherent(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+WGKV_DEVICE f32x4_t load_coherent4(__amdgpu_buffer_rsrc_t r, int byte_off) {
+  return __builtin_bit_cast(f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, byte_off, 0, 16));
+}
+
 // Copies rows r < n of one K/V pair (source row src(r), pool row dst(r)) with
 // the whole workgroup of kThreads, 16 bytes per thread and step.  Eight loads per thread
 // are requested before the first store: one load and one store at a time

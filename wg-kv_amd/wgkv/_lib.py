@@ -208,6 +208,7 @@ SIGNATURES = {
         c_ptr, c_i64, c_ptr, c_i64,
         c_ptr, c_ptr, c_i64, c_i64, c_i64, c_i32,
         c_i32, c_i32, c_i32, c_i32, c_ptr]),
+    "wgkv_kv4_decode_workspace_bytes": (c_size, [c_i32, c_i32, c_i32]),
     "wgkv_kv4_decode_attn": (ctypes.c_int, [
         c_ptr, c_i64, c_i64,
         c_ptr, c_ptr, c_i64, c_i32,
@@ -215,7 +216,7 @@ SIGNATURES = {
         c_ptr, c_i64, c_i64, c_i32,
         c_ptr, c_i64, c_i64,
         c_i32, c_i32, c_i32, c_i32,
-        c_f32, c_ptr]),
+        c_f32, c_ptr, c_size, c_ptr]),
 }
 
 _lib = None

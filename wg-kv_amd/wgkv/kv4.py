@@ -20,6 +20,8 @@ The operators run on torch's current stream of the tensors' device, allocate
 only their outputs and scratch (both through torch, so a call can be captured
 in a HIP graph) and never synchronise with the host.
 """
+import functools
+
 import torch
 
 from . import _lib
@@ -53,14 +55,21 @@ def _same_device(first, *rest):
     return dev
 
 
-def _call(dev, where, fn, *args):
-    """fn(*args, stream) with ``dev`` current: a null stream is the current
-    device's."""
-    if dev.index == torch.cuda.current_device():
-        st = fn(*args, _lib.stream_handle(dev))
-    else:
+def _on_own_device(op):
+    """Runs op with its tensors' device current: a null stream, and whether
+    a stream is being captured, are the current device's."""
+    @functools.wraps(op)
+    def call(first, *args, **kw):
+        dev = first.device
+        if dev.type != "cuda" or dev.index == torch.cuda.current_device():
+            return op(first, *args, **kw)
         with torch.cuda.device(dev):
-            st = fn(*args, _lib.stream_handle(dev))
+            return op(first, *args, **kw)
+    return call
+
+
+def _call(dev, where, fn, *args):
+    st = fn(*args, _lib.stream_handle(dev))
     if st:
         _lib.check(st, where)
 
@@ -106,6 +115,7 @@ def _rows(t):
     return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
 
 
+@_on_own_device
 def kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask=None, out=None, status=None):
     """Quantise tokens into the heads' pages behind the ones already there.
 
@@ -162,6 +172,7 @@ def kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask=None, out=No
     return out
 
 
+@_on_own_device
 def kv4_read(k_cache, v_cache, block_table, lengths, rows, starts=None, dtype=torch.bfloat16, out=None):
     """The cache's rows as dense tensors: (k, v), each (B, rows, Hkv, D) of
     ``dtype`` (bf16, fp16 or fp32).
@@ -207,6 +218,29 @@ def kv4_read(k_cache, v_cache, block_table, lengths, rows, starts=None, dtype=to
     return out
 
 
+_COUNTERS = 8192  # bytes at the start of the attention's workspace that must be zero
+_workspaces = {}
+
+
+def _attn_workspace(dev, nbytes):
+    """Scratch of the attention, its arrival counters zero.  One per device
+    and stream: calls on a stream run in turn and leave the counters zero, and
+    calls on two streams never meet.  A captured call gets scratch of its own
+    from the graph's memory, cleared by the graph, since two graphs that were
+    captured on one stream may run on two."""
+    if torch.cuda.is_current_stream_capturing():
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws[:_COUNTERS].zero_()
+        return ws
+    key = (dev.index, _lib.stream_handle(dev))
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
+        _workspaces[key] = ws
+    return ws
+
+
+@_on_own_device
 def paged_decode_attn_kv4(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, out=None):
     """``paged_decode_attn`` over a 4-bit cache: q (B, 1, Hq, D) bf16 attends
     to the first cache_seqlens[b, h] tokens of its KV head; returns (B, 1, Hq,
@@ -232,8 +266,10 @@ def paged_decode_attn_kv4(q, k_cache, v_cache, cache_seqlens, block_table, softm
         return out.copy_(paged_decode_attn_kv4(q, k_cache, v_cache, lens, table, softmax_scale))
     q = _rows(q)
     qs, os = _strides(q), _strides(out)
-    _call(dev, "wgkv_kv4_decode_attn", _lib.lib().wgkv_kv4_decode_attn,
+    L = _lib.lib()
+    ws = _attn_workspace(dev, L.wgkv_kv4_decode_workspace_bytes(Hq, H, D))
+    _call(dev, "wgkv_kv4_decode_attn", L.wgkv_kv4_decode_attn,
           q.data_ptr(), qs[0], qs[2], k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P,
           lens.data_ptr(), lens.stride(0), table.data_ptr(), table.stride(0), table.stride(1), table.shape[2],
-          out.data_ptr(), os[0], os[2], B, Hq, H, D, float(softmax_scale))
+          out.data_ptr(), os[0], os[2], B, Hq, H, D, float(softmax_scale), ws.data_ptr(), ws.numel())
     return out
