@@ -24,7 +24,7 @@
 // tokens 4q..4q+3 of two tiles), and V words are A operands (rows = d) of
 // pairs of tokens.  Nothing goes through LDS but the merge of the waves.
 //
-// Work split: the heads' sequences, in units of 32 tokens, are one line that
+// Work split: the heads' sequences, in units of 64 tokens, are one line that
 // is cut into equal ranges, one per workgroup (so every workgroup has the
 // same work whatever the lengths); a range may end one head and begin
 // another.  Its waves take units in turn, the next unit's loads in flight.
@@ -40,7 +40,7 @@ constexpr float kRescaleSlack = 8.f;  // log2 units a running maximum may lag th
 constexpr int kMaxBH = 2048;
 constexpr int kMaxG = 8;
 constexpr int kMaxSlots = 1024;  // workgroups of a launch
-constexpr int kFlush = 32;       // units between two corrections of the code offset
+constexpr int kFlush = 16;       // units between two corrections of the code offset
 constexpr uint32_t kCodeMask = 0x000f000fu, kCodeBase = 0x43004300u;  // 128 + c
 constexpr float kOffset = 135.5f;                                     // (128 + c) - (c - 7.5)
 
@@ -55,7 +55,8 @@ struct AttnArgs {
   uint16_t* out;
   int64_t out_sb, out_sh;
   int B, Hkv, G;
-  float scale_log2;
+  float scale_log2;         // |softmax_scale| * log2(e)
+  uint32_t q_and, q_xor;    // its sign (and a scale of 0) is put into the queries
   // pieces: two slots per workgroup (the head it ends, the head it begins);
   // slot s, query head i: part_m[s*G+i], part_l[s*G+i], part_acc[(s*G+i)*D..]
   float *part_m, *part_l, *part_acc;
@@ -68,61 +69,77 @@ WGKV_DEVICE int tokens_of(const AttnArgs& a, int bh) {
   const int64_t n = a.len[(int64_t)b * a.len_sb + h];
   return (int)(n < 0 ? 0 : n > cap ? cap : n);
 }
-WGKV_DEVICE int units_of(int tokens) { return (tokens + 31) >> 5; }
+WGKV_DEVICE int units_of(int tokens) { return (tokens + 63) >> 6; }
 
-// The heads' units as a line, seen by one wave: lane j knows the units of
-// heads [j*per, j*per+per).
-struct Line {
-  int per;
-  int64_t excl;   // units before the lane's heads
-  int64_t total;
-};
-
-WGKV_DEVICE int64_t wave_incl_scan64(int64_t v, int lane) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t u = __shfl_up(v, off, 64);
-    if (lane >= off) v += u;
-  }
+// Inclusive prefix sum over the wave in DPP steps (no LDS round trips):
+// row_shr 1, 2, 4, 8 within 16 lanes, then the rows' ends broadcast onwards.
+WGKV_DEVICE int wave_scan_dpp(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast31 into rows 2 and 3
   return v;
 }
+
+// The heads' units as a line, seen by one wave: lane j knows the units of
+// heads [j*per, j*per+per).  (The host refuses tables whose units could pass
+// 31 bits.)
+struct Line {
+  int per;
+  int tokens;  // of the lane's head where per is 1
+  int excl;    // units before the lane's heads
+  int total;
+};
 
 WGKV_DEVICE Line make_line(const AttnArgs& a, int lane) {
   const int BH = a.B * a.Hkv;
   Line ln;
   ln.per = (BH + 63) >> 6;
-  int64_t n = 0;
-  for (int i = 0; i < ln.per; ++i) {
-    const int bh = lane * ln.per + i;
-    if (bh < BH) n += units_of(tokens_of(a, bh));
+  ln.tokens = 0;
+  int n = 0;
+  if (ln.per == 1) {
+    if (lane < BH) ln.tokens = tokens_of(a, lane);
+    n = units_of(ln.tokens);
+  } else {
+    for (int i = 0; i < ln.per; ++i) {
+      const int bh = lane * ln.per + i;
+      if (bh < BH) n += units_of(tokens_of(a, bh));
+    }
   }
-  const int64_t incl = wave_incl_scan64(n, lane);
+  const int incl = wave_scan_dpp(n);
   ln.excl = incl - n;
-  ln.total = __shfl(incl, 63, 64);
+  ln.total = __builtin_amdgcn_readlane(incl, 63);
   return ln;
 }
 
-// The head that holds unit `pos` < total of the line.
+// The head that holds unit `pos` < total of the line (all wave-uniform).
 struct Head {
   int bh, tokens;
-  int64_t start;  // its first unit on the line
+  int start;  // its first unit on the line
 };
 
-WGKV_DEVICE Head find_head(const AttnArgs& a, const Line& ln, int64_t pos, int lane) {
+WGKV_DEVICE Head find_head(const AttnArgs& a, const Line& ln, int pos, int lane) {
   const int BH = a.B * a.Hkv;
+  Head h;
   // the last lane that starts at or before pos (lanes without units start
   // where the next one does)
   const int o = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(ln.excl <= pos));
-  const int64_t base = __shfl(ln.excl, o, 64);
+  const int base = __builtin_amdgcn_readlane(ln.excl, o);
+  if (ln.per == 1) {
+    h.bh = o;
+    h.tokens = __builtin_amdgcn_readlane(ln.tokens, o);
+    h.start = base;
+    return h;
+  }
   const int bh = o * ln.per + lane;
   const int t = lane < ln.per && bh < BH ? tokens_of(a, bh) : 0;
-  const int64_t incl = wave_incl_scan64(units_of(t), lane);
-  const int64_t excl = base + incl - units_of(t);
+  const int excl = base + wave_scan_dpp(units_of(t)) - units_of(t);
   const int j = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(lane < ln.per && bh < BH && excl <= pos));
-  Head h;
   h.bh = o * ln.per + j;
   h.tokens = __builtin_amdgcn_readlane(t, j);
-  h.start = __shfl(excl, j, 64);
+  h.start = __builtin_amdgcn_readlane(excl, j);
   return h;
 }
 
@@ -132,22 +149,104 @@ WGKV_DEVICE float row_ror_add(float x) {
 }
 
 // A dword of codes as four operand dwords (pairs of 128 + c).
-WGKV_DEVICE void expand(uint32_t w, uint32_t* o) {
+// The constants come in registers, one scalar and one vector: as literals
+// they would make two instructions of one v_and_or.
+WGKV_DEVICE void expand(uint32_t w, uint32_t mask, uint32_t base, uint32_t* o) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = ((w >> (4 * i)) & kCodeMask) | kCodeBase;
+  for (int i = 0; i < 4; ++i) o[i] = ((w >> (4 * i)) & mask) | base;
 }
 
+// The weight of a piece with maximum m under the common maximum M.  A piece
+// without a maximum holds either nothing or only NaN scores, which must come
+// through.
+WGKV_DEVICE float piece_weight(float m, float M) { return m == -INFINITY ? 1.f : fast_exp2(m - M); }
+
+// Merges the pieces that workgroups f..e left of head (b, h) and writes its
+// G rows.  A thread takes four d of a row over every groups-th piece, eight
+// pieces' loads in flight, and the groups meet in LDS (kThreads * 6 floats).
+template <int D, int kThreads>
+WGKV_DEVICE void merge_pieces(const AttnArgs& a, int f, int e, int b, int h, float* lds) {
+  constexpr int kBatch = 8;
+  const int G = a.G, NQ = G * (D / 4);
+  static_assert(kThreads * 4 >= kMaxG * D, "a thread for every four d");
+  const int groups = kThreads / NQ;
+  float* s_m = lds;
+  float* s_l = lds + kThreads;
+  f32x4_t* s_a = (f32x4_t*)(lds + 2 * kThreads);
+  const int t = threadIdx.x;
+  const __amdgpu_buffer_rsrc_t acc = __builtin_amdgcn_make_buffer_rsrc(a.part_acc, (short)0, 0x7fffffff, 0x00020000);
+  const int vq = t % NQ, grp = t / NQ;
+  const int i = vq / (D / 4);
+  float M = -INFINITY, L = 0.f;
+  f32x4_t A = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  if (grp < groups) {
+    for (int x0 = f + grp; x0 <= e; x0 += groups * kBatch) {
+      float m[kBatch], l[kBatch];
+      f32x4_t ac[kBatch];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int x = min(x0 + k * groups, e);
+        const int s = (2 * x + (x == f ? 1 : 0)) * G;
+        m[k] = load_coherent(&a.part_m[s + i]);
+        l[k] = load_coherent(&a.part_l[s + i]);
+        ac[k] = load_coherent4(acc, (s * D + vq * 4) * (int)sizeof(float));
+      }
+      float mn = M;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) mn = fmaxf(mn, m[k]);
+      const float sa = piece_weight(M, mn);
+      L *= sa;
+      A *= sa;
+      M = mn;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        if (x0 + k * groups > e) break;
+        const float sb = piece_weight(m[k], M);
+        L = fmaf(l[k], sb, L);
+        A += ac[k] * sb;
+      }
+    }
+  }
+  s_m[t] = M;
+  s_l[t] = L;
+  s_a[t] = A;
+  __syncthreads();
+  if (grp == 0) {
+    float mn = M;
+    for (int g = 1; g < groups; ++g) mn = fmaxf(mn, s_m[g * NQ + t]);
+    const float sa = piece_weight(M, mn);
+    L *= sa;
+    A *= sa;
+    for (int g = 1; g < groups; ++g) {
+      const float sb = piece_weight(s_m[g * NQ + t], mn);
+      L = fmaf(s_l[g * NQ + t], sb, L);
+      A += s_a[g * NQ + t] * sb;
+    }
+    const float inv = 1.f / L;
+    uint16_t* o = a.out + (int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + (vq * 4) % D;
+    *(uint64_t*)o = (uint64_t)pack_bf16x2(A[2] * inv, A[3] * inv) << 32 | pack_bf16x2(A[0] * inv, A[1] * inv);
+  }
+}
+
+// What a wave leaves in LDS of a head that it has not seen whole.
+struct Piece {
+  int bh;            // -1: none
+  int start, units;  // of the head on the line
+};
+
 template <int D, int NT, int NW>
-__global__ __launch_bounds__(NW * 64) void kv4_attn_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void kv4_attn_kernel(AttnArgs a) {
   constexpr int NG = D / kKv4Group;  // groups
   constexpr int HPT = 16 / NG;       // query heads per 16 columns
   constexpr int KS = D / 32;         // k-steps of the first product, dwords of a lane's K and V chunk per tile
   constexpr int MT = D / 16;         // row tiles of the second product
   constexpr int kThreads = NW * 64;
   typedef __attribute__((__vector_size__(KS * sizeof(uint32_t)))) uint32_t chunk_t;
-  __shared__ float s_acc[NW][NT * HPT][D];
-  __shared__ float s_ml[NW][2][NT * HPT];
-  __shared__ int s_last;
+  static_assert(2 * NW * NT * HPT * D >= kThreads * 6, "LDS of the merge");
+  __shared__ __attribute__((aligned(16))) float s_acc[2 * NW][NT * HPT][D];
+  __shared__ float s_m[2 * NW][NT * HPT], s_l[2 * NW][NT * HPT];
+  __shared__ Piece s_piece[2 * NW];
+  __shared__ int s_last[2];
 
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4;
@@ -155,28 +254,78 @@ __global__ __launch_bounds__(NW * 64) void kv4_attn_kernel(AttnArgs a) {
   const int G = a.G, BH = a.B * a.Hkv;
   const int w = blockIdx.x, n_wg = gridDim.x;
 
-  // heads without tokens
-  for (int bh = w; bh < BH; bh += n_wg) {
-    if (tokens_of(a, bh) != 0) continue;
-    const int b = bh / a.Hkv, h = bh - b * a.Hkv;
-    for (int v = threadIdx.x; v < G * D; v += kThreads)
-      a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + v / D) * a.out_sh + v % D] = 0;
-  }
+  // a lane's places in a tile: K row n, V row n, the pairs of its group
+  const uint32_t koff = n * (D / 2) + quad * (D / 8), voff = quad * (2 * D) + n * (D / 8);
+  const uint32_t soff = kv4_scales_at(D) + (quad * NG + g) * 16;
+  uint32_t mask = kCodeMask, base = kCodeBase;
+  asm("" : "+s"(mask));
+  asm("" : "+v"(base));
 
   const Line ln = make_line(a, lane);
-  // units per workgroup: whole rounds of the waves
-  int64_t cp = (ln.total + n_wg - 1) / n_wg;
-  cp = max((cp + NW - 1) / NW * NW, (int64_t)NW);
-  int64_t pos = w * cp;
-  const int64_t end = min(ln.total, pos + cp);
+  const int cw = max((int)(((unsigned)ln.total + n_wg * NW - 1) / (unsigned)(n_wg * NW)), 1);  // units per wave
+  const int64_t first = (int64_t)(w * NW + wid) * cw;
+  int pos = (int)min(first, (int64_t)ln.total);
+  const int end = (int)min(first + cw, (int64_t)ln.total);
+  if (lane < 2) s_piece[2 * wid + lane].bh = -1;
 
+  // 32 tokens of a head: two tiles of each cache.  Every line is read whole by
+  // one load and once: non-temporal (the default policy reads 5.7 TB/s here,
+  // these 6.3).
+  struct Half {
+    chunk_t k[2], v[2];
+    u32x4_t ks[2], vs[2];
+  };
+  // The place the next loads are for.  Page ids of 64 tiles from tile 4*base
+  // on, one per lane, clamped to the pool.
+  int u = 0, base_u = 0, last_tile = 0, pages = 0;
+  const int32_t* bt_row = nullptr;
+  const auto load_half = [&](Half& x, int half) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int tile = min(4 * u + 2 * half + p, last_tile);
+      const int pg = __builtin_amdgcn_readlane(pages, tile - 4 * base_u);
+      const int64_t at = (((int64_t)pg << a.pg.page_shift) + (tile & ((1 << a.pg.page_shift) - 1))) * kv4_tile_bytes(D);
+      const uint8_t* kt = a.kc + at;
+      const uint8_t* vt = a.vc + at;
+      x.k[p] = __builtin_nontemporal_load((const chunk_t*)(kt + koff));
+      x.ks[p] = __builtin_nontemporal_load((const u32x4_t*)(kt + soff));
+      x.v[p] = __builtin_nontemporal_load((const chunk_t*)(vt + voff));
+      x.vs[p] = __builtin_nontemporal_load((const u32x4_t*)(vt + soff));
+    }
+  };
+  const auto clamp_page = [&](int pg) { return pg < 0 ? 0 : pg >= a.pg.num_pages ? (int)(a.pg.num_pages - 1) : pg; };
+  u32x4_t qraw[NT][KS];
+  const auto load_q = [&](int bh) {
+    const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const uint16_t* qrow = a.q + (int64_t)b * a.q_sb + (int64_t)(h * G + min(nt * HPT + hh, G - 1)) * a.q_sh;
+#pragma unroll
+      for (int i = 0; i < KS; ++i) qraw[nt][i] = *(const u32x4_t*)(qrow + quad * (D / 4) + i * 8);
+    }
+  };
+  const auto table_row = [&](int bh) {
+    const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+    return a.pg.bt + (int64_t)b * a.pg.bt_sb + (int64_t)h * a.pg.bt_sh;
+  };
+
+  Half x, y;
+  Head hd;
+  if (pos < end) {
+    hd = find_head(a, ln, pos, lane);
+    u = base_u = pos - hd.start;
+    last_tile = (hd.tokens - 1) >> 4;
+    bt_row = table_row(hd.bh);
+    const int pg = bt_row[min(4 * u + lane, last_tile) >> a.pg.page_shift];
+    load_q(hd.bh);
+    pages = clamp_page(pg);
+    load_half(x, 0);
+    __builtin_amdgcn_sched_barrier(0);  // the loads stay in front of the queries' wait
+  }
   while (pos < end) {
-    const Head hd = find_head(a, ln, pos, lane);
     const int b = hd.bh / a.Hkv, h = hd.bh - b * a.Hkv;
-    const int T = hd.tokens;
-    const int u0 = (int)(pos - hd.start), u1 = (int)min((int64_t)units_of(T), end - hd.start);
-    const int32_t* bt_row = a.pg.bt + (int64_t)b * a.pg.bt_sb + (int64_t)h * a.pg.bt_sh;
-    const int last_tile = (T - 1) >> 4;
+    const int T = hd.tokens, units = units_of(T);
+    const int u0 = pos - hd.start, cnt = min(units - u0, end - pos);
 
     // queries: column (g, head), k = 8 consecutive d; zeros off the column's group
     bf16x8_t qb[NT][KS];
@@ -184,14 +333,13 @@ __global__ __launch_bounds__(NW * 64) void kv4_attn_kernel(AttnArgs a) {
     float qsum[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int qh = nt * HPT + hh;
-      const uint16_t* qrow = a.q + (int64_t)b * a.q_sb + (int64_t)(h * G + min(qh, G - 1)) * a.q_sh;
-      const bool mine = quad * NG / 4 == g && qh < G;
+      const bool mine = quad * NG / 4 == g && nt * HPT + hh < G;
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
-        u32x4_t v = *(const u32x4_t*)(qrow + quad * (D / 4) + i * 8);
-        if (!mine) v = (u32x4_t){0u, 0u, 0u, 0u};
+        u32x4_t v = qraw[nt][i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = mine ? (v[j] & a.q_and) ^ a.q_xor : 0u;
 #pragma unroll
         for (int j = 0; j < 4; ++j) sum += bf16lo(v[j]) + bf16hi(v[j]);
         qb[nt][i] = __builtin_bit_cast(bf16x8_t, v);
@@ -204,83 +352,49 @@ __global__ __launch_bounds__(NW * 64) void kv4_attn_kernel(AttnArgs a) {
     }
 
     float m_run[NT], l_run[NT], corr[NT];
-    f32x4_t acc[NT][MT];
+    f32x4_t acc[NT][MT], usum[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m_run[nt] = -INFINITY;
       l_run[nt] = corr[nt] = 0.f;
+      usum[nt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int j = 0; j < MT; ++j) acc[nt][j] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
-
-    struct Unit {
-      chunk_t k[2], v[2];
-      u32x4_t ks[2], vs[2];
-    };
-    // page ids of the wave's next 32 units, two tiles each, one per lane
-    int pages = 0;
-    const auto load_pages = [&](int u) {
-      const int tile = min(2 * (u + (lane >> 1) * NW) + (lane & 1), last_tile);
-      const int pg = bt_row[tile >> a.pg.page_shift];
-      pages = pg < 0 ? 0 : pg >= a.pg.num_pages ? (int)(a.pg.num_pages - 1) : pg;
-    };
-    const auto load_unit = [&](Unit& x, int u, int it) {
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const int tile = min(2 * u + p, last_tile);
-        const int pg = __builtin_amdgcn_readlane(pages, 2 * (it & 31) + p);
-        const int64_t at = (((int64_t)pg << a.pg.page_shift) + (tile & ((1 << a.pg.page_shift) - 1))) * kv4_tile_bytes(D);
-        const uint8_t* kt = a.kc + at;
-        const uint8_t* vt = a.vc + at;
-        x.k[p] = *(const chunk_t*)(kt + n * (D / 2) + quad * (D / 8));
-        x.ks[p] = *(const u32x4_t*)(kt + kv4_scales_at(D) + (quad * NG + g) * 16);
-        x.v[p] = *(const chunk_t*)(vt + quad * (2 * D) + n * (D / 8));
-        x.vs[p] = *(const u32x4_t*)(vt + kv4_scales_at(D) + (quad * NG + g) * 16);
-      }
-    };
-    // takes the offset's part out of the accumulators: they and the
-    // correction grow with the tokens, their difference does not
+    // takes the offset's part out of the accumulators and adds the middles':
+    // they and the offset's sum grow with the tokens, their difference does not
     const auto flush = [&]() {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float c = corr[nt];
         c += __shfl_xor(c, 16, 64);
         c += __shfl_xor(c, 32, 64);
+        c = fmaf(-kOffset, usum[nt][0], c);
         corr[nt] = 0.f;
+        usum[nt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < MT; ++j) acc[nt][j] += c;
       }
     };
 
-    Unit cur;
-    int u = u0 + wid, it = 0;
-    if (u < u1) {
-      load_pages(u);
-      load_unit(cur, u, 0);
-    }
-    for (; u < u1; u += NW, ++it) {
-      Unit nxt;
-      const int un = u + NW;
-      if (un < u1) {
-        if (((it + 1) & 31) == 0) load_pages(un);
-        load_unit(nxt, un, it + 1);
-      }
-      if (u * 32 + 32 > T) {  // rows past the end hold anything: step and middle 0
+    // tokens t0..t0+31 of the head
+    const auto step = [&](Half& t, int t0) {
+      const bool tail = t0 + 32 > T;  // rows past the head's end among them
+      if (tail) {                         // those rows hold anything: step and middle 0
 #pragma unroll
         for (int p = 0; p < 2; ++p)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (u * 32 + p * 16 + quad * 4 + i >= T) cur.ks[p][i] = cur.vs[p][i] = 0u;
+            if (t0 + p * 16 + quad * 4 + i >= T) t.ks[p][i] = t.vs[p][i] = 0u;
       }
       f32x4_t z[NT][2];
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
 #pragma unroll
         for (int i = 0; i < KS; ++i) {
-          u32x4_t o;
           uint32_t e[4];
-          expand(cur.k[p][i], e);
-          o = (u32x4_t){e[0], e[1], e[2], e[3]};
+          expand(t.k[p][i], mask, base, e);
+          const u32x4_t o = (u32x4_t){e[0], e[1], e[2], e[3]};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
             z[nt][p] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, o), qb[nt][i],
@@ -290,36 +404,39 @@ __global__ __launch_bounds__(NW * 64) void kv4_attn_kernel(AttnArgs a) {
       u32x4_t pb[NT];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float t[2][4];
+        float s[2][4];
 #pragma unroll
         for (int p = 0; p < 2; ++p)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float x = fmaf(z[nt][p][i], bf16lo(cur.ks[p][i]), bf16hi(cur.ks[p][i]) * qsum[nt]);
-            x = row_ror_add<8>(x);
-            if constexpr (NG == 4) x = row_ror_add<4>(x);
-            t[p][i] = x * a.scale_log2;
+            float v = fmaf(z[nt][p][i], bf16lo(t.ks[p][i]), bf16hi(t.ks[p][i]) * qsum[nt]);
+            v = row_ror_add<8>(v);
+            if constexpr (NG == 4) v = row_ror_add<4>(v);
+            s[p][i] = v;
           }
-        if (u * 32 + 32 > T) {
+        if (tail) {
 #pragma unroll
           for (int p = 0; p < 2; ++p)
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              if (u * 32 + p * 16 + quad * 4 + i >= T) t[p][i] = -INFINITY;
+            for (int i = 0; i < 4; ++i) {
+              asm volatile("" : "+v"(s[p][i]));  // a branch, not selects in every unit
+              if (t0 + p * 16 + quad * 4 + i >= T) s[p][i] = -INFINITY;
+            }
         }
-        const float top = fmaxf(fmaxf(fmaxf(t[0][0], t[0][1]), fmaxf(t[0][2], t[0][3])),
-                                fmaxf(fmaxf(t[1][0], t[1][1]), fmaxf(t[1][2], t[1][3])));
+        const float top = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
+                                fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
         // The maximum of a column moves only when a score exceeds it by more
         // than the slack (p <= 2^slack); it is the same in the column's four
         // lanes, whose accumulators hold sums over all of them.
-        if (__builtin_amdgcn_ballot_w64(top > m_run[nt] + kRescaleSlack)) {
+        if (__builtin_amdgcn_ballot_w64(top * a.scale_log2 > m_run[nt] + kRescaleSlack)) {
           float mx = fmaxf(top, __shfl_xor(top, 16, 64));
           mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-          const float mn = fmaxf(m_run[nt], mx);
+          const float mn = fmaxf(m_run[nt], mx * a.scale_log2);
           const float alpha = mn == -INFINITY ? 1.f : fast_exp2(m_run[nt] - mn);
           m_run[nt] = mn;
           l_run[nt] *= alpha;
           corr[nt] *= alpha;
+          usum[nt] *= alpha;
 #pragma unroll
           for (int j = 0; j < MT; ++j) acc[nt][j] *= alpha;
         }
@@ -328,19 +445,18 @@ __global__ __launch_bounds__(NW * 64) void kv4_attn_kernel(AttnArgs a) {
         for (int p = 0; p < 2; ++p)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const int i0 = 2 * j, i1 = 2 * j + 1;
-            const float p0 = fast_exp2(t[p][i0] - m_run[nt]), p1 = fast_exp2(t[p][i1] - m_run[nt]);
+            const uint32_t s0 = t.vs[p][2 * j], s1 = t.vs[p][2 * j + 1];
+            const float p0 = fast_exp2(fmaf(s[p][2 * j], a.scale_log2, -m_run[nt]));
+            const float p1 = fast_exp2(fmaf(s[p][2 * j + 1], a.scale_log2, -m_run[nt]));
             l_run[nt] += p0 + p1;
-            const uint32_t s0 = cur.vs[p][i0], s1 = cur.vs[p][i1];
-            const uint32_t pr = pack_bf16x2(p0 * bf16lo(s0), p1 * bf16lo(s1));
-            pk[2 * p + j] = pr;
-            // with the rounded products: the offset must cancel exactly
-            float c = fmaf(-kOffset, bf16lo(pr), corr[nt]);
-            c = fmaf(-kOffset, bf16hi(pr), c);
-            c = fmaf(p0, bf16hi(s0), c);
-            corr[nt] = fmaf(p1, bf16hi(s1), c);
+            corr[nt] = fmaf(p1, bf16hi(s1), fmaf(p0, bf16hi(s0), corr[nt]));
+            pk[2 * p + j] = pack_bf16x2(p0 * bf16lo(s0), p1 * bf16lo(s1));
           }
         pb[nt] = (u32x4_t){pk[0], pk[1], pk[2], pk[3]};
+        // the sum of the rounded products, for the offset to cancel exactly
+        const u32x4_t ones = (u32x4_t){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+        usum[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ones),
+                                                           __builtin_bit_cast(bf16x8_t, pb[nt]), usum[nt], 0, 0, 0);
       }
       // row tile j holds d = MT*r + j: code j%4 of the words of half j/4
 #pragma unroll
@@ -349,7 +465,7 @@ __global__ __launch_bounds__(NW * 64) void kv4_attn_kernel(AttnArgs a) {
 #pragma unroll
         for (int p = 0; p < 2; ++p)
 #pragma unroll
-          for (int pr = 0; pr < 2; ++pr) expand(cur.v[p][pr * (KS / 2) + hf], e[2 * p + pr]);
+          for (int pr = 0; pr < 2; ++pr) expand(t.v[p][pr * (KS / 2) + hf], mask, base, e[2 * p + pr]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const u32x4_t o = (u32x4_t){e[0][c], e[1][c], e[2][c], e[3][c]};
@@ -359,117 +475,185 @@ __global__ __launch_bounds__(NW * 64) void kv4_attn_kernel(AttnArgs a) {
                 __builtin_bit_cast(bf16x8_t, o), __builtin_bit_cast(bf16x8_t, pb[nt]), acc[nt][hf * 4 + c], 0, 0, 0);
         }
       }
+    };
+
+    Head nx = hd;  // the next unit's head
+    for (int it = 0; it < cnt; ++it) {
+      // what the next unit needs before its tiles can be asked for -- new
+      // page ids, the next head's queries -- is requested ahead of this
+      // unit's second half, and so is there when that half is
+      const int t0 = (u0 + it) * 64;
+      const bool cross = it + 1 == cnt && pos + cnt < end;
+      const bool refill = cross || u0 + it + 1 - base_u == 16;
+      int pg = 0;
+      if (refill) {
+        if (cross) {
+          nx = find_head(a, ln, pos + cnt, lane);
+          load_q(nx.bh);
+        }
+        const int first_u = cross ? 0 : u0 + it + 1;
+        pg = table_row(nx.bh)[min(4 * first_u + lane, (nx.tokens - 1) >> 4) >> a.pg.page_shift];
+      }
+      load_half(y, 1);
+      step(x, t0);
+      if (refill) {
+        u = base_u = cross ? 0 : u0 + it + 1;
+        last_tile = (nx.tokens - 1) >> 4;
+        pages = clamp_page(pg);
+      } else {
+        ++u;
+      }
+      load_half(x, 0);  // past the range's end: any of its tiles
+      step(y, t0 + 32);
       if ((it & (kFlush - 1)) == kFlush - 1) flush();
-      cur = nxt;
     }
     flush();
 
-    // ---- merge the waves ---------------------------------------------------
     // lane (quad, g, hh) holds rows 4*quad + i of column (g, hh): d = MT *
     // (4*quad + i) + j, of the column's group where quad*NG/4 == g
+    const bool whole = cnt == units;
+    const int slot = 2 * wid + (u0 > 0 ? 0 : 1);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float l = l_run[nt];
       l += __shfl_xor(l, 16, 64);
       l += __shfl_xor(l, 32, 64);
       const int qh = nt * HPT + hh;
-      if (quad * NG / 4 == g) {
+      if (quad * NG / 4 == g && qh < G) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+          const int d = MT * (4 * quad + i);
+          if (whole) {
+            const float inv = 1.f / l;
+            uint32_t o[MT / 2];
 #pragma unroll
-          for (int j = 0; j < MT; ++j) s_acc[wid][qh][MT * (4 * quad + i) + j] = acc[nt][j][i];
+            for (int j = 0; j < MT / 2; ++j) o[j] = pack_bf16x2(acc[nt][2 * j][i] * inv, acc[nt][2 * j + 1][i] * inv);
+            uint16_t* dst = a.out + (int64_t)b * a.out_sb + (int64_t)(h * G + qh) * a.out_sh + d;
+            if constexpr (MT == 8) *(u32x4_t*)dst = (u32x4_t){o[0], o[1], o[2], o[3]};
+            else *(uint64_t*)dst = (uint64_t)o[1] << 32 | o[0];
+          } else {
+#pragma unroll
+            for (int j = 0; j < MT; ++j) s_acc[slot][qh][d + j] = acc[nt][j][i];
+          }
+        }
       }
-      if (quad == 0 && g == 0) {
-        s_ml[wid][0][qh] = m_run[nt];
-        s_ml[wid][1][qh] = l;
+      if (!whole && quad == 0 && g == 0) {
+        s_m[slot][qh] = m_run[nt];
+        s_l[slot][qh] = l;
       }
     }
-    __syncthreads();
+    if (!whole && lane == 0) s_piece[slot] = Piece{hd.bh, hd.start, units};
+    pos += cnt;
+    hd = nx;
+  }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the loads past the end
+  __syncthreads();
 
-    const int64_t f = hd.start / cp;                                    // the head's first and
-    const int64_t e = (hd.start + units_of(T) - 1) / cp;                // last workgroup
-    const bool single = f == e;
-    const int slot = 2 * w + (f == w ? 1 : 0);
+  // ---- the workgroup's heads -----------------------------------------------
+  // Waves hold consecutive ranges, so a head's pieces are neighbours in LDS.
+  // What the workgroup does not hold whole goes to the workspace: at most the
+  // head that it ends and the one that it begins.
+  const int cg = cw * NW;  // units per workgroup
+  const Piece mine = s_piece[lane & (2 * NW - 1)];
+  uint64_t todo = __builtin_amdgcn_ballot_w64(lane < 2 * NW && mine.bh >= 0);
+  int n_open = 0, open_bh[2], open_f[2], open_e[2];
+  while (todo) {
+    const int s0 = __builtin_ctzll(todo);
+    const int bh = __builtin_amdgcn_readlane(mine.bh, s0);
+    const int start = __builtin_amdgcn_readlane(mine.start, s0), units = __builtin_amdgcn_readlane(mine.units, s0);
+    const uint64_t run = __builtin_amdgcn_ballot_w64(lane < 2 * NW && mine.bh == bh);
+    todo &= ~run;
+    const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+    const int f = (int)((unsigned)start / (unsigned)cg), e = (int)((unsigned)(start + units - 1) / (unsigned)cg);
+    const int64_t to = (int64_t)(2 * w + (f == w ? 1 : 0)) * G;
     for (int v = threadIdx.x; v < G * D; v += kThreads) {
       const int i = v / D, d = v - i * D;
-      float M = -INFINITY;
+      float m[2 * NW], M = -INFINITY, L = 0.f, A = 0.f;
 #pragma unroll
-      for (int ww = 0; ww < NW; ++ww) M = fmaxf(M, s_ml[ww][0][i]);
-      float L = 0.f, A = 0.f;
-#pragma unroll
-      for (int ww = 0; ww < NW; ++ww) {
-        // a wave without a score has l = acc = 0; NaN scores leave m = -inf
-        // and must come through
-        const float mw = s_ml[ww][0][i];
-        const float sc = mw == -INFINITY ? 1.f : fast_exp2(mw - M);
-        L = fmaf(sc, s_ml[ww][1][i], L);
-        A = fmaf(sc, s_acc[ww][i][d], A);
+      for (int s = 0; s < 2 * NW; ++s) {
+        m[s] = run >> s & 1 ? s_m[s][i] : -INFINITY;
+        M = fmaxf(M, m[s]);
       }
-      if (single) {
+#pragma unroll
+      for (int s = 0; s < 2 * NW; ++s) {
+        const float l = s_l[s][i], ac = s_acc[s][i][d], c = piece_weight(m[s], M);
+        if (run >> s & 1) {  // other slots hold anything
+          L = fmaf(l, c, L);
+          A = fmaf(ac, c, A);
+        }
+      }
+      if (f == e) {
         a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + d] = f32_to_bf16(A / L);
       } else {
         if (d == 0) {
-          store_coherent(&a.part_m[(int64_t)slot * G + i], M);
-          store_coherent(&a.part_l[(int64_t)slot * G + i], L);
+          store_coherent(&a.part_m[to + i], M);
+          store_coherent(&a.part_l[to + i], L);
         }
-        store_coherent(&a.part_acc[((int64_t)slot * G + i) * D + d], A);
+        store_coherent(&a.part_acc[(to + i) * D + d], A);
       }
     }
-    if (!single) {
-      // The last workgroup of the head to arrive merges.  Its loads see the
-      // others' pieces without cache write-backs: the stores above are
-      // device-coherent (written through to the point of coherence, where
-      // the counter's atomics are performed too), vmcnt(0) waits until they
-      // are acknowledged there, the barrier holds the arrival until every
-      // wave has waited, and the merge's loads bypass this XCD's L2.
+    if (f != e) {
+      if (n_open == 0) open_bh[0] = bh, open_f[0] = f, open_e[0] = e;
+      else open_bh[1] = bh, open_f[1] = f, open_e[1] = e;
+      ++n_open;
+    }
+  }
+
+  if (n_open > 0) {
+    // The last workgroup of a head to arrive merges.  Its loads see the
+    // others' pieces without cache write-backs: the stores above are
+    // device-coherent (written through to the point of coherence, where the
+    // counter's atomics are performed too), vmcnt(0) waits until they are
+    // acknowledged there, the barrier holds the arrival until every wave has
+    // waited, and the merge's loads bypass this XCD's L2.
 #if defined(__HIP_DEVICE_COMPILE__) && !defined(__gfx950__)
 #error "the merge relies on gfx950 store acknowledgement and sc1 ordering"
 #endif
-      __atomic_signal_fence(__ATOMIC_SEQ_CST);
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-      __atomic_signal_fence(__ATOMIC_SEQ_CST);
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        const int prev = __hip_atomic_fetch_add(&a.counter[hd.bh], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        const int last = prev == (int)(e - f);
-        if (last) __hip_atomic_store(&a.counter[hd.bh], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        s_last = last;
-      }
-      __syncthreads();
-      if (s_last) {
-        __atomic_signal_fence(__ATOMIC_SEQ_CST);
-        for (int v = threadIdx.x; v < G * D; v += kThreads) {
-          const int i = v / D, d = v - i * D;
-          float M = -INFINITY, L = 0.f, A = 0.f;
-          for (int64_t x = f; x <= e; ++x) {
-            const int64_t s = 2 * x + (x == f ? 1 : 0);
-            const float m = load_coherent(&a.part_m[s * G + i]);
-            const float l = load_coherent(&a.part_l[s * G + i]);
-            const float ac = load_coherent(&a.part_acc[(s * G + i) * D + d]);
-            const float mn = fmaxf(M, m);
-            const float sa = M == -INFINITY ? 1.f : fast_exp2(M - mn), sb = m == -INFINITY ? 1.f : fast_exp2(m - mn);
-            L = L * sa + l * sb;
-            A = A * sa + ac * sb;
-            M = mn;
-          }
-          a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + d] = f32_to_bf16(A / L);
-        }
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __syncthreads();
+    if (threadIdx.x < n_open) {
+      const int t = threadIdx.x;
+      const int bh = t ? open_bh[1] : open_bh[0], others = t ? open_e[1] - open_f[1] : open_e[0] - open_f[0];
+      const int prev = __hip_atomic_fetch_add(&a.counter[bh], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const int last = prev == others;
+      if (last) __hip_atomic_store(&a.counter[bh], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      s_last[t] = last;
+    }
+    __syncthreads();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (t < n_open && __builtin_amdgcn_readfirstlane(s_last[t])) {
+        const int b = open_bh[t] / a.Hkv;
+        if (t) __syncthreads();  // the first one's LDS
+        merge_pieces<D, kThreads>(a, open_f[t], open_e[t], b, open_bh[t] - b * a.Hkv, &s_acc[0][0][0]);
       }
     }
-    pos = hd.start + units_of(T);
-    __syncthreads();  // LDS is free for the next head
+  }
+
+  // heads without tokens
+  for (int bh = w; bh < BH; bh += n_wg) {
+    const int t = ln.per == 1 ? __builtin_amdgcn_readlane(ln.tokens, bh) : tokens_of(a, bh);
+    if (t != 0) continue;
+    const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+    for (int v = threadIdx.x; v < G * D; v += kThreads)
+      a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + v / D) * a.out_sh + v % D] = 0;
   }
 }
 
 size_t part_floats(int G, int D) { return (size_t)2 * kMaxSlots * G * (2 + (size_t)D); }
 constexpr size_t kCounterBytes = (size_t)kMaxBH * sizeof(int);
 
+// One workgroup per CU: 8 waves, two per SIMD, or with two column tiles, whose
+// accumulators and queries take twice the registers, 4.
 template <int D, int NT>
 hipError_t launch(const AttnArgs& a, hipStream_t st) {
-  constexpr int NW = 4, kPerCU = 3;
-  // no more workgroups than the tables have rounds of units for
-  const int64_t most = ((kv4_capacity(a.pg) + 31) / 32 * a.B * a.Hkv + NW - 1) / NW;
-  const int slots = min(kMaxSlots, cu_count() * kPerCU);
+  constexpr int NW = NT == 1 ? 8 : 4;
+  // no more workgroups than the tables have units for
+  const int64_t most = ((kv4_capacity(a.pg) + 63) / 64 * a.B * a.Hkv + NW - 1) / NW;
+  const int slots = min(kMaxSlots, cu_count());
   hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW>), dim3((unsigned)(most < slots ? most : slots)), dim3(NW * 64), 0, st, a);
   return hipGetLastError();
 }
@@ -497,8 +681,10 @@ extern "C" int wgkv_kv4_decode_attn(
   AttnArgs a{};
   const int st = kv4_pages(&a.pg, num_pages, page_size, block_table, bt_stride_b, bt_stride_h, max_pages);
   if (st != WGKV_OK) return st;
+  if ((kv4_capacity(a.pg) + 63) / 64 * batch * num_kv_heads > 0x7fffffff) return WGKV_ERR_UNSUPPORTED;
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return WGKV_ERR_UNSUPPORTED;
   if ((q_stride_b | q_stride_h) & 7) return WGKV_ERR_UNSUPPORTED;
+  if (((uintptr_t)out & 15) || ((out_stride_b | out_stride_h) & 7)) return WGKV_ERR_UNSUPPORTED;
   if (!workspace || ((uintptr_t)workspace & 15) ||
       workspace_bytes < wgkv_kv4_decode_workspace_bytes(num_q_heads, num_kv_heads, head_dim))
     return WGKV_ERR_WORKSPACE;
@@ -515,7 +701,12 @@ extern "C" int wgkv_kv4_decode_attn(
   a.B = batch;
   a.Hkv = num_kv_heads;
   a.G = G;
-  a.scale_log2 = softmax_scale * kLog2e;
+  // scores in the order of the products: a negative scale negates the
+  // queries, and a scale of 0 clears them (masked rows hold -inf, and -inf * 0
+  // is not a number)
+  a.scale_log2 = softmax_scale == 0.f ? 1.f : fabsf(softmax_scale) * kLog2e;
+  a.q_and = softmax_scale == 0.f ? 0u : ~0u;
+  a.q_xor = softmax_scale < 0.f ? 0x80008000u : 0u;
   a.counter = (int*)workspace;
   const size_t slots = (size_t)2 * kMaxSlots * G;
   a.part_m = (float*)((char*)workspace + kCounterBytes);
