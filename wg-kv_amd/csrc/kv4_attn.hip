@@ -55,6 +55,8 @@ struct AttnArgs {
   uint16_t* out;
   int64_t out_sb, out_sh;
   int B, Hkv, G;
+  int cap;            // tokens a head's table row has pages for
+  uint32_t hkv_inv;   // ceil(2^32 / Hkv), 0 for 1: see sequence_of
   float scale_log2;         // |softmax_scale| * log2(e)
   uint32_t q_and, q_xor;    // its sign (and a scale of 0) is put into the queries
   // pieces: two slots per workgroup (the head it ends, the head it begins);
@@ -63,11 +65,16 @@ struct AttnArgs {
   int* counter;  // arrivals per (b, h), zero between calls
 };
 
+// bh / Hkv by a multiplication: exact while bh * Hkv < 2^32 (both are at most
+// 2048).  A division's code costs more than its time: instructions that run
+// once come cold from memory.
+WGKV_DEVICE int sequence_of(const AttnArgs& a, int bh) {
+  return a.hkv_inv ? (int)__umulhi((uint32_t)bh, a.hkv_inv) : bh;
+}
+
 WGKV_DEVICE int tokens_of(const AttnArgs& a, int bh) {
-  const int b = bh / a.Hkv, h = bh - b * a.Hkv;
-  const int64_t cap = kv4_capacity(a.pg);
-  const int64_t n = a.len[(int64_t)b * a.len_sb + h];
-  return (int)(n < 0 ? 0 : n > cap ? cap : n);
+  const int b = sequence_of(a, bh), h = bh - b * a.Hkv;
+  return min(max(a.len[(int64_t)b * a.len_sb + h], 0), a.cap);
 }
 WGKV_DEVICE int units_of(int tokens) { return (tokens + 63) >> 6; }
 
@@ -88,25 +95,27 @@ WGKV_DEVICE int wave_scan_dpp(int v) {
 // 31 bits.)
 struct Line {
   int per;
-  int tokens;  // of the lane's head where per is 1
+  int tokens;  // of the lane's head (up to 64 heads)
   int excl;    // units before the lane's heads
   int total;
 };
 
+// kMany: more than 64 heads.
+template <bool kMany>
 WGKV_DEVICE Line make_line(const AttnArgs& a, int lane) {
   const int BH = a.B * a.Hkv;
   Line ln;
-  ln.per = (BH + 63) >> 6;
+  ln.per = kMany ? (BH + 63) >> 6 : 1;
   ln.tokens = 0;
   int n = 0;
-  if (ln.per == 1) {
-    if (lane < BH) ln.tokens = tokens_of(a, lane);
-    n = units_of(ln.tokens);
-  } else {
+  if constexpr (kMany) {
     for (int i = 0; i < ln.per; ++i) {
       const int bh = lane * ln.per + i;
       if (bh < BH) n += units_of(tokens_of(a, bh));
     }
+  } else {
+    if (lane < BH) ln.tokens = tokens_of(a, lane);
+    n = units_of(ln.tokens);
   }
   const int incl = wave_scan_dpp(n);
   ln.excl = incl - n;
@@ -120,26 +129,27 @@ struct Head {
   int start;  // its first unit on the line
 };
 
+template <bool kMany>
 WGKV_DEVICE Head find_head(const AttnArgs& a, const Line& ln, int pos, int lane) {
-  const int BH = a.B * a.Hkv;
   Head h;
   // the last lane that starts at or before pos (lanes without units start
   // where the next one does)
   const int o = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(ln.excl <= pos));
   const int base = __builtin_amdgcn_readlane(ln.excl, o);
-  if (ln.per == 1) {
+  if constexpr (kMany) {
+    const int bh = o * ln.per + lane;
+    const bool in = lane < ln.per && bh < a.B * a.Hkv;
+    const int t = in ? tokens_of(a, bh) : 0;
+    const int excl = base + wave_scan_dpp(units_of(t)) - units_of(t);
+    const int j = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(in && excl <= pos));
+    h.bh = o * ln.per + j;
+    h.tokens = __builtin_amdgcn_readlane(t, j);
+    h.start = __builtin_amdgcn_readlane(excl, j);
+  } else {
     h.bh = o;
     h.tokens = __builtin_amdgcn_readlane(ln.tokens, o);
     h.start = base;
-    return h;
   }
-  const int bh = o * ln.per + lane;
-  const int t = lane < ln.per && bh < BH ? tokens_of(a, bh) : 0;
-  const int excl = base + wave_scan_dpp(units_of(t)) - units_of(t);
-  const int j = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(lane < ln.per && bh < BH && excl <= pos));
-  h.bh = o * ln.per + j;
-  h.tokens = __builtin_amdgcn_readlane(t, j);
-  h.start = __builtin_amdgcn_readlane(excl, j);
   return h;
 }
 
@@ -234,7 +244,7 @@ struct Piece {
   int start, units;  // of the head on the line
 };
 
-template <int D, int NT, int NW>
+template <int D, int NT, int NW, bool kMany>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void kv4_attn_kernel(AttnArgs a) {
   constexpr int NG = D / kKv4Group;  // groups
   constexpr int HPT = 16 / NG;       // query heads per 16 columns
@@ -261,7 +271,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
   asm("" : "+s"(mask));
   asm("" : "+v"(base));
 
-  const Line ln = make_line(a, lane);
+  const Line ln = make_line<kMany>(a, lane);
   const int cw = max((int)(((unsigned)ln.total + n_wg * NW - 1) / (unsigned)(n_wg * NW)), 1);  // units per wave
   const int64_t first = (int64_t)(w * NW + wid) * cw;
   int pos = (int)min(first, (int64_t)ln.total);
@@ -296,7 +306,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
   const auto clamp_page = [&](int pg) { return pg < 0 ? 0 : pg >= a.pg.num_pages ? (int)(a.pg.num_pages - 1) : pg; };
   u32x4_t qraw[NT][KS];
   const auto load_q = [&](int bh) {
-    const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+    const int b = sequence_of(a, bh), h = bh - b * a.Hkv;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const uint16_t* qrow = a.q + (int64_t)b * a.q_sb + (int64_t)(h * G + min(nt * HPT + hh, G - 1)) * a.q_sh;
@@ -305,14 +315,14 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     }
   };
   const auto table_row = [&](int bh) {
-    const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+    const int b = sequence_of(a, bh), h = bh - b * a.Hkv;
     return a.pg.bt + (int64_t)b * a.pg.bt_sb + (int64_t)h * a.pg.bt_sh;
   };
 
   Half x, y;
   Head hd;
   if (pos < end) {
-    hd = find_head(a, ln, pos, lane);
+    hd = find_head<kMany>(a, ln, pos, lane);
     u = base_u = pos - hd.start;
     last_tile = (hd.tokens - 1) >> 4;
     bt_row = table_row(hd.bh);
@@ -323,7 +333,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     __builtin_amdgcn_sched_barrier(0);  // the loads stay in front of the queries' wait
   }
   while (pos < end) {
-    const int b = hd.bh / a.Hkv, h = hd.bh - b * a.Hkv;
+    const int b = sequence_of(a, hd.bh), h = hd.bh - b * a.Hkv;
     const int T = hd.tokens, units = units_of(T);
     const int u0 = pos - hd.start, cnt = min(units - u0, end - pos);
 
@@ -488,7 +498,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
       int pg = 0;
       if (refill) {
         if (cross) {
-          nx = find_head(a, ln, pos + cnt, lane);
+          nx = find_head<kMany>(a, ln, pos + cnt, lane);
           load_q(nx.bh);
         }
         const int first_u = cross ? 0 : u0 + it + 1;
@@ -563,24 +573,18 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     const int start = __builtin_amdgcn_readlane(mine.start, s0), units = __builtin_amdgcn_readlane(mine.units, s0);
     const uint64_t run = __builtin_amdgcn_ballot_w64(lane < 2 * NW && mine.bh == bh);
     todo &= ~run;
-    const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+    const int b = sequence_of(a, bh), h = bh - b * a.Hkv;
     const int f = (int)((unsigned)start / (unsigned)cg), e = (int)((unsigned)(start + units - 1) / (unsigned)cg);
     const int64_t to = (int64_t)(2 * w + (f == w ? 1 : 0)) * G;
     for (int v = threadIdx.x; v < G * D; v += kThreads) {
       const int i = v / D, d = v - i * D;
-      float m[2 * NW], M = -INFINITY, L = 0.f, A = 0.f;
-#pragma unroll
-      for (int s = 0; s < 2 * NW; ++s) {
-        m[s] = run >> s & 1 ? s_m[s][i] : -INFINITY;
-        M = fmaxf(M, m[s]);
-      }
-#pragma unroll
-      for (int s = 0; s < 2 * NW; ++s) {
-        const float l = s_l[s][i], ac = s_acc[s][i][d], c = piece_weight(m[s], M);
-        if (run >> s & 1) {  // other slots hold anything
-          L = fmaf(l, c, L);
-          A = fmaf(ac, c, A);
-        }
+      float M = -INFINITY, L = 0.f, A = 0.f;
+      for (uint64_t r = run; r; r &= r - 1) M = fmaxf(M, s_m[__builtin_ctzll(r)][i]);
+      for (uint64_t r = run; r; r &= r - 1) {
+        const int s = __builtin_ctzll(r);
+        const float c = piece_weight(s_m[s][i], M);
+        L = fmaf(s_l[s][i], c, L);
+        A = fmaf(s_acc[s][i][d], c, A);
       }
       if (f == e) {
         a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + d] = f32_to_bf16(A / L);
@@ -623,21 +627,20 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     }
     __syncthreads();
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (t < n_open && __builtin_amdgcn_readfirstlane(s_last[t])) {
-        const int b = open_bh[t] / a.Hkv;
-        if (t) __syncthreads();  // the first one's LDS
-        merge_pieces<D, kThreads>(a, open_f[t], open_e[t], b, open_bh[t] - b * a.Hkv, &s_acc[0][0][0]);
-      }
+#pragma unroll 1
+    for (int t = 0; t < n_open; ++t) {
+      if (!__builtin_amdgcn_readfirstlane(s_last[t])) continue;
+      const int bh = t ? open_bh[1] : open_bh[0], b = sequence_of(a, bh);
+      if (t) __syncthreads();  // the first one's LDS
+      merge_pieces<D, kThreads>(a, t ? open_f[1] : open_f[0], t ? open_e[1] : open_e[0], b, bh - b * a.Hkv, &s_acc[0][0][0]);
     }
   }
 
   // heads without tokens
   for (int bh = w; bh < BH; bh += n_wg) {
-    const int t = ln.per == 1 ? __builtin_amdgcn_readlane(ln.tokens, bh) : tokens_of(a, bh);
+    const int t = kMany ? tokens_of(a, bh) : __builtin_amdgcn_readlane(ln.tokens, bh);
     if (t != 0) continue;
-    const int b = bh / a.Hkv, h = bh - b * a.Hkv;
+    const int b = sequence_of(a, bh), h = bh - b * a.Hkv;
     for (int v = threadIdx.x; v < G * D; v += kThreads)
       a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + v / D) * a.out_sh + v % D] = 0;
   }
@@ -654,7 +657,9 @@ hipError_t launch(const AttnArgs& a, hipStream_t st) {
   // no more workgroups than the tables have units for
   const int64_t most = ((kv4_capacity(a.pg) + 63) / 64 * a.B * a.Hkv + NW - 1) / NW;
   const int slots = min(kMaxSlots, cu_count());
-  hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW>), dim3((unsigned)(most < slots ? most : slots)), dim3(NW * 64), 0, st, a);
+  const dim3 grid((unsigned)(most < slots ? most : slots));
+  if (a.B * a.Hkv > 64) hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, true>), grid, dim3(NW * 64), 0, st, a);
+  else hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, false>), grid, dim3(NW * 64), 0, st, a);
   return hipGetLastError();
 }
 
@@ -701,6 +706,8 @@ extern "C" int wgkv_kv4_decode_attn(
   a.B = batch;
   a.Hkv = num_kv_heads;
   a.G = G;
+  a.cap = (int)kv4_capacity(a.pg);
+  a.hkv_inv = num_kv_heads == 1 ? 0u : (uint32_t)((0x100000000ull + num_kv_heads - 1) / num_kv_heads);
   // scores in the order of the products: a negative scale negates the
   // queries, and a scale of 0 clears them (masked rows hold -inf, and -inf * 0
   // is not a number)
