@@ -20,14 +20,16 @@ The operators run on torch's current stream of the tensors' device, allocate
 only their outputs and scratch (both through torch, so a call can be captured
 in a HIP graph) and never synchronise with the host.
 """
-import functools
-
 import torch
 
 from . import _lib
 from .ops import _u8
 
+# A small call's time is its host time: the operators read each tensor's
+# shape, strides and device once and leave to the C ABI what it checks itself.
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
+_I32, _U8, _BF16 = torch.int32, torch.uint8, torch.bfloat16
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def kv4_cache_shape(num_blocks, block_size, head_dim):
@@ -45,40 +47,24 @@ def kv4_cache(num_blocks, block_size, head_dim, device="cuda"):
     return tuple(torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2))
 
 
-def _same_device(first, *rest):
-    if not first.is_cuda:
-        raise ValueError("wgkv kernels take device tensors (no CPU fallback)")
-    dev = first.device
-    for t in rest:
-        if t is not None and t.device != dev:
-            raise ValueError("all tensors must be on one device")
-    return dev
+def _host_tensor():
+    raise ValueError("wgkv kernels take device tensors (no CPU fallback)")
 
 
-def _on_own_device(op):
-    """Runs op with its tensors' device current: a null stream, and whether
-    a stream is being captured, are the current device's."""
-    @functools.wraps(op)
-    def call(first, *args, **kw):
-        dev = first.device
-        if dev.type != "cuda" or dev.index == torch.cuda.current_device():
-            return op(first, *args, **kw)
-        with torch.cuda.device(dev):
-            return op(first, *args, **kw)
-    return call
+def _two_devices():
+    raise ValueError("all tensors must be on one device")
 
 
-def _call(dev, where, fn, *args):
-    st = fn(*args, _lib.stream_handle(dev))
-    if st:
-        _lib.check(st, where)
+def _stream(index):
+    raw = _lib._raw_stream
+    return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
 
 
 def _check_cache(k_cache, v_cache):
     shape = k_cache.shape
     if len(shape) != 3 or v_cache.shape != shape or shape[2] not in (640, 1280) or shape[1] not in (1, 2, 4):
         raise AssertionError("k_cache/v_cache must be (num_blocks, block_size/16, 10*head_dim), as kv4_cache makes them")
-    if k_cache.dtype != torch.uint8 or v_cache.dtype != torch.uint8:
+    if k_cache.dtype is not _U8 or v_cache.dtype is not _U8:
         raise TypeError("k_cache/v_cache must be uint8")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
         raise ValueError("k_cache/v_cache must be contiguous")
@@ -86,36 +72,42 @@ def _check_cache(k_cache, v_cache):
 
 
 def _check_heads(block_table, lengths, B, H):
-    if block_table.dim() != 3 or block_table.shape[0] != B or block_table.shape[1] != H:
+    """The page table and the lengths, copied where their last dimension is
+    not contiguous, with their strides and the table's width."""
+    shape = block_table.shape
+    if len(shape) != 3 or shape[0] != B or shape[1] != H:
         raise AssertionError("block_table must be (batch, num_kv_heads, max_blocks)")
     if lengths.shape != (B, H):
         raise AssertionError("lengths must be (batch, num_kv_heads)")
-    if block_table.dtype != torch.int32 or lengths.dtype != torch.int32:
+    if block_table.dtype is not _I32 or lengths.dtype is not _I32:
         raise TypeError("block_table and lengths must be int32")
-    if block_table.stride(2) != 1:
+    bs, ls = block_table.stride(), lengths.stride()
+    if bs[2] != 1:
         block_table = block_table.contiguous()
-    if lengths.stride(1) != 1:
+        bs = block_table.stride()
+    if ls[1] != 1:
         lengths = lengths.contiguous()
-    return block_table, lengths
+        ls = lengths.stride()
+    return block_table, bs, shape[2], lengths, ls[0]
 
 
-def _strides(t):
-    """Element strides, 0 for dimensions of one entry (theirs mean nothing)."""
-    return [0 if n == 1 else s for n, s in zip(t.shape, t.stride())]
-
-
-def _aligned(t):
-    """Whether t's rows can be read and written 16 bytes at a time."""
+def _rows(t, copy=True):
+    """t and its strides if its rows can be read and written 16 bytes at a
+    time, else (``copy``) a contiguous copy's, or None."""
     unit = 16 // t.element_size()
-    return t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s % unit for s in _strides(t)[:-1])
+    st = t.stride()
+    if st[3] == 1 and not (st[0] | st[1] | st[2]) % unit and not t.data_ptr() % 16:
+        return t, st
+    # the stride of a dimension of one entry means nothing
+    st = tuple(0 if n == 1 else x for n, x in zip(t.shape, st))
+    if t.stride(3) == 1 and not (st[0] | st[1] | st[2]) % unit and not t.data_ptr() % 16:
+        return t, st
+    if not copy:
+        return None
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride()
 
 
-def _rows(t):
-    """t itself where its rows are 16-byte aligned, else a copy."""
-    return t if _aligned(t) else t.clone(memory_format=torch.contiguous_format)
-
-
-@_on_own_device
 def kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask=None, out=None, status=None):
     """Quantise tokens into the heads' pages behind the ones already there.
 
@@ -134,45 +126,55 @@ def kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask=None, out=No
     to WGKV_ERR_CAPACITY, as the dual cache's is.
     """
     num_blocks, P, D = _check_cache(k_cache, v_cache)
-    if k.dim() != 4 or v.shape != k.shape or k.shape[3] != D:
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or shape[3] != D:
         raise AssertionError("k/v must be (batch, tokens, num_kv_heads, head_dim)")
-    B, T, H, _ = k.shape
-    if k.dtype not in _DTYPES or v.dtype != k.dtype:
+    B, T, H, _ = shape
+    code = _DTYPES.get(k.dtype)
+    if code is None or v.dtype is not k.dtype:
         raise TypeError("k/v must be bf16, fp16 or fp32, both alike")
-    if out is not None and (out.shape != (B, H) or out.dtype != torch.int32 or (H > 1 and out.stride(1) != 1)):
+    if out is not None and (out.shape != (B, H) or out.dtype is not _I32 or (H > 1 and out.stride(1) != 1)):
         raise AssertionError("out must be int32 (batch, num_kv_heads), heads contiguous")
-    if status is not None and (status.dtype != torch.int32 or status.numel() < 1):
+    if status is not None and (status.dtype is not _I32 or status.numel() < 1):
         raise TypeError("status must be an int32 tensor")
     if g_mask is not None and g_mask.shape != (B, H, T):
         raise AssertionError("g_mask must be (batch, num_kv_heads, tokens)")
-    table, lens = _check_heads(block_table, lengths, B, H)
-    dev = _same_device(k, v, k_cache, v_cache, table, lens, g_mask, out, status)
+    table, bs, width, lens, ls = _check_heads(block_table, lengths, B, H)
+    dev = k.get_device()
+    if dev < 0:
+        _host_tensor()
+    if (v.get_device() != dev or k_cache.get_device() != dev or v_cache.get_device() != dev or table.get_device() != dev
+            or lens.get_device() != dev or (g_mask is not None and g_mask.get_device() != dev)
+            or (out is not None and out.get_device() != dev) or (status is not None and status.get_device() != dev)):
+        _two_devices()
+    if dev != _current_device():  # a null stream is the current device's
+        with torch.cuda.device(dev):
+            return kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask, out, status)
     m, ms = None, (0, 0)
     if g_mask is not None:
         m = _u8(g_mask)
         if T > 1 and m.stride(2) != 1:
             m = m.contiguous()
         ms = m.stride()
-    k, v = _rows(k), _rows(v)
-    ks, vs = _strides(k), _strides(v)
+        m = m.data_ptr()
+    k, ks = _rows(k)
+    v, vs = _rows(v)
     if out is None:
-        out = torch.empty(B, H, dtype=torch.int32, device=dev)
+        out = torch.empty_like(lens, memory_format=torch.contiguous_format)
     L = _lib.lib()
-    nbytes = L.wgkv_kv4_append_workspace_bytes(B, H, T)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _call(dev, "wgkv_kv4_append", L.wgkv_kv4_append,
-          k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], _DTYPES[k.dtype],
-          m.data_ptr() if m is not None else None, ms[0], ms[1],
-          lens.data_ptr(), lens.stride(0), out.data_ptr(), out.stride(0),
-          k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P,
-          table.data_ptr(), table.stride(0), table.stride(1), table.shape[2],
-          B, T, H, D,
-          status.data_ptr() if status is not None else None,
-          ws.data_ptr() if ws is not None else None, nbytes)
+    nbytes = L.wgkv_kv4_append_workspace_bytes(B, H, T) if T > 64 else 0
+    ws = torch.empty(nbytes, dtype=_U8, device=dev) if nbytes else None
+    st = L.wgkv_kv4_append(
+        k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], code,
+        m, ms[0], ms[1], lens.data_ptr(), ls, out.data_ptr(), out.stride(0),
+        k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P,
+        table.data_ptr(), bs[0], bs[1], width, B, T, H, D,
+        None if status is None else status.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _stream(dev))
+    if st:
+        _lib.check(st, "wgkv_kv4_append")
     return out
 
 
-@_on_own_device
 def kv4_read(k_cache, v_cache, block_table, lengths, rows, starts=None, dtype=torch.bfloat16, out=None):
     """The cache's rows as dense tensors: (k, v), each (B, rows, Hkv, D) of
     ``dtype`` (bf16, fp16 or fp32).
@@ -184,37 +186,52 @@ def kv4_read(k_cache, v_cache, block_table, lengths, rows, starts=None, dtype=to
     """
     num_blocks, P, D = _check_cache(k_cache, v_cache)
     B, H = lengths.shape if lengths.dim() == 2 else (-1, -1)
-    table, lens = _check_heads(block_table, lengths, B, H)
-    if dtype not in _DTYPES:
+    table, bs, width, lens, ls = _check_heads(block_table, lengths, B, H)
+    code = _DTYPES.get(dtype)
+    if code is None:
         raise TypeError("kv4_read gives bf16, fp16 or fp32")
     if rows < 0:
         raise AssertionError("rows must not be negative")
+    sp, ss = None, 0
     if starts is not None:
-        if starts.shape != (B, H) or starts.dtype != torch.int32:
+        if starts.shape != (B, H) or starts.dtype is not _I32:
             raise AssertionError("starts must be int32 (batch, num_kv_heads)")
         if starts.stride(1) != 1:
             starts = starts.contiguous()
-    dev = _same_device(k_cache, v_cache, table, lens, starts)
+        sp, ss = starts.data_ptr(), starts.stride(0)
+    dev = k_cache.get_device()
+    if dev < 0:
+        _host_tensor()
+    if (v_cache.get_device() != dev or table.get_device() != dev or lens.get_device() != dev
+            or (starts is not None and starts.get_device() != dev)):
+        _two_devices()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return kv4_read(k_cache, v_cache, block_table, lengths, rows, starts, dtype, out)
     if out is None:
-        out = tuple(torch.empty(B, rows, H, D, dtype=dtype, device=dev) for _ in range(2))
-    ko, vo = out
-    if ko.shape != (B, rows, H, D) or vo.shape != ko.shape or ko.dtype != dtype or vo.dtype != dtype:
-        raise AssertionError("out must be two (batch, rows, num_kv_heads, head_dim) tensors of dtype")
-    _same_device(k_cache, ko, vo)
+        ko = torch.empty((B, rows, H, D), dtype=dtype, device=dev)
+        vo = torch.empty_like(ko)
+        out = (ko, vo)
+        st = ko.stride()
+    else:
+        ko, vo = out
+        if ko.shape != (B, rows, H, D) or vo.shape != ko.shape or ko.dtype != dtype or vo.dtype != dtype:
+            raise AssertionError("out must be two (batch, rows, num_kv_heads, head_dim) tensors of dtype")
+        if ko.get_device() != dev or vo.get_device() != dev:
+            _two_devices()
+        kr, vr = _rows(ko, copy=False), _rows(vo, copy=False)
+        if kr is None or vr is None or kr[1] != vr[1]:  # no rows of 16-byte steps, or two layouts
+            for dst, src in zip(out, kv4_read(k_cache, v_cache, table, lens, rows, starts, dtype)):
+                dst.copy_(src)
+            return out
+        st = kr[1]
     if rows == 0:
         return out
-    st = _strides(ko)
-    if _strides(vo) != st or not (_aligned(ko) and _aligned(vo)):  # rows cannot be written 16 bytes at a time
-        for dst, src in zip(out, kv4_read(k_cache, v_cache, table, lens, rows, starts, dtype)):
-            dst.copy_(src)
-        return out
-    _call(dev, "wgkv_kv4_read", _lib.lib().wgkv_kv4_read,
-          k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P,
-          table.data_ptr(), table.stride(0), table.stride(1), table.shape[2],
-          lens.data_ptr(), lens.stride(0), starts.data_ptr() if starts is not None else None,
-          starts.stride(0) if starts is not None else 0,
-          ko.data_ptr(), vo.data_ptr(), st[0], st[1], st[2], _DTYPES[dtype],
-          B, rows, H, D)
+    err = _lib.lib().wgkv_kv4_read(
+        k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P, table.data_ptr(), bs[0], bs[1], width,
+        lens.data_ptr(), ls, sp, ss, ko.data_ptr(), vo.data_ptr(), st[0], st[1], st[2], code, B, rows, H, D, _stream(dev))
+    if err:
+        _lib.check(err, "wgkv_kv4_read")
     return out
 
 
@@ -222,25 +239,23 @@ _COUNTERS = 8192  # bytes at the start of the attention's workspace that must be
 _workspaces = {}
 
 
-def _attn_workspace(dev, nbytes):
+def _attn_workspace(dev, stream, nbytes):
     """Scratch of the attention, its arrival counters zero.  One per device
     and stream: calls on a stream run in turn and leave the counters zero, and
     calls on two streams never meet.  A captured call gets scratch of its own
     from the graph's memory, cleared by the graph, since two graphs that were
     captured on one stream may run on two."""
     if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws = torch.empty(nbytes, dtype=_U8, device=dev)
         ws[:_COUNTERS].zero_()
         return ws
-    key = (dev.index, _lib.stream_handle(dev))
-    ws = _workspaces.get(key)
+    ws = _workspaces.get((dev, stream))
     if ws is None or ws.numel() < nbytes:
-        ws = torch.zeros(nbytes, dtype=torch.uint8, device=dev)
-        _workspaces[key] = ws
+        ws = torch.zeros(nbytes, dtype=_U8, device=dev)
+        _workspaces[(dev, stream)] = ws
     return ws
 
 
-@_on_own_device
 def paged_decode_attn_kv4(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, out=None):
     """``paged_decode_attn`` over a 4-bit cache: q (B, 1, Hq, D) bf16 attends
     to the first cache_seqlens[b, h] tokens of its KV head; returns (B, 1, Hq,
@@ -248,28 +263,43 @@ def paged_decode_attn_kv4(q, k_cache, v_cache, cache_seqlens, block_table, softm
     to bf16 for their product with the values; sums are fp32.  Lengths and
     page ids out of range are clamped to the table and the pool."""
     num_blocks, P, D = _check_cache(k_cache, v_cache)
-    if q.dim() != 4 or q.shape[1] != 1 or q.shape[3] != D:
+    shape = q.shape
+    if len(shape) != 4 or shape[1] != 1 or shape[3] != D:
         raise AssertionError("q must be (batch, 1, num_query_heads, head_dim)")
-    B, _, Hq, _ = q.shape
-    if q.dtype != torch.bfloat16:
+    B, _, Hq, _ = shape
+    if q.dtype is not _BF16:
         raise TypeError("q must be bf16")
     H = cache_seqlens.shape[1] if cache_seqlens.dim() == 2 else -1
-    table, lens = _check_heads(block_table, cache_seqlens, B, H)
+    table, bs, width, lens, ls = _check_heads(block_table, cache_seqlens, B, H)
     if H < 1 or Hq % H:
         raise AssertionError("num_query_heads must be a multiple of num_kv_heads")
-    dev = _same_device(q, k_cache, v_cache, table, lens, out)
+    dev = q.get_device()
+    if dev < 0:
+        _host_tensor()
+    if (k_cache.get_device() != dev or v_cache.get_device() != dev or table.get_device() != dev
+            or lens.get_device() != dev or (out is not None and out.get_device() != dev)):
+        _two_devices()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return paged_decode_attn_kv4(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, out)
+    q, qs = _rows(q)
     if out is None:
-        out = torch.empty(B, 1, Hq, D, dtype=torch.bfloat16, device=dev)
-    elif out.shape != (B, 1, Hq, D) or out.dtype != torch.bfloat16:
-        raise AssertionError("out must be (batch, 1, num_query_heads, head_dim) bf16")
-    elif not _aligned(out):  # rows cannot be written 16 bytes at a time
-        return out.copy_(paged_decode_attn_kv4(q, k_cache, v_cache, lens, table, softmax_scale))
-    q = _rows(q)
-    qs, os = _strides(q), _strides(out)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        os = out.stride()
+    else:
+        if out.shape != shape or out.dtype is not _BF16:
+            raise AssertionError("out must be (batch, 1, num_query_heads, head_dim) bf16")
+        os = _rows(out, copy=False)
+        if os is None:  # rows cannot be written 16 bytes at a time
+            return out.copy_(paged_decode_attn_kv4(q, k_cache, v_cache, lens, table, softmax_scale))
+        os = os[1]
     L = _lib.lib()
-    ws = _attn_workspace(dev, L.wgkv_kv4_decode_workspace_bytes(Hq, H, D))
-    _call(dev, "wgkv_kv4_decode_attn", L.wgkv_kv4_decode_attn,
-          q.data_ptr(), qs[0], qs[2], k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P,
-          lens.data_ptr(), lens.stride(0), table.data_ptr(), table.stride(0), table.stride(1), table.shape[2],
-          out.data_ptr(), os[0], os[2], B, Hq, H, D, float(softmax_scale), ws.data_ptr(), ws.numel())
+    stream = _stream(dev)
+    ws = _attn_workspace(dev, stream, L.wgkv_kv4_decode_workspace_bytes(Hq, H, D))
+    st = L.wgkv_kv4_decode_attn(
+        q.data_ptr(), qs[0], qs[2], k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P,
+        lens.data_ptr(), ls, table.data_ptr(), bs[0], bs[1], width,
+        out.data_ptr(), os[0], os[2], B, Hq, H, D, softmax_scale, ws.data_ptr(), ws.numel(), stream)
+    if st:
+        _lib.check(st, "wgkv_kv4_decode_attn")
     return out
