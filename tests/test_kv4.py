@@ -121,8 +121,8 @@ def test_c_entry_points_check_arguments_without_gpu():
     from wgkv import _lib
     L = _lib.lib()
     x = 4096  # an aligned, never dereferenced address
-    assert L.wgkv_kv4_append_workspace_bytes(1, 8, 64) == 0
-    assert L.wgkv_kv4_append_workspace_bytes(2, 3, 65) == 4 * 6 * (1 + 1 + 2)
+    assert L.wgkv_kv4_append_workspace_bytes(1, 8, 256) == 0
+    assert L.wgkv_kv4_append_workspace_bytes(2, 3, 257) == 4 * 6 * (1 + 1 + 2)
 
     def append(key=x, sk=64, dtype=0, cache=x, pages=4, page=16, maxp=4, B=1, T=4, H=1, D=64, ws=None, n=0):
         return L.wgkv_kv4_append(key, sk, sk, sk, x, sk, sk, sk, dtype, None, 0, 0, x, 1, x, 1, cache, x, pages, page,
@@ -134,7 +134,7 @@ def test_c_entry_points_check_arguments_without_gpu():
                      (dict(dtype=3), _lib.ERR_UNSUPPORTED), (dict(D=96), _lib.ERR_UNSUPPORTED),
                      (dict(page=8), _lib.ERR_UNSUPPORTED), (dict(cache=x + 8), _lib.ERR_UNSUPPORTED),
                      (dict(maxp=1 << 28), _lib.ERR_UNSUPPORTED), (dict(B=256, H=257), _lib.ERR_UNSUPPORTED),
-                     (dict(T=65), _lib.ERR_WORKSPACE), (dict(T=65, ws=x, n=8), _lib.ERR_WORKSPACE)]:
+                     (dict(T=257), _lib.ERR_WORKSPACE), (dict(T=257, ws=x, n=8), _lib.ERR_WORKSPACE)]:
         assert append(**kw) == want, kw
 
     def read(out=x, so=64, rows=4, dtype=0, D=64):

@@ -80,27 +80,35 @@ inline int kv4_pages(Kv4Pages* p, int64_t num_pages, int32_t page_size, const in
 // ---- element types of the rows quantised or read back -------------------------
 enum Kv4Type { kKv4Bf16 = 0, kKv4F32 = 1, kKv4F16 = 2 };
 
-// Eight consecutive values of a row as fp32.
+// Eight consecutive values of a row as they are in memory.
 template <int TY>
-WGKV_DEVICE void kv4_load8(const void* p, int64_t off, float (&x)[8]) {
+struct Kv4Raw {
+  u32x4_t w[TY == kKv4F32 ? 2 : 1];
+};
+
+template <int TY>
+WGKV_DEVICE void kv4_fetch(const void* p, int64_t off, Kv4Raw<TY>& r) {
   if constexpr (TY == kKv4F32) {
-    const f32x4_t a = *(const f32x4_t*)((const float*)p + off), b = *(const f32x4_t*)((const float*)p + off + 4);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = a[i];
-      x[4 + i] = b[i];
-    }
+    r.w[0] = *(const u32x4_t*)((const float*)p + off);
+    r.w[1] = *(const u32x4_t*)((const float*)p + off + 4);
   } else {
-    const u32x4_t w = *(const u32x4_t*)((const uint16_t*)p + off);
+    r.w[0] = *(const u32x4_t*)((const uint16_t*)p + off);
+  }
+}
+
+template <int TY>
+WGKV_DEVICE void kv4_widen(const Kv4Raw<TY>& r, float (&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (TY == kKv4Bf16) {
-        x[2 * i] = bf16lo(w[i]);
-        x[2 * i + 1] = bf16hi(w[i]);
-      } else {
-        x[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] & 0xffffu));
-        x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(w[i] >> 16));
-      }
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (TY == kKv4F32) {
+      x[i] = __uint_as_float(r.w[0][i]);
+      x[4 + i] = __uint_as_float(r.w[1][i]);
+    } else if constexpr (TY == kKv4Bf16) {
+      x[2 * i] = bf16lo(r.w[0][i]);
+      x[2 * i + 1] = bf16hi(r.w[0][i]);
+    } else {
+      x[2 * i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(r.w[0][i] & 0xffffu));
+      x[2 * i + 1] = (float)__builtin_bit_cast(_Float16, (uint16_t)(r.w[0][i] >> 16));
     }
   }
 }

@@ -12,9 +12,13 @@
 
 namespace {
 
-constexpr int kTile = 64;          // source tokens per append workgroup (one wave)
+constexpr int kFew = 64;           // up to this many tokens a call is one-wave workgroups
+constexpr int kTile = 256;         // source tokens per append workgroup otherwise
 constexpr int kSegment = 4096;     // flags per counting workgroup
 constexpr int kSegTiles = kSegment / kTile;
+// Up to this many tokens a workgroup counts the flags in front of its tile
+// itself; beyond, kv4_count_kernel does, in a launch before.
+constexpr int kCountsItself = 16384;
 
 struct AppendArgs {
   const void* src[2];
@@ -29,9 +33,9 @@ struct AppendArgs {
   Kv4Pages pg;
   int B, T, H;
   int32_t* status;  // or null
-  // more than one tile: the lengths before the call (B*H), the admitted
-  // tokens of each segment (B*H, segments) and those before each tile within
-  // its segment (B*H, tiles)
+  // what kv4_count_kernel leaves, or null: the lengths before the call
+  // (B*H), the admitted tokens of each segment (B*H, segments) and those
+  // before each tile within its segment (B*H, tiles)
   int32_t *ws_len, *ws_seg, *ws_tile;
   int tiles, segments;
 };
@@ -75,167 +79,227 @@ __global__ __launch_bounds__(256) void kv4_count_kernel(AppendArgs a) {
   }
 }
 
-WGKV_DEVICE float quad_max(float x) {
-  x = fmaxf(x, dpp_f32<WGKV_DPP_QP_1032>(x));
-  return fmaxf(x, dpp_f32<WGKV_DPP_QP_2301>(x));
+// NaN-propagating maximum and minimum (v_maximum3 / v_minimum3), over a
+// lane's values and then its quad of lanes.
+WGKV_DEVICE float quad_maximum(float x) {
+  x = __builtin_elementwise_maximum(x, dpp_f32<WGKV_DPP_QP_1032>(x));
+  return __builtin_elementwise_maximum(x, dpp_f32<WGKV_DPP_QP_2301>(x));
 }
-WGKV_DEVICE float quad_min(float x) {
-  x = fminf(x, dpp_f32<WGKV_DPP_QP_1032>(x));
-  return fminf(x, dpp_f32<WGKV_DPP_QP_2301>(x));
+WGKV_DEVICE float quad_minimum(float x) {
+  x = __builtin_elementwise_minimum(x, dpp_f32<WGKV_DPP_QP_1032>(x));
+  return __builtin_elementwise_minimum(x, dpp_f32<WGKV_DPP_QP_2301>(x));
 }
 
-// Nearest bf16 of an fp32 value, in integers: a conversion instruction after
-// one from fp64 is folded into a single rounding from fp64, another number
-// where the fp32 value lies halfway between two bf16 ones.
-WGKV_DEVICE float bf16_of(float x) { return __uint_as_float((uint32_t)f32_to_bf16(x) << 16); }
+// Nearest bf16 of a finite fp32 value, in integers: a conversion instruction
+// after one from fp64 is folded into a single rounding from fp64, another
+// number where the fp32 value lies halfway between two bf16 ones.
+WGKV_DEVICE float bf16_of(float x) {
+  const uint32_t u = __float_as_uint(x);
+  return __uint_as_float((u + 0x7fffu + (u >> 16 & 1u)) & 0xffff0000u);
+}
 
 // Quantises a lane's 8 values of a group that four neighbouring lanes share.
-// Returns (s, m) as a packed pair; codes 0..3 and 4..7 in c[0..7].
-WGKV_DEVICE uint32_t quantise8(const float (&x)[8], uint32_t (&c)[8]) {
-  float hi = x[0], lo = x[0], finite = x[0] * 0.f;
+// Returns (s, m) as a packed pair; the codes as numbers in c[0..7].
+//
+// The code is k + 7.5 rounded to even for x = m + k s exactly, k + 8 beyond
+// and k + 7 below, for an integer k next to (x - m) / s: that need not be the
+// nearest, so the quotient may be approximate (v_rcp), and the side is
+// decided by the sign of the residue x - m - k s.  k s has 12 bits and is
+// exact; x - m is within one fp32 rounding, whose error counts only where the
+// rounded difference equals k s (a nonzero residue is at least one ulp of
+// it).  For 16-bit inputs the difference is inexact only where x is tiny
+// beside m, and one addition recovers the error; fp32 takes the full two-sum.
+template <int TY>
+WGKV_DEVICE uint32_t quantise8(const float (&x)[8], float (&c)[8]) {
+  float hi = x[0], lo = x[0];
 #pragma unroll
   for (int i = 1; i < 8; ++i) {
-    hi = fmaxf(hi, x[i]);
-    lo = fminf(lo, x[i]);
-    finite = fmaf(x[i], 0.f, finite);  // NaN once a value is not finite
+    hi = __builtin_elementwise_maximum(hi, x[i]);
+    lo = __builtin_elementwise_minimum(lo, x[i]);
   }
-  hi = quad_max(hi);
-  lo = quad_min(lo);
-  finite += dpp_f32<WGKV_DPP_QP_1032>(finite);
-  finite += dpp_f32<WGKV_DPP_QP_2301>(finite);
+  hi = quad_maximum(hi);
+  lo = quad_minimum(lo);
   // In 64 bits, as a multiplication: 1/15 in fp64 is 2^-56 off, too little
   // to move the quotient across a border of fp32 or bf16.
-  float s = bf16_of((float)(((double)hi - (double)lo) * (1.0 / 15.0)));
+  const float sf = (float)(((double)hi - (double)lo) * (1.0 / 15.0));
+  float s = bf16_of(sf);
   const float m = bf16_of(0.5f * hi + 0.5f * lo);
+  const bool bad = !(sf < INFINITY) || !(fabsf(m) < INFINITY);
   if (!(s >= 0x1p-126f)) s = 0.f;
-  const bool bad = finite != 0.f || !(fabsf(m) <= 0x1.fep127f);
-  // code = 8 + k for x beyond m + k s, 7 + k below it, the even one on it,
-  // for an integer k next to (x - m) / s: that need not be the nearest, so
-  // the quotient may be approximate, and the side is decided by an exact
-  // residue (fp64 holds x - m and k s).  A rounded fp32 quotient would put
-  // values near a border on the wrong side.
+  const bool none = s == 0.f || bad;
   const float inv = __builtin_amdgcn_rcpf(s);
-  const double md = (double)m, sd = (double)s;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float k = rintf((x[i] - m) * inv);
-    const double r = fma(-(double)k, sd, (double)x[i] - md);
-    const int ki = (int)fminf(fmaxf(k, -9.f), 9.f);
-    const int up = r > 0.0 || (r == 0.0 && !(ki & 1));
-    const int code = min(15, max(0, ki + 7 + up));
-    c[i] = s == 0.f || bad ? 0u : (uint32_t)code;
+    const float d = x[i] - m;
+    const float k = rintf(d * inv);
+    float r = fmaf(-k, s, d);
+    if constexpr (TY == kKv4F32) {
+      const float bb = d - x[i];
+      r += (x[i] - (d - bb)) - (m + bb);
+    } else {
+      r += x[i] - (d + m);
+    }
+    // 7.25, 7.5 or 7.75 by the residue's sign (one below 2^-148 counts as 0)
+    const float side = __builtin_amdgcn_fmed3f(fmaf(r, 0x1p127f, 7.5f), 7.25f, 7.75f);
+    c[i] = none ? 0.f : rintf(__builtin_amdgcn_fmed3f(k + side, 0.f, 15.f));
   }
-  const uint32_t w = (__float_as_uint(s) >> 16) | (__float_as_uint(m) & 0xffff0000u);
+  const uint32_t w = (__float_as_uint(s) >> 16) | __float_as_uint(m);
   return bad ? 0x7fc07fc0u : w;
 }
 
-template <int D, int TY>
-__global__ __launch_bounds__(64) void kv4_append_kernel(AppendArgs a) {
-  constexpr int LPR = D / 8;        // lanes per quad
-  constexpr int QPW = 64 / LPR;     // quads per step
+// Four codes as a 16-bit word, the first in the lowest bits.
+WGKV_DEVICE uint32_t pack4(float a, float b, float c, float d) {
+  return (uint32_t)fmaf(d, 4096.f, fmaf(c, 256.f, fmaf(b, 16.f, a)));
+}
+
+// One quad of positions quantised and written: kKeys or values, the four
+// tokens' values x, those of them that are there (ok).
+template <int D, int TY, bool kKeys>
+WGKV_DEVICE void write_quad(uint8_t* tile, int qi, int L, const Kv4Raw<TY> (&raw)[4], const bool (&ok)[4]) {
   constexpr int NG = D / kKv4Group;
-  __shared__ uint8_t s_src[kTile];
+  uint32_t w[4][2], sm[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float x[8], c[8];
+    kv4_widen<TY>(raw[i], x);
+    sm[i] = quantise8<TY>(x, c);
+    if constexpr (kKeys) {
+      w[i][0] = pack4(c[0], c[2], c[4], c[6]);
+      w[i][1] = pack4(c[1], c[3], c[5], c[7]);
+    } else {
+      w[i][0] = pack4(c[0], c[1], c[2], c[3]);
+      w[i][1] = pack4(c[4], c[5], c[6], c[7]);
+    }
+  }
+  const bool whole = ok[0] && ok[1] && ok[2] && ok[3];
+  if constexpr (kKeys) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (ok[i]) *(uint32_t*)(tile + (qi * 4 + i) * (D / 2) + L * 4) = w[i][0] | w[i][1] << 16;
+  } else {
+    // words of lane L: D = 128: row r = L, halves 0 and 1; D = 64: rows 2L
+    // and 2L + 1.  Both are 16 consecutive bytes of the quad.
+    uint8_t* vp = tile + qi * (2 * D) + L * 16;
+    constexpr int kWord = D == 128 ? 4 : 8, kPair = D == 128 ? 8 : 4;  // strides of w[.][1] and of t%4/2
+    if (whole) {
+      u32x4_t v;
+#pragma unroll
+      for (int pr = 0; pr < 2; ++pr)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) v[(pr * kPair + j * kWord) / 4] = w[2 * pr][j] | w[2 * pr + 1][j] << 16;
+      *(u32x4_t*)vp = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (ok[i]) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            *(uint16_t*)(vp + (i >> 1) * kPair + j * kWord + (i & 1) * 2) = (uint16_t)w[i][j];
+        }
+    }
+  }
+  if (L % 4 == 0) {
+    uint32_t* sp = (uint32_t*)(tile + kv4_scales_at(D)) + (qi * NG + L / 4) * 4;
+    if (whole) {
+      *(u32x4_t*)sp = (u32x4_t){sm[0], sm[1], sm[2], sm[3]};
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (ok[i]) sp[i] = sm[i];
+    }
+  }
+}
+
+// One workgroup per tile of source tokens and head; NW waves, 64 tokens each.
+template <int D, int TY, int NW>
+__global__ __launch_bounds__(NW * 64) void kv4_append_kernel(AppendArgs a) {
+  constexpr int LPR = D / 8;             // lanes per quad
+  constexpr int kSlots = NW * 64 / LPR;  // quads per step
+  __shared__ uint8_t s_src[NW * 64];
+  __shared__ int s_adm[NW], s_before[NW], s_len;
   const int tile = blockIdx.x, bh = blockIdx.y;
   const int b = bh / a.H, h = bh - b * a.H;
-  const int lane = threadIdx.x;
-  const int t0 = tile * kTile;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  const int t0 = tile * (NW * 64);
+  const uint8_t* mask = a.mask ? a.mask + (int64_t)b * a.m_b + (int64_t)h * a.m_h : nullptr;
 
-  bool f = t0 + lane < a.T;
-  if (f && a.mask) f = a.mask[(int64_t)b * a.m_b + (int64_t)h * a.m_h + t0 + lane] != 0;
+  // The head's length, through one thread: the new one may be written over it
+  // by the same thread.  Then the admitted tokens in front of the tile.
+  int len = 0, before = 0;
+  if (NW == 1 || tid == 0) len = NW > 1 && a.ws_len ? a.ws_len[bh] : clamped_len(a, b, h);
+  if (NW > 1 && a.ws_len) {
+    const int seg = tile / kSegTiles;
+    if (wid == 0)
+      for (int i = lane; i < seg; i += 64) before += a.ws_seg[(int64_t)bh * a.segments + i];
+    if (tid == 0) before += a.ws_tile[(int64_t)bh * a.tiles + tile];
+  } else {
+    if (NW > 1) {
+      if (mask) before = count_flags(mask, 0, t0, tid, NW * 64);
+      else if (tid == 0) before = t0;
+    }
+  }
+  bool f = t0 + tid < a.T;
+  if (f && mask) f = mask[t0 + tid] != 0;
   const uint64_t bits = __builtin_amdgcn_ballot_w64(f);
-  if (f) s_src[__builtin_popcountll(bits & ((1ull << lane) - 1))] = (uint8_t)lane;
-  wave_lds_sync();
-  const int n_adm = __builtin_popcountll(bits);
+  int rank = __builtin_popcountll(bits & ((1ull << lane) - 1));
+  int n_adm = __builtin_popcountll(bits);
+  if constexpr (NW > 1) {
+    before = wave_sum_int(before);
+    if (lane == 0) {
+      s_adm[wid] = n_adm;
+      s_before[wid] = before;
+    }
+    if (tid == 0) s_len = len;
+    __syncthreads();
+    len = s_len;
+    n_adm = before = 0;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      if (i < wid) rank += s_adm[i];
+      n_adm += s_adm[i];
+      before += s_before[i];
+    }
+  }
+  if (f) s_src[rank] = (uint8_t)tid;
+  if constexpr (NW > 1) __syncthreads();
+  else wave_lds_sync();
 
   // positions [p0, p1) take the tile's admitted tokens
-  int64_t first;
-  if (a.tiles > 1) {
-    const int seg = tile / kSegTiles;
-    int before = 0;
-    for (int i = lane; i < seg; i += 64) before += a.ws_seg[(int64_t)bh * a.segments + i];
-    first = (int64_t)a.ws_len[bh] + wave_sum_int(before) + a.ws_tile[(int64_t)bh * a.tiles + tile];
-  } else {
-    first = clamped_len(a, b, h);
-  }
-  const int64_t cap = kv4_capacity(a.pg);
+  const int64_t first = (int64_t)len + before, cap = kv4_capacity(a.pg);
   const int p0 = (int)min(first, cap), p1 = (int)min(first + n_adm, cap);
   bool lost = first + n_adm > cap;
-  if (tile == max(a.tiles, 1) - 1 && lane == 0) a.new_len[(int64_t)b * a.new_sb + h] = p1;
+  if (tile == max(a.tiles, 1) - 1 && tid == 0) a.new_len[(int64_t)b * a.new_sb + h] = p1;
 
   const int32_t* bt_row = a.pg.bt + (int64_t)b * a.pg.bt_sb + (int64_t)h * a.pg.bt_sh;
-  const int L = lane % LPR, slot = lane / LPR;
+  const int L = tid % LPR, slot = tid / LPR;
+  const int64_t kb = (int64_t)b * a.s_b[0] + (int64_t)h * a.s_h[0] + L * 8;
+  const int64_t vb = (int64_t)b * a.s_b[1] + (int64_t)h * a.s_h[1] + L * 8;
   const int q0 = p0 >> 2, nq = p1 > p0 ? ((p1 - 1) >> 2) - q0 + 1 : 0;
-  // items: keys and values of each quad in turn, so that a single token's
-  // key and value are quantised side by side
-  for (int it = slot; it < 2 * nq; it += QPW) {
-    const int quad = q0 + (it >> 1), kind = it & 1;
+  // A step takes keys and values of a quad per group of lanes, their eight
+  // rows and the page id asked for together.  Few quads (a decode step) give
+  // keys and values to neighbouring groups instead.
+  const bool apart = 2 * nq <= kSlots;
+  const int n_items = apart ? 2 * nq : nq;
+  for (int it = slot; it < n_items; it += kSlots) {
+    const int quad = q0 + (apart ? it >> 1 : it);
+    const bool do_k = !apart || !(it & 1), do_v = !apart || (it & 1);
+    Kv4Raw<TY> kr[4], vr[4];
+    bool ok[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = quad * 4 + i;
+      ok[i] = p >= p0 && p < p1;
+      const int64_t src = t0 + s_src[min(max(p - p0, 0), n_adm - 1)];
+      if (do_k) kv4_fetch<TY>(a.src[0], kb + src * a.s_t[0], kr[i]);
+      if (do_v) kv4_fetch<TY>(a.src[1], vb + src * a.s_t[1], vr[i]);
+    }
     const int64_t at = kv4_tile_at<D>(a.pg, bt_row, quad >> 2);
     if (at < 0) {
       lost = true;
       continue;
     }
-    uint32_t w[4][2], sm[4];
-    bool ok[4];
-    float x[4][8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int p = quad * 4 + i;
-      ok[i] = p >= p0 && p < p1;
-      const int src = t0 + s_src[min(max(p - p0, 0), n_adm - 1)];
-      kv4_load8<TY>(a.src[kind], (int64_t)b * a.s_b[kind] + (int64_t)src * a.s_t[kind] + (int64_t)h * a.s_h[kind] + L * 8,
-                    x[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t c[8];
-      sm[i] = quantise8(x[i], c);
-      if (kind == 0) {
-        w[i][0] = c[0] | c[2] << 4 | c[4] << 8 | c[6] << 12;
-        w[i][1] = c[1] | c[3] << 4 | c[5] << 8 | c[7] << 12;
-      } else {
-        w[i][0] = c[0] | c[1] << 4 | c[2] << 8 | c[3] << 12;
-        w[i][1] = c[4] | c[5] << 4 | c[6] << 8 | c[7] << 12;
-      }
-    }
-    uint8_t* tp = a.cache[kind] + at;
-    const int qi = quad & 3;
-    const bool whole = ok[0] && ok[1] && ok[2] && ok[3];
-    if (kind == 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (ok[i]) *(uint32_t*)(tp + (qi * 4 + i) * (D / 2) + L * 4) = w[i][0] | w[i][1] << 16;
-    } else {
-      // words of lane L: D = 128: row r = L, halves 0 and 1; D = 64: rows
-      // 2L and 2L + 1.  Both are 16 consecutive bytes of the quad.
-      uint8_t* vp = tp + qi * (2 * D) + L * 16;
-      constexpr int kWord = D == 128 ? 4 : 8, kPair = D == 128 ? 8 : 4;  // strides of w[.][1] and of t%4/2
-      if (whole) {
-        u32x4_t v;
-#pragma unroll
-        for (int pr = 0; pr < 2; ++pr)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) v[(pr * kPair + j * kWord) / 4] = w[2 * pr][j] | w[2 * pr + 1][j] << 16;
-        *(u32x4_t*)vp = v;
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (ok[i]) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-              *(uint16_t*)(vp + (i >> 1) * kPair + j * kWord + (i & 1) * 2) = (uint16_t)w[i][j];
-          }
-      }
-    }
-    if (L % 4 == 0) {
-      uint32_t* sp = (uint32_t*)(tp + kv4_scales_at(D)) + (qi * NG + L / 4) * 4;
-      if (whole) {
-        *(u32x4_t*)sp = (u32x4_t){sm[0], sm[1], sm[2], sm[3]};
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (ok[i]) sp[i] = sm[i];
-      }
-    }
+    if (do_k) write_quad<D, TY, true>(a.cache[0] + at, quad & 3, L, kr, ok);
+    if (do_v) write_quad<D, TY, false>(a.cache[1] + at, quad & 3, L, vr, ok);
   }
   if (a.status && lost) atomicMax(a.status, WGKV_ERR_CAPACITY);
 }
@@ -252,14 +316,41 @@ struct ReadArgs {
   int B, rows, H;
 };
 
+// A lane's 8 d of four tokens, from the words and pairs of their quad.
+template <int D, bool kKeys>
+WGKV_DEVICE void quad_values(const uint8_t* tile, int qi, int L, float (&x)[4][8]) {
+  constexpr int NG = D / kKv4Group;
+  const u32x4_t sm = *(const u32x4_t*)(tile + kv4_scales_at(D) + (qi * NG + L / 4) * 16);
+  uint32_t w[4];  // token i's two words
+  if constexpr (kKeys) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = *(const uint32_t*)(tile + (qi * 4 + i) * (D / 2) + L * 4);
+  } else {
+    const u32x4_t v = *(const u32x4_t*)(tile + qi * (2 * D) + L * 16);
+    constexpr int kWord = D == 128 ? 1 : 2, kPair = D == 128 ? 2 : 1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t a = v[(i >> 1) * kPair], b = v[(i >> 1) * kPair + kWord];
+      w[i] = i & 1 ? a >> 16 | (b & 0xffff0000u) : (a & 0xffffu) | b << 16;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float s = bf16lo(sm[i]), m = bf16hi(sm[i]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int sh = kKeys ? 4 * (j >> 1) + 16 * (j & 1) : 4 * j;  // word of d, code in it
+      x[i][j] = fmaf(s, (float)(w[i] >> sh & 15u) - 7.5f, m);
+    }
+  }
+}
+
 // One wave per 64 positions of a head's keys or values.
 constexpr int kReadTile = 64;
 
-template <int D, int TY>
-__global__ __launch_bounds__(64) void kv4_read_kernel(ReadArgs a) {
-  constexpr int LPR = D / 8, QPW = 64 / LPR, NG = D / kKv4Group;
-  const int bh = blockIdx.y, kind = blockIdx.z;
-  const int b = bh / a.H, h = bh - b * a.H;
+template <int D, int TY, bool kKeys>
+WGKV_DEVICE void read_tile(const ReadArgs& a, int b, int h) {
+  constexpr int LPR = D / 8, QPW = 64 / LPR;
   const int64_t cap = kv4_capacity(a.pg);
   int64_t len = a.len[(int64_t)b * a.len_sb + h];
   len = len < 0 ? 0 : len > cap ? cap : len;
@@ -274,57 +365,39 @@ __global__ __launch_bounds__(64) void kv4_read_kernel(ReadArgs a) {
     const int64_t quad = quad0 + i0, p = quad * 4;
     if (p >= end) break;
     float x[4][8];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[i][j] = 0.f;
     const int64_t at = p < len ? kv4_tile_at<D>(a.pg, bt_row, (int)(quad >> 2)) : -1;
     if (at >= 0) {
-      const uint8_t* tp = a.cache[kind] + at;
-      const int qi = (int)(quad & 3);
-      const u32x4_t sm = *(const u32x4_t*)(tp + kv4_scales_at(D) + (qi * NG + L / 4) * 16);
-      uint32_t w[4][2];  // codes of token i: K even / odd d, V first / second four
-      if (kind == 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t v = *(const uint32_t*)(tp + (qi * 4 + i) * (D / 2) + L * 4);
-          w[i][0] = v & 0xffffu;
-          w[i][1] = v >> 16;
-        }
-      } else {
-        const u32x4_t v = *(const u32x4_t*)(tp + qi * (2 * D) + L * 16);
-        constexpr int kWord = D == 128 ? 1 : 2, kPair = D == 128 ? 2 : 1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) w[i][j] = (v[(i >> 1) * kPair + j * kWord] >> (16 * (i & 1))) & 0xffffu;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (p + i >= len) continue;
-        const float s = bf16lo(sm[i]), m = bf16hi(sm[i]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float c0 = (float)(w[i][0] >> (4 * j) & 15u) - 7.5f, c1 = (float)(w[i][1] >> (4 * j) & 15u) - 7.5f;
-          x[i][kind == 0 ? 2 * j : j] = fmaf(s, c0, m);
-          x[i][kind == 0 ? 2 * j + 1 : 4 + j] = fmaf(s, c1, m);
-        }
-      }
+      quad_values<D, kKeys>(a.cache[kKeys ? 0 : 1] + at, (int)(quad & 3), L, x);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      const bool there = at >= 0 && p + i < len;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[i][j] = there ? x[i][j] : 0.f;
       const int64_t row = p + i - start;
-      if (row >= 0 && row < a.rows) kv4_store8<TY>(a.out[kind], ob + row * a.o_t, x[i]);
+      if (row >= 0 && row < a.rows) kv4_store8<TY>(a.out[kKeys ? 0 : 1], ob + row * a.o_t, x[i]);
     }
   }
 }
 
+template <int D, int TY>
+__global__ __launch_bounds__(64) void kv4_read_kernel(ReadArgs a) {
+  const int bh = blockIdx.y, b = bh / a.H, h = bh - b * a.H;
+  if (blockIdx.z == 0) read_tile<D, TY, true>(a, b, h);
+  else read_tile<D, TY, false>(a, b, h);
+}
+
+template <int D, int TY>
+void launch_append(const AppendArgs& a, hipStream_t st) {
+  if (a.T <= kFew) hipLaunchKernelGGL((kv4_append_kernel<D, TY, 1>), dim3(1, a.B * a.H), dim3(64), 0, st, a);
+  else hipLaunchKernelGGL((kv4_append_kernel<D, TY, kTile / 64>), dim3(a.tiles, a.B * a.H), dim3(kTile), 0, st, a);
+}
+
 template <int D>
 void launch_append(const AppendArgs& a, int ty, hipStream_t st) {
-  const dim3 g(max(a.tiles, 1), a.B * a.H);
-  if (ty == kKv4Bf16) hipLaunchKernelGGL((kv4_append_kernel<D, kKv4Bf16>), g, dim3(64), 0, st, a);
-  else if (ty == kKv4F32) hipLaunchKernelGGL((kv4_append_kernel<D, kKv4F32>), g, dim3(64), 0, st, a);
-  else hipLaunchKernelGGL((kv4_append_kernel<D, kKv4F16>), g, dim3(64), 0, st, a);
+  if (ty == kKv4Bf16) launch_append<D, kKv4Bf16>(a, st);
+  else if (ty == kKv4F32) launch_append<D, kKv4F32>(a, st);
+  else launch_append<D, kKv4F16>(a, st);
 }
 
 template <int D>
@@ -393,12 +466,19 @@ extern "C" int wgkv_kv4_append(
     if (!workspace || ((uintptr_t)workspace & 3) ||
         workspace_bytes < wgkv_kv4_append_workspace_bytes(batch, num_kv_heads, tokens))
       return WGKV_ERR_WORKSPACE;
-    const int64_t bh = (int64_t)batch * num_kv_heads;
-    a.ws_len = (int32_t*)workspace;
-    a.ws_seg = a.ws_len + bh;
-    a.ws_tile = a.ws_seg + bh * a.segments;
-    hipLaunchKernelGGL(kv4_count_kernel, dim3(a.segments, (unsigned)bh), dim3(256), 0, s, a);
-    if (hipGetLastError() != hipSuccess) return WGKV_ERR_HIP;
+    // Several workgroups read a head's length and one writes the new one: if
+    // that may be the same memory, the lengths are copied first too.
+    const int32_t* len_end = lengths + (batch - 1) * len_stride_b + num_kv_heads;
+    const int32_t* new_end = new_lengths + (batch - 1) * new_stride_b + num_kv_heads;
+    const bool apart = (uintptr_t)len_end <= (uintptr_t)new_lengths || (uintptr_t)new_end <= (uintptr_t)lengths;
+    if (!apart || (g_mask && tokens > kCountsItself)) {
+      const int64_t bh = (int64_t)batch * num_kv_heads;
+      a.ws_len = (int32_t*)workspace;
+      a.ws_seg = a.ws_len + bh;
+      a.ws_tile = a.ws_seg + bh * a.segments;
+      hipLaunchKernelGGL(kv4_count_kernel, dim3(a.segments, (unsigned)bh), dim3(256), 0, s, a);
+      if (hipGetLastError() != hipSuccess) return WGKV_ERR_HIP;
+    }
   }
   if (head_dim == 128) launch_append<128>(a, dtype, s);
   else launch_append<64>(a, dtype, s);

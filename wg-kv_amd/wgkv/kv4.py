@@ -162,7 +162,7 @@ def kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask=None, out=No
     if out is None:
         out = torch.empty_like(lens, memory_format=torch.contiguous_format)
     L = _lib.lib()
-    nbytes = L.wgkv_kv4_append_workspace_bytes(B, H, T) if T > 64 else 0
+    nbytes = L.wgkv_kv4_append_workspace_bytes(B, H, T) if T > 256 else 0
     ws = torch.empty(nbytes, dtype=_U8, device=dev) if nbytes else None
     st = L.wgkv_kv4_append(
         k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], code,
