@@ -31,6 +31,8 @@
 // A head inside one range is written directly; otherwise the pieces' (max,
 // sum, acc) go to the workspace and the head's last workgroup to arrive
 // merges them, in the order of the sequence.
+#include <string.h>
+
 #include "kv4.h"
 
 namespace {
@@ -722,4 +724,15 @@ extern "C" int wgkv_kv4_decode_attn(
   hipStream_t s = (hipStream_t)stream;
   const hipError_t e = head_dim == 64 ? launch<64, 1>(a, s) : G <= 4 ? launch<128, 1>(a, s) : launch<128, 2>(a, s);
   return e == hipSuccess ? WGKV_OK : WGKV_ERR_HIP;
+}
+
+extern "C" int wgkv_kv4_decode_attn_block(const void* args) {
+  int64_t a[24];
+  memcpy(a, args, sizeof a);
+  double scale;
+  memcpy(&scale, &a[20], sizeof scale);
+  return wgkv_kv4_decode_attn((const void*)a[0], a[1], a[2], (const void*)a[3], (const void*)a[4], a[5], (int32_t)a[6],
+                              (const int32_t*)a[7], a[8], (const int32_t*)a[9], a[10], a[11], (int32_t)a[12],
+                              (void*)a[13], a[14], a[15], (int32_t)a[16], (int32_t)a[17], (int32_t)a[18],
+                              (int32_t)a[19], (float)scale, (void*)a[21], (size_t)a[22], (void*)a[23]);
 }

@@ -217,6 +217,9 @@ SIGNATURES = {
         c_ptr, c_i64, c_i64,
         c_i32, c_i32, c_i32, c_i32,
         c_f32, c_ptr, c_size, c_ptr]),
+    "wgkv_kv4_append_block": (ctypes.c_int, [ctypes.c_char_p]),
+    "wgkv_kv4_read_block": (ctypes.c_int, [ctypes.c_char_p]),
+    "wgkv_kv4_decode_attn_block": (ctypes.c_int, [ctypes.c_char_p]),
 }
 
 _lib = None

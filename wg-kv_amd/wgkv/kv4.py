@@ -20,6 +20,8 @@ The operators run on torch's current stream of the tensors' device, allocate
 only their outputs and scratch (both through torch, so a call can be captured
 in a HIP graph) and never synchronise with the host.
 """
+import struct
+
 import torch
 
 from . import _lib
@@ -29,6 +31,10 @@ from .ops import _u8
 # shape, strides and device once and leave to the C ABI what it checks itself.
 _DTYPES = {torch.bfloat16: 0, torch.float32: 1, torch.float16: 2}
 _I32, _U8, _BF16 = torch.int32, torch.uint8, torch.bfloat16
+# arguments of the C calls as blocks of 8-byte words (wgkv_kv4_*_block)
+_pack_append = struct.Struct("32q").pack
+_pack_read = struct.Struct("23q").pack
+_pack_attn = struct.Struct("20qd3q").pack
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
@@ -91,21 +97,22 @@ def _check_heads(block_table, lengths, B, H):
     return block_table, bs, shape[2], lengths, ls[0]
 
 
-def _rows(t, copy=True):
-    """t and its strides if its rows can be read and written 16 bytes at a
-    time, else (``copy``) a contiguous copy's, or None."""
-    unit = 16 // t.element_size()
+def _rows(t, unit, copy=True):
+    """t, its address and strides if its rows can be read and written 16
+    bytes (``unit`` elements) at a time, else (``copy``) a contiguous copy's,
+    or None."""
     st = t.stride()
-    if st[3] == 1 and not (st[0] | st[1] | st[2]) % unit and not t.data_ptr() % 16:
-        return t, st
+    p = t.data_ptr()
+    if st[3] == 1 and not (st[0] | st[1] | st[2]) % unit and not p % 16:
+        return t, p, st
     # the stride of a dimension of one entry means nothing
-    st = tuple(0 if n == 1 else x for n, x in zip(t.shape, st))
-    if t.stride(3) == 1 and not (st[0] | st[1] | st[2]) % unit and not t.data_ptr() % 16:
-        return t, st
+    sz = tuple(0 if n == 1 else x for n, x in zip(t.shape, st))
+    if st[3] == 1 and not (sz[0] | sz[1] | sz[2]) % unit and not p % 16:
+        return t, p, sz
     if not copy:
         return None
     t = t.clone(memory_format=torch.contiguous_format)
-    return t, t.stride()
+    return t, t.data_ptr(), t.stride()
 
 
 def kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask=None, out=None, status=None):
@@ -150,26 +157,26 @@ def kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask=None, out=No
     if dev != _current_device():  # a null stream is the current device's
         with torch.cuda.device(dev):
             return kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask, out, status)
-    m, ms = None, (0, 0)
+    mp, ms = 0, (0, 0)
     if g_mask is not None:
         m = _u8(g_mask)
         if T > 1 and m.stride(2) != 1:
             m = m.contiguous()
         ms = m.stride()
-        m = m.data_ptr()
-    k, ks = _rows(k)
-    v, vs = _rows(v)
+        mp = m.data_ptr()
+    unit = 4 if code == 1 else 8
+    k, kp, ks = _rows(k, unit)
+    v, vp, vs = _rows(v, unit)
     if out is None:
         out = torch.empty_like(lens, memory_format=torch.contiguous_format)
     L = _lib.lib()
     nbytes = L.wgkv_kv4_append_workspace_bytes(B, H, T) if T > 256 else 0
     ws = torch.empty(nbytes, dtype=_U8, device=dev) if nbytes else None
-    st = L.wgkv_kv4_append(
-        k.data_ptr(), ks[0], ks[1], ks[2], v.data_ptr(), vs[0], vs[1], vs[2], code,
-        m, ms[0], ms[1], lens.data_ptr(), ls, out.data_ptr(), out.stride(0),
-        k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P,
+    st = L.wgkv_kv4_append_block(_pack_append(
+        kp, ks[0], ks[1], ks[2], vp, vs[0], vs[1], vs[2], code, mp, ms[0], ms[1],
+        lens.data_ptr(), ls, out.data_ptr(), out.stride(0), k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P,
         table.data_ptr(), bs[0], bs[1], width, B, T, H, D,
-        None if status is None else status.data_ptr(), None if ws is None else ws.data_ptr(), nbytes, _stream(dev))
+        0 if status is None else status.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes, _stream(dev)))
     if st:
         _lib.check(st, "wgkv_kv4_append")
     return out
@@ -192,7 +199,7 @@ def kv4_read(k_cache, v_cache, block_table, lengths, rows, starts=None, dtype=to
         raise TypeError("kv4_read gives bf16, fp16 or fp32")
     if rows < 0:
         raise AssertionError("rows must not be negative")
-    sp, ss = None, 0
+    sp, ss = 0, 0
     if starts is not None:
         if starts.shape != (B, H) or starts.dtype is not _I32:
             raise AssertionError("starts must be int32 (batch, num_kv_heads)")
@@ -213,23 +220,26 @@ def kv4_read(k_cache, v_cache, block_table, lengths, rows, starts=None, dtype=to
         vo = torch.empty_like(ko)
         out = (ko, vo)
         st = ko.stride()
+        kp, vp = ko.data_ptr(), vo.data_ptr()
     else:
         ko, vo = out
         if ko.shape != (B, rows, H, D) or vo.shape != ko.shape or ko.dtype != dtype or vo.dtype != dtype:
             raise AssertionError("out must be two (batch, rows, num_kv_heads, head_dim) tensors of dtype")
         if ko.get_device() != dev or vo.get_device() != dev:
             _two_devices()
-        kr, vr = _rows(ko, copy=False), _rows(vo, copy=False)
-        if kr is None or vr is None or kr[1] != vr[1]:  # no rows of 16-byte steps, or two layouts
+        unit = 4 if code == 1 else 8
+        kr, vr = _rows(ko, unit, False), _rows(vo, unit, False)
+        if kr is None or vr is None or kr[2] != vr[2]:  # no rows of 16-byte steps, or two layouts
             for dst, src in zip(out, kv4_read(k_cache, v_cache, table, lens, rows, starts, dtype)):
                 dst.copy_(src)
             return out
-        st = kr[1]
+        _, kp, st = kr
+        vp = vr[1]
     if rows == 0:
         return out
-    err = _lib.lib().wgkv_kv4_read(
+    err = _lib.lib().wgkv_kv4_read_block(_pack_read(
         k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P, table.data_ptr(), bs[0], bs[1], width,
-        lens.data_ptr(), ls, sp, ss, ko.data_ptr(), vo.data_ptr(), st[0], st[1], st[2], code, B, rows, H, D, _stream(dev))
+        lens.data_ptr(), ls, sp, ss, kp, vp, st[0], st[1], st[2], code, B, rows, H, D, _stream(dev)))
     if err:
         _lib.check(err, "wgkv_kv4_read")
     return out
@@ -282,24 +292,24 @@ def paged_decode_attn_kv4(q, k_cache, v_cache, cache_seqlens, block_table, softm
     if dev != _current_device():
         with torch.cuda.device(dev):
             return paged_decode_attn_kv4(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, out)
-    q, qs = _rows(q)
+    q, qp, qs = _rows(q, 8)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
-        os = out.stride()
+        op, os = out.data_ptr(), out.stride()
     else:
         if out.shape != shape or out.dtype is not _BF16:
             raise AssertionError("out must be (batch, 1, num_query_heads, head_dim) bf16")
-        os = _rows(out, copy=False)
-        if os is None:  # rows cannot be written 16 bytes at a time
+        rows = _rows(out, 8, False)
+        if rows is None:  # they cannot be written 16 bytes at a time
             return out.copy_(paged_decode_attn_kv4(q, k_cache, v_cache, lens, table, softmax_scale))
-        os = os[1]
+        _, op, os = rows
     L = _lib.lib()
     stream = _stream(dev)
     ws = _attn_workspace(dev, stream, L.wgkv_kv4_decode_workspace_bytes(Hq, H, D))
-    st = L.wgkv_kv4_decode_attn(
-        q.data_ptr(), qs[0], qs[2], k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P,
-        lens.data_ptr(), ls, table.data_ptr(), bs[0], bs[1], width,
-        out.data_ptr(), os[0], os[2], B, Hq, H, D, softmax_scale, ws.data_ptr(), ws.numel(), stream)
+    st = L.wgkv_kv4_decode_attn_block(_pack_attn(
+        qp, qs[0], qs[2], k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P, lens.data_ptr(), ls,
+        table.data_ptr(), bs[0], bs[1], width, op, os[0], os[2], B, Hq, H, D, softmax_scale, ws.data_ptr(), ws.numel(),
+        stream))
     if st:
         _lib.check(st, "wgkv_kv4_decode_attn")
     return out
