@@ -582,3 +582,50 @@ def test_calls_on_two_streams_at_once():
                 assert torch.equal(o[0], rk[0]) and torch.equal(o[1], rk[1])
             else:
                 assert torch.equal(o, refs[j])
+
+
+def test_dispatcher_operators_run_the_kernels():
+    import wgkv
+    gen = torch.Generator().manual_seed(91)
+    lens = torch.tensor([[70, 33]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, 32, 128)
+    dk, dv, sl, tb = torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV), lens.to(DEV), bt.to(DEV)
+    q = torch.randn(1, 1, 8, 128, generator=gen).to(torch.bfloat16).to(DEV)
+    assert torch.equal(torch.ops.wgkv.paged_decode_attn_kv4(q, dk, dv, sl, tb, 0.1),
+                       wgkv.paged_decode_attn_kv4(q, dk, dv, sl, tb, 0.1))
+    for a, b in zip(torch.ops.wgkv.kv4_read(dk, dv, tb, sl, 40, dtype=torch.float32),
+                    wgkv.kv4_read(dk, dv, tb, sl, 40, dtype=torch.float32)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("units", [16, 17, 32, 33])
+def test_attend_page_windows(units):
+    """Ranges that end with or just behind a window of page ids (16 units of
+    64 tokens): one head on one workgroup's waves, many units each."""
+    import wgkv
+    ln = torch.full((64, 32), 1, dtype=I32)  # 2048 heads fill the line's other ranges
+    ln[5, 7] = units * 64
+    ln[63, 31] = units * 64 - 40
+    kc, vc, bt = device_cache(ln, 64, 64, seed=units)
+    gen = torch.Generator().manual_seed(units)
+    q = torch.randn(64, 1, 32, 64, generator=gen).to(torch.bfloat16)
+    check_attend(q, kc.cpu().numpy(), vc.cpu().numpy(), bt, ln, 0.125)
+    # the same heads alone, whole ranges of many units per wave
+    long = torch.full((8, 8), units * 64 * 4, dtype=I32)
+    kc, vc, bt = device_cache(long, 64, 64, seed=units + 1)
+    q = torch.randn(8, 1, 32, 64, generator=gen).to(torch.bfloat16).to(DEV)
+    sl, tb = long.to(DEV), bt.to(DEV)
+    got = wgkv.paged_decode_attn_kv4(q, kc, vc, sl, tb, 0.125)
+    k, v = wgkv.kv4_read(kc, vc, tb, sl, units * 256, dtype=torch.float32)
+    k, v = (x.cpu().double().transpose(1, 2).repeat_interleave(4, 1) for x in (k, v))
+    p = torch.softmax((q.cpu().double().transpose(1, 2) @ k.transpose(2, 3)) * 0.125, -1)
+    want = (p @ v).transpose(1, 2)
+    # half a bf16 step, 2^-8, of what the codes add (a group's middle is that
+    # of its read values, whose ends are codes 0 and 15) and of the output;
+    # fp32 sums: 32 accumulations of codes offset by 143 steps of at most 0.5
+    # between two corrections, and as much for their offset: 2 * 32 * 2^-24 *
+    # 143 * 0.5 = 2.8e-4
+    g = v.view(*v.shape[:-1], 2, 32)
+    spread = (g - (g.amax(-1, keepdim=True) + g.amin(-1, keepdim=True)) / 2).abs().view_as(v)
+    bound = 2.0 ** -8 * ((p @ spread).transpose(1, 2) + want.abs()) + 2.8e-4
+    assert ((got.cpu().double() - want).abs() <= bound).all()

@@ -143,3 +143,40 @@ def test_c_entry_points_check_arguments_without_gpu():
     for kw, want in [(dict(out=None), _lib.ERR_ARG), (dict(rows=0), _lib.ERR_ARG), (dict(so=4), _lib.ERR_UNSUPPORTED),
                      (dict(dtype=-1), _lib.ERR_UNSUPPORTED), (dict(D=32), _lib.ERR_UNSUPPORTED)]:
         assert read(**kw) == want, kw
+
+
+@pytest.mark.parametrize("D,P", [(64, 16), (128, 64)])
+def test_dispatcher_operators(D, P):
+    """Registered with their schemas; the Meta kernels give the shapes."""
+    import wgkv  # noqa: F401
+    for n in ("paged_decode_attn_kv4", "kv4_read"):
+        assert str(getattr(torch.ops.wgkv, n).default._schema).startswith(f"wgkv::{n}(")
+    meta = dict(device="meta")
+    kc = torch.empty(7, P // 16, 10 * D, dtype=torch.uint8, **meta)
+    q = torch.empty(2, 1, 8, D, dtype=torch.bfloat16, **meta)
+    sl, bt = torch.empty(2, 4, dtype=torch.int32, **meta), torch.empty(2, 4, 9, dtype=torch.int32, **meta)
+    out = torch.ops.wgkv.paged_decode_attn_kv4(q, kc, kc, sl, bt, 0.1)
+    assert out.shape == q.shape and out.dtype == q.dtype
+    k, v = torch.ops.wgkv.kv4_read(kc, kc, bt, sl, 33, dtype=torch.float32)
+    assert k.shape == v.shape == (2, 33, 4, D) and k.dtype == torch.float32
+
+
+def test_argument_blocks_are_the_calls_arguments():
+    """The block entry points check what the plain ones check (a null query,
+    cache or output is refused before any HIP call)."""
+    from wgkv import _lib, kv4
+    L = _lib.lib()
+    assert L.wgkv_kv4_append_block(kv4._pack_append(*[0] * 32)) == _lib.ERR_ARG
+    assert L.wgkv_kv4_read_block(kv4._pack_read(*[0] * 23)) == _lib.ERR_ARG
+    assert L.wgkv_kv4_decode_attn_block(kv4._pack_attn(*[0] * 20, 1.0, 0, 0, 0)) == _lib.ERR_ARG
+    x = 4096
+    sizes = dict(append=(len(_lib.SIGNATURES["wgkv_kv4_append"][1]), 32), read=(len(_lib.SIGNATURES["wgkv_kv4_read"][1]), 23),
+                 attn=(len(_lib.SIGNATURES["wgkv_kv4_decode_attn"][1]), 24))
+    assert all(a == b for a, b in sizes.values()), sizes
+    # every word reaches its argument: the last checks before a launch
+    words = [x, 64, 64, 64, x, 64, 64, 64, 0, 0, 0, 0, x, 1, x, 1, x, x, 4, 16, x, 4, 4, 4, 1, 257, 1, 64, 0, x, 8, 0]
+    assert L.wgkv_kv4_append_block(kv4._pack_append(*words)) == _lib.ERR_WORKSPACE
+    words = [x, x, 4, 16, x, 4, 4, 4, x, 1, 0, 0, x, x, 64, 64, 4, 0, 1, 4, 1, 64, 0]
+    assert L.wgkv_kv4_read_block(kv4._pack_read(*words)) == _lib.ERR_UNSUPPORTED
+    words = [x, 64, 64, x, x, 4, 16, x, 1, x, 4, 4, 4, x, 64, 64, 1, 4, 1, 64, 0.125, x, 8, 0]
+    assert L.wgkv_kv4_decode_attn_block(kv4._pack_attn(*words)) == _lib.ERR_WORKSPACE

@@ -41,7 +41,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;  // log2 units a running maximum may lag the scores
 constexpr int kMaxBH = 2048;
 constexpr int kMaxG = 8;
-constexpr int kMaxSlots = 1024;  // workgroups of a launch
+constexpr int kMaxSlots = 512;  // workgroups of a launch
 constexpr int kFlush = 16;       // units between two corrections of the code offset
 constexpr uint32_t kCodeMask = 0x000f000fu, kCodeBase = 0x43004300u;  // 128 + c
 constexpr float kOffset = 135.5f;                                     // (128 + c) - (c - 7.5)
@@ -295,7 +295,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       const int tile = min(4 * u + 2 * half + p, last_tile);
-      const int pg = __builtin_amdgcn_readlane(pages, tile - 4 * base_u);
+      const int pg = __builtin_amdgcn_readlane(pages, max(tile - 4 * base_u, 0));
       const int64_t at = (((int64_t)pg << a.pg.page_shift) + (tile & ((1 << a.pg.page_shift) - 1))) * kv4_tile_bytes(D);
       const uint8_t* kt = a.kc + at;
       const uint8_t* vt = a.vc + at;

@@ -17,12 +17,17 @@ Operators (schemas below):
                              the optional packed first layer)
   gate_pack_weights       -- the packed first layer of the bf16
                              matrix-core gate path (no reference counterpart)
+  paged_decode_attn_kv4   -- paged_decode_attn over a cache held in 4 bits
+  kv4_read                -- such a cache's rows as dense tensors (no
+                             reference counterpart, both)
 """
 import torch
 
 from . import ops as _ops
 from .gate import gate_scores_and_mask as _gate_scores_and_mask
 from .gate import pack_weights as _pack_weights
+from .kv4 import kv4_read as _kv4_read
+from .kv4 import paged_decode_attn_kv4 as _paged_decode_attn_kv4
 
 _INPUT_NAMES = ("pre_k", "post_k", "v")
 
@@ -38,6 +43,10 @@ _LIB.define("gate_scores_and_mask(Tensor? pre_key, Tensor? post_key, Tensor? val
             "bool rms, float clamp_min, float threshold, Tensor? w1_packed=None, int precision=0) -> (Tensor, Tensor)")
 _LIB.define("gate_pack_weights(Tensor? w_pre, Tensor? w_post, Tensor? w_v, Tensor w1, int inputs_mask, bool rms, "
             "int num_kv_heads, int head_dim, int inner, int precision=0) -> Tensor")
+_LIB.define("paged_decode_attn_kv4(Tensor q, Tensor k_cache, Tensor v_cache, Tensor cache_seqlens, "
+            "Tensor block_table, float softmax_scale) -> Tensor")
+_LIB.define("kv4_read(Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor lengths, int rows, "
+            "Tensor? starts=None, ScalarType dtype=bfloat16) -> (Tensor, Tensor)")
 
 
 # ---- CUDA (HIP) kernels: the library calls ----------------------------------
@@ -66,7 +75,13 @@ def _gate_pack(w_pre, w_post, w_v, w1, inputs_mask, rms, num_kv_heads, head_dim,
     return _pack_weights(w_pre, w_post, w_v, w1, names, rms, num_kv_heads, head_dim, inner, precision=precision)
 
 
+def _kv4_read_op(k_cache, v_cache, block_table, lengths, rows, starts=None, dtype=torch.bfloat16):
+    return _kv4_read(k_cache, v_cache, block_table, lengths, rows, starts, dtype)
+
+
 _LIB.impl("sparse_attn", _sparse_attn, "CUDA")
+_LIB.impl("paged_decode_attn_kv4", _paged_decode_attn_kv4, "CUDA")
+_LIB.impl("kv4_read", _kv4_read_op, "CUDA")
 _LIB.impl("paged_decode_attn", _paged_decode_attn, "CUDA")
 _LIB.impl("generate_sparse_indices", _generate_sparse_indices, "CUDA")
 _LIB.impl("gate_scores_and_mask", _gate, "CUDA")
@@ -110,6 +125,18 @@ def _gate_pack_meta(w_pre, w_post, w_v, w1, inputs_mask, rms, num_kv_heads, head
                        device=w1.device)
 
 
+def _paged_decode_attn_kv4_meta(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale):
+    return torch.empty_like(q, memory_format=torch.contiguous_format)
+
+
+def _kv4_read_meta(k_cache, v_cache, block_table, lengths, rows, starts=None, dtype=torch.bfloat16):
+    B, H = lengths.shape
+    shape = (B, rows, H, k_cache.shape[2] // 10)
+    return tuple(torch.empty(shape, dtype=dtype, device=k_cache.device) for _ in range(2))
+
+
+_LIB.impl("paged_decode_attn_kv4", _paged_decode_attn_kv4_meta, "Meta")
+_LIB.impl("kv4_read", _kv4_read_meta, "Meta")
 _LIB.impl("gate_scores_and_mask", _gate_meta, "Meta")
 _LIB.impl("gate_pack_weights", _gate_pack_meta, "Meta")
 
