@@ -37,6 +37,8 @@
 
 namespace {
 
+typedef __attribute__((__vector_size__(2 * sizeof(uint32_t)))) uint32_t u32x2_t;
+
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;  // log2 units a running maximum may lag the scores
 constexpr int kMaxBH = 2048;
@@ -62,8 +64,8 @@ struct AttnArgs {
   float scale_log2;         // |softmax_scale| * log2(e)
   uint32_t q_and, q_xor;    // its sign (and a scale of 0) is put into the queries
   // pieces: two slots per workgroup (the head it ends, the head it begins);
-  // slot s, query head i: part_m[s*G+i], part_l[s*G+i], part_acc[(s*G+i)*D..]
-  float *part_m, *part_l, *part_acc;
+  // slot s, query head i: (max, sum) at part_ml[(s*G+i)*2], part_acc[(s*G+i)*D..]
+  float *part_ml, *part_acc;
   int* counter;  // arrivals per (b, h), zero between calls
 };
 
@@ -160,6 +162,23 @@ WGKV_DEVICE float row_ror_add(float x) {
   return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x120 + CTRL, 0xf, 0xf, false));
 }
 
+// Sum and maximum over the four 16-lane rows of a wave, lane by lane
+// (v_permlane32_swap, v_permlane16_swap: no LDS round trip).
+template <typename Op>
+WGKV_DEVICE float over_rows(float x, Op op) {
+  uint32_t u = __float_as_uint(x);
+  u32x2_t r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  u = __float_as_uint(op(__uint_as_float(r[0]), __uint_as_float(r[1])));
+  r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+WGKV_DEVICE float rows_sum(float x) {
+  return over_rows(x, [](float a, float b) { return a + b; });
+}
+WGKV_DEVICE float rows_max(float x) {
+  return over_rows(x, [](float a, float b) { return fmaxf(a, b); });
+}
+
 // A dword of codes as four operand dwords (pairs of 128 + c).
 // The constants come in registers, one scalar and one vector: as literals
 // they would make two instructions of one v_and_or.
@@ -174,11 +193,11 @@ WGKV_DEVICE void expand(uint32_t w, uint32_t mask, uint32_t base, uint32_t* o) {
 WGKV_DEVICE float piece_weight(float m, float M) { return m == -INFINITY ? 1.f : fast_exp2(m - M); }
 
 // Merges the pieces that workgroups f..e left of head (b, h) and writes its
-// G rows.  A thread takes four d of a row over every groups-th piece, eight
+// G rows.  A thread takes four d of a row over every groups-th piece, four
 // pieces' loads in flight, and the groups meet in LDS (kThreads * 6 floats).
 template <int D, int kThreads>
 WGKV_DEVICE void merge_pieces(const AttnArgs& a, int f, int e, int b, int h, float* lds) {
-  constexpr int kBatch = 8;
+  constexpr int kBatch = 4;
   const int G = a.G, NQ = G * (D / 4);
   static_assert(kThreads * 4 >= kMaxG * D, "a thread for every four d");
   const int groups = kThreads / NQ;
@@ -187,6 +206,7 @@ WGKV_DEVICE void merge_pieces(const AttnArgs& a, int f, int e, int b, int h, flo
   f32x4_t* s_a = (f32x4_t*)(lds + 2 * kThreads);
   const int t = threadIdx.x;
   const __amdgpu_buffer_rsrc_t acc = __builtin_amdgcn_make_buffer_rsrc(a.part_acc, (short)0, 0x7fffffff, 0x00020000);
+  const __amdgpu_buffer_rsrc_t ml_rsrc = __builtin_amdgcn_make_buffer_rsrc(a.part_ml, (short)0, 0x7fffffff, 0x00020000);
   const int vq = t % NQ, grp = t / NQ;
   const int i = vq / (D / 4);
   float M = -INFINITY, L = 0.f;
@@ -199,8 +219,10 @@ WGKV_DEVICE void merge_pieces(const AttnArgs& a, int f, int e, int b, int h, flo
       for (int k = 0; k < kBatch; ++k) {
         const int x = min(x0 + k * groups, e);
         const int s = (2 * x + (x == f ? 1 : 0)) * G;
-        m[k] = load_coherent(&a.part_m[s + i]);
-        l[k] = load_coherent(&a.part_l[s + i]);
+        const u32x2_t ml = __builtin_bit_cast(
+            u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(ml_rsrc, (s + i) * 2 * (int)sizeof(float), 0, 16));
+        m[k] = __uint_as_float(ml[0]);
+        l[k] = __uint_as_float(ml[1]);
         ac[k] = load_coherent4(acc, (s * D + vq * 4) * (int)sizeof(float));
       }
       float mn = M;
@@ -272,6 +294,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
   uint32_t mask = kCodeMask, base = kCodeBase;
   asm("" : "+s"(mask));
   asm("" : "+v"(base));
+
+  const u32x4_t ones = (u32x4_t){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // bf16 1.0
 
   const Line ln = make_line<kMany>(a, lane);
   const int cw = max((int)(((unsigned)ln.total + n_wg * NW - 1) / (unsigned)(n_wg * NW)), 1);  // units per wave
@@ -346,21 +370,16 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const bool mine = quad * NG / 4 == g && nt * HPT + hh < G;
-      float sum = 0.f;
+      const uint32_t keep = mine ? a.q_and : 0u, flip = mine ? a.q_xor : 0u;
+      f32x4_t sum = (f32x4_t){0.f, 0.f, 0.f, 0.f};  // of the column, in every row
 #pragma unroll
       for (int i = 0; i < KS; ++i) {
-        u32x4_t v = qraw[nt][i];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = mine ? (v[j] & a.q_and) ^ a.q_xor : 0u;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sum += bf16lo(v[j]) + bf16hi(v[j]);
+        const u32x4_t v = (qraw[nt][i] & keep) ^ flip;
         qb[nt][i] = __builtin_bit_cast(bf16x8_t, v);
+        sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ones), qb[nt][i], sum, 0, 0, 0);
       }
-      sum += __shfl_xor(sum, 16, 64);  // over the quads: the column's group
-      sum += __shfl_xor(sum, 32, 64);
-      qsum[nt] = sum;
-      const float c = -kOffset * sum;
-      c0[nt] = (f32x4_t){c, c, c, c};
+      qsum[nt] = sum[0];
+      c0[nt] = sum * -kOffset;
     }
 
     float m_run[NT], l_run[NT], corr[NT];
@@ -378,10 +397,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     const auto flush = [&]() {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float c = corr[nt];
-        c += __shfl_xor(c, 16, 64);
-        c += __shfl_xor(c, 32, 64);
-        c = fmaf(-kOffset, usum[nt][0], c);
+        const float c = fmaf(-kOffset, usum[nt][0], rows_sum(corr[nt]));
         corr[nt] = 0.f;
         usum[nt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -441,9 +457,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
         // than the slack (p <= 2^slack); it is the same in the column's four
         // lanes, whose accumulators hold sums over all of them.
         if (__builtin_amdgcn_ballot_w64(top * a.scale_log2 > m_run[nt] + kRescaleSlack)) {
-          float mx = fmaxf(top, __shfl_xor(top, 16, 64));
-          mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-          const float mn = fmaxf(m_run[nt], mx * a.scale_log2);
+          const float mn = fmaxf(m_run[nt], rows_max(top) * a.scale_log2);
           const float alpha = mn == -INFINITY ? 1.f : fast_exp2(m_run[nt] - mn);
           m_run[nt] = mn;
           l_run[nt] *= alpha;
@@ -466,7 +480,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
           }
         pb[nt] = (u32x4_t){pk[0], pk[1], pk[2], pk[3]};
         // the sum of the rounded products, for the offset to cancel exactly
-        const u32x4_t ones = (u32x4_t){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
         usum[nt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ones),
                                                            __builtin_bit_cast(bf16x8_t, pb[nt]), usum[nt], 0, 0, 0);
       }
@@ -527,9 +540,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     const int slot = 2 * wid + (u0 > 0 ? 0 : 1);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      float l = l_run[nt];
-      l += __shfl_xor(l, 16, 64);
-      l += __shfl_xor(l, 32, 64);
+      const float l = rows_sum(l_run[nt]);
       const int qh = nt * HPT + hh;
       if (quad * NG / 4 == g && qh < G) {
 #pragma unroll
@@ -592,8 +603,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
         a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + d] = f32_to_bf16(A / L);
       } else {
         if (d == 0) {
-          store_coherent(&a.part_m[to + i], M);
-          store_coherent(&a.part_l[to + i], L);
+          store_coherent(&a.part_ml[(to + i) * 2], M);
+          store_coherent(&a.part_ml[(to + i) * 2 + 1], L);
         }
         store_coherent(&a.part_acc[(to + i) * D + d], A);
       }
@@ -718,9 +729,8 @@ extern "C" int wgkv_kv4_decode_attn(
   a.q_xor = softmax_scale < 0.f ? 0x80008000u : 0u;
   a.counter = (int*)workspace;
   const size_t slots = (size_t)2 * kMaxSlots * G;
-  a.part_m = (float*)((char*)workspace + kCounterBytes);
-  a.part_l = a.part_m + slots;
-  a.part_acc = a.part_l + slots;
+  a.part_ml = (float*)((char*)workspace + kCounterBytes);
+  a.part_acc = a.part_ml + slots * 2;
   hipStream_t s = (hipStream_t)stream;
   const hipError_t e = head_dim == 64 ? launch<64, 1>(a, s) : G <= 4 ? launch<128, 1>(a, s) : launch<128, 2>(a, s);
   return e == hipSuccess ? WGKV_OK : WGKV_ERR_HIP;
