@@ -100,27 +100,52 @@ WGKV_DEVICE float bf16_of(float x) {
   return __uint_as_float((u + 0x7fffu + (u >> 16 & 1u)) & 0xffff0000u);
 }
 
-// The codes of 8 values exactly: k + 7.5 rounded to even for x = m + k s, k + 8
-// beyond it and k + 7 below, for an integer k next to (x - m) / s.  That need
-// not be the nearest, so the quotient may be approximate (v_rcp), and the
-// side is decided by the sign of the residue x - m - k s.  k s has 12 bits
-// and is exact; x - m is within one fp32 rounding, whose error counts only
-// where the rounded difference equals k s (a nonzero residue is at least one
-// ulp of it).  For 16-bit inputs the difference is inexact only where x is
-// tiny beside m, and one addition recovers the error; fp32 takes the full
-// two-sum.
+// A group's step, middle and reciprocal step; the step is 0 where the group
+// has none (all values alike, or one not finite: `pair` says which).
+struct Group {
+  float s, m, inv;
+  uint32_t pair;  // (s, m) as they are stored
+};
+
+WGKV_DEVICE Group group_of(float hi, float lo) {
+  // In 64 bits, as a multiplication: 1/15 in fp64 is 2^-56 off, too little
+  // to move the quotient across a border of fp32 or bf16.
+  const float sf = (float)(((double)hi - (double)lo) * (1.0 / 15.0));
+  Group g;
+  g.s = bf16_of(sf);
+  g.m = bf16_of(0.5f * hi + 0.5f * lo);
+  const bool bad = !(sf < INFINITY) || !(fabsf(g.m) < INFINITY);
+  if (!(g.s >= 0x1p-126f) || bad) g.s = 0.f;
+  g.inv = __builtin_amdgcn_rcpf(g.s);
+  g.pair = bad ? 0x7fc07fc0u : (__float_as_uint(g.s) >> 16) | __float_as_uint(g.m);
+  return g;
+}
+
+// The code of x is k + 7.5 rounded to even for x = m + k s, k + 8 beyond it
+// and k + 7 below, for an integer k next to (x - m) / s.  That need not be
+// the nearest, so the quotient may be approximate (v_rcp is good to 2^-23),
+// and the side is decided by the sign of an exact residue:
+//   * 16-bit inputs: x - (m + k s).  The border m + k s is exact in fp32 for
+//     the |k| <= 8 that matter: m has 8 bits and k s 12, m is 0 or at least
+//     2^-13 of the range (a sum of two 11-bit numbers), and s is at least
+//     2^-15 of m (values that differ do so by a unit of their 11 bits).
+//   * fp32: (x - m) - k s with the two-sum error of x - m, which counts only
+//     where the rounded difference equals k s (a nonzero residue is at least
+//     one ulp of it).
 template <int TY>
 WGKV_DEVICE void exact_codes(const float (&x)[8], float s, float m, float inv, float (&c)[8]) {
+  const float nb = -m * inv;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float d = x[i] - m;
-    const float k = rintf(d * inv);
-    float r = fmaf(-k, s, d);
+    float k, r;
     if constexpr (TY == kKv4F32) {
+      const float d = x[i] - m;
+      k = rintf(d * inv);
       const float bb = d - x[i];
-      r += (x[i] - (d - bb)) - (m + bb);
+      r = fmaf(-k, s, d) + ((x[i] - (d - bb)) - (m + bb));
     } else {
-      r += x[i] - (d + m);
+      k = rintf(fmaf(x[i], inv, nb));
+      r = x[i] - fmaf(k, s, m);
     }
     // 7.25, 7.5 or 7.75 by the residue's sign (one below 2^-148 counts as 0)
     const float side = __builtin_amdgcn_fmed3f(fmaf(r, 0x1p127f, 7.5f), 7.25f, 7.75f);
@@ -128,33 +153,14 @@ WGKV_DEVICE void exact_codes(const float (&x)[8], float s, float m, float inv, f
   }
 }
 
-// Quantises a lane's 8 values of a group that four neighbouring lanes share.
-// Returns (s, m) as a packed pair; the codes as numbers in c[0..7], all 0
-// where `none` comes back true (no step).
+// The codes of a lane's 8 values, as numbers.
 template <int TY>
-WGKV_DEVICE uint32_t quantise8(const float (&x)[8], float (&c)[8], bool& none) {
-  float hi = x[0], lo = x[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    hi = __builtin_elementwise_maximum(hi, x[i]);
-    lo = __builtin_elementwise_minimum(lo, x[i]);
-  }
-  hi = quad_maximum(hi);
-  lo = quad_minimum(lo);
-  // In 64 bits, as a multiplication: 1/15 in fp64 is 2^-56 off, too little
-  // to move the quotient across a border of fp32 or bf16.
-  const float sf = (float)(((double)hi - (double)lo) * (1.0 / 15.0));
-  float s = bf16_of(sf);
-  const float m = bf16_of(0.5f * hi + 0.5f * lo);
-  const bool bad = !(sf < INFINITY) || !(fabsf(m) < INFINITY);
-  if (!(s >= 0x1p-126f)) s = 0.f;
-  none = s == 0.f || bad;
-  const float inv = __builtin_amdgcn_rcpf(s);
+WGKV_DEVICE void codes_of(const float (&x)[8], float s, float m, float inv, float (&c)[8]) {
   if constexpr (TY == kKv4F32) {
-    // (x - m) / s + 7.5 by one fma is within 2^-24 (|bias| + 32) of itself
-    // (v_rcp is good to 2^-23).  Rows of a wave with a value that near to a
-    // border between two codes are taken exactly.  (Not for 16-bit inputs:
-    // 0.7 % of bf16 values lie on a border, some in every wave.)
+    // (x - m) / s + 7.5 by one fma is within 2^-24 (|bias| + 32) of itself.
+    // Rows of a wave with a value that near to a border between two codes are
+    // taken exactly.  (Not for 16-bit inputs: 0.7 % of bf16 values lie on a
+    // border, some in every wave.)
     const float bias = fmaf(-m, inv, 7.5f);
     float far = 0.f;
 #pragma unroll
@@ -164,12 +170,15 @@ WGKV_DEVICE uint32_t quantise8(const float (&x)[8], float (&c)[8], bool& none) {
       c[i] = __builtin_amdgcn_fmed3f(r, 0.f, 15.f);
     }
     const bool near = far >= 0.5f - 0x1p-23f * (fabsf(bias) + 32.f);
-    if (__builtin_amdgcn_ballot_w64(near && !none)) exact_codes<TY>(x, s, m, inv, c);
+    if (__builtin_amdgcn_ballot_w64(near && s != 0.f)) exact_codes<TY>(x, s, m, inv, c);
   } else {
     exact_codes<TY>(x, s, m, inv, c);
   }
-  const uint32_t w = (__float_as_uint(s) >> 16) | __float_as_uint(m);
-  return bad ? 0x7fc07fc0u : w;
+}
+
+template <int I>
+WGKV_DEVICE float quad_lane(float x) {  // lane I of each four
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), I * 0x55, 0xf, 0xf, true));
 }
 
 // Four codes as a 16-bit word, the first in the lowest bits.
@@ -182,13 +191,31 @@ WGKV_DEVICE uint32_t pack4(float a, float b, float c, float d) {
 template <int D, int TY, bool kKeys>
 WGKV_DEVICE void write_quad(uint8_t* tile, int qi, int L, const Kv4Raw<TY> (&raw)[4], const bool (&ok)[4]) {
   constexpr int NG = D / kKv4Group;
-  uint32_t w[4][2], sm[4];
+  uint32_t w[4][2];
+  float x[4][8], hi[4], lo[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    float x[8], c[8];
-    bool none;
-    kv4_widen<TY>(raw[i], x);
-    sm[i] = quantise8<TY>(x, c, none);
+    kv4_widen<TY>(raw[i], x[i]);
+    hi[i] = lo[i] = x[i][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) {
+      hi[i] = __builtin_elementwise_maximum(hi[i], x[i][j]);
+      lo[i] = __builtin_elementwise_minimum(lo[i], x[i][j]);
+    }
+    hi[i] = quad_maximum(hi[i]);
+    lo[i] = quad_minimum(lo[i]);
+  }
+  // four lanes share the four tokens' groups: lane j works token j's out
+  const int j = L & 3;
+  const Group g = group_of(j == 0 ? hi[0] : j == 1 ? hi[1] : j == 2 ? hi[2] : hi[3],
+                           j == 0 ? lo[0] : j == 1 ? lo[1] : j == 2 ? lo[2] : lo[3]);
+  const float gs[4] = {quad_lane<0>(g.s), quad_lane<1>(g.s), quad_lane<2>(g.s), quad_lane<3>(g.s)};
+  const float gm[4] = {quad_lane<0>(g.m), quad_lane<1>(g.m), quad_lane<2>(g.m), quad_lane<3>(g.m)};
+  const float gi[4] = {quad_lane<0>(g.inv), quad_lane<1>(g.inv), quad_lane<2>(g.inv), quad_lane<3>(g.inv)};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float c[8];
+    codes_of<TY>(x[i], gs[i], gm[i], gi[i], c);
     if constexpr (kKeys) {
       w[i][0] = pack4(c[0], c[2], c[4], c[6]);
       w[i][1] = pack4(c[1], c[3], c[5], c[7]);
@@ -196,7 +223,7 @@ WGKV_DEVICE void write_quad(uint8_t* tile, int qi, int L, const Kv4Raw<TY> (&raw
       w[i][0] = pack4(c[0], c[1], c[2], c[3]);
       w[i][1] = pack4(c[4], c[5], c[6], c[7]);
     }
-    if (none) w[i][0] = w[i][1] = 0u;
+    if (gs[i] == 0.f) w[i][0] = w[i][1] = 0u;
   }
   const bool whole = ok[0] && ok[1] && ok[2] && ok[3];
   if constexpr (kKeys) {
@@ -225,16 +252,8 @@ WGKV_DEVICE void write_quad(uint8_t* tile, int qi, int L, const Kv4Raw<TY> (&raw
         }
     }
   }
-  if (L % 4 == 0) {
-    uint32_t* sp = (uint32_t*)(tile + kv4_scales_at(D)) + (qi * NG + L / 4) * 4;
-    if (whole) {
-      *(u32x4_t*)sp = (u32x4_t){sm[0], sm[1], sm[2], sm[3]};
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (ok[i]) sp[i] = sm[i];
-    }
-  }
+  if (j == 0 ? ok[0] : j == 1 ? ok[1] : j == 2 ? ok[2] : ok[3])
+    *((uint32_t*)(tile + kv4_scales_at(D)) + (qi * NG + L / 4) * 4 + j) = g.pair;
 }
 
 // One workgroup per tile of source tokens and head; NW waves, 64 tokens each.
@@ -299,8 +318,9 @@ __global__ __launch_bounds__(NW * 64) void kv4_append_kernel(AppendArgs a) {
 
   const int32_t* bt_row = a.pg.bt + (int64_t)b * a.pg.bt_sb + (int64_t)h * a.pg.bt_sh;
   const int L = tid % LPR, slot = tid / LPR;
-  const int64_t kb = (int64_t)b * a.s_b[0] + (int64_t)h * a.s_h[0] + L * 8;
-  const int64_t vb = (int64_t)b * a.s_b[1] + (int64_t)h * a.s_h[1] + L * 8;
+  const int64_t kb = (int64_t)b * a.s_b[0] + (int64_t)h * a.s_h[0] + (int64_t)t0 * a.s_t[0] + L * 8;
+  const int64_t vb = (int64_t)b * a.s_b[1] + (int64_t)h * a.s_h[1] + (int64_t)t0 * a.s_t[1] + L * 8;
+  const uint32_t kst = (uint32_t)a.s_t[0], vst = (uint32_t)a.s_t[1];  // below 2^32 (the host's check)
   const int q0 = p0 >> 2, nq = p1 > p0 ? ((p1 - 1) >> 2) - q0 + 1 : 0;
   // A step takes keys and values of a quad per group of lanes, their eight
   // rows and the page id asked for together.  Few quads (a decode step) give
@@ -316,9 +336,9 @@ __global__ __launch_bounds__(NW * 64) void kv4_append_kernel(AppendArgs a) {
     for (int i = 0; i < 4; ++i) {
       const int p = quad * 4 + i;
       ok[i] = p >= p0 && p < p1;
-      const int64_t src = t0 + s_src[min(max(p - p0, 0), n_adm - 1)];
-      if (do_k) kv4_fetch<TY>(a.src[0], kb + src * a.s_t[0], kr[i]);
-      if (do_v) kv4_fetch<TY>(a.src[1], vb + src * a.s_t[1], vr[i]);
+      const uint32_t src = s_src[min(max(p - p0, 0), n_adm - 1)];
+      if (do_k) kv4_fetch<TY>(a.src[0], kb + (int64_t)((uint64_t)src * kst), kr[i]);
+      if (do_v) kv4_fetch<TY>(a.src[1], vb + (int64_t)((uint64_t)src * vst), vr[i]);
     }
     const int64_t at = kv4_tile_at<D>(a.pg, bt_row, quad >> 2);
     if (at < 0) {
@@ -469,6 +489,7 @@ extern "C" int wgkv_kv4_append(
   const int64_t unit = dtype == kKv4F32 ? 3 : 7;
   if (((uintptr_t)key | (uintptr_t)value | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return WGKV_ERR_UNSUPPORTED;
   if ((k_stride_b | k_stride_t | k_stride_h | v_stride_b | v_stride_t | v_stride_h) & unit) return WGKV_ERR_UNSUPPORTED;
+  if (((uint64_t)k_stride_t | (uint64_t)v_stride_t) >> 32) return WGKV_ERR_UNSUPPORTED;
   a.src[0] = key;
   a.src[1] = value;
   a.s_b[0] = k_stride_b, a.s_t[0] = k_stride_t, a.s_h[0] = k_stride_h;
