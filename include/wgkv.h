@@ -634,11 +634,12 @@ int wgkv_rope_qkv_norm_ring_write(const void* q, int64_t q_sh, const void* k, in
  *   both rounded to fp32 first;
  *   c = round((x - m)/s + 7.5) clamped to 0..15, ties to even; a group that
  *   holds a NaN or an infinity gets s = m = NaN.
- * new_lengths (B, H) receives the lengths after the call and may be lengths.
+ * new_lengths (B, H) receives the lengths after the call; it may be lengths
+ * and shares no entry with it otherwise.
  * Positions beyond max_pages*page_size and pages outside the pool are not
  * written; *status (or NULL) is then raised to WGKV_ERR_CAPACITY.  B*H <=
- * 65535.  Two launches for T > 64 (workspace as sized, else 0 bytes), else
- * one.
+ * 65535.  One launch; T > 256 needs a workspace (as sized, any contents), and
+ * takes a second launch in place or for a mask of more than 16384 tokens.
  *
  * wgkv_kv4_read writes rows i < rows of each head to key/value (B, rows, H,
  * D; shared element strides, aligned as above): position starts[b,h] + i

@@ -629,3 +629,151 @@ def test_attend_page_windows(units):
     spread = (g - (g.amax(-1, keepdim=True) + g.amin(-1, keepdim=True)) / 2).abs().view_as(v)
     bound = 2.0 ** -8 * ((p @ spread).transpose(1, 2) + want.abs()) + 2.8e-4
     assert ((got.cpu().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("T,masked", [(17161, True), (16384, True), (5000, False)])
+def test_append_long_prompts_in_place(T, masked):
+    """Prompts of several counting segments, their lengths written apart and
+    in place; the mask's rows start at any byte."""
+    import wgkv
+    gen = torch.Generator().manual_seed(T)
+    B, H, D, P = 1, 3, 64, 32
+    k, v = rows(gen, B, T, H, D), rows(gen, B, T, H, D)
+    lens = torch.tensor([[5, 0, 77]], dtype=I32)
+    mask = torch.rand(B, H, T, generator=gen) < 0.05 if masked else None
+    if masked:
+        mask[0, 1, 4090:12300] = False
+        mask[0, 2, T - 300:] = True
+    dk, dv, bt, new = check_append(k, v, lens, mask, P, D, seed=3)
+    b = [t.to(DEV) for t in pool(dk.shape[0], P, D)]
+    sl = lens.to(DEV)
+    wgkv.kv4_append(k.to(DEV), v.to(DEV), *b, bt.to(DEV), sl, g_mask=None if mask is None else mask.to(DEV), out=sl)
+    assert torch.equal(sl, new) and torch.equal(b[0], dk) and torch.equal(b[1], dv)
+
+
+def test_append_lengths_beside_each_other():
+    """Lengths read from one half of an array and written to the other, and
+    lengths of one row for every sequence."""
+    import wgkv
+    gen = torch.Generator().manual_seed(103)
+    k, v = rows(gen, 2, 300, 3, 64).to(DEV), rows(gen, 2, 300, 3, 64).to(DEV)
+    lens = torch.tensor([[4, 0, 19]], dtype=I32).expand(2, 3)
+    bt, total = table_for(lens + 300, 16, gen)
+    both = torch.cat([lens, torch.full_like(lens, -7)], 1).to(DEV)
+    a, b = [[t.to(DEV) for t in pool(total, 16, 64)] for _ in range(2)]
+    wgkv.kv4_append(k, v, *a, bt.to(DEV), both[:, :3], out=both[:, 3:])
+    new = wgkv.kv4_append(k, v, *b, bt.to(DEV), lens[:1].to(DEV).expand(2, 3))
+    assert torch.equal(both[:, :3].cpu(), lens) and torch.equal(both[:, 3:], new) and torch.equal(new.cpu(), lens + 300)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_overlapping_outputs_are_refused():
+    import wgkv
+    from wgkv import _lib
+    gen = torch.Generator().manual_seed(105)
+    lens = torch.tensor([[20, 3], [0, 9]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, 16, 64)
+    dk, dv, tb = torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV), bt.to(DEV)
+    k = rows(gen, 2, 4, 2, 64).to(DEV)
+    buf = torch.zeros(3, 2, dtype=I32, device=DEV)
+    for sl, out in [(buf[:2], buf[1:]), (buf[1:], buf[:2]), (buf[:2], torch.zeros(1, 2, dtype=I32, device=DEV).expand(2, 2))]:
+        with pytest.raises(_lib.WGKVError):
+            wgkv.kv4_append(k, k.clone(), dk, dv, tb, sl, out=out)
+    sl = lens.to(DEV)
+    q = torch.zeros(2, 1, 4, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(_lib.WGKVError):
+        wgkv.paged_decode_attn_kv4(q, dk, dv, sl, tb, 0.1, out=q[:1].expand(2, 1, 4, 64))
+    one = torch.zeros(2, 2, 1, 8, 64, dtype=torch.bfloat16, device=DEV)
+    with pytest.raises(_lib.WGKVError):
+        wgkv.kv4_read(dk, dv, tb, sl, 8, out=tuple(one.transpose(2, 3).expand(2, 2, 8, 2, 64)))
+    assert torch.equal(dk.cpu(), torch.from_numpy(kc)) and not buf.any()
+
+
+def test_captured_prompt_append():
+    """A gated prompt's append of two launches, its scratch the graph's."""
+    import wgkv
+    gen = torch.Generator().manual_seed(107)
+    B, T, H, D, P = 1, 16500, 2, 64, 32
+    k, v = rows(gen, B, T, H, D).to(DEV), rows(gen, B, T, H, D).to(DEV)
+    masks = [(torch.rand(B, H, T, generator=gen) < p).to(torch.uint8).to(DEV) for p in (0.02, 0.3, 0.1)]
+    lens = torch.tensor([[9, 100]], dtype=I32, device=DEV)
+    bt, total = table_for(torch.full((B, H), 3 * T), P, gen)
+    tb = bt.to(DEV)
+    ea, ga = ([t.to(DEV) for t in pool(total, P, D)] + [lens.clone()] for _ in range(2))
+    m = masks[0].clone()
+
+    def step(st, mask):
+        wgkv.kv4_append(k, v, st[0], st[1], tb, st[2], g_mask=mask, out=st[2])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step([t.clone() for t in ga], m)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step(ga, m)
+    for mask in masks:
+        step(ea, mask)
+        m.copy_(mask)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(ea, ga))
+
+
+@pytest.mark.parametrize("B,H,G,D", [(3, 30, 8, 128), (7, 11, 5, 128), (9, 13, 3, 64)])
+def test_attend_many_heads_of_wide_groups(B, H, G, D):
+    gen = torch.Generator().manual_seed(B * G)
+    ln = torch.randint(0, 90, (B, H), generator=gen, dtype=I32)
+    ln[0, 0], ln[B - 1, H - 1], ln[1, 2] = 0, 2100, 900
+    kc, vc, bt = device_cache(ln, 32, D, seed=B + H)
+    q = torch.randn(B, 1, H * G, D, generator=gen).to(torch.bfloat16)
+    check_attend(q, kc.cpu().numpy(), vc.cpu().numpy(), bt, ln, D ** -0.5)
+
+
+def test_attend_nothing_anywhere():
+    """No head has a token: zeros, whatever the pages and the table hold."""
+    import wgkv
+    for B, H, G, D in [(1, 1, 1, 64), (2, 3, 8, 128), (40, 5, 2, 64)]:
+        kc, vc = (t.to(DEV) for t in pool(2, 16, D))
+        bt = torch.full((B, H, 1), -1, dtype=I32, device=DEV)
+        q = torch.full((B, 1, H * G, D), float("nan"), dtype=torch.bfloat16, device=DEV)
+        out = torch.full_like(q, 3.0)
+        for n in (0, -5):
+            sl = torch.full((B, H), n, dtype=I32, device=DEV)
+            assert not wgkv.paged_decode_attn_kv4(q, kc, vc, sl, bt, 0.1, out=out).any()
+
+
+def test_attend_nan_in_a_query_stays_there():
+    import wgkv
+    gen = torch.Generator().manual_seed(109)
+    lens = torch.tensor([[700, 33]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, 16, 128)
+    args = (torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV), lens.to(DEV), bt.to(DEV), 0.09)
+    for G in (4, 7):
+        q = torch.randn(1, 1, 2 * G, 128, generator=gen).to(torch.bfloat16).to(DEV)
+        want, bound = ok.attend(q[:, 0].double().cpu().numpy(), kc, vc, bt.numpy(), lens.numpy(), 0.09)
+        for bad in (0, G + 2):
+            x = q.clone()
+            x[0, 0, bad, 77] = float("nan")
+            got = wgkv.paged_decode_attn_kv4(x, *args)[:, 0].double().cpu().numpy()
+            keep = [i for i in range(2 * G) if i != bad]
+            assert (np.abs(got - want) <= bound)[:, keep].all() and np.isnan(got[:, bad]).all()
+
+
+def test_attend_scales_with_its_values():
+    """Steps and middles of the values times a power of two: the output times
+    the same, to the last bit (nothing under- or overflows on the way)."""
+    import wgkv
+    gen = torch.Generator().manual_seed(111)
+    lens = torch.tensor([[1500, 70]], dtype=I32)
+    P, D = 16, 64
+    kc, vc, bt = random_cache(gen, lens, P, D)
+    q = (torch.randn(1, 1, 8, D, generator=gen) * 0.5).to(torch.bfloat16).to(DEV)
+    sl, tb, dk = lens.to(DEV), bt.to(DEV), torch.from_numpy(kc).to(DEV)
+    ref = wgkv.paged_decode_attn_kv4(q, dk, torch.from_numpy(vc).to(DEV), sl, tb, 0.125)
+    for e in (96, -60):
+        x = torch.from_numpy(vc.copy())
+        pairs = x[..., 8 * D:].contiguous().view(torch.bfloat16)
+        x[..., 8 * D:] = (pairs.float() * 2.0 ** e).to(torch.bfloat16).view(torch.uint8)
+        got = wgkv.paged_decode_attn_kv4(q, dk, x.to(DEV), sl, tb, 0.125)
+        assert torch.equal(got.float(), ref.float() * 2.0 ** e)

@@ -180,3 +180,41 @@ def test_argument_blocks_are_the_calls_arguments():
     assert L.wgkv_kv4_read_block(kv4._pack_read(*words)) == _lib.ERR_UNSUPPORTED
     words = [x, 64, 64, x, x, 4, 16, x, 1, x, 4, 4, 4, x, 64, 64, 1, 4, 1, 64, 0.125, x, 8, 0]
     assert L.wgkv_kv4_decode_attn_block(kv4._pack_attn(*words)) == _lib.ERR_WORKSPACE
+
+
+def test_outputs_that_overlap_are_refused():
+    """Lengths written in place or apart from those read, rows written once;
+    what passes these checks fails on the missing workspace."""
+    import wgkv
+    from wgkv import _lib
+    L = _lib.lib()
+    x = 1 << 20
+
+    def append(new, new_sb, B=3, H=4, len_sb=4):
+        return L.wgkv_kv4_append(x, 64, 64, 64, x, 64, 64, 64, 0, None, 0, 0, x, len_sb, new, new_sb, x, x, 4, 16,
+                                 x, 4, 4, 4, B, 257, H, 64, None, None, 0, None)
+    for good in [dict(new=x, new_sb=4), dict(new=x + 48, new_sb=4), dict(new=x - 48, new_sb=4),
+                 dict(new=x, new_sb=9, B=1),
+                 dict(new=x + 16, new_sb=8, len_sb=8), dict(new=x - 16, new_sb=8, len_sb=8),  # slices of one array
+                 dict(new=x + 48, new_sb=8, len_sb=8), dict(new=x + 48, new_sb=4, len_sb=0)]:
+        assert append(**good) == _lib.ERR_WORKSPACE, good
+    for bad in [dict(new=x + 4, new_sb=4), dict(new=x - 44, new_sb=4), dict(new=x + 44, new_sb=4),
+                dict(new=x, new_sb=8), dict(new=x + 12, new_sb=8, len_sb=8), dict(new=x - 12, new_sb=8, len_sb=8),
+                dict(new=x + 64, new_sb=0), dict(new=x + 4, new_sb=4, B=1), dict(new=x + 64, new_sb=3),
+                dict(new=x + 8, new_sb=4, len_sb=0)]:
+        assert append(**bad) == _lib.ERR_ARG, bad
+
+    def read(sb=4096, st=128, sh=64, key=x, value=2 * x, B=2, H=2):
+        return L.wgkv_kv4_read(x, x, 4, 16, x, 4, 4, 4, x, 2, None, 0, key, value, sb, st, sh, 0, B, 8, H, 64, None)
+    for bad in [dict(sb=0), dict(st=0), dict(sh=0), dict(value=x)]:
+        assert read(**bad) == _lib.ERR_ARG, bad
+
+    def attend(sb, sh, B=2, Hq=4):
+        return L.wgkv_kv4_decode_attn(x, 256, 64, x, x, 4, 16, x, 4, x, 4, 4, 4, 2 * x, sb, sh, B, Hq, 1, 64, 0.1,
+                                      None, 0, None)
+    assert attend(256, 64) == attend(0, 64, B=1) == attend(64, 0, Hq=1) == _lib.ERR_WORKSPACE
+    assert attend(0, 64) == attend(256, 0) == _lib.ERR_ARG
+    _, _, kc, vc, bt, sl = _args()
+    out = torch.zeros(2, 4, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises((AssertionError, ValueError)):
+        wgkv.kv4_read(kc, vc, bt, sl, 4, out=(out, out))

@@ -644,7 +644,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     __syncthreads();
-    if (threadIdx.x < n_open) {
+    if ((int)threadIdx.x < n_open) {
       const int t = threadIdx.x;
       const int bh = t ? open_bh[1] : open_bh[0], others = t ? open_e[1] - open_f[1] : open_e[0] - open_f[0];
       const int prev = __hip_atomic_fetch_add(&a.counter[bh], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -717,6 +717,7 @@ extern "C" int wgkv_kv4_decode_attn(
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return WGKV_ERR_UNSUPPORTED;
   if ((q_stride_b | q_stride_h) & 7) return WGKV_ERR_UNSUPPORTED;
   if (((uintptr_t)out & 15) || ((out_stride_b | out_stride_h) & 7)) return WGKV_ERR_UNSUPPORTED;
+  if ((batch > 1 && !out_stride_b) || (num_q_heads > 1 && !out_stride_h)) return WGKV_ERR_ARG;  // rows written twice
   if (!workspace || ((uintptr_t)workspace & 15) ||
       workspace_bytes < wgkv_kv4_decode_workspace_bytes(num_q_heads, num_kv_heads, head_dim))
     return WGKV_ERR_WORKSPACE;

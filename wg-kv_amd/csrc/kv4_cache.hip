@@ -465,6 +465,16 @@ int segments_of(int T) { return (T + kSegment - 1) / kSegment; }
 
 constexpr int kMaxBH = 65535;  // grid y
 
+// Whether two arrays (B, H) with these row strides may share an entry: exact
+// for slices of one array, else by their extents.
+bool may_meet(const int32_t* x, int64_t sx, const int32_t* y, int64_t sy, int B, int H) {
+  const int64_t d = ((intptr_t)y - (intptr_t)x) / (int64_t)sizeof(int32_t);
+  if (d >= (B - 1) * sx + H || -d >= (B - 1) * sy + H) return false;
+  if (B == 1 || sx != sy || sx <= 0) return true;
+  const int64_t r = (d % sx + sx) % sx;
+  return r < H || sx - r < H;
+}
+
 }  // namespace
 
 extern "C" size_t wgkv_kv4_append_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t tokens) {
@@ -486,6 +496,11 @@ extern "C" int wgkv_kv4_append(
   if (head_dim != 64 && head_dim != 128) return WGKV_ERR_UNSUPPORTED;
   if (dtype != kKv4Bf16 && dtype != kKv4F32 && dtype != kKv4F16) return WGKV_ERR_UNSUPPORTED;
   if ((int64_t)batch * num_kv_heads > kMaxBH || tokens > (1 << 30)) return WGKV_ERR_UNSUPPORTED;
+  // Workgroups read a head's length and write another's new one: the same
+  // array, or none of its entries.
+  const bool in_place = new_lengths == lengths && (batch == 1 || new_stride_b == len_stride_b);
+  if (batch > 1 && new_stride_b < num_kv_heads) return WGKV_ERR_ARG;
+  if (!in_place && may_meet(lengths, len_stride_b, new_lengths, new_stride_b, batch, num_kv_heads)) return WGKV_ERR_ARG;
   AppendArgs a{};
   const int st = kv4_pages(&a.pg, num_pages, page_size, block_table, bt_stride_b, bt_stride_h, max_pages);
   if (st != WGKV_OK) return st;
@@ -518,12 +533,9 @@ extern "C" int wgkv_kv4_append(
     if (!workspace || ((uintptr_t)workspace & 3) ||
         workspace_bytes < wgkv_kv4_append_workspace_bytes(batch, num_kv_heads, tokens))
       return WGKV_ERR_WORKSPACE;
-    // Several workgroups read a head's length and one writes the new one: if
-    // that may be the same memory, the lengths are copied first too.
-    const int32_t* len_end = lengths + (batch - 1) * len_stride_b + num_kv_heads;
-    const int32_t* new_end = new_lengths + (batch - 1) * new_stride_b + num_kv_heads;
-    const bool apart = (uintptr_t)len_end <= (uintptr_t)new_lengths || (uintptr_t)new_end <= (uintptr_t)lengths;
-    if (!apart || (g_mask && tokens > kCountsItself)) {
+    // Several workgroups read a head's length and one writes the new one: in
+    // place, the lengths are copied first too.
+    if (in_place || (g_mask && tokens > kCountsItself)) {
       const int64_t bh = (int64_t)batch * num_kv_heads;
       a.ws_len = (int32_t*)workspace;
       a.ws_seg = a.ws_len + bh;
@@ -554,6 +566,9 @@ extern "C" int wgkv_kv4_read(
   const int64_t unit = dtype == kKv4F32 ? 3 : 7;
   if (((uintptr_t)key | (uintptr_t)value | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return WGKV_ERR_UNSUPPORTED;
   if ((out_stride_b | out_stride_t | out_stride_h) & unit) return WGKV_ERR_UNSUPPORTED;
+  // rows that are written more than once
+  if ((batch > 1 && !out_stride_b) || (rows > 1 && !out_stride_t) || (num_kv_heads > 1 && !out_stride_h) || key == value)
+    return WGKV_ERR_ARG;
   a.cache[0] = (const uint8_t*)k_cache;
   a.cache[1] = (const uint8_t*)v_cache;
   a.len = lengths;

@@ -18,7 +18,9 @@ Page tables, lengths and heads are those of ``paged_decode_attn``: per
 (sequence, KV head) a row of page ids ``block_table[b, h]`` and a length.
 The operators run on torch's current stream of the tensors' device, allocate
 only their outputs and scratch (both through torch, so a call can be captured
-in a HIP graph) and never synchronise with the host.
+in a HIP graph) and never synchronise with the host.  A tensor they write must
+not overlap itself (an expanded one) or, but for kv4_append's lengths in place,
+one they read.
 """
 import struct
 
@@ -122,7 +124,7 @@ def kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask=None, out=No
     ``g_mask`` (B, Hkv, T) nonzero -- all without it -- go, in order, to
     positions lengths[b, h], lengths[b, h] + 1, ... of their head, whose page
     ``p // block_size`` is ``block_table[b, h, p // block_size]``: pages are
-    the caller's to provide and must not be shared between heads.  Tokens the
+    the caller's to provide, and those written must stand in the table once.  Tokens the
     mask leaves out are not read into the cache whatever they hold (padding,
     NaN), and bytes of other tokens are left as they were.
 
@@ -223,6 +225,8 @@ def kv4_read(k_cache, v_cache, block_table, lengths, rows, starts=None, dtype=to
         kp, vp = ko.data_ptr(), vo.data_ptr()
     else:
         ko, vo = out
+        if ko is vo:
+            raise AssertionError("out must be two tensors")
         if ko.shape != (B, rows, H, D) or vo.shape != ko.shape or ko.dtype != dtype or vo.dtype != dtype:
             raise AssertionError("out must be two (batch, rows, num_kv_heads, head_dim) tensors of dtype")
         if ko.get_device() != dev or vo.get_device() != dev:
@@ -269,9 +273,11 @@ def _attn_workspace(dev, stream, nbytes):
 def paged_decode_attn_kv4(q, k_cache, v_cache, cache_seqlens, block_table, softmax_scale, out=None):
     """``paged_decode_attn`` over a 4-bit cache: q (B, 1, Hq, D) bf16 attends
     to the first cache_seqlens[b, h] tokens of its KV head; returns (B, 1, Hq,
-    D) bf16, zeros for a head without tokens.  The probabilities are rounded
-    to bf16 for their product with the values; sums are fp32.  Lengths and
-    page ids out of range are clamped to the table and the pool."""
+    D) bf16, zeros for a head without tokens.  Hq / Hkv may be up to 8, B * Hkv
+    up to 2048.  The probabilities are rounded to bf16 for their product with
+    the values; sums are fp32, before their division by the probabilities' sum
+    (so values beyond 2^100 may overflow to NaN).  Lengths and page ids out of
+    range are clamped to the table and the pool."""
     num_blocks, P, D = _check_cache(k_cache, v_cache)
     shape = q.shape
     if len(shape) != 4 or shape[1] != 1 or shape[3] != D:
