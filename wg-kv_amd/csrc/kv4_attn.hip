@@ -68,7 +68,9 @@ struct AttnArgs {
   uint16_t* out;
   int64_t out_sb, out_sh;
   int B, Hkv, G;
+  int g_shift;        // G <= 1 << g_shift
   int cap;            // tokens a head's table row has pages for
+  uint32_t waves_inv; // ceil(2^32 / waves of the launch)
   uint32_t hkv_inv;   // ceil(2^32 / Hkv), 0 for 1: see sequence_of
   float scale_log2;         // |softmax_scale| * log2(e)
   uint32_t q_and, q_xor;    // its sign (and a scale of 0) is put into the queries
@@ -206,66 +208,71 @@ WGKV_DEVICE float piece_weight(float m, float M) { return m == -INFINITY ? 1.f :
 // pieces' loads in flight, and the groups meet in LDS (kThreads * 6 floats).
 template <int D, int kThreads>
 WGKV_DEVICE void merge_pieces(const AttnArgs& a, int f, int e, int b, int h, float* lds) {
-  constexpr int kBatch = 4;
-  const int G = a.G, NQ = G * (D / 4);
-  static_assert(kThreads * 4 >= kMaxG * D, "a thread for every four d");
-  const int groups = kThreads / NQ;
+  constexpr int kBatch = 4, kRow = D / 4;  // threads of a row
+  const int G = a.G;
+  static_assert(kThreads >= kMaxG * kRow, "a thread for every four d");
+  const int t = threadIdx.x, d = t % kRow * 4;
+  const int i = t / kRow & ((1 << a.g_shift) - 1), grp = t / kRow >> a.g_shift;
+  const int groups = kThreads / kRow >> a.g_shift;
   float* s_m = lds;
   float* s_l = lds + kThreads;
   f32x4_t* s_a = (f32x4_t*)(lds + 2 * kThreads);
-  const int t = threadIdx.x;
   const __amdgpu_buffer_rsrc_t acc = __builtin_amdgcn_make_buffer_rsrc(a.part_acc, (short)0, 0x7fffffff, 0x00020000);
-  const int vq = t % NQ, grp = t / NQ;
-  const int i = vq / (D / 4);
+  const int row = min(i, G - 1);
   float M = -INFINITY, L = 0.f;
   f32x4_t A = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-  if (grp < groups) {
-    for (int x0 = f + grp; x0 <= e; x0 += groups * kBatch) {
-      float m[kBatch], l[kBatch];
-      f32x4_t ac[kBatch];
+#pragma unroll 1
+  for (int x0 = f + grp; x0 <= e; x0 += groups * kBatch) {
+    float m[kBatch], l[kBatch];
+    f32x4_t ac[kBatch];
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int x = min(x0 + k * groups, e);
-        const int s = (2 * x + (x == f ? 1 : 0)) * G;
-        m[k] = load_coherent(&a.part_ml[(s + i) * 2]);
-        l[k] = load_coherent(&a.part_ml[(s + i) * 2 + 1]);
-        ac[k] = load_coherent4(acc, (s * D + vq * 4) * (int)sizeof(float));
-      }
-      float mn = M;
+    for (int k = 0; k < kBatch; ++k) {
+      const int x = min(x0 + k * groups, e);
+      const int s = (2 * x + (x == f ? 1 : 0)) * G + row;
+      m[k] = load_coherent(&a.part_ml[s * 2]);
+      l[k] = load_coherent(&a.part_ml[s * 2 + 1]);
+      ac[k] = load_coherent4(acc, (s * D + d) * (int)sizeof(float));
+    }
+    float mn = M;
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) mn = fmaxf(mn, m[k]);
-      const float sa = piece_weight(M, mn);
-      L *= sa;
-      A *= sa;
-      M = mn;
+    for (int k = 0; k < kBatch; ++k) mn = fmaxf(mn, m[k]);
+    const float sa = piece_weight(M, mn);
+    L *= sa;
+    A *= sa;
+    M = mn;
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        if (x0 + k * groups > e) break;
-        const float sb = piece_weight(m[k], M);
-        L = fmaf(l[k], sb, L);
-        A += ac[k] * sb;
-      }
+    for (int k = 0; k < kBatch; ++k) {
+      if (x0 + k * groups > e) break;
+      const float sb = piece_weight(m[k], M);
+      L = fmaf(l[k], sb, L);
+      A += ac[k] * sb;
     }
   }
   s_m[t] = M;
   s_l[t] = L;
   s_a[t] = A;
   __syncthreads();
-  if (grp == 0) {
-    float mn = M;
-    for (int g = 1; g < groups; ++g) mn = fmaxf(mn, s_m[g * NQ + t]);
-    const float sa = piece_weight(M, mn);
-    L *= sa;
-    A *= sa;
-    for (int g = 1; g < groups; ++g) {
-      const float sb = piece_weight(s_m[g * NQ + t], mn);
-      L = fmaf(s_l[g * NQ + t], sb, L);
-      A += s_a[g * NQ + t] * sb;
+  if (grp == 0 && i < G) {
+#pragma unroll 1
+    for (int x = t + (kRow << a.g_shift); x < kThreads; x += kRow << a.g_shift) {
+      const float mn = fmaxf(M, s_m[x]);
+      const float sa = piece_weight(M, mn), sb = piece_weight(s_m[x], mn);
+      L = fmaf(s_l[x], sb, L * sa);
+      A = A * sa + s_a[x] * sb;
+      M = mn;
     }
-    const float inv = 1.f / L;
-    uint16_t* o = a.out + (int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + (vq * 4) % D;
+    const float inv = __builtin_amdgcn_rcpf(L);
+    uint16_t* o = a.out + (int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + d;
     *(uint64_t*)o = (uint64_t)pack_bf16x2(A[2] * inv, A[3] * inv) << 32 | pack_bf16x2(A[0] * inv, A[1] * inv);
   }
+}
+
+// unit / per, exact: the quotient is a workgroup's index (below 2^9), so that
+// the approximate one is at most 1 off.
+WGKV_DEVICE int owner(int unit, int per) {
+  const int q = (int)((float)unit * __builtin_amdgcn_rcpf((float)per));
+  const int r = unit - q * per;
+  return r < 0 ? q - 1 : r >= per ? q + 1 : q;
 }
 
 // What a wave leaves in LDS of a head that it has not seen whole.
@@ -286,7 +293,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
   __shared__ __attribute__((aligned(16))) float s_acc[2 * NW][NT * HPT][D];
   __shared__ float s_m[2 * NW][NT * HPT], s_l[2 * NW][NT * HPT];
   __shared__ Piece s_piece[2 * NW];
-  __shared__ int s_last[2];
+  __shared__ int s_first[2], s_end[2];
 
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n = lane & 15, quad = lane >> 4;
@@ -304,10 +311,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
   const u32x4_t ones = (u32x4_t){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // bf16 1.0
 
   const Line ln = make_line<kMany>(a, lane);
-  const int cw = max((int)(((unsigned)ln.total + n_wg * NW - 1) / (unsigned)(n_wg * NW)), 1);  // units per wave
-  const int64_t first = (int64_t)(w * NW + wid) * cw;
-  int pos = (int)min(first, (int64_t)ln.total);
-  const int end = (int)min(first + cw, (int64_t)ln.total);
+  // units per wave (the host keeps all of this within 31 bits; the
+  // multiplication may give one more than the division, never less)
+  const int cw = max((int)__umulhi((uint32_t)ln.total + n_wg * NW - 1, a.waves_inv), 1);
+  int pos = min((w * NW + wid) * cw, ln.total);
+  const int end = min(pos + cw, ln.total);
   if (lane < 2) s_piece[2 * wid + lane].bh = -1;
 
   // 32 tokens of a head: two tiles of each cache.  Every line is read whole by
@@ -364,6 +372,16 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     load_half(x, 0);
     __builtin_amdgcn_sched_barrier(0);  // the loads stay in front of the queries' wait
   }
+  // Heads without tokens, while the first tiles are in flight: code after the
+  // last tile is time of its own.
+  for (int bh = w; bh < BH; bh += n_wg) {
+    const int t = kMany ? tokens_of(a, bh) : __builtin_amdgcn_readlane(ln.tokens, bh);
+    if (t != 0) continue;
+    const int b = sequence_of(a, bh), h = bh - b * a.Hkv;
+    for (int v = threadIdx.x; v < G * D; v += kThreads)
+      a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + v / D) * a.out_sh + v % D] = 0;
+  }
+
   while (pos < end) {
     const int b = sequence_of(a, hd.bh), h = hd.bh - b * a.Hkv;
     const int T = hd.tokens, units = units_of(T);
@@ -561,7 +579,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
         for (int i = 0; i < 4; ++i) {
           const int d = MT * (4 * quad + i);
           if (whole) {
-            const float inv = 1.f / l;
+            const float inv = __builtin_amdgcn_rcpf(l);
             uint32_t o[MT / 2];
 #pragma unroll
             for (int j = 0; j < MT / 2; ++j) o[j] = pack_bf16x2(acc[nt][2 * j][i] * inv, acc[nt][2 * j + 1][i] * inv);
@@ -593,7 +611,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
   const int cg = cw * NW;  // units per workgroup
   const Piece mine = s_piece[lane & (2 * NW - 1)];
   uint64_t todo = __builtin_amdgcn_ballot_w64(lane < 2 * NW && mine.bh >= 0);
-  int n_open = 0, open_bh[2], open_f[2], open_e[2];
+  int n_open = 0, open_bh[2], open_start[2], open_units[2];
   while (todo) {
     const int s0 = __builtin_ctzll(todo);
     const int bh = __builtin_amdgcn_readlane(mine.bh, s0);
@@ -601,8 +619,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     const uint64_t run = __builtin_amdgcn_ballot_w64(lane < 2 * NW && mine.bh == bh);
     todo &= ~run;
     const int b = sequence_of(a, bh), h = bh - b * a.Hkv;
-    const int f = (int)((unsigned)start / (unsigned)cg), e = (int)((unsigned)(start + units - 1) / (unsigned)cg);
-    const int64_t to = (int64_t)(2 * w + (f == w ? 1 : 0)) * G;
+    const bool begins = start >= w * cg, whole = begins && start + units <= (w + 1) * cg;
+    const int to = (2 * w + (begins ? 1 : 0)) * G;
     for (int v = threadIdx.x; v < G * D; v += kThreads) {
       const int i = v / D, d = v - i * D;
       float M = -INFINITY, L = 0.f, A = 0.f;
@@ -613,8 +631,8 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
         L = fmaf(s_l[s][i], c, L);
         A = fmaf(s_acc[s][i][d], c, A);
       }
-      if (f == e) {
-        a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + d] = f32_to_bf16(A / L);
+      if (whole) {
+        a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + d] = f32_to_bf16(A * __builtin_amdgcn_rcpf(L));
       } else {
         if (d == 0) {
           store_coherent(&a.part_ml[(to + i) * 2], M);
@@ -623,9 +641,9 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
         store_coherent(&a.part_acc[(to + i) * D + d], A);
       }
     }
-    if (f != e) {
-      if (n_open == 0) open_bh[0] = bh, open_f[0] = f, open_e[0] = e;
-      else open_bh[1] = bh, open_f[1] = f, open_e[1] = e;
+    if (!whole) {
+      if (n_open == 0) open_bh[0] = bh, open_start[0] = start, open_units[0] = units;
+      else open_bh[1] = bh, open_start[1] = start, open_units[1] = units;
       ++n_open;
     }
   }
@@ -646,30 +664,24 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     __syncthreads();
     if ((int)threadIdx.x < n_open) {
       const int t = threadIdx.x;
-      const int bh = t ? open_bh[1] : open_bh[0], others = t ? open_e[1] - open_f[1] : open_e[0] - open_f[0];
+      const int bh = t ? open_bh[1] : open_bh[0], start = t ? open_start[1] : open_start[0];
       const int prev = __hip_atomic_fetch_add(&a.counter[bh], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const int last = prev == others;
+      const int f = owner(start, cg), e = owner(start + (t ? open_units[1] : open_units[0]) - 1, cg);
+      const bool last = prev == e - f;
       if (last) __hip_atomic_store(&a.counter[bh], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      s_last[t] = last;
+      s_first[t] = last ? f : -1;
+      s_end[t] = e;
     }
     __syncthreads();
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
 #pragma unroll 1
     for (int t = 0; t < n_open; ++t) {
-      if (!__builtin_amdgcn_readfirstlane(s_last[t])) continue;
+      const int f = __builtin_amdgcn_readfirstlane(s_first[t]), e = __builtin_amdgcn_readfirstlane(s_end[t]);
+      if (f < 0) continue;
       const int bh = t ? open_bh[1] : open_bh[0], b = sequence_of(a, bh);
       if (t) __syncthreads();  // the first one's LDS
-      merge_pieces<D, kThreads>(a, t ? open_f[1] : open_f[0], t ? open_e[1] : open_e[0], b, bh - b * a.Hkv, &s_acc[0][0][0]);
+      merge_pieces<D, kThreads>(a, f, e, b, bh - b * a.Hkv, &s_acc[0][0][0]);
     }
-  }
-
-  // heads without tokens
-  for (int bh = w; bh < BH; bh += n_wg) {
-    const int t = kMany ? tokens_of(a, bh) : __builtin_amdgcn_readlane(ln.tokens, bh);
-    if (t != 0) continue;
-    const int b = sequence_of(a, bh), h = bh - b * a.Hkv;
-    for (int v = threadIdx.x; v < G * D; v += kThreads)
-      a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + v / D) * a.out_sh + v % D] = 0;
   }
 }
 
@@ -685,8 +697,10 @@ hipError_t launch(const AttnArgs& a, hipStream_t st) {
   const int64_t most = ((kv4_capacity(a.pg) + 63) / 64 * a.B * a.Hkv + NW - 1) / NW;
   const int slots = min(kMaxSlots, cu_count());
   const dim3 grid((unsigned)(most < slots ? most : slots));
-  if (a.B * a.Hkv > 64) hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, true>), grid, dim3(NW * 64), 0, st, a);
-  else hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, false>), grid, dim3(NW * 64), 0, st, a);
+  AttnArgs b = a;
+  b.waves_inv = (uint32_t)((0x100000000ull + grid.x * NW - 1) / (grid.x * NW));
+  if (a.B * a.Hkv > 64) hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, true>), grid, dim3(NW * 64), 0, st, b);
+  else hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, false>), grid, dim3(NW * 64), 0, st, b);
   return hipGetLastError();
 }
 
@@ -713,7 +727,7 @@ extern "C" int wgkv_kv4_decode_attn(
   AttnArgs a{};
   const int st = kv4_pages(&a.pg, num_pages, page_size, block_table, bt_stride_b, bt_stride_h, max_pages);
   if (st != WGKV_OK) return st;
-  if ((kv4_capacity(a.pg) + 63) / 64 * batch * num_kv_heads > 0x7fffffff) return WGKV_ERR_UNSUPPORTED;
+  if ((kv4_capacity(a.pg) + 63) / 64 * batch * num_kv_heads > 0x7f000000) return WGKV_ERR_UNSUPPORTED;
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return WGKV_ERR_UNSUPPORTED;
   if ((q_stride_b | q_stride_h) & 7) return WGKV_ERR_UNSUPPORTED;
   if (((uintptr_t)out & 15) || ((out_stride_b | out_stride_h) & 7)) return WGKV_ERR_UNSUPPORTED;
@@ -734,6 +748,7 @@ extern "C" int wgkv_kv4_decode_attn(
   a.B = batch;
   a.Hkv = num_kv_heads;
   a.G = G;
+  a.g_shift = G <= 1 ? 0 : G <= 2 ? 1 : G <= 4 ? 2 : 3;
   a.cap = (int)kv4_capacity(a.pg);
   a.hkv_inv = num_kv_heads == 1 ? 0u : (uint32_t)((0x100000000ull + num_kv_heads - 1) / num_kv_heads);
   // scores in the order of the products: a negative scale negates the
