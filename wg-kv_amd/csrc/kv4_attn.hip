@@ -106,31 +106,45 @@ WGKV_DEVICE int wave_scan_dpp(int v) {
 }
 
 // The heads' units as a line, seen by one wave: lane j knows the units of
-// heads [j*per, j*per+per).  (The host refuses tables whose units could pass
-// 31 bits.)
+// heads [j*per, j*per+per).  kPer bounds per: 1, 4 (then the lane keeps its
+// heads' tokens) or 32 (then they are read again where they are needed).
+template <int kPer>
 struct Line {
+  static constexpr int kKept = kPer <= 4 ? kPer : 1;
   int per;
-  int tokens;  // of the lane's head (up to 64 heads)
-  int excl;    // units before the lane's heads
+  int tokens[kKept];  // of the lane's heads, 0 past the last one
+  int excl;           // units before the lane's heads
   int total;
 };
 
-// kMany: more than 64 heads.
-template <bool kMany>
-WGKV_DEVICE Line make_line(const AttnArgs& a, int lane) {
+// Tokens of heads first..first+kN-1, their loads in flight together.
+template <int kN>
+WGKV_DEVICE void tokens_of_run(const AttnArgs& a, int first, int n, int (&t)[kN]) {
   const int BH = a.B * a.Hkv;
-  Line ln;
-  ln.per = kMany ? (BH + 63) >> 6 : 1;
-  ln.tokens = 0;
+#pragma unroll
+  for (int k = 0; k < kN; ++k) t[k] = tokens_of(a, min(first + k, BH - 1));
+#pragma unroll
+  for (int k = 0; k < kN; ++k)
+    if (k >= n || first + k >= BH) t[k] = 0;
+}
+
+template <int kPer>
+WGKV_DEVICE Line<kPer> make_line(const AttnArgs& a, int lane) {
+  Line<kPer> ln;
+  ln.per = kPer == 1 ? 1 : (a.B * a.Hkv + 63) >> 6;
   int n = 0;
-  if constexpr (kMany) {
-    for (int i = 0; i < ln.per; ++i) {
-      const int bh = lane * ln.per + i;
-      if (bh < BH) n += units_of(tokens_of(a, bh));
-    }
+  if constexpr (kPer <= 4) {
+    tokens_of_run(a, lane * ln.per, ln.per, ln.tokens);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) n += units_of(ln.tokens[k]);
   } else {
-    if (lane < BH) ln.tokens = tokens_of(a, lane);
-    n = units_of(ln.tokens);
+#pragma unroll 1
+    for (int i = 0; i < ln.per; i += 4) {
+      int t[4];
+      tokens_of_run(a, lane * ln.per + i, ln.per - i, t);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) n += units_of(t[k]);
+    }
   }
   const int incl = wave_scan_dpp(n);
   ln.excl = incl - n;
@@ -144,14 +158,27 @@ struct Head {
   int start;  // its first unit on the line
 };
 
-template <bool kMany>
-WGKV_DEVICE Head find_head(const AttnArgs& a, const Line& ln, int pos, int lane) {
+template <int kPer>
+WGKV_DEVICE Head find_head(const AttnArgs& a, const Line<kPer>& ln, int pos, int lane) {
   Head h;
   // the last lane that starts at or before pos (lanes without units start
   // where the next one does)
   const int o = 63 - __builtin_clzll(__builtin_amdgcn_ballot_w64(ln.excl <= pos));
   const int base = __builtin_amdgcn_readlane(ln.excl, o);
-  if constexpr (kMany) {
+  if constexpr (kPer <= 4) {
+    h.bh = o * ln.per;
+    h.tokens = __builtin_amdgcn_readlane(ln.tokens[0], o);
+    h.start = base;
+#pragma unroll
+    for (int k = 1; k < kPer; ++k) {
+      const int next = h.start + units_of(h.tokens);  // of head o*per + k, where the search has come this far
+      if (h.bh == o * ln.per + k - 1 && pos >= next) {
+        h.bh = o * ln.per + k;
+        h.tokens = __builtin_amdgcn_readlane(ln.tokens[k], o);
+        h.start = next;
+      }
+    }
+  } else {
     const int bh = o * ln.per + lane;
     const bool in = lane < ln.per && bh < a.B * a.Hkv;
     const int t = in ? tokens_of(a, bh) : 0;
@@ -160,10 +187,6 @@ WGKV_DEVICE Head find_head(const AttnArgs& a, const Line& ln, int pos, int lane)
     h.bh = o * ln.per + j;
     h.tokens = __builtin_amdgcn_readlane(t, j);
     h.start = __builtin_amdgcn_readlane(excl, j);
-  } else {
-    h.bh = o;
-    h.tokens = __builtin_amdgcn_readlane(ln.tokens, o);
-    h.start = base;
   }
   return h;
 }
@@ -281,7 +304,7 @@ struct Piece {
   int start, units;  // of the head on the line
 };
 
-template <int D, int NT, int NW, bool kMany>
+template <int D, int NT, int NW, int kPer>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void kv4_attn_kernel(AttnArgs a) {
   constexpr int NG = D / kKv4Group;  // groups
   constexpr int HPT = 16 / NG;       // query heads per 16 columns
@@ -310,7 +333,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
 
   const u32x4_t ones = (u32x4_t){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // bf16 1.0
 
-  const Line ln = make_line<kMany>(a, lane);
+  const Line<kPer> ln = make_line<kPer>(a, lane);
   // units per wave (the host keeps all of this within 31 bits; the
   // multiplication may give one more than the division, never less)
   const int cw = max((int)__umulhi((uint32_t)ln.total + n_wg * NW - 1, a.waves_inv), 1);
@@ -362,7 +385,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
   Half x, y;
   Head hd;
   if (pos < end) {
-    hd = find_head<kMany>(a, ln, pos, lane);
+    hd = find_head<kPer>(a, ln, pos, lane);
     u = base_u = pos - hd.start;
     last_tile = (hd.tokens - 1) >> 4;
     bt_row = table_row(hd.bh);
@@ -375,7 +398,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
   // Heads without tokens, while the first tiles are in flight: code after the
   // last tile is time of its own.
   for (int bh = w; bh < BH; bh += n_wg) {
-    const int t = kMany ? tokens_of(a, bh) : __builtin_amdgcn_readlane(ln.tokens, bh);
+    const int t = kPer > 1 ? tokens_of(a, bh) : __builtin_amdgcn_readlane(ln.tokens[0], bh);
     if (t != 0) continue;
     const int b = sequence_of(a, bh), h = bh - b * a.Hkv;
     for (int v = threadIdx.x; v < G * D; v += kThreads)
@@ -545,7 +568,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
       int pg = 0;
       if (refill) {
         if (cross) {
-          nx = find_head<kMany>(a, ln, pos + cnt, lane);
+          nx = find_head<kPer>(a, ln, pos + cnt, lane);
           load_q(nx.bh);
         }
         const int first_u = cross ? 0 : u0 + it + 1;
@@ -699,8 +722,11 @@ hipError_t launch(const AttnArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)(most < slots ? most : slots));
   AttnArgs b = a;
   b.waves_inv = (uint32_t)((0x100000000ull + grid.x * NW - 1) / (grid.x * NW));
-  if (a.B * a.Hkv > 64) hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, true>), grid, dim3(NW * 64), 0, st, b);
-  else hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, false>), grid, dim3(NW * 64), 0, st, b);
+  const dim3 block(NW * 64);
+  const int heads = a.B * a.Hkv;
+  if (heads <= 64) hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, 1>), grid, block, 0, st, b);
+  else if (heads <= 256) hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, 4>), grid, block, 0, st, b);
+  else hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, 32>), grid, block, 0, st, b);
   return hipGetLastError();
 }
 
