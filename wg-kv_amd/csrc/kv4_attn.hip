@@ -25,9 +25,9 @@
 // pairs of tokens.  Nothing goes through LDS but the merge of the waves.
 //
 // Work split: the heads' sequences, in units of 64 tokens, are one line that
-// is cut into equal ranges, one per wave (so all have the same work whatever
-// the lengths; 8 waves per CU, in one workgroup); a range may end one head
-// and begin another.  Half a unit is worked on while the next half's tiles
+// is cut into ranges that differ by one unit, one per wave (so all have the
+// same work whatever the lengths; 8 waves per CU, in one workgroup); a range
+// may end one head and begin another.  Half a unit is worked on while the next half's tiles
 // are in flight, and what a new head needs is asked for before that.  A head
 // inside one range is written by its wave, one inside a workgroup after its
 // waves' pieces (max, sum, acc) met in LDS; otherwise the workgroups' pieces
@@ -37,9 +37,9 @@
 // Bound by reads where the caches are long: 8 sequences of 128K, 2-60 %
 // admitted (424 MB), 73 us, 5.8 TB/s (loads of this pattern alone 6.3); 8
 // heads of 400K tokens (513 MB) 86 us, 6.0 TB/s, vector instructions half of
-// the time.  Short ones are latency: 8 heads of ~1300 tokens 11.7 us, of
-// which 2.4 pass before the first tile, 2 for a unit, 1.5 in the workgroup's
-// merge and 4.5 between workgroups.
+// the time.  Short ones are latency: 8 heads of ~1300 tokens 12 us in a graph,
+// of which 2.4 pass before the first tile, 2 for a unit, 1.5 in the
+// workgroup's merge and 4.5 between workgroups.
 #include <string.h>
 
 #include "kv4.h"
@@ -53,6 +53,8 @@ constexpr float kRescaleSlack = 8.f;  // log2 units a running maximum may lag th
 constexpr int kMaxBH = 2048;
 constexpr int kMaxG = 8;
 constexpr int kMaxSlots = 512;  // workgroups of a launch
+constexpr int kUnit = 64;        // tokens
+constexpr int kFewest = 4;       // units of a workgroup before more workgroups have none
 constexpr int kFlush = 16;       // units between two corrections of the code offset
 constexpr uint32_t kCodeMask = 0x000f000fu, kCodeBase = 0x43004300u;  // 128 + c
 constexpr float kOffset = 135.5f;                                     // (128 + c) - (c - 7.5)
@@ -70,7 +72,6 @@ struct AttnArgs {
   int B, Hkv, G;
   int g_shift;        // G <= 1 << g_shift
   int cap;            // tokens a head's table row has pages for
-  uint32_t waves_inv; // ceil(2^32 / waves of the launch)
   uint32_t hkv_inv;   // ceil(2^32 / Hkv), 0 for 1: see sequence_of
   float scale_log2;         // |softmax_scale| * log2(e)
   uint32_t q_and, q_xor;    // its sign (and a scale of 0) is put into the queries
@@ -91,7 +92,7 @@ WGKV_DEVICE int tokens_of(const AttnArgs& a, int bh) {
   const int b = sequence_of(a, bh), h = bh - b * a.Hkv;
   return min(max(a.len[(int64_t)b * a.len_sb + h], 0), a.cap);
 }
-WGKV_DEVICE int units_of(int tokens) { return (tokens + 63) >> 6; }
+WGKV_DEVICE int units_of(int tokens) { return (tokens + kUnit - 1) / kUnit; }
 
 // Inclusive prefix sum over the wave in DPP steps (no LDS round trips):
 // row_shr 1, 2, 4, 8 within 16 lanes, then the rows' ends broadcast onwards.
@@ -292,10 +293,35 @@ WGKV_DEVICE void merge_pieces(const AttnArgs& a, int f, int e, int b, int h, flo
 
 // unit / per, exact: the quotient is a workgroup's index (below 2^9), so that
 // the approximate one is at most 1 off.
-WGKV_DEVICE int owner(int unit, int per) {
+WGKV_DEVICE int quotient(int unit, int per) {
   const int q = (int)((float)unit * __builtin_amdgcn_rcpf((float)per));
   const int r = unit - q * per;
   return r < 0 ? q - 1 : r >= per ? q + 1 : q;
+}
+
+// The line cut into ranges that differ by a unit: over the workgroups, the
+// first `more` of which get units + 1, and so again over a workgroup's waves.
+// A unit is 1.7 us of one SIMD's vector instructions, so a line too short for
+// all of them goes to workgroups of a unit per SIMD, not per wave (8 heads of
+// 1300 tokens in a graph: 13.9 -> 12.0 us; units of 32 tokens 11.9, but 73.9
+// -> 77 us at 8 sequences of 128K).
+struct Split {
+  int used, units, more;
+  WGKV_DEVICE int first(int w) const { return min(w, used) * units + min(w, more); }
+  WGKV_DEVICE int owner(int unit) const {  // the workgroup that has a unit
+    const int cut = more * (units + 1);
+    const bool late = unit >= cut;
+    return quotient(late ? unit - cut : unit, late ? units : units + 1) + (late ? more : 0);
+  }
+};
+
+// (The host keeps all of this within 31 bits.)
+WGKV_DEVICE Split make_split(int total, int n_wg) {
+  Split s;
+  s.used = max(min((total + kFewest - 1) / kFewest, n_wg), 1);
+  s.units = (int)((unsigned)total / (unsigned)s.used);
+  s.more = total - s.units * s.used;
+  return s;
 }
 
 // What a wave leaves in LDS of a head that it has not seen whole.
@@ -334,11 +360,10 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
   const u32x4_t ones = (u32x4_t){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};  // bf16 1.0
 
   const Line<kPer> ln = make_line<kPer>(a, lane);
-  // units per wave (the host keeps all of this within 31 bits; the
-  // multiplication may give one more than the division, never less)
-  const int cw = max((int)__umulhi((uint32_t)ln.total + n_wg * NW - 1, a.waves_inv), 1);
-  int pos = min((w * NW + wid) * cw, ln.total);
-  const int end = min(pos + cw, ln.total);
+  const Split sp = make_split(ln.total, n_wg);
+  const int wg_first = sp.first(w), wg_units = sp.first(w + 1) - wg_first;
+  int pos = wg_first + wid * (wg_units / NW) + min(wid, wg_units % NW);
+  const int end = pos + wg_units / NW + (wid < wg_units % NW ? 1 : 0);
   if (lane < 2) s_piece[2 * wid + lane].bh = -1;
 
   // 32 tokens of a head: two tiles of each cache.  Every line is read whole by
@@ -631,7 +656,6 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
   // Waves hold consecutive ranges, so a head's pieces are neighbours in LDS.
   // What the workgroup does not hold whole goes to the workspace: at most the
   // head that it ends and the one that it begins.
-  const int cg = cw * NW;  // units per workgroup
   const Piece mine = s_piece[lane & (2 * NW - 1)];
   uint64_t todo = __builtin_amdgcn_ballot_w64(lane < 2 * NW && mine.bh >= 0);
   int n_open = 0, open_bh[2], open_start[2], open_units[2];
@@ -642,7 +666,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     const uint64_t run = __builtin_amdgcn_ballot_w64(lane < 2 * NW && mine.bh == bh);
     todo &= ~run;
     const int b = sequence_of(a, bh), h = bh - b * a.Hkv;
-    const bool begins = start >= w * cg, whole = begins && start + units <= (w + 1) * cg;
+    const bool begins = start >= wg_first, whole = begins && start + units <= wg_first + wg_units;
     const int to = (2 * w + (begins ? 1 : 0)) * G;
     for (int v = threadIdx.x; v < G * D; v += kThreads) {
       const int i = v / D, d = v - i * D;
@@ -689,7 +713,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
       const int t = threadIdx.x;
       const int bh = t ? open_bh[1] : open_bh[0], start = t ? open_start[1] : open_start[0];
       const int prev = __hip_atomic_fetch_add(&a.counter[bh], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      const int f = owner(start, cg), e = owner(start + (t ? open_units[1] : open_units[0]) - 1, cg);
+      const int f = sp.owner(start), e = sp.owner(start + (t ? open_units[1] : open_units[0]) - 1);
       const bool last = prev == e - f;
       if (last) __hip_atomic_store(&a.counter[bh], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       s_first[t] = last ? f : -1;
@@ -717,16 +741,14 @@ template <int D, int NT>
 hipError_t launch(const AttnArgs& a, hipStream_t st) {
   constexpr int NW = NT == 1 ? 8 : 4;
   // no more workgroups than the tables have units for
-  const int64_t most = ((kv4_capacity(a.pg) + 63) / 64 * a.B * a.Hkv + NW - 1) / NW;
+  const int64_t most = ((kv4_capacity(a.pg) + kUnit - 1) / kUnit * a.B * a.Hkv + kFewest - 1) / kFewest;
   const int slots = min(kMaxSlots, cu_count());
   const dim3 grid((unsigned)(most < slots ? most : slots));
-  AttnArgs b = a;
-  b.waves_inv = (uint32_t)((0x100000000ull + grid.x * NW - 1) / (grid.x * NW));
   const dim3 block(NW * 64);
   const int heads = a.B * a.Hkv;
-  if (heads <= 64) hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, 1>), grid, block, 0, st, b);
-  else if (heads <= 256) hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, 4>), grid, block, 0, st, b);
-  else hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, 32>), grid, block, 0, st, b);
+  if (heads <= 64) hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, 1>), grid, block, 0, st, a);
+  else if (heads <= 256) hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, 4>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((kv4_attn_kernel<D, NT, NW, 32>), grid, block, 0, st, a);
   return hipGetLastError();
 }
 
@@ -753,7 +775,7 @@ extern "C" int wgkv_kv4_decode_attn(
   AttnArgs a{};
   const int st = kv4_pages(&a.pg, num_pages, page_size, block_table, bt_stride_b, bt_stride_h, max_pages);
   if (st != WGKV_OK) return st;
-  if ((kv4_capacity(a.pg) + 63) / 64 * batch * num_kv_heads > 0x7f000000) return WGKV_ERR_UNSUPPORTED;
+  if ((kv4_capacity(a.pg) + kUnit - 1) / kUnit * batch * num_kv_heads > 0x7f000000) return WGKV_ERR_UNSUPPORTED;
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return WGKV_ERR_UNSUPPORTED;
   if ((q_stride_b | q_stride_h) & 7) return WGKV_ERR_UNSUPPORTED;
   if (((uintptr_t)out & 15) || ((out_stride_b | out_stride_h) & 7)) return WGKV_ERR_UNSUPPORTED;
