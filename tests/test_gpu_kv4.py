@@ -777,3 +777,18 @@ def test_attend_scales_with_its_values():
         x[..., 8 * D:] = (pairs.float() * 2.0 ** e).to(torch.bfloat16).view(torch.uint8)
         got = wgkv.paged_decode_attn_kv4(q, dk, x.to(DEV), sl, tb, 0.125)
         assert torch.equal(got.float(), ref.float() * 2.0 ** e)
+
+
+def test_append_borders_of_the_smallest_steps():
+    """The same at the least step, 2^-126, where neighbours of a border lie
+    2^-149 (fp32) and 2^-133 (bf16) from it."""
+    D = 64
+    for s in (2.0 ** -126, 1.5 * 2.0 ** -126):
+        for m in (0.0, 2.0 ** -122):
+            ticks = m + s * np.arange(-7, 8)
+            for dt, least in ((torch.float32, 2.0 ** -149), (torch.bfloat16, 2.0 ** -133)):
+                rows_ = [np.concatenate([[m - 7.5 * s, m + 7.5 * s], ticks + e * least, ticks]) for e in (-1, 0, 1)]
+                x = torch.from_numpy(np.concatenate([*rows_, rows_[0]]).reshape(2, D)).to(dt).view(1, 2, 1, D)
+                want = ok.quantise(x.double().numpy())[1]
+                assert np.isfinite(want).all() and (want > 0).all()
+                check_append(x, -x, torch.zeros(1, 1, dtype=I32), None, 16, D, seed=7)

@@ -126,9 +126,10 @@ WGKV_DEVICE Group group_of(float hi, float lo) {
 }
 
 // The code of x is k + 7.5 rounded to even for x = m + k s, k + 8 beyond it
-// and k + 7 below, for an integer k next to (x - m) / s.  That need not be
-// the nearest, so the quotient may be approximate (v_rcp is good to 2^-23),
-// and the side is decided by the sign of an exact residue:
+// and k + 7 below, for an integer k next to (x - m) / s.  That need not be the
+// nearest, so the quotient may be approximate (v_rcp is good to 2^-23), and
+// the side is decided by the sign of an exact residue (k here is k + 7, and m7
+// its zero):
 //   * 16-bit inputs: x - (m + k s).  The border m + k s is exact in fp32 for
 //     the |k| <= 8 that matter: m has 8 bits and k s 12, m is 0 or at least
 //     2^-13 of the range (a sum of two 11-bit numbers), and s is at least
@@ -138,7 +139,7 @@ WGKV_DEVICE Group group_of(float hi, float lo) {
 //     one ulp of it).
 template <int TY>
 WGKV_DEVICE void exact_codes(const float (&x)[8], float s, float m, float inv, float (&c)[8]) {
-  const float nb = -m * inv;
+  const float nb = fmaf(-m, inv, 7.f), m7 = fmaf(-7.f, s, m);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     float k, r;
@@ -146,13 +147,16 @@ WGKV_DEVICE void exact_codes(const float (&x)[8], float s, float m, float inv, f
       const float d = x[i] - m;
       k = rintf(d * inv);
       const float bb = d - x[i];
-      r = fmaf(-k, s, d) + ((x[i] - (d - bb)) - (m + bb));
+      r = (fmaf(-k, s, d) + ((x[i] - (d - bb)) - (m + bb))) * inv * 0x1p-97f;
+      k += 7.f;
     } else {
       k = rintf(fmaf(x[i], inv, nb));
-      r = x[i] - fmaf(k, s, m);
+      r = x[i] - fmaf(k, s, m7);
     }
-    // 7.25, 7.5 or 7.75 by the residue's sign (one below 2^-148 counts as 0)
-    const float side = __builtin_amdgcn_fmed3f(fmaf(r, 0x1p127f, 7.5f), 7.25f, 7.75f);
+    // 0, 0.5 or 1 by the residue's sign: for 16-bit inputs any (the least is
+    // 2^-133, at steps of 2^-126), for fp32 those above 2^-51 of a step, which
+    // arithmetic in 64 bits tells from a border too.
+    const float side = __builtin_amdgcn_fmed3f(fmaf(r, 0x1p127f, 0.5f), 0.f, 1.f);
     c[i] = rintf(__builtin_amdgcn_fmed3f(k + side, 0.f, 15.f));
   }
 }
