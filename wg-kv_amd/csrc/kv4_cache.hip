@@ -9,9 +9,9 @@
 // whole by neighbouring lanes, and the values' words of a quad are one
 // 16-byte access.  The read-back is bound by its writes (24K rows of 64 heads,
 // 994 MB, 186 us, 5.35 TB/s; a copy reaches 4.9), the append by its rounding
-// (26K admitted rows of a 128K prompt in 8 heads: 48 us, two thirds of it
-// vector instructions, 143 MB moved; 400 instructions less per wave took 6 us
-// off).
+// (26K admitted rows of a 128K prompt in 8 heads: 46 us, two thirds of it
+// vector instructions, 143 MB moved; 460 instructions less per wave took 8 us
+// off; registers for more waves spill: 87 us for both calls instead of 79).
 #include <string.h>
 
 #include "kv4.h"
