@@ -792,3 +792,29 @@ def test_append_borders_of_the_smallest_steps():
                 want = ok.quantise(x.double().numpy())[1]
                 assert np.isfinite(want).all() and (want > 0).all()
                 check_append(x, -x, torch.zeros(1, 1, dtype=I32), None, 16, D, seed=7)
+
+
+@pytest.mark.parametrize("B,H,G,D", [(64, 1, 2, 64), (5, 13, 1, 128), (4, 64, 4, 128), (257, 1, 3, 64), (5, 60, 8, 128)])
+def test_attend_heads_per_lane(B, H, G, D):
+    """64, 65, 256, 257 and 300 heads: 1 to 5 of them per lane of the line,
+    empty ones in all places, a long one among the last."""
+    gen = torch.Generator().manual_seed(B + H)
+    ln = torch.randint(0, 70, (B, H), generator=gen, dtype=I32)
+    ln[torch.rand(B, H, generator=gen) < 0.4] = 0
+    ln.view(-1)[-2] = 1700
+    kc, vc, bt = device_cache(ln, 16, D, seed=B * H)
+    q = torch.randn(B, 1, H * G, D, generator=gen).to(torch.bfloat16)
+    got = check_attend(q, kc.cpu().numpy(), vc.cpu().numpy(), bt, ln, D ** -0.5)
+    assert not got.view(B, H, G * D)[(ln == 0).to(DEV)].any()
+
+
+@pytest.mark.parametrize("extra", [0, 1, 63, 65, 129, 500])
+def test_attend_uneven_ranges(extra):
+    """Lines of a few units more than the workgroups and waves have ranges
+    for: the first ranges are a unit longer than the others."""
+    gen = torch.Generator().manual_seed(extra)
+    units = 1024 + 3 * extra  # 256 workgroups of 4 units, and some
+    ln = torch.tensor([[units * 64 // 4 - 640, units * 64 // 4 + 640 - 63, 70, units * 64 // 2 - 100]], dtype=I32)
+    kc, vc, bt = device_cache(ln, 64, 64, seed=extra)
+    q = torch.randn(1, 1, 8, 64, generator=gen).to(torch.bfloat16)
+    check_attend(q, kc.cpu().numpy(), vc.cpu().numpy(), bt, ln, 0.125)
