@@ -58,15 +58,6 @@ WGKV_DEVICE int64_t kv4_tile_at(const Kv4Pages& p, const int32_t* bt_row, int ti
   return (((int64_t)pg << p.page_shift) + within) * kv4_tile_bytes(D);
 }
 
-// The same with a page id outside the pool clamped to it, so that a corrupt
-// table cannot make the attention read out of bounds.
-template <int D>
-WGKV_DEVICE int64_t kv4_tile_clamped(const Kv4Pages& p, const int32_t* bt_row, int tile) {
-  const int pg = bt_row[tile >> p.page_shift];
-  const int64_t in = pg < 0 ? 0 : pg >= p.num_pages ? p.num_pages - 1 : pg;
-  return ((in << p.page_shift) + (tile & ((1 << p.page_shift) - 1))) * kv4_tile_bytes(D);
-}
-
 inline int kv4_pages(Kv4Pages* p, int64_t num_pages, int32_t page_size, const int32_t* bt, int64_t sb, int64_t sh,
                      int32_t max_pages) {
   if (!bt || num_pages <= 0 || max_pages <= 0) return WGKV_ERR_ARG;
