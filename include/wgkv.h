@@ -35,6 +35,9 @@ int wgkv_version(void);
 /* Human-readable text of a status code (static storage). */
 const char* wgkv_status_string(int status);
 
+/* *id names the graph capture that the stream takes part in; 0 if none. */
+int wgkv_stream_capture_id(void* stream, uint64_t* id);
+
 /* ------------------------------------------------------------------------
  * Ragged paged decode attention over the dual cache.
  *

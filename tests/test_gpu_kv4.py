@@ -818,3 +818,53 @@ def test_attend_uneven_ranges(extra):
     kc, vc, bt = device_cache(ln, 64, 64, seed=extra)
     q = torch.randn(1, 1, 8, 64, generator=gen).to(torch.bfloat16)
     check_attend(q, kc.cpu().numpy(), vc.cpu().numpy(), bt, ln, 0.125)
+
+
+def test_captured_calls_share_one_scratch():
+    """Graphs of several attention calls, on one stream and forked: a capture
+    clears its scratch once per stream, whatever the calls' sizes, and no two
+    captures share it."""
+    import wgkv
+    from wgkv import kv4
+    gen = torch.Generator().manual_seed(121)
+    ln = torch.tensor([[900, 3000, 0, 77]], dtype=I32)
+    kc, vc, bt = device_cache(ln, 16, 128, seed=122)
+    sl, tb = ln.to(DEV), bt.to(DEV)
+    qs = [torch.randn(1, 1, 4 * g, 128, generator=gen).to(torch.bfloat16).to(DEV) for g in (1, 4, 2, 8, 8, 3)]
+    want = [wgkv.paged_decode_attn_kv4(q, kc, vc, sl, tb, 0.09) for q in qs]
+    torch.cuda.synchronize()
+    graphs, seen = [], []
+    fork = torch.cuda.Stream()
+    for forked in (False, True, False):
+        g, outs = torch.cuda.CUDAGraph(), []
+        with torch.cuda.graph(g):
+            main = torch.cuda.current_stream()
+            for i, q in enumerate(qs):
+                if forked and i == 1:
+                    fork.wait_stream(main)
+                    with torch.cuda.stream(fork):
+                        outs.append(wgkv.paged_decode_attn_kv4(q, kc, vc, sl, tb, 0.09))
+                        seen.append(kv4._captured[(0, fork.cuda_stream)])
+                    main.wait_stream(fork)
+                else:
+                    outs.append(wgkv.paged_decode_attn_kv4(q, kc, vc, sl, tb, 0.09))
+                seen.append(kv4._captured[(0, main.cuda_stream)])
+        graphs.append((g, outs))
+    ids = [i for i, _ in seen]
+    assert len(set(ids)) == 3 and 0 not in ids
+    # of the sizes G = 1, 4, 2, 8, 8, 3 only 1, 4 and 8 asked for more
+    assert len({ws.data_ptr() for i, ws in seen if i == ids[0]}) == 3
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(4):
+        for (g, outs), s in zip(graphs, streams):
+            for o in outs:
+                o.fill_(9.0)
+        torch.cuda.synchronize()
+        for (g, outs), s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = wgkv.paged_decode_attn_kv4(qs[1], kc, vc, sl, tb, 0.09)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[1])
+        for _, outs in graphs:
+            assert all(torch.equal(o, w) for o, w in zip(outs, want))

@@ -218,3 +218,8 @@ def test_outputs_that_overlap_are_refused():
     out = torch.zeros(2, 4, 2, 64, dtype=torch.bfloat16)
     with pytest.raises((AssertionError, ValueError)):
         wgkv.kv4_read(kc, vc, bt, sl, 4, out=(out, out))
+
+
+def test_capture_id_needs_somewhere_to_go():
+    from wgkv import _lib
+    assert _lib.lib().wgkv_stream_capture_id(None, None) == _lib.ERR_ARG

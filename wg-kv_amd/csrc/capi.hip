@@ -1,4 +1,4 @@
-// Library-level C entry points: version and status text.
+// Library-level C entry points: version, status text and a stream's capture.
 #include "wgkv_common.h"
 
 extern "C" int wgkv_version(void) { return 1; }
@@ -13,4 +13,13 @@ extern "C" const char* wgkv_status_string(int status) {
     case WGKV_ERR_HIP: return "HIP runtime error";
     default: return "unknown status";
   }
+}
+
+extern "C" int wgkv_stream_capture_id(void* stream, uint64_t* id) {
+  if (!id) return WGKV_ERR_ARG;
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long n = 0;
+  if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &n) != hipSuccess) return WGKV_ERR_HIP;
+  *id = status == hipStreamCaptureStatusActive ? n : 0;
+  return WGKV_OK;
 }

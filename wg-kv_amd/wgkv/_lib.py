@@ -32,6 +32,7 @@ c_size = ctypes.c_size_t
 SIGNATURES = {
     "wgkv_version": (ctypes.c_int, []),
     "wgkv_status_string": (ctypes.c_char_p, [ctypes.c_int]),
+    "wgkv_stream_capture_id": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "wgkv_paged_decode_workspace_bytes": (c_size, [c_i32, c_i32, c_i32]),
     "wgkv_paged_decode_attn": (ctypes.c_int, [
         c_ptr, c_i64, c_i64,
