@@ -641,8 +641,8 @@ int wgkv_rope_qkv_norm_ring_write(const void* q, int64_t q_sh, const void* k, in
  * and shares no entry with it otherwise.
  * Positions beyond max_pages*page_size and pages outside the pool are not
  * written; *status (or NULL) is then raised to WGKV_ERR_CAPACITY.  B*H <=
- * 65535.  One launch; T > 256 needs a workspace (as sized, any contents), and
- * takes a second launch in place or for a mask of more than 16384 tokens.
+ * 65535.  One launch; T > 256 in place, or T > 16384 with a mask, takes a
+ * second one and a workspace (as sized, any contents).
  *
  * wgkv_kv4_read writes rows i < rows of each head to key/value (B, rows, H,
  * D; shared element strides, aligned as above): position starts[b,h] + i

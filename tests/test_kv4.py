@@ -191,8 +191,8 @@ def test_outputs_that_overlap_are_refused():
     x = 1 << 20
 
     def append(new, new_sb, B=3, H=4, len_sb=4):
-        return L.wgkv_kv4_append(x, 64, 64, 64, x, 64, 64, 64, 0, None, 0, 0, x, len_sb, new, new_sb, x, x, 4, 16,
-                                 x, 4, 4, 4, B, 257, H, 64, None, None, 0, None)
+        return L.wgkv_kv4_append(x, 64, 64, 64, x, 64, 64, 64, 0, x, 0, 0, x, len_sb, new, new_sb, x, x, 4, 16,
+                                 x, 4, 4, 4, B, 16385, H, 64, None, None, 0, None)
     for good in [dict(new=x, new_sb=4), dict(new=x + 48, new_sb=4), dict(new=x - 48, new_sb=4),
                  dict(new=x, new_sb=9, B=1),
                  dict(new=x + 16, new_sb=8, len_sb=8), dict(new=x - 16, new_sb=8, len_sb=8),  # slices of one array

@@ -533,20 +533,18 @@ extern "C" int wgkv_kv4_append(
   a.tiles = tiles_of(tokens);
   a.segments = segments_of(tokens);
   hipStream_t s = (hipStream_t)stream;
-  if (a.tiles > 1) {
+  // Several workgroups read a head's length and one writes the new one: in
+  // place, the lengths are copied first too.
+  if (a.tiles > 1 && (in_place || (g_mask && tokens > kCountsItself))) {
     if (!workspace || ((uintptr_t)workspace & 3) ||
         workspace_bytes < wgkv_kv4_append_workspace_bytes(batch, num_kv_heads, tokens))
       return WGKV_ERR_WORKSPACE;
-    // Several workgroups read a head's length and one writes the new one: in
-    // place, the lengths are copied first too.
-    if (in_place || (g_mask && tokens > kCountsItself)) {
-      const int64_t bh = (int64_t)batch * num_kv_heads;
-      a.ws_len = (int32_t*)workspace;
-      a.ws_seg = a.ws_len + bh;
-      a.ws_tile = a.ws_seg + bh * a.segments;
-      hipLaunchKernelGGL(kv4_count_kernel, dim3(a.segments, (unsigned)bh), dim3(256), 0, s, a);
-      if (hipGetLastError() != hipSuccess) return WGKV_ERR_HIP;
-    }
+    const int64_t bh = (int64_t)batch * num_kv_heads;
+    a.ws_len = (int32_t*)workspace;
+    a.ws_seg = a.ws_len + bh;
+    a.ws_tile = a.ws_seg + bh * a.segments;
+    hipLaunchKernelGGL(kv4_count_kernel, dim3(a.segments, (unsigned)bh), dim3(256), 0, s, a);
+    if (hipGetLastError() != hipSuccess) return WGKV_ERR_HIP;
   }
   if (head_dim == 128) launch_append<128>(a, dtype, s);
   else launch_append<64>(a, dtype, s);

@@ -23,6 +23,7 @@ not overlap itself (an expanded one) or, but for kv4_append's lengths in place,
 one they read.
 """
 import ctypes
+import functools
 import struct
 
 import torch
@@ -39,6 +40,7 @@ _pack_append = struct.Struct("32q").pack
 _pack_read = struct.Struct("23q").pack
 _pack_attn = struct.Struct("20qd3q").pack
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 
 
 def kv4_cache_shape(num_blocks, block_size, head_dim):
@@ -118,6 +120,9 @@ def _rows(t, unit, copy=True):
     return t, t.data_ptr(), t.stride()
 
 
+_COUNTS_ITSELF = 16384  # tokens of a mask that the append counts in its own launch
+
+
 def kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask=None, out=None, status=None):
     """Quantise tokens into the heads' pages behind the ones already there.
 
@@ -170,10 +175,13 @@ def kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask=None, out=No
     unit = 4 if code == 1 else 8
     k, kp, ks = _rows(k, unit)
     v, vp, vs = _rows(v, unit)
-    if out is None:
+    given = out is not None
+    if not given:
         out = torch.empty_like(lens, memory_format=torch.contiguous_format)
     L = _lib.lib()
-    nbytes = L.wgkv_kv4_append_workspace_bytes(B, H, T) if T > 256 else 0
+    # a launch before counts the mask, and copies lengths written in place
+    counted = T > 256 and (given or (g_mask is not None and T > _COUNTS_ITSELF))
+    nbytes = L.wgkv_kv4_append_workspace_bytes(B, H, T) if counted else 0
     ws = torch.empty(nbytes, dtype=_U8, device=dev) if nbytes else None
     st = L.wgkv_kv4_append_block(_pack_append(
         kp, ks[0], ks[1], ks[2], vp, vs[0], vs[1], vs[2], code, mp, ms[0], ms[1],
@@ -255,6 +263,11 @@ _workspaces = {}
 _captured = {}
 
 
+@functools.lru_cache(maxsize=None)
+def _attn_bytes(Hq, H, D):
+    return _lib.lib().wgkv_kv4_decode_workspace_bytes(Hq, H, D)
+
+
 def _attn_workspace(dev, stream, nbytes):
     """Scratch of the attention, its arrival counters zero.  One per device
     and stream: calls on a stream run in turn and leave the counters zero, and
@@ -264,7 +277,7 @@ def _attn_workspace(dev, stream, nbytes):
     that a graph holds of a stream run in turn too (32 calls of 8 heads x 1300
     tokens: 9.6 us each, 10.9 with scratch for each), and held here until the
     stream's next capture."""
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         capture = ctypes.c_uint64()
         _lib.check(_lib.lib().wgkv_stream_capture_id(stream, ctypes.byref(capture)), "wgkv_stream_capture_id")
         held, ws = _captured.get((dev, stream), (0, None))
@@ -321,7 +334,7 @@ def paged_decode_attn_kv4(q, k_cache, v_cache, cache_seqlens, block_table, softm
         _, op, os = rows
     L = _lib.lib()
     stream = _stream(dev)
-    ws = _attn_workspace(dev, stream, L.wgkv_kv4_decode_workspace_bytes(Hq, H, D))
+    ws = _attn_workspace(dev, stream, _attn_bytes(Hq, H, D))
     st = L.wgkv_kv4_decode_attn_block(_pack_attn(
         qp, qs[0], qs[2], k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, P, lens.data_ptr(), ls,
         table.data_ptr(), bs[0], bs[1], width, op, os[0], os[2], B, Hq, H, D, softmax_scale, ws.data_ptr(), ws.numel(),
