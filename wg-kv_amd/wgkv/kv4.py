@@ -130,9 +130,9 @@ def kv4_append(k, v, k_cache, v_cache, block_table, lengths, g_mask=None, out=No
     ``g_mask`` (B, Hkv, T) nonzero -- all without it -- go, in order, to
     positions lengths[b, h], lengths[b, h] + 1, ... of their head, whose page
     ``p // block_size`` is ``block_table[b, h, p // block_size]``: pages are
-    the caller's to provide, and those written must stand in the table once.  Tokens the
-    mask leaves out are not read into the cache whatever they hold (padding,
-    NaN), and bytes of other tokens are left as they were.
+    the caller's to provide, and those written must stand in the table once.
+    Tokens the mask leaves out are not read into the cache whatever they hold
+    (padding, NaN), and bytes of other tokens are left as they were.
 
     Returns the new lengths, int32 (B, Hkv): ``out`` where given, which may
     be ``lengths`` itself.  Lengths never exceed max_blocks * block_size: what
