@@ -868,3 +868,47 @@ def test_captured_calls_share_one_scratch():
         assert torch.equal(eager, want[1])
         for _, outs in graphs:
             assert all(torch.equal(o, w) for o, w in zip(outs, want))
+
+
+def minus_infinity_case(D, G, dead, n, seed):
+    """One sequence of two heads whose first ``dead`` tokens (whole pages) have
+    keys that every query of ones scores below the least fp32 number, before
+    ``n`` ordinary ones: (q, kc, vc, table, lens, pages to skip)."""
+    P = 16
+    gen = torch.Generator().manual_seed(seed)
+    lens = torch.tensor([[dead + n, dead + max(n - 30, 0)]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, P, D)
+    for h in range(2):
+        for p in range(dead):  # constant rows: step 0, -1e37 in every place
+            ok.put(kc[int(bt[0, h, p // P]), 0], p % P, np.zeros(D, np.int64), np.zeros(D // 32), ok.bf16(np.full(D // 32, -1e37)), True)
+    q = torch.randn(1, 1, 2 * G, D, generator=gen) * 0.1 + 1
+    return q.to(torch.bfloat16), kc, vc, bt, lens, dead // P
+
+
+@pytest.mark.parametrize("D,G", [(64, 8), (128, 4), (128, 7)])
+@pytest.mark.parametrize("dead,n", [(16, 40), (64, 300), (320, 70), (1600, 33)])
+def test_attend_scores_of_minus_infinity(D, G, dead, n):
+    """Tokens whose score falls below fp32's range weigh nothing, wherever
+    they stand: among a half's others, alone in a wave's range, in a piece."""
+    import wgkv
+    q, kc, vc, bt, lens, skip = minus_infinity_case(D, G, dead, n, seed=D + G + dead)
+    want, bound = ok.attend(q[:, 0].double().numpy(), kc, vc, bt[..., skip:].numpy(), (lens - dead).numpy(), 0.125)
+    dk, dv = torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV)
+    print(f"[kv4 attend -inf] D={D} G={G} dead={dead} n={n}", flush=True)
+    got = wgkv.paged_decode_attn_kv4(q.to(DEV), dk, dv, lens.to(DEV), bt.to(DEV), 0.125)
+    assert (np.abs(got[:, 0].double().cpu().numpy() - want) <= bound).all()
+    # scores that only the scale takes there: -1e37 * sum q is 1000 times too small
+    x = (q.float() / 1000).to(torch.bfloat16)
+    want, bound = ok.attend(x[:, 0].double().numpy(), kc, vc, bt[..., skip:].numpy(), (lens - dead).numpy(), 900.0)
+    got = wgkv.paged_decode_attn_kv4(x.to(DEV), dk, dv, lens.to(DEV), bt.to(DEV), 900.0)
+    assert (np.abs(got[:, 0].double().cpu().numpy() - want) <= bound).all()
+
+
+@pytest.mark.parametrize("dead", [16, 400])
+def test_attend_only_scores_of_minus_infinity(dead):
+    """No token left with any weight: zeros, as of a head without tokens."""
+    import wgkv
+    q, kc, vc, bt, lens, _ = minus_infinity_case(128, 4, dead, 0, seed=dead)
+    got = wgkv.paged_decode_attn_kv4(q.to(DEV), torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV),
+                                     lens.to(DEV), bt.to(DEV), 0.125)
+    assert not got.any()

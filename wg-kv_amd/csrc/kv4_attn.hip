@@ -50,6 +50,11 @@ typedef __attribute__((__vector_size__(2 * sizeof(uint32_t)))) uint32_t u32x2_t;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleSlack = 8.f;  // log2 units a running maximum may lag the scores
+// Where a running maximum begins.  Finite: a score of -inf (a finite one may
+// fall there too, by its sum or its scale) then weighs exp2(-inf) = 0 and a
+// piece that saw no other weighs 0 against one that did, without a case of
+// their own; from -inf both would be exp2(-inf + inf), not a number.
+constexpr float kNoMax = -3.402823466e38f;
 constexpr int kMaxBH = 2048;
 constexpr int kMaxG = 8;
 constexpr int kMaxSlots = 512;  // workgroups of a launch
@@ -222,10 +227,13 @@ WGKV_DEVICE void expand(uint32_t w, uint32_t mask, uint32_t base, uint32_t* o) {
   for (int i = 0; i < 4; ++i) o[i] = ((w >> (4 * i)) & mask) | base;
 }
 
-// The weight of a piece with maximum m under the common maximum M.  A piece
-// without a maximum holds either nothing or only NaN scores, which must come
-// through.
-WGKV_DEVICE float piece_weight(float m, float M) { return m == -INFINITY ? 1.f : fast_exp2(m - M); }
+// The weight of a piece with maximum m under the common maximum M >= kNoMax.
+// One without a score above it holds zeros, or a NaN that any weight keeps.
+WGKV_DEVICE float piece_weight(float m, float M) { return fast_exp2(m - M); }
+
+// 1 / sum of the weights.  The sum is 0 where every score is -inf (else one
+// weight is 1): zeros then, as of a head without tokens.
+WGKV_DEVICE float inverse_sum(float l) { return l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l); }
 
 // Merges the pieces that workgroups f..e left of head (b, h) and writes its
 // G rows.  A thread takes four d of a row over every groups-th piece, four
@@ -243,7 +251,7 @@ WGKV_DEVICE void merge_pieces(const AttnArgs& a, int f, int e, int b, int h, flo
   f32x4_t* s_a = (f32x4_t*)(lds + 2 * kThreads);
   const __amdgpu_buffer_rsrc_t acc = __builtin_amdgcn_make_buffer_rsrc(a.part_acc, (short)0, 0x7fffffff, 0x00020000);
   const int row = min(i, G - 1);
-  float M = -INFINITY, L = 0.f;
+  float M = kNoMax, L = 0.f;
   f32x4_t A = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll 1
   for (int x0 = f + grp; x0 <= e; x0 += groups * kBatch) {
@@ -285,7 +293,7 @@ WGKV_DEVICE void merge_pieces(const AttnArgs& a, int f, int e, int b, int h, flo
       A = A * sa + s_a[x] * sb;
       M = mn;
     }
-    const float inv = __builtin_amdgcn_rcpf(L);
+    const float inv = inverse_sum(L);
     uint16_t* o = a.out + (int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + d;
     *(uint64_t*)o = (uint64_t)pack_bf16x2(A[2] * inv, A[3] * inv) << 32 | pack_bf16x2(A[0] * inv, A[1] * inv);
   }
@@ -458,7 +466,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     f32x4_t acc[NT][MT], usum[NT];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m_run[nt] = -INFINITY;
+      m_run[nt] = kNoMax;
       l_run[nt] = corr[nt] = 0.f;
       usum[nt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -530,7 +538,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
         // lanes, whose accumulators hold sums over all of them.
         if (__builtin_amdgcn_ballot_w64(top * a.scale_log2 > m_run[nt] + kRescaleSlack)) {
           const float mn = fmaxf(m_run[nt], rows_max(top) * a.scale_log2);
-          const float alpha = mn == -INFINITY ? 1.f : fast_exp2(m_run[nt] - mn);
+          const float alpha = fast_exp2(m_run[nt] - mn);
           m_run[nt] = mn;
           l_run[nt] *= alpha;
           corr[nt] *= alpha;
@@ -627,7 +635,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
         for (int i = 0; i < 4; ++i) {
           const int d = MT * (4 * quad + i);
           if (whole) {
-            const float inv = __builtin_amdgcn_rcpf(l);
+            const float inv = inverse_sum(l);
             uint32_t o[MT / 2];
 #pragma unroll
             for (int j = 0; j < MT / 2; ++j) o[j] = pack_bf16x2(acc[nt][2 * j][i] * inv, acc[nt][2 * j + 1][i] * inv);
@@ -670,7 +678,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     const int to = (2 * w + (begins ? 1 : 0)) * G;
     for (int v = threadIdx.x; v < G * D; v += kThreads) {
       const int i = v / D, d = v - i * D;
-      float M = -INFINITY, L = 0.f, A = 0.f;
+      float M = kNoMax, L = 0.f, A = 0.f;
       for (uint64_t r = run; r; r &= r - 1) M = fmaxf(M, s_m[__builtin_ctzll(r)][i]);
       for (uint64_t r = run; r; r &= r - 1) {
         const int s = __builtin_ctzll(r);
@@ -679,7 +687,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
         A = fmaf(s_acc[s][i][d], c, A);
       }
       if (whole) {
-        a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + d] = f32_to_bf16(A * __builtin_amdgcn_rcpf(L));
+        a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + d] = f32_to_bf16(A * inverse_sum(L));
       } else {
         if (d == 0) {
           store_coherent(&a.part_ml[(to + i) * 2], M);

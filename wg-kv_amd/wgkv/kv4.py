@@ -299,8 +299,9 @@ def paged_decode_attn_kv4(q, k_cache, v_cache, cache_seqlens, block_table, softm
     D) bf16, zeros for a head without tokens.  Hq / Hkv may be up to 8, B * Hkv
     up to 2048.  The probabilities are rounded to bf16 for their product with
     the values; sums are fp32, before their division by the probabilities' sum
-    (so values beyond 2^100 may overflow to NaN).  Lengths and page ids out of
-    range are clamped to the table and the pool."""
+    (so values beyond 2^100 may overflow to NaN).  Tokens whose score falls
+    below fp32's range weigh nothing, and a head that has no others gives zeros.
+    Lengths and page ids out of range are clamped to the table and the pool."""
     num_blocks, P, D = _check_cache(k_cache, v_cache)
     shape = q.shape
     if len(shape) != 4 or shape[1] != 1 or shape[3] != D:
