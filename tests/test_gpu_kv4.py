@@ -912,3 +912,21 @@ def test_attend_only_scores_of_minus_infinity(dead):
     got = wgkv.paged_decode_attn_kv4(q.to(DEV), torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV),
                                      lens.to(DEV), bt.to(DEV), 0.125)
     assert not got.any()
+
+
+def test_append_middles_of_subnormal_groups():
+    """fp32 groups below 2^-126, whose halves fp32 does not hold: middles next
+    to a border between two bf16 values, and any others."""
+    D, T = 64, 512
+    unit = 2.0 ** -149  # of fp32; a bf16 unit there is 2^16 of them
+    rng = np.random.default_rng(131)
+    mid = rng.integers(1, 120, (1, T, 2, D // 32, 1)) * 2 ** 16 + 2 ** 15
+    odd = np.stack([mid + rng.integers(-2, 3, mid.shape) for _ in range(2)])  # the ends: hi + lo odd in half of them
+    pick = rng.integers(0, 2, (2, 1, T, 2, D // 32, 32))
+    near = np.where(pick == 1, odd[0], odd[1])
+    near[..., :1], near[..., 1:2] = odd[0], odd[1]
+    wide = rng.integers(-2 ** 23 + 1, 2 ** 23, near.shape)
+    for x in (near, wide):
+        k, v = (torch.from_numpy((y * unit).reshape(1, T, 2, D)).float() for y in x)
+        assert np.array_equal(k.double().numpy(), (x[0] * unit).reshape(1, T, 2, D))
+        check_append(k, -v, torch.zeros(1, 2, dtype=I32), None, 16, D, seed=133)

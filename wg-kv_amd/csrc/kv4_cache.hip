@@ -117,7 +117,8 @@ WGKV_DEVICE Group group_of(float hi, float lo) {
   const float sf = (float)(((double)hi - (double)lo) * (1.0 / 15.0));
   Group g;
   g.s = bf16_of(sf);
-  g.m = bf16_of(0.5f * hi + 0.5f * lo);
+  // The sum in 64 bits too: half of an odd fp32 subnormal is not an fp32 number.
+  g.m = bf16_of((float)(((double)hi + (double)lo) * 0.5));
   const bool bad = !(sf < INFINITY) || !(fabsf(g.m) < INFINITY);
   if (!(g.s >= 0x1p-126f) || bad) g.s = 0.f;
   g.inv = __builtin_amdgcn_rcpf(g.s);
