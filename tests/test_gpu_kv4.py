@@ -930,3 +930,17 @@ def test_append_middles_of_subnormal_groups():
         k, v = (torch.from_numpy((y * unit).reshape(1, T, 2, D)).float() for y in x)
         assert np.array_equal(k.double().numpy(), (x[0] * unit).reshape(1, T, 2, D))
         check_append(k, -v, torch.zeros(1, 2, dtype=I32), None, 16, D, seed=133)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_read_of_subnormal_values(dtype):
+    """Middles below 2^-126 and, for fp16, values below 2^-14."""
+    import wgkv
+    gen = torch.Generator().manual_seed(137)
+    x = torch.randn(1, 60, 1, 64, generator=gen)
+    x = x * torch.tensor([2.0 ** -6, 2.0 ** -14, 2.0 ** -20, 2.0 ** -124, 2.0 ** -128, 2.0 ** -133]).repeat(10)[None, :, None, None]
+    lens = torch.zeros(1, 1, dtype=I32)
+    dk, dv, bt, new = check_append(x, -x, lens, None, 16, 64, seed=138)
+    want = oracle_read(dk.cpu().numpy(), dv.cpu().numpy(), bt, new.cpu(), 60, lens)
+    for g, w in zip(wgkv.kv4_read(dk, dv, bt.to(DEV), new, 60, dtype=dtype), want):
+        assert torch.equal(g.cpu(), w.float().to(dtype))
