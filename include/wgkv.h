@@ -639,6 +639,7 @@ int wgkv_rope_qkv_norm_ring_write(const void* q, int64_t q_sh, const void* k, in
  *   holds a NaN or an infinity gets s = m = NaN.
  * new_lengths (B, H) receives the lengths after the call; it may be lengths
  * and shares no entry with it otherwise.
+ * k_cache and v_cache share no byte.
  * Positions beyond max_pages*page_size and pages outside the pool are not
  * written; *status (or NULL) is then raised to WGKV_ERR_CAPACITY.  B*H <=
  * 65535.  One launch; T > 256 in place, or T > 16384 with a mask, takes a

@@ -944,3 +944,24 @@ def test_read_of_subnormal_values(dtype):
     want = oracle_read(dk.cpu().numpy(), dv.cpu().numpy(), bt, new.cpu(), 60, lens)
     for g, w in zip(wgkv.kv4_read(dk, dv, bt.to(DEV), new, 60, dtype=dtype), want):
         assert torch.equal(g.cpu(), w.float().to(dtype))
+
+
+def test_pools_of_one_buffer():
+    """Pools side by side in one buffer are taken; the same pool for both, or
+    pools that share a page, are refused before anything is written."""
+    import wgkv
+    from wgkv import _lib
+    gen = torch.Generator().manual_seed(141)
+    lens = torch.tensor([[5, 17]], dtype=I32)
+    bt, n = table_for(lens + 9, 16, gen)
+    k, v = rows(gen, 1, 9, 2, 64).to(DEV), rows(gen, 1, 9, 2, 64).to(DEV)
+    both = torch.zeros(2 * n, 1, 640, dtype=torch.uint8, device=DEV)
+    args = (bt.to(DEV), lens.to(DEV))
+    for kc, vc in [(both[:n], both[:n]), (both[:n], both[n - 1:-1]), (both[n - 1:-1], both[:n])]:
+        with pytest.raises(_lib.WGKVError):
+            wgkv.kv4_append(k, v, kc, vc, *args)
+    assert not both.any()
+    apart = [torch.zeros(n, 1, 640, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    for kc, vc in [(both[:n], both[n:]), apart]:
+        wgkv.kv4_append(k, v, kc, vc, *args)
+    assert torch.equal(both, torch.cat(apart))

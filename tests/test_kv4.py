@@ -223,3 +223,18 @@ def test_outputs_that_overlap_are_refused():
 def test_capture_id_needs_somewhere_to_go():
     from wgkv import _lib
     assert _lib.lib().wgkv_stream_capture_id(None, None) == _lib.ERR_ARG
+
+
+def test_append_refuses_pools_that_meet():
+    """Keys and values of one page are written by different lanes: two pools
+    that share bytes, wholly or in part, would be left to a race."""
+    from wgkv import _lib
+    L = _lib.lib()
+    x, pages, P, D = 1 << 20, 4, 32, 64
+    size = pages * P // 16 * 10 * D
+
+    def append(kc, vc):
+        return L.wgkv_kv4_append(x, 64, 64, 64, x, 64, 64, 64, 0, None, 0, 0, x, 1, x, 1, kc, vc, pages, P,
+                                 x, 4, 4, 4, 1, 4, 1, D, None, None, 0, None)
+    for kc, vc in [(x, x), (x, x + size - 16), (x + size - 16, x), (x, x + 16)]:
+        assert append(kc, vc) == _lib.ERR_ARG, (kc, vc)

@@ -34,7 +34,7 @@
 constexpr int kKv4Group = 32;
 constexpr int kKv4Tile = 16;
 
-WGKV_DEVICE constexpr int kv4_tile_bytes(int D) { return 10 * D; }
+__host__ __device__ constexpr int kv4_tile_bytes(int D) { return 10 * D; }
 WGKV_DEVICE constexpr int kv4_scales_at(int D) { return 8 * D; }
 
 // A caller's paged 4-bit cache (all entry points share these checks).

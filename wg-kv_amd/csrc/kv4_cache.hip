@@ -533,13 +533,18 @@ extern "C" int wgkv_kv4_append(
   a.status = status;
   a.tiles = tiles_of(tokens);
   a.segments = segments_of(tokens);
-  hipStream_t s = (hipStream_t)stream;
   // Several workgroups read a head's length and one writes the new one: in
   // place, the lengths are copied first too.
-  if (a.tiles > 1 && (in_place || (g_mask && tokens > kCountsItself))) {
-    if (!workspace || ((uintptr_t)workspace & 3) ||
-        workspace_bytes < wgkv_kv4_append_workspace_bytes(batch, num_kv_heads, tokens))
-      return WGKV_ERR_WORKSPACE;
+  const bool counted = a.tiles > 1 && (in_place || (g_mask && tokens > kCountsItself));
+  if (counted && (!workspace || ((uintptr_t)workspace & 3) ||
+                  workspace_bytes < wgkv_kv4_append_workspace_bytes(batch, num_kv_heads, tokens)))
+    return WGKV_ERR_WORKSPACE;
+  // keys and values are written by different lanes
+  const int64_t pool = num_pages * (page_size / kKv4Tile) * kv4_tile_bytes(head_dim);
+  const intptr_t apart = (intptr_t)v_cache - (intptr_t)k_cache;
+  if (apart < pool && -apart < pool) return WGKV_ERR_ARG;
+  hipStream_t s = (hipStream_t)stream;
+  if (counted) {
     const int64_t bh = (int64_t)batch * num_kv_heads;
     a.ws_len = (int32_t*)workspace;
     a.ws_seg = a.ws_len + bh;
