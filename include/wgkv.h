@@ -648,7 +648,8 @@ int wgkv_rope_qkv_norm_ring_write(const void* q, int64_t q_sh, const void* k, in
  * wgkv_kv4_read writes rows i < rows of each head to key/value (B, rows, H,
  * D; shared element strides, aligned as above): position starts[b,h] + i
  * (NULL: 0; negative starts count as 0), zeros from lengths[b,h] on and where
- * the page is outside the pool.
+ * the page is outside the pool.  No two rows written, of key and value
+ * together, share an element; nor do two rows of the attention's out.
  *
  * wgkv_kv4_decode_attn has wgkv_paged_decode_attn's contract over such a
  * cache, in one launch.  Its workspace's first 8192 bytes (per-head arrival

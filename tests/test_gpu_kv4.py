@@ -965,3 +965,41 @@ def test_pools_of_one_buffer():
     for kc, vc in [(both[:n], both[n:]), apart]:
         wgkv.kv4_append(k, v, kc, vc, *args)
     assert torch.equal(both, torch.cat(apart))
+
+
+def test_read_into_rows_of_any_layout():
+    """Random layouts of a pair of outputs in one buffer, rows of both
+    interleaved among others: filled where no two rows meet, else refused."""
+    import wgkv
+    from wgkv import _lib
+    gen = torch.Generator().manual_seed(143)
+    rng = np.random.default_rng(144)
+    lens = torch.tensor([[3, 7], [5, 0], [1, 6]], dtype=I32)
+    kc, vc, bt = random_cache(gen, lens, 16, 64)
+    dk, dv, sl, tb = torch.from_numpy(kc).to(DEV), torch.from_numpy(vc).to(DEV), lens.to(DEV), bt.to(DEV)
+    counts = [0, 0]
+    for i in range(300):
+        B, n, H = int(rng.integers(1, 4)), int(rng.integers(1, 6)), int(rng.integers(1, 3))
+        sizes, strides, step = [2, B, n, H], [0] * 4, 64 + 8 * int(rng.integers(0, 2))
+        for d in rng.permutation(4):  # nested, and in two of three cases one stride changed
+            strides[d] = step
+            step *= sizes[d]
+        if i % 3:
+            strides[int(rng.integers(0, 4))] = 8 * int(rng.integers(0, 8 * (i % 3) * B * n))
+        at = np.add.outer(np.add.outer(np.arange(2) * strides[0], np.arange(B) * strides[1]),
+                          np.add.outer(np.arange(n) * strides[2], np.arange(H) * strides[3])).ravel()
+        meets = bool((np.diff(np.sort(at)) < 64).any())
+        buf = torch.full((int(at.max()) + 64,), 7.0, dtype=torch.float16, device=DEV)
+        out = tuple(torch.as_strided(buf, (B, n, H, 64), (*strides[1:], 1), j * strides[0]) for j in range(2))
+        args = (dk, dv, tb[:B, :H], sl[:B, :H], n)
+        counts[meets] += 1
+        if meets:
+            with pytest.raises(_lib.WGKVError):
+                wgkv.kv4_read(*args, dtype=torch.float16, out=out)
+            assert (buf == 7).all()
+            continue
+        wgkv.kv4_read(*args, dtype=torch.float16, out=out)
+        want = wgkv.kv4_read(*args, dtype=torch.float16)
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), (sizes, strides)
+        assert int((buf == 7).sum()) >= buf.numel() - 64 * len(at)  # nothing between the rows is written
+    assert min(counts) > 60, counts

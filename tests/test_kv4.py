@@ -238,3 +238,33 @@ def test_append_refuses_pools_that_meet():
                                  x, 4, 4, 4, 1, 4, 1, D, None, None, 0, None)
     for kc, vc in [(x, x), (x, x + size - 16), (x + size - 16, x), (x, x + 16)]:
         assert append(kc, vc) == _lib.ERR_ARG, (kc, vc)
+
+
+def test_output_rows_that_meet_are_refused():
+    """Rows of an output may lie anyhow but on each other: in strides smaller
+    than a row, interleaved, keys' rows among values'."""
+    from wgkv import _lib
+    L = _lib.lib()
+    x = 1 << 20
+
+    def read(sb=4096, st=128, sh=64, apart=1 << 20, B=2, H=2):
+        return L.wgkv_kv4_read(x, x, 4, 16, x, 4, 4, 4, x, 2, None, 0, x, x + 2 * apart, sb, st, sh, 0, B, 8, H, 64, None)
+    for bad in [dict(st=120), dict(sh=8), dict(sb=8 * 128 - 64), dict(apart=0), dict(apart=56), dict(apart=-56),
+                dict(apart=64), dict(apart=4096), dict(apart=8 * 128 - 8), dict(sb=256, st=128, sh=64),
+                dict(st=-128, sb=128), dict(sb=1 << 60, st=1 << 61, sh=32)]:
+        assert read(**bad) == _lib.ERR_ARG, bad
+
+    def attend(sb, sh, B, Hq):
+        return L.wgkv_kv4_decode_attn(x, 256, 64, x, x, 4, 16, x, 4, x, 4, 4, 4, 2 * x, sb, sh, B, Hq, 1, 64, 0.1,
+                                      None, 0, None)
+    rng = np.random.default_rng(3)
+    seen = set()
+    for _ in range(2000):
+        B, Hq = int(rng.integers(1, 9)), int(rng.integers(1, 9))
+        sb, sh = (int(rng.integers(0, 9) * rng.choice([8, 64, 128, 192])) for _ in range(2))
+        at = np.sort([b * sb + h * sh for b in range(B) for h in range(Hq)])
+        meets = bool((np.diff(at) < 64).any())
+        nested = all(s >= 64 and (n == 1 or s >= (n - 1) * t + 64) for s, t, n in [sorted([(sb, sh, Hq), (sh, sb, B)])[1]])
+        seen.add((meets, nested))
+        assert attend(sb, sh, B, Hq) == (_lib.ERR_ARG if meets else _lib.ERR_WORKSPACE), (B, Hq, sb, sh)
+    assert seen >= {(True, False), (False, False), (False, True)}

@@ -68,6 +68,61 @@ inline int kv4_pages(Kv4Pages* p, int64_t num_pages, int32_t page_size, const in
   return WGKV_OK;
 }
 
+// Whether two rows of `row` elements, spread over four dimensions of these
+// sizes and strides, share an element (an output's rows are written by
+// workgroups that do not wait for each other).  Layouts whose every stride
+// spans what the smaller ones reach cannot; of others, the differences of two
+// rows' places are gone through in three dimensions and solved for the largest.
+inline bool kv4_rows_meet(const int64_t (&sizes)[4], const int64_t (&strides)[4], int64_t row) {
+  typedef __int128 wide;
+  wide n[4], s[4];
+  int dims = 0;
+  for (int i = 0; i < 4; ++i) {
+    if (sizes[i] <= 1) continue;
+    const wide st = strides[i] < 0 ? -(wide)strides[i] : (wide)strides[i];  // a difference's sign does not matter
+    int j = dims++;
+    for (; j > 0 && s[j - 1] > st; --j) s[j] = s[j - 1], n[j] = n[j - 1];
+    s[j] = st, n[j] = sizes[i];
+  }
+  wide reach = row;
+  bool nested = true;
+  for (int i = 0; i < dims; ++i) {
+    nested = nested && s[i] >= reach;
+    reach += (n[i] - 1) * s[i];
+  }
+  if (nested) return false;
+  int most = 0;
+  for (int i = 1; i < dims; ++i)
+    if (n[i] > n[most]) most = i;
+  const wide step = s[most], far = n[most] - 1;
+  if (step < row) return true;  // neighbours in this dimension
+  wide d[4];
+  for (int i = 0; i < dims; ++i) d[i] = 1 - n[i];
+  for (;;) {
+    wide x = 0;
+    bool same = true;
+    for (int i = 0; i < dims; ++i) {
+      if (i == most) continue;
+      x += d[i] * s[i];
+      same = same && d[i] == 0;
+    }
+    if (!same) {  // the two multiples of `step` next to -x, within reach
+      wide k = -x / step - (-x % step < 0 ? 1 : 0);
+      for (int i = 0; i < 2; ++i, ++k) {
+        const wide c = k < -far ? -far : k > far ? far : k, y = x + c * step;
+        if (y < row && -y < row) return true;
+      }
+    }
+    int i = 0;
+    for (; i < dims; ++i) {
+      if (i == most) continue;
+      if (++d[i] < n[i]) break;
+      d[i] = 1 - n[i];
+    }
+    if (i == dims) return false;
+  }
+}
+
 // ---- element types of the rows quantised or read back -------------------------
 enum Kv4Type { kKv4Bf16 = 0, kKv4F32 = 1, kKv4F16 = 2 };
 

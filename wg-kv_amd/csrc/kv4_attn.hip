@@ -787,7 +787,7 @@ extern "C" int wgkv_kv4_decode_attn(
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return WGKV_ERR_UNSUPPORTED;
   if ((q_stride_b | q_stride_h) & 7) return WGKV_ERR_UNSUPPORTED;
   if (((uintptr_t)out & 15) || ((out_stride_b | out_stride_h) & 7)) return WGKV_ERR_UNSUPPORTED;
-  if ((batch > 1 && !out_stride_b) || (num_q_heads > 1 && !out_stride_h)) return WGKV_ERR_ARG;  // rows written twice
+  if (kv4_rows_meet({batch, num_q_heads, 1, 1}, {out_stride_b, out_stride_h, 0, 0}, head_dim)) return WGKV_ERR_ARG;
   if (!workspace || ((uintptr_t)workspace & 15) ||
       workspace_bytes < wgkv_kv4_decode_workspace_bytes(num_q_heads, num_kv_heads, head_dim))
     return WGKV_ERR_WORKSPACE;

@@ -574,8 +574,9 @@ extern "C" int wgkv_kv4_read(
   const int64_t unit = dtype == kKv4F32 ? 3 : 7;
   if (((uintptr_t)key | (uintptr_t)value | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return WGKV_ERR_UNSUPPORTED;
   if ((out_stride_b | out_stride_t | out_stride_h) & unit) return WGKV_ERR_UNSUPPORTED;
-  // rows that are written more than once
-  if ((batch > 1 && !out_stride_b) || (rows > 1 && !out_stride_t) || (num_kv_heads > 1 && !out_stride_h) || key == value)
+  // (both bases are 16-byte aligned, so they are whole elements apart)
+  const int64_t apart = ((intptr_t)value - (intptr_t)key) / (dtype == kKv4F32 ? 4 : 2);
+  if (kv4_rows_meet({batch, rows, num_kv_heads, 2}, {out_stride_b, out_stride_t, out_stride_h, apart}, head_dim))
     return WGKV_ERR_ARG;
   a.cache[0] = (const uint8_t*)k_cache;
   a.cache[1] = (const uint8_t*)v_cache;
