@@ -688,9 +688,9 @@ int wgkv_kv4_decode_attn(
 
 /* The three calls with their arguments in a block: the same ones in the same
  * order, each in 8 bytes (pointers and integers as int64, softmax_scale as a
- * double).  For callers whose foreign-function interface converts arguments
- * one at a time: a Python call spends 0.6 us on a block, 2.3 to 2.9 us on the
- * arguments. */
+ * double); a 32-bit argument's word that does not fit it is unsupported.  For
+ * callers whose foreign-function interface converts arguments one at a time: a
+ * Python call spends 0.6 us on a block, 2.3 to 2.9 us on the arguments. */
 int wgkv_kv4_append_block(const void* args);
 int wgkv_kv4_read_block(const void* args);
 int wgkv_kv4_decode_attn_block(const void* args);

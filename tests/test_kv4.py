@@ -268,3 +268,25 @@ def test_output_rows_that_meet_are_refused():
         seen.add((meets, nested))
         assert attend(sb, sh, B, Hq) == (_lib.ERR_ARG if meets else _lib.ERR_WORKSPACE), (B, Hq, sb, sh)
     assert seen >= {(True, False), (False, False), (False, True)}
+
+
+def test_sizes_past_32_bits_are_refused():
+    """The C calls' 32-bit sizes come from 64-bit ones in the argument blocks:
+    what does not fit is refused, not cut off (an expanded tensor may have 2^32
+    + 1 tokens).  What passes fails on a missing workspace or argument."""
+    from wgkv import _lib, kv4
+    L = _lib.lib()
+    x = 4096
+    append = [x, 64, 64, 64, x, 64, 64, 64, 0, 0, 0, 0, x, 1, x, 1, x, x, 4, 16, x, 4, 4, 4, 1, 257, 1, 64, 0, x, 8, 0]
+    read = [x, x, 4, 16, x, 4, 4, 4, x, 1, 0, 0, 0, x, 64, 64, 64, 0, 1, 4, 1, 64, 0]
+    attn = [x, 64, 64, x, x, 4, 16, x, 1, x, 4, 4, 4, x, 64, 64, 1, 4, 1, 64, 0.125, x, 8, 0]
+    for call, pack, words, narrow, otherwise in [
+            (L.wgkv_kv4_append_block, kv4._pack_append, append, (8, 19, 23, 24, 25, 26, 27), _lib.ERR_WORKSPACE),
+            (L.wgkv_kv4_read_block, kv4._pack_read, read, (3, 7, 17, 18, 19, 20, 21), _lib.ERR_ARG),
+            (L.wgkv_kv4_decode_attn_block, kv4._pack_attn, attn, (6, 12, 16, 17, 18, 19), _lib.ERR_WORKSPACE)]:
+        assert call(pack(*words)) == otherwise
+        for i in narrow:
+            for more in (1 << 32, -(1 << 32), 1 << 40):
+                wide = list(words)
+                wide[i] += more
+                assert call(pack(*wide)) == _lib.ERR_UNSUPPORTED, (i, more)

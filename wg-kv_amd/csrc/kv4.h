@@ -123,6 +123,12 @@ inline bool kv4_rows_meet(const int64_t (&sizes)[4], const int64_t (&strides)[4]
   }
 }
 
+// Whether a block's 8-byte words fit the 32-bit arguments they become.
+template <typename... I>
+inline bool kv4_narrow(const int64_t* a, I... at) {
+  return ((a[at] == (int32_t)a[at]) && ...);
+}
+
 // ---- element types of the rows quantised or read back -------------------------
 enum Kv4Type { kKv4Bf16 = 0, kKv4F32 = 1, kKv4F16 = 2 };
 

@@ -825,6 +825,7 @@ extern "C" int wgkv_kv4_decode_attn(
 extern "C" int wgkv_kv4_decode_attn_block(const void* args) {
   int64_t a[24];
   memcpy(a, args, sizeof a);
+  if (!kv4_narrow(a, 6, 12, 16, 17, 18, 19)) return WGKV_ERR_UNSUPPORTED;
   double scale;
   memcpy(&scale, &a[20], sizeof scale);
   return wgkv_kv4_decode_attn((const void*)a[0], a[1], a[2], (const void*)a[3], (const void*)a[4], a[5], (int32_t)a[6],

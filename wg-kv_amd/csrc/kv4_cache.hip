@@ -600,6 +600,7 @@ extern "C" int wgkv_kv4_read(
 extern "C" int wgkv_kv4_append_block(const void* args) {
   int64_t a[32];
   memcpy(a, args, sizeof a);
+  if (!kv4_narrow(a, 8, 19, 23, 24, 25, 26, 27)) return WGKV_ERR_UNSUPPORTED;
   return wgkv_kv4_append((const void*)a[0], a[1], a[2], a[3], (const void*)a[4], a[5], a[6], a[7], (int32_t)a[8],
                          (const uint8_t*)a[9], a[10], a[11], (const int32_t*)a[12], a[13], (int32_t*)a[14], a[15],
                          (void*)a[16], (void*)a[17], a[18], (int32_t)a[19], (const int32_t*)a[20], a[21], a[22],
@@ -610,6 +611,7 @@ extern "C" int wgkv_kv4_append_block(const void* args) {
 extern "C" int wgkv_kv4_read_block(const void* args) {
   int64_t a[23];
   memcpy(a, args, sizeof a);
+  if (!kv4_narrow(a, 3, 7, 17, 18, 19, 20, 21)) return WGKV_ERR_UNSUPPORTED;
   return wgkv_kv4_read((const void*)a[0], (const void*)a[1], a[2], (int32_t)a[3], (const int32_t*)a[4], a[5], a[6],
                        (int32_t)a[7], (const int32_t*)a[8], a[9], (const int32_t*)a[10], a[11], (void*)a[12],
                        (void*)a[13], a[14], a[15], a[16], (int32_t)a[17], (int32_t)a[18], (int32_t)a[19],
