@@ -290,3 +290,61 @@ def test_sizes_past_32_bits_are_refused():
                 wide = list(words)
                 wide[i] += more
                 assert call(pack(*wide)) == _lib.ERR_UNSUPPORTED, (i, more)
+
+
+class _Captures:
+    """The scratch's view of a capture: its state and id."""
+
+    def __init__(self, monkeypatch):
+        from wgkv import kv4
+        self.id = 0
+        monkeypatch.setattr(kv4, "_capturing", lambda: self.id is not None)
+        monkeypatch.setattr(kv4, "_workspaces", {})
+        monkeypatch.setattr(kv4, "_captured", {})
+        monkeypatch.setattr(kv4._lib, "lib", lambda: self)
+
+    def wgkv_stream_capture_id(self, stream, ref):
+        ref._obj.value = self.id
+        return 0
+
+
+def test_scratch_is_let_go(monkeypatch):
+    """Attention scratch: a capture's is held no longer than to the next
+    capture or uncaptured call, a stream's until many others had theirs."""
+    import gc
+    import weakref
+    from wgkv import kv4
+    cap = _Captures(monkeypatch)
+
+    def scratch(stream, n=kv4._COUNTERS + 64):
+        return weakref.ref(kv4._attn_workspace("cpu", stream, n))
+    cap.id = 7
+    a, b = scratch(1), scratch(2)
+    assert a() is not None and scratch(1)() is a() and scratch(2)() is b()  # shared within the capture
+    big = scratch(1, kv4._COUNTERS + 4096)
+    gc.collect()
+    assert a() is None and big() is not None and scratch(1)() is big()
+    cap.id = 8
+    c = scratch(3)
+    gc.collect()
+    assert big() is None and b() is None and c() is not None  # another capture's
+    cap.id = None
+    e = scratch(1)
+    gc.collect()
+    assert c() is None and not kv4._captured
+    assert e() is not None and scratch(1)() is e()
+    for s in range(100, 400):
+        assert int(kv4._attn_workspace("cpu", s, kv4._COUNTERS)[:kv4._COUNTERS].max()) == 0
+    gc.collect()
+    assert e() is None and len(kv4._workspaces) <= 32
+    assert scratch(399)() is not None and int(scratch(1)().max()) == 0
+
+
+def test_scratch_of_a_capture_without_id(monkeypatch):
+    """A capture that was invalidated has no id: scratch of its own, shared
+    with no other call."""
+    from wgkv import kv4
+    cap = _Captures(monkeypatch)
+    cap.id = 0
+    x, y = (kv4._attn_workspace("cpu", 5, kv4._COUNTERS + 64) for _ in range(2))
+    assert x.data_ptr() != y.data_ptr() and not x[:kv4._COUNTERS].any()

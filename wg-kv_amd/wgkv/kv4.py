@@ -259,6 +259,7 @@ def kv4_read(k_cache, v_cache, block_table, lengths, rows, starts=None, dtype=to
 
 
 _COUNTERS = 8192  # bytes at the start of the attention's workspace that must be zero
+_KEPT = 32  # streams whose scratch is kept, the last to have asked for one
 _workspaces = {}
 _captured = {}
 
@@ -275,21 +276,37 @@ def _attn_workspace(dev, stream, nbytes):
     graph's memory, cleared by the graph, since two graphs that were captured
     on one stream may run on two: one per capture and stream, for the calls
     that a graph holds of a stream run in turn too (32 calls of 8 heads x 1300
-    tokens: 9.6 us each, 10.9 with scratch for each), and held here until the
-    stream's next capture."""
+    tokens: 9.6 us each, 10.9 with scratch for each).
+
+    Letting scratch go is safe at any time: its memory then serves later calls
+    of the same stream, or stays with the graph.  A capture's is held up to
+    the next capture's first call or the next uncaptured one, so that a graph
+    that is gone can return its memory; a stream's until _KEPT others had
+    theirs, since streams come and go."""
+    key = (dev, stream)
     if _capturing():
         capture = ctypes.c_uint64()
         _lib.check(_lib.lib().wgkv_stream_capture_id(stream, ctypes.byref(capture)), "wgkv_stream_capture_id")
-        held, ws = _captured.get((dev, stream), (0, None))
-        if held != capture.value or ws.numel() < nbytes:
+        now = capture.value
+        held, ws = _captured.get(key, (0, None))
+        if not now or held != now or ws.numel() < nbytes:
             ws = torch.empty(nbytes, dtype=_U8, device=dev)
             ws[:_COUNTERS].zero_()
-            _captured[(dev, stream)] = (capture.value, ws)
+            for other, (i, _) in list(_captured.items()):
+                if i != now:
+                    _captured.pop(other, None)
+            if now:  # 0: a capture that was invalidated
+                _captured[key] = (now, ws)
         return ws
-    ws = _workspaces.get((dev, stream))
+    if _captured:
+        _captured.clear()
+    ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
         ws = torch.zeros(nbytes, dtype=_U8, device=dev)
-        _workspaces[(dev, stream)] = ws
+        _workspaces.pop(key, None)
+        _workspaces[key] = ws
+        for other in list(_workspaces)[:-_KEPT]:
+            _workspaces.pop(other, None)
     return ws
 
 
