@@ -119,13 +119,50 @@ def rows(cache, table_row, n, keys):
     return c, s, m
 
 
+WINDOW = 1024  # tokens a wave adds up before it takes the codes' offset out of its sums
+PIECES = 272   # sums of waves (8) and workgroups (256) that are added up for a head, and a few more
+
+
+def attend_head(x, kk, vv, scale, counts=None, run=None):
+    """One query x (D) over a head's tokens, kk and vv their (codes, s, m):
+    (out, bound), both (D).  A token may stand in the sequence ``counts``
+    times.  The bound is how far a bf16 result may be off whose probabilities
+    are rounded to bf16 for the product with the values (half a step, 2^-8, of
+    p times what the code adds, s |c - 7.5|; the middles' part keeps fp32), with
+    the scores' fp32 sums of D products of codes offset by up to 143, the final
+    rounding (2^-8), and the fp32 sums over the tokens:
+      * codes offset by up to 143 are added up over a window only, at most
+        WINDOW tokens of one wave, before their offset goes (and the windows'
+        errors are relative to the windows' own weights);
+      * middles, windows without the offset and the weights, over the tokens
+        that one wave takes (``run`` of them, all without it), then the pieces.
+    An addition is off by 2^-24 of the sum so far, which is at most the whole;
+    a token counts as one, though the matrix core adds 32 of them in a step,
+    which leaves room for the sum that the offset is taken from."""
+    D = x.shape[0]
+    k, v = values(*kk), values(*vv)
+    z = k @ x * scale
+    w = np.ones(len(z)) if counts is None else np.asarray(counts, np.float64)
+    n = w.sum()
+    p = w * np.exp(z - z[w > 0].max(initial=-np.inf))
+    p /= p.sum()
+    o = p @ v
+    steps, middles = np.repeat(vv[1], GROUP, 1), np.abs(np.repeat(vv[2], GROUP, 1))
+    spread = steps * np.abs(vv[0] - 7.5)
+    reach = np.repeat(kk[1], GROUP, 1) * 143 + np.abs(np.repeat(kk[2], GROUP, 1))
+    dz = abs(scale) * (reach @ np.abs(x)) * (D + 8) * 2.0 ** -24 + (np.abs(z).max() + 8) * 2.0 ** -22
+    sums = (min(n, WINDOW) + 8) * 143 * (p @ steps)
+    if run is None:
+        sums += (n + 8) * (p @ middles) + max(n - WINDOW, 0) * (p @ spread)
+    else:
+        sums += (run + PIECES) * (p @ middles + p @ spread + np.abs(o))
+    return o, (2.0 ** -8 * np.abs(o) + 2.0 ** -8 * (p @ spread) * (1 + 2.0 ** -8)
+               + 2 * (p * dz) @ np.abs(v) + 2 * (p @ dz) * np.abs(o) + 2.0 ** -24 * sums + 1e-30)
+
+
 def attend(q, kc, vc, table, lengths, scale):
     """q (B, Hq, D) float64 -> (out, bound), both (B, Hq, D) float64: the
-    attention, and how far a bf16 result may be from it whose probabilities
-    are rounded to bf16 for the product with the values (half a step, 2^-8,
-    of p times what the code adds, s |c - 7.5|; the middles' part keeps
-    fp32), with fp32 sums of D products of codes offset by up to 143 and the
-    final rounding (2^-8)."""
+    attention, and how far a bf16 result may be from it (attend_head)."""
     B, Hq, D = q.shape
     H = table.shape[1]
     G = Hq // H
@@ -137,19 +174,41 @@ def attend(q, kc, vc, table, lengths, scale):
             if n == 0:
                 continue
             kk, vv = rows(kc, table[b, h], n, True), rows(vc, table[b, h], n, False)
-            kx, vx = values(*kk), values(*vv)
-            spread = np.repeat(vv[1], GROUP, 1) * np.abs(vv[0] - 7.5)
-            reach = np.repeat(kk[1], GROUP, 1) * 143 + np.abs(np.repeat(kk[2], GROUP, 1))
-            vreach = np.repeat(vv[1], GROUP, 1) * 143 + np.abs(np.repeat(vv[2], GROUP, 1))
-            for i in range(G):
-                x = q[b, h * G + i]
-                z = kx @ x * scale
-                p = np.exp(z - z.max())
-                p /= p.sum()
-                o = p @ vx
-                dz = abs(scale) * (reach @ np.abs(x)) * (D + 8) * 2.0 ** -24 + (np.abs(z).max() + 8) * 2.0 ** -22
-                out[b, h * G + i] = o
-                tail = (n + 8) * 2.0 ** -24 * (p @ vreach)  # fp32 sums over the tokens
-                bound[b, h * G + i] = (2.0 ** -8 * np.abs(o) + 2.0 ** -8 * (p @ spread) * (1 + 2.0 ** -8)
-                                       + 2 * (p * dz) @ np.abs(vx) + 2 * (p @ dz) * np.abs(o) + tail + 1e-30)
+            for i in range(h * G, h * G + G):
+                out[b, i], bound[b, i] = attend_head(q[b, i], kk, vv, scale)
+    return out, bound
+
+
+def pool_rows(kc, vc):
+    """Every token of a pair of pools, in the pages' order."""
+    N, P = kc.shape[0], kc.shape[1] * TILE
+    return rows(kc, np.arange(N), N * P, True), rows(vc, np.arange(N), N * P, False)
+
+
+def token_counts(table_row, n, pages, P):
+    """How often each token of the pool stands among a head's first n."""
+    counts = np.repeat(np.bincount(np.asarray(table_row[:n // P], np.int64), minlength=pages), P)
+    if n % P:
+        last = int(table_row[n // P]) * P
+        counts[last:last + n % P] += 1
+    return counts
+
+
+def attend_shared(q, held, P, table, lengths, scale, run=None):
+    """``attend`` for long sequences over few pages, which their tables name
+    many times: each token of the pool (``held``: pool_rows) once, with its
+    count in the head."""
+    B, Hq, D = q.shape
+    H = table.shape[1]
+    G = Hq // H
+    out, bound = np.zeros((B, Hq, D)), np.zeros((B, Hq, D))
+    for b in range(B):
+        for h in range(H):
+            counts = token_counts(table[b, h], int(lengths[b, h]), len(held[0][0]) // P, P)
+            live = counts > 0
+            if not live.any():
+                continue
+            kk, vv = (tuple(y[live] for y in c) for c in held)
+            for i in range(h * G, h * G + G):
+                out[b, i], bound[b, i] = attend_head(q[b, i], kk, vv, scale, counts[live], run)
     return out, bound
