@@ -37,7 +37,11 @@
 // Bound by reads where the caches are long: 8 sequences of 128K, 2-60 %
 // admitted (424 MB), 73 us, 5.8 TB/s (loads of this pattern alone 6.3); 8
 // heads of 400K tokens (513 MB) 86 us, 6.0 TB/s, vector instructions half of
-// the time.  Short ones are latency: 8 heads of ~1300 tokens 12 us in a graph,
+// the time.  With 5 to 8 query heads per KV head at D = 128 the first of these
+// takes 113 us: two column tiles, half the waves, and one group of threads to
+// merge a head's pieces, which also costs lines of one or two heads (one of
+// 400K tokens: 31 us, with 8 query heads 76; 10 at the rate of its reads).
+// Short ones are latency: 8 heads of ~1300 tokens 12 us in a graph,
 // of which 2.4 pass before the first tile, 2 for a unit, 1.5 in the
 // workgroup's merge and 4.5 between workgroups.
 #include <string.h>
@@ -556,6 +560,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
             const float p1 = fast_exp2(fmaf(s[p][2 * j + 1], a.scale_log2, -m_run[nt]));
             l_run[nt] += p0 + p1;
             corr[nt] = fmaf(p1, bf16hi(s1), fmaf(p0, bf16hi(s0), corr[nt]));
+            // Rounded to bf16 for the matrix core, as the bf16 cache's
+            // probabilities are: 2^-8 at most of what a code adds, and the
+            // middles' part (corr) keeps fp32.  Against 64 bits the outputs
+            // are 2.1e-3 to 2.4e-3 off (rms over rms), of which their own
+            // rounding is 1.7e-3.
             pk[2 * p + j] = pack_bf16x2(p0 * bf16lo(s0), p1 * bf16lo(s1));
           }
         pb[nt] = (u32x4_t){pk[0], pk[1], pk[2], pk[3]};

@@ -8,10 +8,13 @@
 // 64/(D/8) quads at a time, every row of the dense side is read or written
 // whole by neighbouring lanes, and the values' words of a quad are one
 // 16-byte access.  The read-back is bound by its writes (24K rows of 64 heads,
-// 994 MB, 186 us, 5.35 TB/s; a copy reaches 4.9), the append by its rounding
-// (26K admitted rows of a 128K prompt in 8 heads: 46 us, two thirds of it
-// vector instructions, 143 MB moved; 460 instructions less per wave took 8 us
-// off; registers for more waves spill: 87 us for both calls instead of 79).
+// 994 MB, 186 us, 5.35 TB/s; a copy reaches 4.9).  The append is bound by
+// nothing alone (26K admitted rows of a 128K prompt in 8 heads, 143 MB moved:
+// 45 us, of which 30 are vector instructions' issue, the rounding's above all):
+// a tile with a fifth of its tokens admitted is one step, whose flags, page
+// id, rows and arithmetic follow each other.  460 instructions less per wave
+// took 8 us off; registers for more waves spill (87 us for both calls instead
+// of 79).
 #include <string.h>
 
 #include "kv4.h"
