@@ -695,6 +695,120 @@ int wgkv_kv4_append_block(const void* args);
 int wgkv_kv4_read_block(const void* args);
 int wgkv_kv4_decode_attn_block(const void* args);
 
+/* ------------------------------------------------------------------------
+ * Serving a packed batch of requests over paged per-head caches.  No
+ * counterpart in the reference, whose cache serves one sequence; page tables,
+ * lengths and pools are those of wgkv_paged_decode_attn.
+ *
+ * wgkv_build_block_tables: pages, lengths and cache rows of a step's tokens.
+ *   cu_seqlens  i32 (B+1), ascending: request b's new tokens are rows
+ *               cu[b] .. cu[b+1]-1 of num_tokens (N)
+ *   lengths     i32 (B, H) tokens held; new_lengths (B, H) receives them with
+ *               the kept ones (it may be lengths; no entry shared otherwise)
+ *   g_mask      u8 (H, N), n contiguous: nonzero = kept; NULL: all kept
+ *   block_table i32 (B, H, max_pages), updated in place: a head's new pages
+ *               are entries ceil(len/page) .. ceil(new/page)-1
+ *   page_state  i32 [2]: next unused page, entries of free_ids; state_out
+ *               receives it after the step (it may be page_state)
+ *   free_ids    i32 (free_capacity) pages given back, or NULL
+ *   slots       i32 (N, H): the pool row of each kept token (page *
+ *               page_size + position % page_size), -1 for the others and for
+ *               rows of no request
+ * New pages are handed out in row-major (b, h) order, the free list's last
+ * entries first (in list order), then page_state[0], page_state[0]+1, ...
+ * If the pages do not suffice or a head would outgrow its table, nothing is
+ * written but slots (-1), unchanged lengths and state, and *status (or NULL) =
+ * WGKV_ERR_CAPACITY; a held page id outside the pool sets it too, and its
+ * tokens' slots are -1.  num_pages * page_size and N*H < 2^31, (B+1)*H <=
+ * 2^24.  One launch for N <= 256 and (B+1)*H <= 4096; two otherwise, three
+ * with a mask, and then a workspace (as sized, any contents).
+ *
+ * wgkv_paged_append copies rows of key/value bf16 (N, H, D) (element strides,
+ * d contiguous; 16-byte aligned, strides multiples of 8) to rows slots[n,h]
+ * of the pools (cache_rows, D); slots outside [0, cache_rows) are left out.
+ * D a multiple of 8.  The pools share no byte; of two tokens with one slot
+ * either may stay.
+ *
+ * wgkv_sink_window_attn: q, out bf16 (N, Hq, D), k, v (Nk, Hkv, D) (element
+ * strides, d contiguous, 16-byte aligned).  Sequence b holds rows cu_seqlens_q[b]
+ * .. cu_seqlens_q[b+1]-1 and keys cu_seqlens_k[b] .. cu_seqlens_k[b+1]-1; with
+ * nq rows and nk keys its row i is at position p = i + nk - nq and sees key j
+ * iff j <= p and (j > p - window or j < num_sinks).  Rows that see nothing
+ * give zeros; what a row does not see has no part in it, NaN included.  Rows
+ * of no sequence are left as they are, or cleared (clear_rest != 0).  window
+ * >= 1; D in {64,128}; G = Hq/Hkv in 1..8; up to 2048 sequences and 2^30
+ * rows.
+ *
+ * wgkv_paged_decode_attn_window: wgkv_paged_decode_attn where a head of T
+ * tokens shows those t with t >= T - window or t < num_sinks.  Page ids of the
+ * others are not read.  Same workspace (its counters zero before a call and
+ * after it).
+ *
+ * wgkv_shared_decode_attn: wgkv_paged_decode_attn where sequences
+ * group_starts[n] .. group_starts[n+1]-1 (i32 (num_groups+1), ascending) also
+ * attend, under the same softmax, to the first prefix_lens[n,h] tokens of
+ * prefix n, whose pages are prefix_table (num_groups, Hkv, prefix_pages).
+ * Sequences of no group have none.  B*Hkv and num_groups*Hkv <= 2048.  Two
+ * launches; workspace as sized, any contents, calls that share one ordered.
+ * ---------------------------------------------------------------------- */
+size_t wgkv_block_tables_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t num_tokens);
+
+int wgkv_build_block_tables(
+    const int32_t* lengths, int64_t len_stride_b, const int32_t* cu_seqlens, int32_t num_tokens,
+    const uint8_t* g_mask, int64_t gm_stride_h,
+    int32_t* block_table, int64_t bt_stride_b, int64_t bt_stride_h, int32_t max_pages,
+    const int32_t* page_state, int32_t* state_out, const int32_t* free_ids, int32_t free_capacity,
+    int64_t num_pages, int32_t page_size,
+    int32_t* new_lengths, int64_t new_stride_b, int32_t* slots,
+    int32_t batch, int32_t num_kv_heads, int32_t* status,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+int wgkv_paged_append(
+    const void* key, int64_t k_stride_n, int64_t k_stride_h, const void* value, int64_t v_stride_n, int64_t v_stride_h,
+    void* k_cache, void* v_cache, int64_t cache_rows, const int32_t* slots,
+    int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim, void* stream);
+
+int wgkv_sink_window_attn(
+    const void* q, int64_t q_stride_n, int64_t q_stride_h,
+    const void* k, int64_t k_stride_n, int64_t k_stride_h,
+    const void* v, int64_t v_stride_n, int64_t v_stride_h,
+    void* out, int64_t out_stride_n, int64_t out_stride_h,
+    const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int32_t batch, int32_t num_rows, int32_t num_keys,
+    int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t window, int32_t num_sinks, float softmax_scale, int32_t clear_rest, void* stream);
+
+int wgkv_paged_decode_attn_window(
+    const void* q, int64_t q_stride_b, int64_t q_stride_h,
+    const void* k_cache, const void* v_cache, int64_t num_pages, int32_t page_size,
+    const int32_t* cache_seqlens, int64_t sl_stride_b,
+    const int32_t* block_table, int64_t bt_stride_b, int64_t bt_stride_h, int32_t max_pages,
+    void* out, int64_t out_stride_b, int64_t out_stride_h,
+    int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t window, int32_t num_sinks, float softmax_scale,
+    void* workspace, size_t workspace_bytes, void* stream);
+
+size_t wgkv_shared_decode_workspace_bytes(int32_t batch, int32_t num_groups, int32_t num_q_heads,
+                                          int32_t num_kv_heads, int32_t head_dim);
+
+int wgkv_shared_decode_attn(
+    const void* q, int64_t q_stride_b, int64_t q_stride_h,
+    const void* k_cache, const void* v_cache, int64_t num_pages, int32_t page_size,
+    const int32_t* cache_seqlens, int64_t sl_stride_b,
+    const int32_t* block_table, int64_t bt_stride_b, int64_t bt_stride_h, int32_t max_pages,
+    const int32_t* prefix_lens, int64_t pl_stride_n,
+    const int32_t* prefix_table, int64_t pt_stride_n, int64_t pt_stride_h, int32_t prefix_pages,
+    const int32_t* group_starts, int32_t num_groups,
+    void* out, int64_t out_stride_b, int64_t out_stride_h,
+    int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The five calls with their arguments in a block, as wgkv_kv4_*_block. */
+int wgkv_build_block_tables_block(const void* args);
+int wgkv_paged_append_block(const void* args);
+int wgkv_sink_window_attn_block(const void* args);
+int wgkv_paged_decode_attn_window_block(const void* args);
+int wgkv_shared_decode_attn_block(const void* args);
+
 #ifdef __cplusplus
 }
 #endif

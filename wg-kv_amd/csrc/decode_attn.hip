@@ -38,9 +38,11 @@
 //     kernel (at batch 8 the last arriver's write-through stores and
 //     arrival count cost as much as the second launch, which spreads the
 //     merge over B*Hkv*G workgroups).
+#include <string.h>
+
 #include <mutex>
 
-#include "wgkv_common.h"
+#include "kv4.h"
 
 namespace {
 
@@ -77,6 +79,9 @@ struct DecodeArgs {
   int64_t out_sb, out_sh;
   int B, Hkv;
   float scale_log2;
+  // windowed calls: a token t of T is seen iff t >= T - window or t < sinks
+  int window, sinks;
+  uint32_t q_and, q_xor;  // the queries' bits: a scale of 0 clears them, a negative one negates them
   int target_chunks;  // resident workgroup slots: the plan aims at one chunk per slot
   // partials of chunk w, query head i (i < G): m at part_m[w*G+i], l at
   // part_l[w*G+i], acc at part_acc[(w*G+i)*D ..]
@@ -97,6 +102,29 @@ __device__ __forceinline__ int clamped_tokens(const DecodeArgs& a, int bh) {
   const int cap = a.max_pages * a.page_size;
   T = T < 0 ? 0 : (T > cap ? cap : T);
   return T;
+}
+
+// The sub-pages of a head that a call reads, counted through: those of the
+// first tokens, then those from the window's first token on (all of them
+// without a window).  Sub-page j of them is j, or j + skip from `cut` on.
+struct Visible {
+  int nsub, cut, skip;
+};
+
+template <bool WIN>
+__device__ __forceinline__ Visible visible_subpages(const DecodeArgs& a, int T) {
+  const int all = (T + 15) >> 4;
+  Visible v = {all, all, 0};
+  if constexpr (WIN) {
+    const int ns = (min(T, a.sinks) + 15) >> 4, w0 = max(0, T - a.window) >> 4;
+    if (w0 > ns) v = {ns + all - w0, ns, w0 - ns};
+  }
+  return v;
+}
+
+template <bool WIN>
+__device__ __forceinline__ int head_subpages(const DecodeArgs& a, int bh) {
+  return visible_subpages<WIN>(a, clamped_tokens(a, bh)).nsub;
 }
 
 // This workgroup's share of the device-side split plan (replaces the host
@@ -123,11 +151,11 @@ __device__ __forceinline__ int chunk_subpages(int total, int target) {
 // scans in registers, no LDS and no barrier.  With 4-wave workgroups,
 // workgroup 0 stores the plan (first chunk of each head, then the chunk
 // count) for the merge kernel.
-template <int NW>
+template <int NW, bool WIN>
 __device__ Plan plan_wave(const DecodeArgs& a, int w) {
   const int BH = a.B * a.Hkv;
   const int lane = threadIdx.x & 63;
-  const int ns = lane < BH ? (clamped_tokens(a, lane) + 15) >> 4 : 0;
+  const int ns = lane < BH ? head_subpages<WIN>(a, lane) : 0;
   const int total = __builtin_amdgcn_readlane(wave_incl_scan(ns, lane), 63);
   int cp = chunk_subpages<NW>(total, a.target_chunks);
   int ch = lane < BH ? max(1, (ns + cp - 1) / cp) : 0;
@@ -158,26 +186,27 @@ __device__ Plan plan_wave(const DecodeArgs& a, int w) {
 
 // B*Hkv > 64 (4-wave workgroups): block scans over the heads through LDS
 // (workgroup 0 stores the plan for the merge kernel).
+template <bool WIN>
 __device__ Plan plan_block(const DecodeArgs& a, int w, int* s_pref, int* s_tmp) {
   const int BH = a.B * a.Hkv;
   const int t = threadIdx.x;
   const int per = (BH + kPlanThreads - 1) / kPlanThreads;
   const int lo = min(BH, t * per), hi = min(BH, lo + per);
   int subs = 0;
-  for (int bh = lo; bh < hi; ++bh) subs += (clamped_tokens(a, bh) + 15) >> 4;
+  for (int bh = lo; bh < hi; ++bh) subs += head_subpages<WIN>(a, bh);
   int total = 0;
   block_exclusive_scan_256(subs, s_tmp, &total);
   const int cp = chunk_subpages<4>(total, a.target_chunks);
   int chunks = 0;
   for (int bh = lo; bh < hi; ++bh) {
-    const int ns = (clamped_tokens(a, bh) + 15) >> 4;
+    const int ns = head_subpages<WIN>(a, bh);
     chunks += max(1, (ns + cp - 1) / cp);
   }
   int n_chunks = 0;
   int run = block_exclusive_scan_256(chunks, s_tmp, &n_chunks);
   for (int bh = lo; bh < hi; ++bh) {
     s_pref[bh] = run;
-    const int ns = (clamped_tokens(a, bh) + 15) >> 4;
+    const int ns = head_subpages<WIN>(a, bh);
     run += max(1, (ns + cp - 1) / cp);
   }
   if (t == 0) s_pref[BH] = n_chunks;
@@ -244,7 +273,7 @@ __device__ __forceinline__ float dot2_bf16(uint32_t a, uint32_t b, float c) {
   return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, a), __builtin_bit_cast(bf16x2_t, b), c, false);
 }
 
-template <int D, int G, int NW>
+template <int D, int G, int NW, bool WIN>
 __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(waves_per_simd(G, NW), waves_per_simd(G, NW))))
 void decode_split_kernel(DecodeArgs a) {
   constexpr int kThreads = NW * 64;
@@ -270,16 +299,17 @@ void decode_split_kernel(DecodeArgs a) {
   if constexpr (NW == 4) {
     __shared__ int s_pref[kMaxBH + 1];
     __shared__ int s_tmp[kPlanThreads];
-    pl = a.B * a.Hkv <= kWaveBH ? plan_wave<NW>(a, w) : plan_block(a, w, s_pref, s_tmp);
+    pl = a.B * a.Hkv <= kWaveBH ? plan_wave<NW, WIN>(a, w) : plan_block<WIN>(a, w, s_pref, s_tmp);
   } else {
-    pl = plan_wave<NW>(a, w);  // the host takes 8 waves only for B*Hkv < 32
+    pl = plan_wave<NW, WIN>(a, w);  // the host takes 8 waves only for B*Hkv < 32
   }
   if (w >= pl.n_chunks) return;
   const int bh = pl.bh;
   const int ci = w - pl.first;
   const int b = bh / a.Hkv, h = bh - b * a.Hkv;
   const int T = clamped_tokens(a, bh);
-  const int nsub = (T + 15) >> 4;
+  const Visible vis = visible_subpages<WIN>(a, T);
+  const int nsub = vis.nsub;
   const int s0 = ci * pl.cp;
   const int s1 = min(nsub, s0 + pl.cp);
   const int tok_end = min(T, s1 * 16);
@@ -301,6 +331,7 @@ void decode_split_kernel(DecodeArgs a) {
     for (int j = 0; j < KS; ++j) {
       u32x4_t v = *(const u32x4_t*)(qrow + (j * 4 + g) * 8);
       if (qh >= G) v = (u32x4_t){0u, 0u, 0u, 0u};
+      if constexpr (WIN) v = (v & a.q_and) ^ a.q_xor;
       qa[gi][j] = __builtin_bit_cast(bf16x8_t, v);
     }
   }
@@ -319,7 +350,10 @@ void decode_split_kernel(DecodeArgs a) {
     const int sp0 = s0 + jq * 4;
     int64_t off[4];
 #pragma unroll
-    for (int p = 0; p < 4; ++p) off[p] = subpage_row(a, bt_row, min(sp0 + p, s1 - 1)) * D;
+    for (int p = 0; p < 4; ++p) {
+      const int sp = min(sp0 + p, s1 - 1);
+      off[p] = subpage_row(a, bt_row, WIN && sp >= vis.cut ? sp + vis.skip : sp) * D;
+    }
     u32x4_t kr[4][KS];
     u32x4_t vr[NV];
     load_k<D>(a, kr, off, n, g);
@@ -343,7 +377,11 @@ void decode_split_kernel(DecodeArgs a) {
     // p <= 2^kRescaleSlack and most quads need neither a maximum nor a
     // rescale -- one compare and ballot per head.  Lane (n, g) holds token n
     // of sub-page g (rows 4g..4g+3 of its MFMA are the group's heads).
-    const bool ok = (sp0 + g) * 16 + n < tok_end;
+    bool ok = (sp0 + g) * 16 + n < tok_end;
+    if constexpr (WIN) {
+      const int t = (sp0 + g + (sp0 + g >= vis.cut ? vis.skip : 0)) * 16 + n;
+      ok = sp0 + g < s1 && t < T && (t < a.sinks || T - t <= a.window);
+    }
     float s[G], pr[NG][4];
 #pragma unroll
     for (int i = 0; i < G; ++i) {
@@ -385,13 +423,16 @@ void decode_split_kernel(DecodeArgs a) {
     // so that one instruction adds p_r * v_r + p_r' * v_r' for one d; the
     // probabilities are rounded to bf16 for the product, as the reference's
     // kernel does (src/modeling_layers.py:930-931).
-    const bool full = sp0 * 16 + 64 <= tok_end;
+    // Rows that no query sees are cleared: whatever they hold, times 0, must
+    // be 0 (row r of the quad is lane r's token).
+    const uint64_t seen = WIN ? __builtin_amdgcn_ballot_w64(ok) : 0;
+    const bool full = WIN ? seen == ~0ull : sp0 * 16 + 64 <= tok_end;
 #pragma unroll
     for (int i = 0; i < NV; i += 2) {
       const int r0 = i * RPI + lane / CH, r1 = r0 + RPI;
       u32x4_t v0 = vr[i], v1 = vr[i + 1];
-      if (!full && sp0 * 16 + r0 >= tok_end) v0 = (u32x4_t){0u, 0u, 0u, 0u};
-      if (!full && sp0 * 16 + r1 >= tok_end) v1 = (u32x4_t){0u, 0u, 0u, 0u};
+      if (!full && (WIN ? !(seen >> r0 & 1) : sp0 * 16 + r0 >= tok_end)) v0 = (u32x4_t){0u, 0u, 0u, 0u};
+      if (!full && (WIN ? !(seen >> r1 & 1) : sp0 * 16 + r1 >= tok_end)) v1 = (u32x4_t){0u, 0u, 0u, 0u};
       uint32_t pp[G];
 #pragma unroll
       for (int gi = 0; gi < NG; ++gi) {
@@ -654,7 +695,7 @@ __global__ void zero_counters_kernel(int* c, int n) {
   if (i < n) c[i] = 0;
 }
 
-template <int D, int G, int NW>
+template <int D, int G, int NW, bool WIN>
 hipError_t launch_nw(DecodeArgs a, hipStream_t st) {
   const int BH = a.B * a.Hkv;
   const int slots = min(kMaxSlots, cu_count() * wg_per_cu(G, NW));
@@ -663,32 +704,32 @@ hipError_t launch_nw(DecodeArgs a, hipStream_t st) {
   // per CU a few chunks beyond the slots only fill the first free slots
   // (aiming at slots - BH measured 0.5 % slower at batch 8).
   a.target_chunks = slots;
-  hipLaunchKernelGGL((decode_split_kernel<D, G, NW>), dim3(a.target_chunks + BH), dim3(NW * 64), 0, st, a);
+  hipLaunchKernelGGL((decode_split_kernel<D, G, NW, WIN>), dim3(a.target_chunks + BH), dim3(NW * 64), 0, st, a);
   const hipError_t e = hipGetLastError();
   if (NW > 4 || e != hipSuccess) return e;
   hipLaunchKernelGGL((decode_merge_kernel<D, G>), dim3(BH, G), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
-template <int D, int G>
+template <int D, int G, bool WIN>
 hipError_t launch(const DecodeArgs& a, hipStream_t st) {
   if constexpr (G <= 4) {
-    if (a.B * a.Hkv < kWideBelowBH) return launch_nw<D, G, 8>(a, st);
+    if (a.B * a.Hkv < kWideBelowBH) return launch_nw<D, G, 8, WIN>(a, st);
   }
-  return launch_nw<D, G, 4>(a, st);
+  return launch_nw<D, G, 4, WIN>(a, st);
 }
 
-template <int D>
+template <int D, bool WIN>
 hipError_t launch_g(const DecodeArgs& a, int G, hipStream_t st) {
   switch (G) {
-    case 1: return launch<D, 1>(a, st);
-    case 2: return launch<D, 2>(a, st);
-    case 3: return launch<D, 3>(a, st);
-    case 4: return launch<D, 4>(a, st);
-    case 5: return launch<D, 5>(a, st);
-    case 6: return launch<D, 6>(a, st);
-    case 7: return launch<D, 7>(a, st);
-    default: return launch<D, 8>(a, st);
+    case 1: return launch<D, 1, WIN>(a, st);
+    case 2: return launch<D, 2, WIN>(a, st);
+    case 3: return launch<D, 3, WIN>(a, st);
+    case 4: return launch<D, 4, WIN>(a, st);
+    case 5: return launch<D, 5, WIN>(a, st);
+    case 6: return launch<D, 6, WIN>(a, st);
+    case 7: return launch<D, 7, WIN>(a, st);
+    default: return launch<D, 8, WIN>(a, st);
   }
 }
 
@@ -805,6 +846,9 @@ extern "C" int wgkv_paged_decode_attn(
   a.B = batch;
   a.Hkv = num_kv_heads;
   a.scale_log2 = softmax_scale * kLog2e;
+  a.window = a.sinks = 0;
+  a.q_and = ~0u;
+  a.q_xor = 0;
   a.counter = (int*)workspace;
   float* ws = (float*)((char*)workspace + kCounterBytes);
   a.part_m = ws;
@@ -813,7 +857,7 @@ extern "C" int wgkv_paged_decode_attn(
   a.plan = (int*)(ws + part_floats(head_dim));
 
   hipStream_t st = (hipStream_t)stream;
-  const hipError_t e = head_dim == 128 ? launch_g<128>(a, G, st) : launch_g<64>(a, G, st);
+  const hipError_t e = head_dim == 128 ? launch_g<128, false>(a, G, st) : launch_g<64, false>(a, G, st);
   return e == hipSuccess ? WGKV_OK : WGKV_ERR_HIP;
 }
 
@@ -835,4 +879,80 @@ extern "C" int wgkv_paged_decode_attn_noalloc(
                                 sl_stride_b, block_table, bt_stride_b, bt_stride_h, max_pages, out, out_stride_b,
                                 out_stride_h, batch, num_q_heads, num_kv_heads, head_dim, softmax_scale, ws,
                                 kScratchBytes, stream);
+}
+
+extern "C" int wgkv_paged_decode_attn_window(
+    const void* q, int64_t q_stride_b, int64_t q_stride_h,
+    const void* k_cache, const void* v_cache, int64_t num_pages, int32_t page_size,
+    const int32_t* cache_seqlens, int64_t sl_stride_b,
+    const int32_t* block_table, int64_t bt_stride_b, int64_t bt_stride_h, int32_t max_pages,
+    void* out, int64_t out_stride_b, int64_t out_stride_h,
+    int32_t batch, int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
+    int32_t window, int32_t num_sinks, float softmax_scale,
+    void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !k_cache || !v_cache || !cache_seqlens || !block_table || !out) return WGKV_ERR_ARG;
+  if (batch <= 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_pages <= 0 || max_pages <= 0) return WGKV_ERR_ARG;
+  if (num_q_heads % num_kv_heads || window < 1 || num_sinks < 0) return WGKV_ERR_ARG;
+  if ((int64_t)batch * num_kv_heads > kMaxBH) return WGKV_ERR_UNSUPPORTED;
+  const int G = num_q_heads / num_kv_heads;
+  if (head_dim != 64 && head_dim != 128) return WGKV_ERR_UNSUPPORTED;
+  if (G > kMaxG || (page_size != 16 && page_size != 32 && page_size != 64)) return WGKV_ERR_UNSUPPORTED;
+  // positions, and the sub-pages of all heads together, are 32-bit
+  const int64_t cap = (int64_t)max_pages * page_size;
+  if (cap > 0x7fffff00 || (cap / 16) * batch * num_kv_heads > 0x7f000000) return WGKV_ERR_UNSUPPORTED;
+  if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return WGKV_ERR_UNSUPPORTED;
+  if ((q_stride_b | q_stride_h) & 7) return WGKV_ERR_UNSUPPORTED;
+  if (kv4_rows_meet({batch, num_q_heads, 1, 1}, {out_stride_b, out_stride_h, 0, 0}, head_dim)) return WGKV_ERR_ARG;
+  if (!workspace || workspace_bytes < wgkv_paged_decode_workspace_bytes(batch, num_kv_heads, head_dim) ||
+      ((uintptr_t)workspace & 15))
+    return WGKV_ERR_WORKSPACE;
+  DecodeArgs a;
+  a.q = (const uint16_t*)q;
+  a.q_sb = q_stride_b;
+  a.q_sh = q_stride_h;
+  a.kc = (const uint16_t*)k_cache;
+  a.vc = (const uint16_t*)v_cache;
+  a.num_pages = num_pages;
+  a.page_size = page_size;
+  a.page_shift = page_size == 16 ? 0 : page_size == 32 ? 1 : 2;
+  a.seqlens = cache_seqlens;
+  a.sl_sb = sl_stride_b;
+  a.bt = block_table;
+  a.bt_sb = bt_stride_b;
+  a.bt_sh = bt_stride_h;
+  a.max_pages = max_pages;
+  a.out = (uint16_t*)out;
+  a.out_sb = out_stride_b;
+  a.out_sh = out_stride_h;
+  a.B = batch;
+  a.Hkv = num_kv_heads;
+  a.window = window;
+  a.sinks = num_sinks;
+  // a negative scale negates the queries, and a scale of 0 clears them: masked
+  // scores are -inf, and -inf * 0 is not a number
+  a.scale_log2 = softmax_scale == 0.f ? 1.f : fabsf(softmax_scale) * kLog2e;
+  a.q_and = softmax_scale == 0.f ? 0u : ~0u;
+  a.q_xor = softmax_scale < 0.f ? 0x80008000u : 0u;
+  a.counter = (int*)workspace;
+  float* ws = (float*)((char*)workspace + kCounterBytes);
+  a.part_m = ws;
+  a.part_l = ws + (size_t)kMaxChunks * kMaxG;
+  a.part_acc = ws + (size_t)kMaxChunks * kMaxG * 2;
+  a.plan = (int*)(ws + part_floats(head_dim));
+  hipStream_t st = (hipStream_t)stream;
+  const hipError_t e = head_dim == 128 ? launch_g<128, true>(a, G, st) : launch_g<64, true>(a, G, st);
+  return e == hipSuccess ? WGKV_OK : WGKV_ERR_HIP;
+}
+
+extern "C" int wgkv_paged_decode_attn_window_block(const void* args) {
+  int64_t a[26];
+  memcpy(a, args, sizeof a);
+  if (!kv4_narrow(a, 6, 12, 16, 17, 18, 19, 20, 21)) return WGKV_ERR_UNSUPPORTED;
+  double scale;
+  memcpy(&scale, &a[22], sizeof scale);
+  return wgkv_paged_decode_attn_window(
+      (const void*)a[0], a[1], a[2], (const void*)a[3], (const void*)a[4], a[5], (int32_t)a[6], (const int32_t*)a[7],
+      a[8], (const int32_t*)a[9], a[10], a[11], (int32_t)a[12], (void*)a[13], a[14], a[15], (int32_t)a[16],
+      (int32_t)a[17], (int32_t)a[18], (int32_t)a[19], (int32_t)a[20], (int32_t)a[21], (float)scale, (void*)a[23],
+      (size_t)a[24], (void*)a[25]);
 }

@@ -221,6 +221,54 @@ SIGNATURES = {
     "wgkv_kv4_append_block": (ctypes.c_int, [ctypes.c_char_p]),
     "wgkv_kv4_read_block": (ctypes.c_int, [ctypes.c_char_p]),
     "wgkv_kv4_decode_attn_block": (ctypes.c_int, [ctypes.c_char_p]),
+    "wgkv_block_tables_workspace_bytes": (c_size, [c_i32, c_i32, c_i32]),
+    "wgkv_build_block_tables": (ctypes.c_int, [
+        c_ptr, c_i64, c_ptr, c_i32,
+        c_ptr, c_i64,
+        c_ptr, c_i64, c_i64, c_i32,
+        c_ptr, c_ptr, c_ptr, c_i32,
+        c_i64, c_i32,
+        c_ptr, c_i64, c_ptr,
+        c_i32, c_i32, c_ptr,
+        c_ptr, c_size, c_ptr]),
+    "wgkv_paged_append": (ctypes.c_int, [
+        c_ptr, c_i64, c_i64, c_ptr, c_i64, c_i64,
+        c_ptr, c_ptr, c_i64, c_ptr,
+        c_i32, c_i32, c_i32, c_ptr]),
+    "wgkv_sink_window_attn": (ctypes.c_int, [
+        c_ptr, c_i64, c_i64,
+        c_ptr, c_i64, c_i64,
+        c_ptr, c_i64, c_i64,
+        c_ptr, c_i64, c_i64,
+        c_ptr, c_ptr, c_i32, c_i32, c_i32,
+        c_i32, c_i32, c_i32,
+        c_i32, c_i32, c_f32, c_i32, c_ptr]),
+    "wgkv_paged_decode_attn_window": (ctypes.c_int, [
+        c_ptr, c_i64, c_i64,
+        c_ptr, c_ptr, c_i64, c_i32,
+        c_ptr, c_i64,
+        c_ptr, c_i64, c_i64, c_i32,
+        c_ptr, c_i64, c_i64,
+        c_i32, c_i32, c_i32, c_i32,
+        c_i32, c_i32, c_f32,
+        c_ptr, c_size, c_ptr]),
+    "wgkv_shared_decode_workspace_bytes": (c_size, [c_i32, c_i32, c_i32, c_i32, c_i32]),
+    "wgkv_shared_decode_attn": (ctypes.c_int, [
+        c_ptr, c_i64, c_i64,
+        c_ptr, c_ptr, c_i64, c_i32,
+        c_ptr, c_i64,
+        c_ptr, c_i64, c_i64, c_i32,
+        c_ptr, c_i64,
+        c_ptr, c_i64, c_i64, c_i32,
+        c_ptr, c_i32,
+        c_ptr, c_i64, c_i64,
+        c_i32, c_i32, c_i32, c_i32,
+        c_f32, c_ptr, c_size, c_ptr]),
+    "wgkv_build_block_tables_block": (ctypes.c_int, [ctypes.c_char_p]),
+    "wgkv_paged_append_block": (ctypes.c_int, [ctypes.c_char_p]),
+    "wgkv_sink_window_attn_block": (ctypes.c_int, [ctypes.c_char_p]),
+    "wgkv_paged_decode_attn_window_block": (ctypes.c_int, [ctypes.c_char_p]),
+    "wgkv_shared_decode_attn_block": (ctypes.c_int, [ctypes.c_char_p]),
 }
 
 _lib = None

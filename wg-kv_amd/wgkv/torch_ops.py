@@ -20,10 +20,17 @@ Operators (schemas below):
   paged_decode_attn_kv4   -- paged_decode_attn over a cache held in 4 bits
   kv4_read                -- such a cache's rows as dense tensors (no
                              reference counterpart, both)
+  sink_window_attn        -- packed prompts, a sliding window and first tokens
+  paged_decode_attn_window -- the same for one token over a paged cache
+  paged_decode_attn_shared -- one token over a prefix that sequences share (no
+                             reference counterpart, the three)
 """
 import torch
 
 from . import ops as _ops
+from .batch import paged_decode_attn_shared as _paged_decode_attn_shared
+from .batch import paged_decode_attn_window as _paged_decode_attn_window
+from .batch import sink_window_attn as _sink_window_attn
 from .gate import gate_scores_and_mask as _gate_scores_and_mask
 from .gate import pack_weights as _pack_weights
 from .kv4 import kv4_read as _kv4_read
@@ -47,6 +54,13 @@ _LIB.define("paged_decode_attn_kv4(Tensor q, Tensor k_cache, Tensor v_cache, Ten
             "Tensor block_table, float softmax_scale) -> Tensor")
 _LIB.define("kv4_read(Tensor k_cache, Tensor v_cache, Tensor block_table, Tensor lengths, int rows, "
             "Tensor? starts=None, ScalarType dtype=bfloat16) -> (Tensor, Tensor)")
+_LIB.define("sink_window_attn(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens, int window, int num_sinks, "
+            "float? softmax_scale=None, Tensor? cu_seqlens_k=None) -> Tensor")
+_LIB.define("paged_decode_attn_window(Tensor q, Tensor k_cache, Tensor v_cache, Tensor cache_seqlens, "
+            "Tensor block_table, int window, int num_sinks, float softmax_scale) -> Tensor")
+_LIB.define("paged_decode_attn_shared(Tensor q, Tensor k_cache, Tensor v_cache, Tensor cache_seqlens, "
+            "Tensor block_table, Tensor prefix_lens, Tensor prefix_table, Tensor group_starts, float softmax_scale) "
+            "-> Tensor")
 
 
 # ---- CUDA (HIP) kernels: the library calls ----------------------------------
@@ -80,6 +94,9 @@ def _kv4_read_op(k_cache, v_cache, block_table, lengths, rows, starts=None, dtyp
 
 
 _LIB.impl("sparse_attn", _sparse_attn, "CUDA")
+_LIB.impl("sink_window_attn", lambda *a: _sink_window_attn(*a), "CUDA")
+_LIB.impl("paged_decode_attn_window", lambda *a: _paged_decode_attn_window(*a), "CUDA")
+_LIB.impl("paged_decode_attn_shared", lambda *a: _paged_decode_attn_shared(*a), "CUDA")
 _LIB.impl("paged_decode_attn_kv4", _paged_decode_attn_kv4, "CUDA")
 _LIB.impl("kv4_read", _kv4_read_op, "CUDA")
 _LIB.impl("paged_decode_attn", _paged_decode_attn, "CUDA")
@@ -135,6 +152,12 @@ def _kv4_read_meta(k_cache, v_cache, block_table, lengths, rows, starts=None, dt
     return tuple(torch.empty(shape, dtype=dtype, device=k_cache.device) for _ in range(2))
 
 
+def _like_q_meta(q, *_):
+    return torch.empty_like(q, memory_format=torch.contiguous_format)
+
+
+for _name in ("sink_window_attn", "paged_decode_attn_window", "paged_decode_attn_shared"):
+    _LIB.impl(_name, _like_q_meta, "Meta")
 _LIB.impl("paged_decode_attn_kv4", _paged_decode_attn_kv4_meta, "Meta")
 _LIB.impl("kv4_read", _kv4_read_meta, "Meta")
 _LIB.impl("gate_scores_and_mask", _gate_meta, "Meta")
