@@ -741,8 +741,9 @@ int wgkv_kv4_decode_attn_block(const void* args);
  *
  * wgkv_paged_decode_attn_window: wgkv_paged_decode_attn where a head of T
  * tokens shows those t with t >= T - window or t < num_sinks.  Page ids of the
- * others are not read.  Same workspace (its counters zero before a call and
- * after it).
+ * others are not read.  The workspace's first 8192 bytes (per-head arrival
+ * counters) must be zero before a call; every call leaves them zero.  Calls
+ * that share a workspace must be ordered.
  *
  * wgkv_shared_decode_attn: wgkv_paged_decode_attn where sequences
  * group_starts[n] .. group_starts[n+1]-1 (i32 (num_groups+1), ascending) also
@@ -776,6 +777,9 @@ int wgkv_sink_window_attn(
     const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int32_t batch, int32_t num_rows, int32_t num_keys,
     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
     int32_t window, int32_t num_sinks, float softmax_scale, int32_t clear_rest, void* stream);
+
+size_t wgkv_paged_decode_window_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                                int32_t head_dim);
 
 int wgkv_paged_decode_attn_window(
     const void* q, int64_t q_stride_b, int64_t q_stride_h,

@@ -39,10 +39,12 @@
 //     arrival count cost as much as the second launch, which spreads the
 //     merge over B*Hkv*G workgroups).
 #include <string.h>
+#include <stdlib.h>
 
 #include <mutex>
 
 #include "kv4.h"
+#include "stream_attn.h"
 
 namespace {
 
@@ -881,6 +883,18 @@ extern "C" int wgkv_paged_decode_attn_noalloc(
                                 kScratchBytes, stream);
 }
 
+namespace {
+bool stream_window(int heads) { return heads > (getenv("SW") ? atoi(getenv("SW")) : 128); }
+}
+
+extern "C" size_t wgkv_paged_decode_window_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
+                                                           int32_t head_dim) {
+  if (batch <= 0 || num_kv_heads <= 0 || num_q_heads < num_kv_heads || head_dim <= 0) return 0;
+  const size_t chunks = wgkv_paged_decode_workspace_bytes(batch, num_kv_heads, head_dim);
+  const size_t stream = kCounterBytes + wgkv_stream_window_bytes(batch, num_kv_heads, num_q_heads / num_kv_heads, head_dim);
+  return chunks > stream ? chunks : stream;
+}
+
 extern "C" int wgkv_paged_decode_attn_window(
     const void* q, int64_t q_stride_b, int64_t q_stride_h,
     const void* k_cache, const void* v_cache, int64_t num_pages, int32_t page_size,
@@ -903,7 +917,7 @@ extern "C" int wgkv_paged_decode_attn_window(
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return WGKV_ERR_UNSUPPORTED;
   if ((q_stride_b | q_stride_h) & 7) return WGKV_ERR_UNSUPPORTED;
   if (kv4_rows_meet({batch, num_q_heads, 1, 1}, {out_stride_b, out_stride_h, 0, 0}, head_dim)) return WGKV_ERR_ARG;
-  if (!workspace || workspace_bytes < wgkv_paged_decode_workspace_bytes(batch, num_kv_heads, head_dim) ||
+  if (!workspace || workspace_bytes < wgkv_paged_decode_window_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim) ||
       ((uintptr_t)workspace & 15))
     return WGKV_ERR_WORKSPACE;
   DecodeArgs a;
@@ -940,6 +954,12 @@ extern "C" int wgkv_paged_decode_attn_window(
   a.part_acc = ws + (size_t)kMaxChunks * kMaxG * 2;
   a.plan = (int*)(ws + part_floats(head_dim));
   hipStream_t st = (hipStream_t)stream;
+  if (stream_window(batch * num_kv_heads)) {
+    const StreamWindow w = {a.q, q_stride_b, q_stride_h, a.kc, a.vc, num_pages, a.page_shift, cache_seqlens, sl_stride_b,
+                            block_table, bt_stride_b, bt_stride_h, (int)cap, a.out, out_stride_b, out_stride_h, batch,
+                            num_kv_heads, G, head_dim, window, num_sinks, a.scale_log2, a.q_and, a.q_xor};
+    return wgkv_stream_window(w, ws, st);
+  }
   const hipError_t e = head_dim == 128 ? launch_g<128, true>(a, G, st) : launch_g<64, true>(a, G, st);
   return e == hipSuccess ? WGKV_OK : WGKV_ERR_HIP;
 }

@@ -280,9 +280,9 @@ def _token_out(q, out):
     return (out, out.data_ptr(), st) if st[3] == 1 else None
 
 
-@functools.lru_cache(maxsize=None)
-def _window_bytes(D):
-    return _lib.lib().wgkv_paged_decode_workspace_bytes(1, 1, D)
+@functools.lru_cache(maxsize=1024)
+def _window_bytes(B, Hq, H, D):
+    return _lib.lib().wgkv_paged_decode_window_workspace_bytes(B, Hq, H, D)
 
 
 def paged_decode_attn_window(q, k_cache, v_cache, cache_seqlens, block_table, window, num_sinks, softmax_scale, out=None):
@@ -311,7 +311,7 @@ def paged_decode_attn_window(q, k_cache, v_cache, cache_seqlens, block_table, wi
     out, op, os = rows
     q, qp, qs = _rows(q, 8)
     stream = _stream(dev)
-    ws = _attn_workspace(dev, stream, _window_bytes(D))
+    ws = _attn_workspace(dev, stream, _window_bytes(B, Hq, H, D))
     st = _lib.lib().wgkv_paged_decode_attn_window_block(_pack_window(
         qp, qs[0], qs[2], k_cache.data_ptr(), v_cache.data_ptr(), pool[0], pool[1], lens.data_ptr(), ls,
         table.data_ptr(), bs[0], bs[1], width, op, os[0], os[2], B, Hq, H, D, min(window, _MOST), min(num_sinks, _MOST),
