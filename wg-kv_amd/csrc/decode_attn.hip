@@ -39,7 +39,6 @@
 //     arrival count cost as much as the second launch, which spreads the
 //     merge over B*Hkv*G workgroups).
 #include <string.h>
-#include <stdlib.h>
 
 #include <mutex>
 
@@ -188,27 +187,26 @@ __device__ Plan plan_wave(const DecodeArgs& a, int w) {
 
 // B*Hkv > 64 (4-wave workgroups): block scans over the heads through LDS
 // (workgroup 0 stores the plan for the merge kernel).
-template <bool WIN>
 __device__ Plan plan_block(const DecodeArgs& a, int w, int* s_pref, int* s_tmp) {
   const int BH = a.B * a.Hkv;
   const int t = threadIdx.x;
   const int per = (BH + kPlanThreads - 1) / kPlanThreads;
   const int lo = min(BH, t * per), hi = min(BH, lo + per);
   int subs = 0;
-  for (int bh = lo; bh < hi; ++bh) subs += head_subpages<WIN>(a, bh);
+  for (int bh = lo; bh < hi; ++bh) subs += head_subpages<false>(a, bh);
   int total = 0;
   block_exclusive_scan_256(subs, s_tmp, &total);
   const int cp = chunk_subpages<4>(total, a.target_chunks);
   int chunks = 0;
   for (int bh = lo; bh < hi; ++bh) {
-    const int ns = head_subpages<WIN>(a, bh);
+    const int ns = head_subpages<false>(a, bh);
     chunks += max(1, (ns + cp - 1) / cp);
   }
   int n_chunks = 0;
   int run = block_exclusive_scan_256(chunks, s_tmp, &n_chunks);
   for (int bh = lo; bh < hi; ++bh) {
     s_pref[bh] = run;
-    const int ns = head_subpages<WIN>(a, bh);
+    const int ns = head_subpages<false>(a, bh);
     run += max(1, (ns + cp - 1) / cp);
   }
   if (t == 0) s_pref[BH] = n_chunks;
@@ -285,7 +283,7 @@ void decode_split_kernel(DecodeArgs a) {
   constexpr int NV = 64 / RPI;     // V loads per quad
   constexpr int NG = (G + 3) / 4;  // groups of 4 query heads (MFMA A operands)
   static_assert(G <= kMaxG, "query heads per KV head");
-  static_assert(NW == 4 || (NW == 8 && G <= 4), "4-wave workgroups, or 8-wave ones for G <= 4");
+  static_assert(NW == 8 ? G <= 4 : NW == 4 && !WIN, "4-wave workgroups, or 8-wave ones (windows too) for G <= 4");
 
   constexpr bool kFused = NW > 4;  // the last chunk of a head merges (see top)
   // s_buf: each wave's (RPI, G, D) accumulators, then the fused merge's
@@ -301,7 +299,7 @@ void decode_split_kernel(DecodeArgs a) {
   if constexpr (NW == 4) {
     __shared__ int s_pref[kMaxBH + 1];
     __shared__ int s_tmp[kPlanThreads];
-    pl = a.B * a.Hkv <= kWaveBH ? plan_wave<NW, WIN>(a, w) : plan_block<WIN>(a, w, s_pref, s_tmp);
+    pl = a.B * a.Hkv <= kWaveBH ? plan_wave<NW, WIN>(a, w) : plan_block(a, w, s_pref, s_tmp);
   } else {
     pl = plan_wave<NW, WIN>(a, w);  // the host takes 8 waves only for B*Hkv < 32
   }
@@ -716,9 +714,10 @@ hipError_t launch_nw(DecodeArgs a, hipStream_t st) {
 template <int D, int G, bool WIN>
 hipError_t launch(const DecodeArgs& a, hipStream_t st) {
   if constexpr (G <= 4) {
-    if (a.B * a.Hkv < kWideBelowBH) return launch_nw<D, G, 8, WIN>(a, st);
+    if (WIN || a.B * a.Hkv < kWideBelowBH) return launch_nw<D, G, 8, WIN>(a, st);
   }
-  return launch_nw<D, G, 4, WIN>(a, st);
+  if constexpr (WIN) return hipErrorInvalidValue;  // (in_ranges)
+  else return launch_nw<D, G, 4, WIN>(a, st);
 }
 
 template <int D, bool WIN>
@@ -884,8 +883,16 @@ extern "C" int wgkv_paged_decode_attn_noalloc(
 }
 
 namespace {
-bool stream_window(int heads) { return heads > (getenv("SW") ? atoi(getenv("SW")) : 128); }
-}
+
+// Windows of a batch with many heads, or more than four query heads each, are
+// cut into even ranges of all heads' tokens (stream_attn.hip): chunks of one
+// size leave heads of about that size a full and a small one (64 x 8 heads of
+// 4160 tokens 303 us in chunks, 194 in ranges; 32 x 8 heads 121 / 104; 16 x 8
+// 67 / 53; 8 x 8 40.5 / 36.2, of 32772 tokens 203 / 192; 5 x 8 of 704 tokens
+// 15.2 / 16.7).  Few heads take the 8-wave chunks, which need one launch.
+bool in_ranges(int heads, int G) { return heads >= kWideBelowBH || G > 4; }
+
+}  // namespace
 
 extern "C" size_t wgkv_paged_decode_window_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                                            int32_t head_dim) {
@@ -954,7 +961,7 @@ extern "C" int wgkv_paged_decode_attn_window(
   a.part_acc = ws + (size_t)kMaxChunks * kMaxG * 2;
   a.plan = (int*)(ws + part_floats(head_dim));
   hipStream_t st = (hipStream_t)stream;
-  if (stream_window(batch * num_kv_heads)) {
+  if (in_ranges(batch * num_kv_heads, G)) {
     const StreamWindow w = {a.q, q_stride_b, q_stride_h, a.kc, a.vc, num_pages, a.page_shift, cache_seqlens, sl_stride_b,
                             block_table, bt_stride_b, bt_stride_h, (int)cap, a.out, out_stride_b, out_stride_h, batch,
                             num_kv_heads, G, head_dim, window, num_sinks, a.scale_log2, a.q_and, a.q_xor};

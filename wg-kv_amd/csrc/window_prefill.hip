@@ -28,41 +28,13 @@
 // (exact_rows).
 #include <string.h>
 
+#include "attn_tile.h"
 #include "kv4.h"
 
 namespace {
 
-constexpr int kBlk = 64;      // query rows per item and keys per tile
+constexpr int kBlk = 64;      // query rows per item
 constexpr int kMaxSeqs = 2048;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSlack = 8.f;  // log2 units a row maximum may lag its scores
-
-WGKV_DEVICE float fmax_ieee(float x, float y) { return __builtin_elementwise_maximum(x, y); }
-WGKV_DEVICE float xor16_max(float x) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmax_ieee(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-WGKV_DEVICE float xor32_max(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return fmax_ieee(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-typedef short v4i16_t __attribute__((ext_vector_type(4)));
-
-// The 16 bytes at g go to LDS at lds + 16 * lane (lds the same in every lane).
-WGKV_DEVICE void lds_dma16(const uint16_t* g, uint16_t* lds) { __builtin_amdgcn_global_load_lds(g, lds, 16, 0, 0); }
-
-WGKV_DEVICE v4i16_t lds_read_tr16(const uint16_t* p) {
-  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4i16_t __attribute__((address_space(3)))*)(p));
-}
-
-// Places of a row's 16-byte slices in an unpadded LDS tile: slice c of row r
-// is at c ^ swz(r).  16 consecutive rows of a K operand, and the 8 rows of a
-// V transpose read, then lie on different banks.
-template <int D>
-WGKV_DEVICE int swz_k(int row) { return D == 128 ? (row & 15) : ((row >> 1) & 7); }
-template <int D>
-WGKV_DEVICE int swz_v(int row) { return D == 128 ? 2 * (row & 7) : 2 * ((row >> 1) & 3); }
 
 struct WindowArgs {
   const uint16_t* q;
@@ -84,18 +56,32 @@ struct WindowArgs {
 
 WGKV_DEVICE int clamp_to(int x, int hi) { return min(max(x, 0), hi); }
 
+// A value that every lane holds, as a scalar.
+WGKV_DEVICE int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+typedef const int32_t __attribute__((address_space(4))) ConstInt;
+
+// A sequence's rows and keys (scalar loads where b is a scalar).
+struct Seq {
+  int q0, nq, k0, nk;
+};
+WGKV_DEVICE Seq seq_of(const WindowArgs& a, int b) {
+  ConstInt *q = (ConstInt*)a.cu_q, *k = (ConstInt*)a.cu_k;
+  const int q0 = clamp_to(q[b], a.N), k0 = clamp_to(k[b], a.Nk);
+  return {q0, max(clamp_to(q[b + 1], a.N) - q0, 0), k0, max(clamp_to(k[b + 1], a.Nk) - k0, 0)};
+}
+
 // The keys of an item as one list: entry x is key x for x < first, else key x + shift.
 struct Keys {
   int first, shift, count;
   WGKV_DEVICE int key(int x) const { return x < first ? x : x + shift; }
 };
 
-// The rows of one wave, key by key, for results that are not finite.  32
-// lanes of a wave would idle in a matrix of one row, so a lane takes D/64
-// values of d and the wave one row.
+// A row key by key, for results that are not finite: a wave, D/64 values of d
+// each lane.
 template <int D>
-WGKV_DEVICE void exact_row(const WindowArgs& a, const uint16_t* q, const uint16_t* k,
-                                                    const uint16_t* v, int p, uint16_t* out, int lane) {
+WGKV_DEVICE void exact_row(const WindowArgs& a, const uint16_t* q, const uint16_t* k, const uint16_t* v, int p,
+                           uint16_t* out, int lane) {
   constexpr int C = D / 64;
   float qf[C], acc[C], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -126,37 +112,74 @@ WGKV_DEVICE void exact_row(const WindowArgs& a, const uint16_t* q, const uint16_
   for (int c = 0; c < C; ++c) out[lane * C + c] = l == 0.f ? 0 : f32_to_bf16(acc[c] * inv);
 }
 
-template <int D, int HPW>
-__global__ __launch_bounds__(128 * HPW) void window_prefill_kernel(WindowArgs a) {
-  constexpr int NT = 128 * HPW;
-  constexpr int KS = D / 32;       // k-steps over head_dim
-  constexpr int DT = D / 16;       // 16-wide d tiles
+struct Item {
+  int q0, nq, nk;     // the sequence's first row, rows and keys
+  int r_blk, p_blk;   // the item's first row in the sequence, and its position
+  int h, hq0;         // KV head, first query head
+  Keys keys;
+  int tiles;
+  const uint16_t *kb, *vb;
+};
+
+WGKV_DEVICE Keys keys_of(const WindowArgs& a, int p_blk, int p_last) {
+  if (p_last < 0) return {0, 0, 0};
+  const int lo = max(0, p_blk - a.window + 1), first = min(a.sinks, lo);
+  return {first, lo - first, first + p_last - lo + 1};
+}
+
+// The block's sequence, rows and keys; s_blocks: row blocks of the sequences before each.
+WGKV_DEVICE void find_block(const WindowArgs& a, const int* s_blocks, int blk, int* seq, int* r_blk, int* p_blk,
+                            Keys* keys) {
+  int b = 0;
+  for (int hi = a.B - 1; b < hi;) {  // the last sequence that begins at or before the block
+    const int mid = (b + hi + 1) >> 1;
+    if (s_blocks[mid] <= blk) b = mid; else hi = mid - 1;
+  }
+  const Seq s = seq_of(a, b);
+  *seq = b;
+  *r_blk = (blk - s_blocks[b]) * kBlk;
+  *p_blk = *r_blk + s.nk - s.nq;
+  *keys = keys_of(a, *p_blk, *p_blk + min(kBlk, s.nq - *r_blk) - 1);
+}
+
+// A buffer of `bytes` at p (a scalar address), and 16 bytes of it to LDS at lds
+// + 16 * lane; beyond its end they are zeros.
+WGKV_DEVICE __amdgpu_buffer_rsrc_t rows_buffer(const uint16_t* p, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)p, (short)0, bytes, 0x00020000);
+}
+WGKV_DEVICE void buffer_to_lds(__amdgpu_buffer_rsrc_t r, uint16_t* lds, int off) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 16, off, 0, 0, 0);
+}
+
+// FAR: keys that may lie 2^31 bytes or more apart.
+template <int D, int HPW, bool FAR>
+__global__ __launch_bounds__(128 * HPW) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void window_prefill_kernel(WindowArgs a) {
+  constexpr int NT = 128 * HPW, NW = 2 * HPW;
   constexpr int CH = D / 8;        // 16-byte slices per row
-  constexpr int NW = 2 * HPW;
   constexpr int RPB = 64 / CH;     // key rows of 1 KB of LDS, one load instruction of a wave
-  constexpr int NBLK = kBlk / RPB;
+  constexpr int NBLK = attn::kKeys / RPB;
   // with four heads only the older wave of each SIMD loads: it reaches the
   // tile's barrier first
   constexpr int NL = HPW == 4 ? NW / 2 : NW;
   constexpr int KPT = NBLK / NL;
   static_assert(NBLK % NL == 0, "every loading wave loads whole 1 KB blocks");
   // four LDS objects: loads into one buffer then provably leave the other alone
-  __shared__ __attribute__((aligned(16))) uint16_t sK0[kBlk * D];
-  __shared__ __attribute__((aligned(16))) uint16_t sK1[kBlk * D];
-  __shared__ __attribute__((aligned(16))) uint16_t sV0[kBlk * D];
-  __shared__ __attribute__((aligned(16))) uint16_t sV1[kBlk * D];
-  __shared__ int s_blocks[kMaxSeqs + 1];  // row blocks of the sequences before
+  __shared__ __attribute__((aligned(16))) uint16_t sK0[attn::kKeys * D];
+  __shared__ __attribute__((aligned(16))) uint16_t sK1[attn::kKeys * D];
+  __shared__ __attribute__((aligned(16))) uint16_t sV0[attn::kKeys * D];
+  __shared__ __attribute__((aligned(16))) uint16_t sV1[attn::kKeys * D];
+  __shared__ int s_blocks[kMaxSeqs + 1];               // row blocks of the sequences before
   __shared__ int s_wave[NW];
 
   const int t = threadIdx.x;
-  const int lane = t & 63, wid = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int lane = t & 63, wid = uniform(t >> 6);
   const int n = lane & 15, g = lane >> 4;
 
   {
     const int per = (a.B + NT - 1) / NT, b0 = min(a.B, t * per), b1 = min(a.B, b0 + per);
     int mine = 0;
-    for (int b = b0; b < b1; ++b)
-      mine += (max(clamp_to(a.cu_q[b + 1], a.N) - clamp_to(a.cu_q[b], a.N), 0) + kBlk - 1) / kBlk;
+    for (int b = b0; b < b1; ++b) mine += (seq_of(a, b).nq + kBlk - 1) / kBlk;
     const int incl = wave_incl_scan(mine, lane);
     if (lane == 63) s_wave[wid] = incl;
     __syncthreads();
@@ -164,11 +187,13 @@ __global__ __launch_bounds__(128 * HPW) void window_prefill_kernel(WindowArgs a)
     for (int i = 0; i < NW; ++i) run += i < wid ? s_wave[i] : 0;
     for (int b = b0; b < b1; ++b) {
       s_blocks[b] = run;
-      run += (max(clamp_to(a.cu_q[b + 1], a.N) - clamp_to(a.cu_q[b], a.N), 0) + kBlk - 1) / kBlk;
+      run += (seq_of(a, b).nq + kBlk - 1) / kBlk;
       if (b == a.B - 1) s_blocks[a.B] = run;
     }
     __syncthreads();
   }
+  const int blocks = uniform(s_blocks[a.B]);
+  const int per_block = a.Hkv * (a.G / HPW);
   if (a.clear_rest) {
     const int head = clamp_to(a.cu_q[0], a.N), tail = max(clamp_to(a.cu_q[a.B], a.N), head);
     const int64_t pieces = (int64_t)(head + a.N - tail) * a.Hkv * a.G * CH;
@@ -178,243 +203,203 @@ __global__ __launch_bounds__(128 * HPW) void window_prefill_kernel(WindowArgs a)
           (u32x4_t){0u, 0u, 0u, 0u};
     }
   }
+  const attn::Offsets<D> at(n, g);
 
-  // Per-lane LDS element offsets of the operands
-  int koff[KS];
-#pragma unroll
-  for (int j = 0; j < KS; ++j) koff[j] = n * D + ((j * 4 + g) ^ swz_k<D>(n)) * 8;
-  const int vrow = 4 * g + (n >> 2);
-  int voff[DT];
-#pragma unroll
-  for (int dt = 0; dt < DT; ++dt)
-    voff[dt] = vrow * D + ((2 * dt + ((n & 3) >> 1)) ^ swz_v<D>(vrow)) * 8 + (n & 1) * 4;
-
-  // Items from the last row block to the first -- later blocks of a sequence
-  // see no fewer keys --, heads innermost: workgroups are dealt to the XCDs in
-  // turn, so with 8 KV heads each XCD's L2 serves one head's keys.  A
-  // workgroup takes items from alternate ends of its rounds.
-  const int per_block = a.Hkv * (a.G / HPW);
-  const int64_t items = (int64_t)s_blocks[a.B] * per_block;
-  for (int round = 0;; ++round) {
+  // A round's item.  Items go from the last row block to the first -- later
+  // blocks of a sequence see no fewer keys --, heads innermost: workgroups are
+  // dealt to the XCDs in turn, so with 8 KV heads each XCD's L2 serves one
+  // head's keys.  A workgroup takes items from alternate ends of its rounds.
+  const auto item_at = [&](int round, Item* p) {
     const int64_t item = (int64_t)round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    if (item >= items) break;
-    if (round) __syncthreads();  // every wave is done with the previous item's tiles
-    const int blk = s_blocks[a.B] - 1 - (int)(item / per_block), rest = (int)(item % per_block);
-    int b = 0;
-    for (int hi = a.B - 1; b < hi;) {  // the last sequence that begins at or before the block
-      const int mid = (b + hi + 1) >> 1;
-      if (s_blocks[mid] <= blk) b = mid; else hi = mid - 1;
-    }
-    const int h = rest % a.Hkv, hq = h * a.G + (rest / a.Hkv) * HPW + (wid >> 1);
-    const int q0 = clamp_to(a.cu_q[b], a.N), nq = max(clamp_to(a.cu_q[b + 1], a.N) - q0, 0);
-    const int k0 = clamp_to(a.cu_k[b], a.Nk), nk = max(clamp_to(a.cu_k[b + 1], a.Nk) - k0, 0);
-    const int r_blk = (blk - s_blocks[b]) * kBlk;             // the item's rows in the sequence
-    const int n_rows = min(kBlk, nq - r_blk);
-    const int p_blk = r_blk + nk - nq;                         // the first row's position
-    const int r0 = r_blk + (wid & 1) * 32, p0 = p_blk + (wid & 1) * 32;  // the wave's
-    const int p_last = p_blk + n_rows - 1;
-    Keys ks = {0, 0, 0};
-    if (p_last >= 0) {
-      const int lo = max(0, p_blk - a.window + 1);
-      ks.first = min(a.sinks, lo);
-      ks.shift = lo - ks.first;
-      ks.count = ks.first + p_last - lo + 1;
-    }
-    const int ntiles = (ks.count + kBlk - 1) / kBlk;
-    const uint16_t* kbase = a.k + (int64_t)k0 * a.k_sn + (int64_t)h * a.k_sh;
-    const uint16_t* vbase = a.v + (int64_t)k0 * a.v_sn + (int64_t)h * a.v_sh;
+    if (item >= (int64_t)blocks * per_block) return false;
+    const int of = uniform((int)(item / per_block)), rest = uniform((int)(item - (int64_t)of * per_block));
+    const int blk = blocks - 1 - of;
+    int seq, r_blk, p_blk;
+    Keys k;
+    find_block(a, s_blocks, blk, &seq, &r_blk, &p_blk, &k);
+    const Seq s = seq_of(a, uniform(seq));
+    p->q0 = uniform(s.q0);
+    p->nq = uniform(s.nq);
+    p->nk = uniform(s.nk);
+    p->r_blk = uniform(r_blk);
+    p->p_blk = uniform(p_blk);
+    p->keys = {uniform(k.first), uniform(k.shift), uniform(k.count)};
+    p->tiles = (p->keys.count + attn::kKeys - 1) / attn::kKeys;
+    p->h = uniform(rest % a.Hkv);
+    p->hq0 = p->h * a.G + uniform(rest / a.Hkv) * HPW;
+    const int k0 = uniform(s.k0);
+    p->kb = a.k + (int64_t)k0 * a.k_sn + (int64_t)p->h * a.k_sh;
+    p->vb = a.v + (int64_t)k0 * a.v_sn + (int64_t)p->h * a.v_sh;
+    return true;
+  };
 
-    // queries as the B operand: lane (row n, slice g) of row tile rt, k-step j
-    bf16x8_t qb[2][KS];
-#pragma unroll
-    for (int rt = 0; rt < 2; ++rt) {
-      const int s = min(r0 + rt * 16 + n, nq - 1);
-      const uint16_t* qrow = a.q + (int64_t)(q0 + s) * a.q_sn + (int64_t)hq * a.q_sh;
-#pragma unroll
-      for (int j = 0; j < KS; ++j) {
-        const u32x4_t w = *(const u32x4_t*)(qrow + (j * 4 + g) * 8);
-        qb[rt][j] = __builtin_bit_cast(bf16x8_t, (w & a.q_and) ^ a.q_xor);
-      }
-    }
-    float m_run[2] = {-INFINITY, -INFINITY};
-    f32x4_t lsum[2] = {(f32x4_t){0.f, 0.f, 0.f, 0.f}, (f32x4_t){0.f, 0.f, 0.f, 0.f}};
-    const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, (u32x4_t){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u});
-    f32x4_t o[DT][2];
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int rt = 0; rt < 2; ++rt) o[dt][rt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-
-    // Loading wave w fills the 1 KB blocks w, w + NL, ...: in block q lane i
-    // loads slice (i % CH) ^ swz of list entry q * RPB + i / CH.
-    auto tile_load = [&](int tl, uint16_t* dK, uint16_t* dV) __attribute__((always_inline)) {
-      if (wid >= NL) return;
+  // Loading wave w fills the 1 KB blocks w, w + NL, ...: in block q lane i
+  // loads slice (i % CH) ^ swz of list entry q * RPB + i / CH.  A lane's offset
+  // within a tile stays, but for the jump behind the first tokens; entries
+  // behind the sequence's keys read as zeros (and are masked).
+  const auto tile_load = [&](const Item& p, int tl, bool on, uint16_t* dK, uint16_t* dV) __attribute__((always_inline)) {
+    if (wid >= NL) return;
+    const Keys& ks = p.keys;
+    const int x0 = tl * attn::kKeys;
+    if constexpr (!FAR) {
+      const int j0 = ks.key(x0);
+      const int rows = p.nk - j0 - 1;  // (nothing is asked for where there is no tile)
+      const auto kr = rows_buffer(p.kb + (int64_t)j0 * a.k_sn, uniform(on ? rows * (int)(a.k_sn * 2) + D * 2 : 0));
+      const auto vr = rows_buffer(p.vb + (int64_t)j0 * a.v_sn, uniform(on ? rows * (int)(a.v_sn * 2) + D * 2 : 0));
+      const int jump = x0 < ks.first ? ks.shift : 0;
+      const int k_jump = jump * (int)(a.k_sn * 2), v_jump = jump * (int)(a.v_sn * 2);
 #pragma unroll
       for (int i = 0; i < KPT; ++i) {
-        const int row = (wid + i * NL) * RPB + lane / CH, blk1k = (wid + i * NL) * 512;
-        const int64_t j = ks.key(min(tl * kBlk + row, ks.count - 1));
-        lds_dma16(kbase + j * a.k_sn + ((lane % CH) ^ swz_k<D>(row)) * 8, dK + blk1k);
-        lds_dma16(vbase + j * a.v_sn + ((lane % CH) ^ swz_v<D>(row)) * 8, dV + blk1k);
+        int row = (wid + i * NL) * RPB + lane / CH;
+        asm volatile("" : "+v"(row));  // worked out here: over the loop there are no registers to keep it in
+        const bool over = x0 + row >= ks.first;
+        buffer_to_lds(kr, dK + (wid + i * NL) * 512,
+                      row * (int)(a.k_sn * 2) + ((lane % CH) ^ attn::swz_k<D>(row)) * 16 + (over ? k_jump : 0));
+        buffer_to_lds(vr, dV + (wid + i * NL) * 512,
+                      row * (int)(a.v_sn * 2) + ((lane % CH) ^ attn::swz_v<D>(row)) * 16 + (over ? v_jump : 0));
       }
-    };
-    if (ntiles > 0) tile_load(0, sK0, sV0);
+    } else if (on) {
+#pragma unroll
+      for (int i = 0; i < KPT; ++i) {
+        const int row = (wid + i * NL) * RPB + lane / CH;
+        const int64_t j = ks.key(min(x0 + row, ks.count - 1));
+        attn::lds_dma16(p.kb + j * a.k_sn + ((lane % CH) ^ attn::swz_k<D>(row)) * 8, dK + (wid + i * NL) * 512);
+        attn::lds_dma16(p.vb + j * a.v_sn + ((lane % CH) ^ attn::swz_v<D>(row)) * 8, dV + (wid + i * NL) * 512);
+      }
+    }
+  };
+  const auto load_rows = [&](const Item& p, attn::Rows32<D>& r) __attribute__((always_inline)) {
+    const int r0 = p.r_blk + (wid & 1) * 32;
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt)
+      r.load_q(rt, a.q + (int64_t)(p.q0 + min(r0 + rt * 16 + n, p.nq - 1)) * a.q_sn + (int64_t)(p.hq0 + (wid >> 1)) * a.q_sh,
+               g, a.q_and, a.q_xor);
+  };
 
-    auto step = [&](int tile, const uint16_t* sK, const uint16_t* sV, uint16_t* nK,
-                    uint16_t* nV) __attribute__((always_inline)) {
+  Item cur = {}, nxt = {};
+  bool more = item_at(0, &cur);
+  if (more) tile_load(cur, 0, cur.tiles > 0, sK0, sV0);
+  for (int round = 1; more; ++round) {
+    more = item_at(round, &nxt);
+    const Keys& ks = cur.keys;
+    const int r0 = cur.r_blk + (wid & 1) * 32, p0 = cur.p_blk + (wid & 1) * 32;  // the wave's rows
+    attn::Rows32<D> r;
+    load_rows(cur, r);
+    r.clear();
+    const auto step = [&](int tile, const uint16_t* sK, const uint16_t* sV, uint16_t* nK, uint16_t* nV,
+                          bool second) __attribute__((always_inline)) {
       __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's loads of the tile have landed
       __syncthreads();
-      if (tile + 1 < ntiles) tile_load(tile + 1, nK, nV);
-      const int x0 = tile * kBlk, x1 = min(x0 + kBlk, ks.count) - 1;  // the tile's list entries
-      // the wave's rows p0 .. p0 + 31 see something of it?  (the list ascends,
-      // so its band part is [max(x0, first), x1])
-      const bool firsts = x0 < ks.first;
-      const int band_lo = max(x0, ks.first) + ks.shift, band_hi = x1 + ks.shift;
-      const bool band = x1 >= ks.first && band_lo <= p0 + 31 && p0 - band_hi < a.window;
-      if (!firsts && !band) return;
+      // the coming tile, of this item or (into the first buffers) the next
+      const bool last = tile + 1 >= cur.tiles;
+      tile_load(last ? nxt : cur, last ? 0 : tile + 1, !last || (second && more && nxt.tiles > 0), nK, nV);
+      // Row p sees the list's entries x <= p - shift, of them those > p -
+      // window - shift or < sinks.  (Of the first tokens, below the band, all
+      // rows see all.)
+      const int x0 = tile * attn::kKeys, x1 = min(x0 + attn::kKeys, ks.count) - 1;
+      const int e0 = p0 - ks.shift, e1 = e0 + 31;  // the last entries of the wave's first and last row
       f32x4_t sc[4][2];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int rt = 0; rt < 2; ++rt) sc[kt][rt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-      bf16x8_t kf[2][4];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-        kf[0][kt] = __builtin_bit_cast(bf16x8_t, *(const u32x4_t*)(&sK[kt * 16 * D + koff[0]]));
-#pragma unroll
-      for (int j = 0; j < KS; ++j) {
-        if (j + 1 < KS)
-#pragma unroll
-          for (int kt = 0; kt < 4; ++kt)
-            kf[(j + 1) & 1][kt] = __builtin_bit_cast(bf16x8_t, *(const u32x4_t*)(&sK[kt * 16 * D + koff[j + 1]]));
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int rt = 0; rt < 2; ++rt)
-            sc[kt][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[j & 1][kt], qb[rt][j], sc[kt][rt], 0, 0, 0);
-      }
-      // all 64 keys visible to all 32 rows?
-      const bool full = x0 + kBlk <= ks.count && p0 >= 0 &&
-                        (x1 < ks.first || (band_hi <= p0 && p0 + 31 - band_lo < a.window));
-      float mxs[2];
-#pragma unroll
-      for (int rt = 0; rt < 2; ++rt) {
-        if (!full) {
-          const int p = p0 + rt * 16 + n;
-#pragma unroll
-          for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int x = x0 + kt * 16 + 4 * g + i, j = ks.key(x);
-              const bool see = x < ks.count && j <= p && (p - j < a.window || j < a.sinks);
-              sc[kt][rt][i] = see ? sc[kt][rt][i] : -INFINITY;
-            }
-        }
-        float mx = sc[0][rt][0];
-#pragma unroll
-        for (int e = 1; e < 16; ++e) mx = fmax_ieee(mx, sc[e >> 2][rt][e & 3]);
-        mxs[rt] = mx * a.scale_log2;
-      }
-      if (__builtin_amdgcn_ballot_w64(mxs[0] > m_run[0] + kSlack || mxs[1] > m_run[1] + kSlack) != 0) {
+      attn::tile_scores<D>(r, sK, at, sc);
+      const bool full = x1 - x0 == attn::kKeys - 1 && x1 <= e0 && (e1 - x0 < a.window || x1 < a.sinks);
+      if (!full) {
 #pragma unroll
         for (int rt = 0; rt < 2; ++rt) {
-          const float mx = xor32_max(xor16_max(mxs[rt]));
-          const float mnew = mx > m_run[rt] + kSlack ? mx : m_run[rt];
-          const float alpha = mnew == m_run[rt] ? 1.f : fast_exp2(m_run[rt] - mnew);
-          m_run[rt] = mnew;
-          lsum[rt] *= alpha;
+          const int top = e0 + rt * 16 + n, hi = min(top, ks.count - 1) - x0 - 4 * g;  // from the lane's first entry
+          const int span = min(a.window - 1, INT32_MAX / 2) - max(0, top - (ks.count - 1));
+          if (x0 >= a.sinks) {  // hi - span <= entry <= hi
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt) o[dt][rt] *= alpha;
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                sc[kt][rt][i] = (uint32_t)(hi - (kt * 16 + i)) <= (uint32_t)span && span >= 0 ? sc[kt][rt][i] : -INFINITY;
+          } else {
+            const int f = a.sinks - x0 - 4 * g;
+#pragma unroll
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int x = kt * 16 + i;
+                sc[kt][rt][i] = x <= hi && (hi - x <= span || x < f) ? sc[kt][rt][i] : -INFINITY;
+              }
+          }
         }
       }
-      bf16x8_t pb[2][2];
-#pragma unroll
-      for (int rt = 0; rt < 2; ++rt) {
-        const float mref = m_run[rt] == -INFINITY ? 0.f : m_run[rt];
-        uint32_t pw[8];
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; i += 2)
-            pw[kt * 2 + i / 2] = pack_bf16x2(fast_exp2(fmaf(sc[kt][rt][i], a.scale_log2, -mref)),
-                                             fast_exp2(fmaf(sc[kt][rt][i + 1], a.scale_log2, -mref)));
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-          pb[rt][s] = __builtin_bit_cast(bf16x8_t, (u32x4_t){pw[4 * s], pw[4 * s + 1], pw[4 * s + 2], pw[4 * s + 3]});
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-#pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          const uint16_t* vrd = sV + voff[dt] + s * 32 * D;
-          const v4i16_t lo = lds_read_tr16(vrd);
-          const v4i16_t hi = lds_read_tr16(vrd + 16 * D);
-          const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-#pragma unroll
-          for (int rt = 0; rt < 2; ++rt)
-            o[dt][rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pb[rt][s], o[dt][rt], 0, 0, 0);
-        }
-#pragma unroll
-        for (int rt = 0; rt < 2; ++rt) lsum[rt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, pb[rt][s], lsum[rt], 0, 0, 0);
-      }
+      attn::tile_attend<D>(r, sc, sV, at, a.scale_log2);
     };
-    for (int tile = 0; tile < ntiles; tile += 2) {
-      step(tile, sK0, sV0, sK1, sV1);
-      if (tile + 1 < ntiles) step(tile + 1, sK1, sV1, sK0, sV0);
+    for (int tile = 0; tile < cur.tiles; tile += 2) {
+      step(tile, sK0, sV0, sK1, sV1, false);
+      if (tile + 1 < cur.tiles) step(tile + 1, sK1, sV1, sK0, sV0, true);
     }
-
-    // lane holds O[row rt*16+n][dt*16 + 4g + i]
+    if (cur.tiles == 0 || cur.tiles % 2 != 0) {  // the first buffers were the last in use, or none were
+      __syncthreads();
+      tile_load(nxt, 0, more && nxt.tiles > 0, sK0, sV0);
+    }
+    const Item done = cur;
+    const int hq = done.hq0 + (wid >> 1);
     uint32_t again = 0;  // rows with a value that is not finite
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
-      float bad = lsum[rt][0] * 0.f;
+      float bad = r.sum[rt][0] * 0.f;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
+      for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad += o[dt][rt][i] * 0.f;
-      const uint64_t y = __builtin_amdgcn_ballot_w64(r0 + rt * 16 + n < nq && bad != bad);
+        for (int i = 0; i < 4; ++i) bad += r.o[dt][rt][i] * 0.f;
+      const uint64_t y = __builtin_amdgcn_ballot_w64(r0 + rt * 16 + n < done.nq && bad != bad);
       again |= (uint32_t)((y | y >> 16 | y >> 32 | y >> 48) & 0xffff) << (16 * rt);
     }
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
-      const float l = lsum[rt][0];
+      const float l = r.sum[rt][0];
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int s = r0 + rt * 16 + n;
-      if (s >= nq || (again >> (rt * 16 + n) & 1)) continue;
-      uint16_t* orow = a.out + (int64_t)(q0 + s) * a.o_sn + (int64_t)hq * a.o_sh;
+      if (s >= done.nq || (again >> (rt * 16 + n) & 1)) continue;
+      uint16_t* orow = a.out + (int64_t)(done.q0 + s) * a.o_sn + (int64_t)hq * a.o_sh;
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        const uint32_t w0 = pack_bf16x2(o[dt][rt][0] * inv, o[dt][rt][1] * inv);
-        const uint32_t w1 = pack_bf16x2(o[dt][rt][2] * inv, o[dt][rt][3] * inv);
+      for (int dt = 0; dt < D / 16; ++dt) {
+        const uint32_t w0 = pack_bf16x2(r.o[dt][rt][0] * inv, r.o[dt][rt][1] * inv);
+        const uint32_t w1 = pack_bf16x2(r.o[dt][rt][2] * inv, r.o[dt][rt][3] * inv);
         *(uint64_t*)(orow + dt * 16 + 4 * g) = (uint64_t)w0 | ((uint64_t)w1 << 32);
       }
     }
     while (again) {
       const int row = r0 + __builtin_ctz(again);
       again &= again - 1;
-      const int64_t at = q0 + row;
-      exact_row<D>(a, a.q + at * a.q_sn + (int64_t)hq * a.q_sh, kbase, vbase, row + nk - nq,
-                   a.out + at * a.o_sn + (int64_t)hq * a.o_sh, lane);
+      const int64_t to = done.q0 + row;
+      exact_row<D>(a, a.q + to * a.q_sn + (int64_t)hq * a.q_sh, done.kb, done.vb, row + done.nk - done.nq,
+                   a.out + to * a.o_sn + (int64_t)hq * a.o_sh, lane);
     }
+    cur = nxt;
   }
 }
 
-// As many workgroups as are resident at once, at most one per item.
-template <int D, int HPW>
-hipError_t launch(const WindowArgs& a, hipStream_t st) {
+template <int D, int HPW, bool FAR>
+int resident() {
   static int per_cu = 0;
   if (per_cu == 0) {
     int nb = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&nb, window_prefill_kernel<D, HPW>, 128 * HPW, 0) != hipSuccess ||
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&nb, window_prefill_kernel<D, HPW, FAR>, 128 * HPW, 0) !=
+            hipSuccess ||
         nb <= 0)
       nb = 1;
     per_cu = nb;
   }
-  const int64_t items = ((int64_t)a.N / kBlk + a.B) * a.Hkv * (a.G / HPW);
-  const int64_t most = (int64_t)per_cu * cu_count();
-  hipLaunchKernelGGL((window_prefill_kernel<D, HPW>), dim3((unsigned)(items < most ? items : most)), dim3(128 * HPW), 0,
-                     st, a);
+  return per_cu * cu_count();
+}
+
+// Workgroups: those resident at once, at most one per item.
+template <int D, int HPW, bool FAR>
+hipError_t launch_items(const WindowArgs& a, hipStream_t st) {
+  const int64_t items = ((int64_t)a.N / kBlk + a.B) * a.Hkv * (a.G / HPW), most = resident<D, HPW, FAR>();
+  hipLaunchKernelGGL((window_prefill_kernel<D, HPW, FAR>), dim3((unsigned)(items < most ? items : most)), dim3(128 * HPW),
+                     0, st, a);
   return hipGetLastError();
+}
+
+template <int D, int HPW>
+hipError_t launch(const WindowArgs& a, hipStream_t st) {
+  const int64_t bytes = ((int64_t)a.Nk + attn::kKeys) * 2 * (a.k_sn > a.v_sn ? a.k_sn : a.v_sn);
+  const bool far = a.k_sn < 0 || a.v_sn < 0 || bytes >= 0x7ffff000;
+  return far ? launch_items<D, HPW, true>(a, st) : launch_items<D, HPW, false>(a, st);
 }
 
 // Query heads per workgroup: as many of 4, 2, 1 as divide G, halved while the
@@ -478,7 +463,7 @@ extern "C" int wgkv_sink_window_attn(
   a.sinks = num_sinks;
   // a negative scale negates the queries, and a scale of 0 clears them: masked
   // scores are -inf, and -inf * 0 is not a number
-  a.scale_log2 = softmax_scale == 0.f ? 1.f : fabsf(softmax_scale) * kLog2e;
+  a.scale_log2 = softmax_scale == 0.f ? 1.f : fabsf(softmax_scale) * attn::kLog2e;
   a.q_and = softmax_scale == 0.f ? 0u : ~0u;
   a.q_xor = softmax_scale < 0.f ? 0x80008000u : 0u;
   a.clear_rest = clear_rest;
