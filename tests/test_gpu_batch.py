@@ -431,7 +431,7 @@ def test_window_masked_tokens_of_a_visible_page():
         check_close(out, *ob.token(q, kc, vc, lens, table, 0.1, 21, 3))
 
 
-def check_shared(lens, plens, starts, Hq, P, D, scale=None, seed=0, spread=1.0):
+def check_shared(lens, plens, starts, Hq, P, D, scale=None, seed=0, spread=1.0, given=None):
     import wgkv
     lens, plens = torch.as_tensor(lens), torch.as_tensor(plens)
     B, H = lens.shape
@@ -451,8 +451,8 @@ def check_shared(lens, plens, starts, Hq, P, D, scale=None, seed=0, spread=1.0):
     q = query(B, Hq, D, seed + 2, spread)
     scale = D ** -0.5 if scale is None else scale
     print(f"[shared] lens={tuple(lens.shape)} prefixes={tuple(plens.shape)} Hq={Hq} P={P} D={D}", flush=True)
-    out = wgkv.paged_decode_attn_shared(q, kc, vc, lens.to(DEV, I32), table, plens.to(DEV, I32), ptable, i32(starts),
-                                        scale)
+    out = wgkv.paged_decode_attn_shared(q, kc, vc, lens.to(DEV, I32), table, plens.to(DEV, I32), ptable,
+                                        i32(given or starts), scale)
     torch.cuda.synchronize()
     check_close(out, *ob.token(q, kc, vc, lens, table, scale, prefix=(plens, ptable, starts)))
     return out
@@ -512,6 +512,17 @@ def test_shared_nan_is_seen_by_those_who_see_it():
     kc[int(ptable[0, 0, 0]), 0] = float("nan")      # the prefix of every sequence's first head
     out = wgkv.paged_decode_attn_shared(q, kc, vc, *args, 0.1)
     assert torch.isnan(out[:, 0, :2]).all() and torch.isfinite(out[2, 0, 2:]).all()
+
+
+@pytest.mark.parametrize("N", [2, 64])
+def test_shared_starts_that_do_not_ascend(N):
+    """They are taken as the greatest so far: here all but the first prefix have
+    no sequence, and nothing is written for them."""
+    B, H = 96, 4
+    starts = [0] + [B, 0] * (N // 2)
+    rng = np.random.default_rng(N)
+    lens, plens = rng.integers(0, 40, (B, H)), rng.integers(100, 300, (N, H))
+    check_shared(lens, plens, [0] + [B] * N, 32, 16, 64, given=starts)
 
 
 def test_shared_equals_one_table():

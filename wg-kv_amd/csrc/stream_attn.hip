@@ -27,15 +27,19 @@
 //     being kept (8 x 128K tokens: 119 -> 104 us).
 //
 // Many rows (a prefix of a larger group): the matrix products count.  A
-// workgroup takes 128 rows, 32 per wave, and tiles of 64 tokens that go from
-// the pages straight into LDS, one tile ahead (attn_tile.h).
+// workgroup of eight waves takes 256 rows, 32 per wave, and tiles of 64 tokens
+// that go from the pages straight into LDS, one tile ahead (attn_tile.h).
 //
 // Split: the tiles of all (prefix, head, row tile) and (sequence, head) are
-// laid end to end, weighted by what they cost, and the workgroups take equal
-// ranges of that line, whatever the lengths.  A workgroup goes through the
-// pieces of its range.  Pieces are numbered (workgroup + position of their
-// entry), store (max, sum, O) there, and a second launch joins the pieces of
-// every query row in a fixed order.
+// laid end to end and the waves take equal ranges of that line, whatever the
+// lengths.  Prefixes of many rows are a line of their own, of which every
+// workgroup takes an equal range, as its waves do of the other: nothing has to
+// be weighed against each other, and one half of the workgroups begins with
+// the prefix and the other with the sequences' own tokens, so that some
+// compute while others read.  A wave (or workgroup) goes through the pieces of
+// its range.  Pieces are numbered (range + position of their entry), store
+// (max, sum, O) there, and a second launch joins the pieces of every query row
+// in a fixed order.
 #include <string.h>
 
 #include "attn_tile.h"
@@ -48,16 +52,12 @@ using attn::fmax_ieee;
 using attn::xor16_max;
 using attn::xor32_max;
 
-constexpr int kWaves = 4;
-constexpr int kThreads = 64 * kWaves;
 constexpr int kMaxHeads = 2048;     // (sequence, head) pairs; (prefix, head) pairs
 constexpr int kMaxG = 8;
-constexpr int kWgsPerCu = 2;        // what the registers hold: two waves per SIMD
-constexpr int kMaxSlots = 1024;     // workgroups of the split launch at most
-constexpr int kFew = 16, kMany = 128;  // rows of a piece
-// What a tile costs along the line, in quarters of a streamed tile of 32
-// tokens.
-constexpr int kStreamed = 4, kTiled = 8;
+constexpr int kWavesPerCu = 8;      // what the registers hold: two per SIMD
+constexpr int kMaxWaves = 4096;     // of the split launch
+constexpr int kFew = 16, kMany = 256;  // rows of a piece
+constexpr int kLeastStreamed = 2, kLeastTiled = 2;  // tiles of a range
 
 struct StreamArgs {
   const uint16_t* q;
@@ -88,16 +88,15 @@ struct StreamArgs {
   float* pre_o;
   float* own_ml;
   float* own_o;
-  int* plan;  // cost before each entry, the total, and the cost of a workgroup's range
+  // tiles (prefixes of many rows: chunks) before each entry and in all, tiles of
+  // a chunk and of a range of the line, groups' first sequences
+  int* plan;
 };
 
 // A value that every lane holds, as a scalar.
 WGKV_DEVICE int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 WGKV_DEVICE int clamp_to(int x, int hi) { return min(max(x, 0), hi); }
-
-WGKV_DEVICE int group_start(const StreamArgs& a, int n) { return clamp_to(a.starts[n], a.B); }
-WGKV_DEVICE int group_size(const StreamArgs& a, int n) { return max(group_start(a, n + 1) - group_start(a, n), 0); }
 
 // What a call is: prefixes of few or many rows, or a window.
 enum Mode { kFewRows, kManyRows, kWindowed };
@@ -126,46 +125,46 @@ WGKV_DEVICE Seen seen_of(const StreamArgs& a, int tokens) {
   return x;
 }
 
-// Entry e of the line, prefixes first: tokens, tiles (per row tile), row tiles,
-// cost of a tile.
-struct Entry {
-  int tokens, tiles, row_tiles, weight;
-  WGKV_DEVICE int cost() const { return tiles * row_tiles * weight; }
-};
-
 template <Mode KIND>
 constexpr int rows_of() { return KIND == kManyRows ? kMany : kFew; }
 
-template <Mode KIND>
-WGKV_DEVICE Entry entry_of(const StreamArgs& a, int e) {
-  Entry x;
+// Tokens of entry e of the call, prefixes (prefix, head) first, then (sequence,
+// head).
+WGKV_DEVICE int entry_tokens(const StreamArgs& a, int e) {
   const int NH = a.N * a.H;
   if (e < NH) {
     const int n = e / a.H, h = e - n * a.H;
-    x.tokens = clamp_to(a.plen[(int64_t)n * a.plen_sb + h], a.pcap);
-    x.row_tiles = (group_size(a, n) * a.G + rows_of<KIND>() - 1) / rows_of<KIND>();
-    x.weight = KIND == kManyRows ? kTiled : kStreamed;
-    x.tiles = KIND == kManyRows ? (x.tokens + 63) >> 6 : (x.tokens + 31) >> 5;
-  } else {
-    const int b = (e - NH) / a.H, h = e - NH - b * a.H;
-    x.tokens = clamp_to(a.len[(int64_t)b * a.len_sb + h], a.cap);
-    x.row_tiles = 1;
-    x.weight = kStreamed;
-    x.tiles = (seen_of<KIND>(a, x.tokens).subs + 1) >> 1;
+    return clamp_to(a.plen[(int64_t)n * a.plen_sb + h], a.pcap);
   }
-  return x;
+  const int b = (e - NH) / a.H, h = e - NH - b * a.H;
+  return clamp_to(a.len[(int64_t)b * a.len_sb + h], a.cap);
 }
 
-// Cost of a workgroup's range: an equal share, but a streamed tile per wave at least.
-WGKV_DEVICE int range_cost(int total, int slots) { return max((total + slots - 1) / slots, kWaves * kStreamed); }
-
-// Number of a (prefix, head, row tile) that only grows along the line: groups
-// before n have at most starts[n] * G / rows + n row tiles.
+// Tiles of an entry's tokens (per row tile), and row tiles of a group.
 template <Mode KIND>
-WGKV_DEVICE int64_t piece_of(const StreamArgs& a, int n, int h, int row_tile) {
-  constexpr int R = rows_of<KIND>();
-  const int row_tiles = (group_size(a, n) * a.G + R - 1) / R;
-  return (int64_t)a.H * (group_start(a, n) * a.G / R + n) + h * row_tiles + row_tile;
+WGKV_DEVICE int entry_tiles(const StreamArgs& a, bool pre, int tokens) {
+  if (KIND == kManyRows && pre) return (tokens + 63) >> 6;
+  return (seen_of<KIND>(a, tokens).subs + 1) >> 1;
+}
+template <Mode KIND>
+WGKV_DEVICE int row_tiles(const StreamArgs& a, int size) { return (size * a.G + rows_of<KIND>() - 1) / rows_of<KIND>(); }
+
+// Tiles of a range of a line: an equal share, but `least` at least.
+WGKV_DEVICE int range_tiles(int total, int ranges, int least) { return max((total + ranges - 1) / ranges, least); }
+
+// Prefixes of few rows: number of a (prefix, head, row tile) that only grows
+// along the line: groups before n have at most starts[n] * G / 16 + n row tiles.
+WGKV_DEVICE int piece_of(const StreamArgs& a, int start, int size, int n, int h, int row_tile) {
+  return a.H * (start * a.G / kFew + n) + h * row_tiles<kFewRows>(a, size) + row_tile;
+}
+
+// Prefixes of many rows: every (prefix, head, row tile) is cut into chunks of
+// equal size, so that a workgroup has one where their number allows it (a
+// second piece costs it 14 us of 70): at most `slots` chunks while there are
+// half as many row tiles.
+WGKV_DEVICE int chunk_tiles(int total, int row_tiles, int slots) {
+  const int left = max(slots - row_tiles, slots / 2);
+  return max((total + left - 1) / left, kLeastTiled);
 }
 
 // Pages of a head, and what the call sees of its tokens.
@@ -359,95 +358,177 @@ WGKV_DEVICE void attend_tile(const StreamArgs& a, Rows16<D>& r, const KTile<D>& 
   for (int e = 0; e < D / 16; ++e) r.o[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[e], pb, r.o[e], 0, 0, 0);
 }
 
-template <int D>
-constexpr int row_stride() { return D + 4; }  // LDS: rows of one operand on different banks
+// What the workgroup keeps of the call's plan in LDS.
+struct Plan {
+  const int* base;   // tiles of the entries before (prefixes of many rows: chunks)
+  const int* tokens;
+  const int* start;  // groups' first sequences
+};
 
-// A wave's 16 rows in LDS: O, then (max, sum).
-template <int D>
-constexpr int wave_floats() { return kFew * row_stride<D>() + 2 * kFew; }
+// A tile on its way through a wave: page ids are asked for three tiles before
+// it is attended to, keys two, values one.
+struct Stage {
+  int pos;             // on the line; >= the range's end: none
+  int e, row_tile;     // its entry
+  int tile, t1;        // within the entry's row tile; the piece's end
+  int tokens;
+  bool first;          // of its piece
+  Ids ids;
+};
 
-// Tiles t0 .. t1 - 1 of a head's tokens for up to 16 rows, the waves taking
-// them in turn and meeting in LDS (part[w] is wave w's).  (max, sum) and O of
-// rows < rows go to ml and o.
 template <int D, Mode KIND>
-WGKV_DEVICE void stream_piece(const StreamArgs& a, const Pages& p, int t0, int t1, const Queries& q, int rows, float* ml,
-                              float* o, float* const (&part)[kWaves]) {
-  constexpr int RS = row_stride<D>();
-  const int t = threadIdx.x, lane = t & 63, w = uniform(t >> 6);
-  const int n = lane & 15, g = lane >> 4;
-  Rows16<D> r;
-  const uint16_t* row = q.row(a, n);
-#pragma unroll
-  for (int j = 0; j < D / 32; ++j) {
-    const u32x4_t x = *(const u32x4_t*)(row + (j * 4 + g) * 8);
-    r.q[j] = __builtin_bit_cast(bf16x8_t, (x & a.q_and) ^ a.q_xor);
+struct Stream {
+  const StreamArgs& a;
+  const Plan& plan;
+  int NH, zero, hi, range;
+  int n, g;
+
+  WGKV_DEVICE const int32_t* table(int e) const {
+    if (KIND != kWindowed && e < NH) {
+      const int i = uniform(e / a.H);
+      return a.pbt + i * a.pbt_sb + (e - i * a.H) * a.pbt_sh;
+    }
+    const int b = uniform((e - NH) / a.H);
+    return a.bt + b * a.bt_sb + (e - NH - b * a.H) * a.bt_sh;
   }
-  r.m = -INFINITY;
-  r.sum = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+
+  // The stage at position pos, which lies in entry e or behind it.
+  WGKV_DEVICE Stage at(int pos, int e) const {
+    Stage x = {pos, e, 0, 0, 0, 1, true, {{0, 0}}};
+    if (pos >= hi) return x;
+    int next = uniform(plan.base[e + 1]) - zero;
+    while (next <= pos) next = uniform(plan.base[++e + 1]) - zero;
+    x.e = e;
+    x.tokens = uniform(plan.tokens[e]);
+    const int begin = uniform(plan.base[e]) - zero, tiles = uniform(entry_tiles<KIND>(a, e < NH, x.tokens));
+    x.row_tile = KIND == kFewRows ? uniform((pos - begin) / tiles) : 0;
+    x.tile = pos - begin - x.row_tile * tiles;
+    x.t1 = min(tiles, x.tile + hi - pos);
+    return x;
+  }
+  WGKV_DEVICE Stage after(const Stage& s) const {
+    if (s.tile + 1 < s.t1) {
+      Stage x = s;
+      ++x.pos;
+      ++x.tile;
+      x.first = false;
+      return x;
+    }
+    return at(s.pos + 1, s.e);
+  }
+  WGKV_DEVICE Pages pages(const Stage& s) const { return {table(s.e), seen_of<KIND>(a, s.tokens)}; }
+  WGKV_DEVICE void ask_ids(Stage& s) const {
+    if (s.pos < hi) s.ids = tile_ids<KIND>(a, pages(s), s.tile);
+  }
+  WGKV_DEVICE int tile_or_none(const Stage& s) const { return s.pos < hi ? s.tile : INT32_MAX / 64; }
+  WGKV_DEVICE Pages seen_pages(const Stage& s) const { return {nullptr, seen_of<KIND>(a, s.tokens)}; }
+
+  WGKV_DEVICE Queries queries(const Stage& s) const {
+    Queries q;
+    if (KIND != kWindowed && s.e < NH) {
+      const int i = uniform(s.e / a.H);
+      q.h = s.e - i * a.H;
+      q.b0 = uniform(plan.start[i]);
+      q.first = s.row_tile * kFew;
+      q.count = (uniform(plan.start[i + 1]) - q.b0) * a.G;
+    } else {
+      q.b0 = uniform((s.e - NH) / a.H);
+      q.h = s.e - NH - q.b0 * a.H;
+      q.first = 0;
+      q.count = a.G;
+    }
+    return q;
+  }
+  WGKV_DEVICE void load_q(const Stage& s, u32x4_t (&q)[D / 32]) const {
+    const uint16_t* row = queries(s).row(a, n);
 #pragma unroll
-  for (int e = 0; e < D / 16; ++e) r.o[e] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-  const int koff = (n * D + g * 8) * 2, voff = (4 * g * D + n * (D / 16)) * 2;
-  const auto or_none = [&](int tile) { return tile < t1 ? tile : INT32_MAX / 64; };
-  int tile = t0 + w;
-  if (tile < t1) {
+    for (int j = 0; j < D / 32; ++j) q[j] = *(const u32x4_t*)(row + (j * 4 + g) * 8);
+  }
+
+  // (max, sum) and O of the stage's piece, and the state for the next one.
+  WGKV_DEVICE void flush(const Stage& s, Rows16<D>& r) const {
+    float *ml, *o;
+    int rows;
+    if (KIND != kWindowed && s.e < NH) {
+      const int i = uniform(s.e / a.H), start = uniform(plan.start[i]), size = uniform(plan.start[i + 1]) - start;
+      const int64_t id = range + piece_of(a, start, size, i, s.e - i * a.H, s.row_tile);
+      ml = a.pre_ml + id * (kFew * 2);
+      o = a.pre_o + id * (kFew * D);
+      rows = min(kFew, size * a.G - s.row_tile * kFew);
+    } else {
+      const int64_t id = range + s.e - NH;
+      ml = a.own_ml + id * (a.G * 2);
+      o = a.own_o + id * (a.G * D);
+      rows = a.G;
+    }
+    if (n < rows) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int e = 0; e < D / 16; e += 4)
+          *(f32x4_t*)(o + n * D + (D / 16) * (4 * g + i) + e) =
+              (f32x4_t){r.o[e][i], r.o[e + 1][i], r.o[e + 2][i], r.o[e + 3][i]};
+      if (g == 0) {
+        ml[n * 2] = r.m;
+        ml[n * 2 + 1] = r.sum[0];
+      }
+    }
+    clear(r);
+  }
+  WGKV_DEVICE static void clear(Rows16<D>& r) {
+    r.m = -INFINITY;
+    r.sum = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int e = 0; e < D / 16; ++e) r.o[e] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  }
+  WGKV_DEVICE void take_q(Rows16<D>& r, const u32x4_t (&q)[D / 32]) const {
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) r.q[j] = __builtin_bit_cast(bf16x8_t, (q[j] & a.q_and) ^ a.q_xor);
+  }
+
+  // One wave's range [lo, hi) of the line (not empty); its first entry is at or
+  // behind `from`.
+  WGKV_DEVICE void run(int lo, int from) const {
+    const int koff = (n * D + g * 8) * 2, voff = (4 * g * D + n * (D / 16)) * 2;
     KTile<D> k0, k1;
     VTile<D> v;
-    Ids i0 = tile_ids<KIND>(a, p, tile), i1 = tile_ids<KIND>(a, p, tile + kWaves), i2 = tile_ids<KIND>(a, p, tile + 2 * kWaves);
-    load_k<D, KIND>(a, p, tile, i0, koff, k0);
-    load_v<D, KIND>(a, p, tile, i0, voff, v);
-    load_k<D, KIND>(a, p, or_none(tile + kWaves), i1, koff, k1);
+    Rows16<D> r;
+    u32x4_t q[D / 32];
+    Stage s0 = at(lo, from);
+    ask_ids(s0);
+    load_q(s0, q);
+    Stage s1 = after(s0);
+    ask_ids(s1);
+    Stage s2 = after(s1);
+    ask_ids(s2);
+    load_k<D, KIND>(a, seen_pages(s0), s0.tile, s0.ids, koff, k0);
+    load_v<D, KIND>(a, seen_pages(s0), s0.tile, s0.ids, voff, v);
+    load_k<D, KIND>(a, seen_pages(s1), tile_or_none(s1), s1.ids, koff, k1);
+    take_q(r, q);
+    if (s1.first && s1.pos < hi) load_q(s1, q);
+    clear(r);
     scores<D>(r, k0);
-    // (kc: the next tile's keys, kn: its buffer; i1, i2: page ids one and two tiles on)
     const auto step = [&](KTile<D>& kc, KTile<D>& kn) __attribute__((always_inline)) {
-      load_k<D, KIND>(a, p, or_none(tile + 2 * kWaves), i2, koff, kn);
-      attend_tile<D, KIND>(a, r, kc, v, p, tile, g, [&] __attribute__((always_inline)) () {
-        load_v<D, KIND>(a, p, or_none(tile + kWaves), i1, voff, v);
-        i1 = i2;
-        i2 = tile_ids<KIND>(a, p, tile + 3 * kWaves);
+      load_k<D, KIND>(a, seen_pages(s2), tile_or_none(s2), s2.ids, koff, kn);
+      if (s1.first) take_q(r, q);  // (its scores come next; s0's are there)
+      if (s2.first && s2.pos < hi) load_q(s2, q);
+      attend_tile<D, KIND>(a, r, kc, v, seen_pages(s0), s0.tile, g, [&] __attribute__((always_inline)) () {
+        load_v<D, KIND>(a, seen_pages(s1), tile_or_none(s1), s1.ids, voff, v);
       });
-      tile += kWaves;
+      if (s0.tile + 1 == s0.t1) flush(s0, r);
+      s0 = s1;
+      s1 = s2;
+      s2 = after(s2);
+      ask_ids(s2);
     };
     for (;;) {
       step(k1, k0);
-      if (tile >= t1) break;
+      if (s0.pos >= hi) break;
       step(k0, k1);
-      if (tile >= t1) break;
+      if (s0.pos >= hi) break;
     }
   }
-  float* mine = w == 0 ? part[0] : w == 1 ? part[1] : w == 2 ? part[2] : part[3];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int e = 0; e < D / 16; e += 4)
-      *(f32x4_t*)(mine + n * RS + (D / 16) * (4 * g + i) + e) = (f32x4_t){r.o[e][i], r.o[e + 1][i], r.o[e + 2][i], r.o[e + 3][i]};
-  if (g == 0) {
-    mine[kFew * RS + 2 * n] = r.m;
-    mine[kFew * RS + 2 * n + 1] = r.sum[0];
-  }
-  __syncthreads();
-  for (int i = t; i < rows * (D / 4); i += kThreads) {
-    const int at = i / (D / 4), d = (i - at * (D / 4)) * 4;
-    float m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) m = fmaxf(m, part[k][kFew * RS + 2 * at]);
-    f32x4_t sum = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < kWaves; ++k) {
-      const float mk = part[k][kFew * RS + 2 * at], lk = part[k][kFew * RS + 2 * at + 1];
-      // a sum of 0 (no token that weighs) has no part; one of NaN (its scores
-      // were) has, whatever its maximum
-      const float c = mk == -INFINITY && lk == 0.f ? 0.f : fast_exp2(mk - m);
-      l += c * lk;
-      sum += c * *(const f32x4_t*)(part[k] + at * RS + d);
-    }
-    *(f32x4_t*)(o + (int64_t)at * D + d) = sum;
-    if (d == 0) {
-      ml[at * 2] = m;
-      ml[at * 2 + 1] = l;
-    }
-  }
-  __syncthreads();
-}
+};
 
 // ---- many rows: tiles in LDS ----------------------------------------------------
 // 16 bytes of the buffer at `off` (zeros behind its end) go to LDS at lds + 16 * lane.
@@ -455,8 +536,8 @@ WGKV_DEVICE void buffer_to_lds(__amdgpu_buffer_rsrc_t r, uint16_t* lds, int off)
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, 16, off, 0, 0, 0);
 }
 
-// Tiles t0 .. t1 - 1 of 64 tokens for `rows` <= 128 rows, 32 per wave.  Wave w
-// loads sub-page w of every tile.
+// Tiles t0 .. t1 - 1 of 64 tokens for `rows` <= 256 rows, 32 per wave of eight.
+// Wave w loads sub-page w % 4 of every tile, the keys or the values.
 template <int D>
 WGKV_DEVICE void tile_piece(const StreamArgs& a, const Pages& p, int t0, int t1, const Queries& q, int rows, float* ml,
                             float* o, uint16_t* sK0, uint16_t* sV0, uint16_t* sK1, uint16_t* sV1) {
@@ -468,33 +549,39 @@ WGKV_DEVICE void tile_piece(const StreamArgs& a, const Pages& p, int t0, int t1,
   r.clear();
 #pragma unroll
   for (int rt = 0; rt < 2; ++rt) r.load_q(rt, q.row(a, w * 32 + rt * 16 + n), g, a.q_and, a.q_xor);
-  int koff[NB], voff[NB];
+  const int sub = w & 3;
+  const bool keys = w < 4;
+  const uint16_t* pool = keys ? a.kc : a.vc;
+  int off[NB];
 #pragma unroll
   for (int i = 0; i < NB; ++i) {
     const int row = i * RPB + lane / CH;
-    koff[i] = row * D * 2 + ((lane % CH) ^ attn::swz_k<D>(row)) * 16;
-    voff[i] = row * D * 2 + ((lane % CH) ^ attn::swz_v<D>(row)) * 16;
+    off[i] = row * D * 2 + ((lane % CH) ^ (keys ? attn::swz_k<D>(row) : attn::swz_v<D>(row))) * 16;
   }
   const auto load = [&](int tile, int id, uint16_t* sK, uint16_t* sV) __attribute__((always_inline)) {
-    const __amdgpu_buffer_rsrc_t k = subpage_rows<D>(a, p, a.kc, 4 * tile + w, id);
-    const __amdgpu_buffer_rsrc_t v = subpage_rows<D>(a, p, a.vc, 4 * tile + w, id);
+    const __amdgpu_buffer_rsrc_t r = subpage_rows<D>(a, p, pool, 4 * tile + sub, id);
+    uint16_t* to = (keys ? sK : sV) + sub * NB * 512;
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      buffer_to_lds(k, sK + (w * NB + i) * 512, koff[i]);
-      buffer_to_lds(v, sV + (w * NB + i) * 512, voff[i]);
-    }
+    for (int i = 0; i < NB; ++i) buffer_to_lds(r, to + i * 512, off[i]);
   };
-  int id = subpage_id(a, p, 4 * t0 + w);
-  load(t0, id, sK0, sV0);
-  id = subpage_id(a, p, 4 * (t0 + 1) + w);
+  // Page ids of 16 tiles are a lane's each, asked for 16 tiles ahead.  (A
+  // scalar load per tile would be waited for by the tile's first LDS read,
+  // with which it shares a counter.)
+  const auto ids_from = [&](int tile) {
+    return p.bt[min(4 * tile + lane, (p.seen.tokens - 1) >> 4) >> a.page_shift];
+  };
+  int ids = ids_from(t0), ids_next = ids_from(t0 + 16);
+  const auto id_of = [&](int tile) { return __builtin_amdgcn_readlane(ids, (tile - t0) % 16 * 4 + sub); };
+  load(t0, id_of(t0), sK0, sV0);
   const auto step = [&](int tile, const uint16_t* sK, const uint16_t* sV, uint16_t* nK, uint16_t* nV)
       __attribute__((always_inline)) {
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the tile has landed
     __syncthreads();                     // every wave's has, and nobody reads the other buffer any more
-    if (tile + 1 < t1) {
-      load(tile + 1, id, nK, nV);
-      id = subpage_id(a, p, 4 * (tile + 2) + w);
+    if ((tile + 1 - t0) % 16 == 0) {
+      ids = ids_next;
+      ids_next = ids_from(tile + 17);
     }
+    if (tile + 1 < t1) load(tile + 1, id_of(tile + 1), nK, nV);
     if (w * 32 >= rows) return;
     f32x4_t sc[4][2];
     attn::tile_scores<D>(r, sK, at, sc);
@@ -529,152 +616,232 @@ WGKV_DEVICE void tile_piece(const StreamArgs& a, const Pages& p, int t0, int t1,
   __syncthreads();  // the buffers are free
 }
 
-template <int D, Mode KIND>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kWgsPerCu, kWgsPerCu)))
-void stream_split_kernel(StreamArgs a) {
-  // four objects: loads into one tile buffer then provably leave the others
-  // alone; between pieces they hold the waves' rows
-  constexpr int kLds = KIND == kManyRows ? attn::kKeys * D * 2 : wave_floats<D>() * 4;
-  static_assert(kLds >= wave_floats<D>() * 4, "a wave's rows fit a tile buffer");
-  __shared__ __attribute__((aligned(16))) uint16_t s0[kLds / 2];
-  __shared__ __attribute__((aligned(16))) uint16_t s1[kLds / 2];
-  __shared__ __attribute__((aligned(16))) uint16_t s2[kLds / 2];
-  __shared__ __attribute__((aligned(16))) uint16_t s3[kLds / 2];
-  // (many rows: at least 17 per prefix, so N * H <= 2048 * 8 / 17)
-  __shared__ int s_base[kMaxHeads + (KIND == kManyRows ? 1024 : KIND == kFewRows ? kMaxHeads : 0) + 1];
-  __shared__ int s_tmp[4];
-  const int t = threadIdx.x, wg = blockIdx.x;
-  const int NH = a.N * a.H, E = NH + a.B * a.H;
-  // cost before every entry, the same in every workgroup
-  const int per_thread = (E + kThreads - 1) / kThreads;
-  const int e0 = min(E, t * per_thread), e1 = min(E, e0 + per_thread);
-  int mine = 0, total;
-  for (int e = e0; e < e1; ++e) mine += entry_of<KIND>(a, e).cost();
-  int run = block_exclusive_scan_256(mine, s_tmp, &total);
-  for (int e = e0; e < e1; ++e) {
-    s_base[e] = run;
-    run += entry_of<KIND>(a, e).cost();
-  }
-  if (t == 0) s_base[E] = total;
+// (max, sum, O) of a second set of tokens into the first's.  A sum of 0 (no
+// token that weighs) has no part; one of NaN (its scores were) has, whatever its
+// maximum.
+WGKV_DEVICE void join(float& m, float& l, f32x4_t& o, float mb, float lb, f32x4_t ob) {
+  const float mn = fmaxf(m, mb);
+  const float ca = m == -INFINITY && l == 0.f ? 0.f : fast_exp2(m - mn);
+  const float cb = mb == -INFINITY && lb == 0.f ? 0.f : fast_exp2(mb - mn);
+  l = l * ca + lb * cb;
+  o = o * ca + ob * cb;
+  m = mn;
+}
+
+// Where the own tokens' line begins among the entries' tiles: prefixes of many
+// rows are not on it.
+template <Mode KIND>
+WGKV_DEVICE int own_zero(const int* base, int NH) { return KIND == kManyRows ? base[NH] : 0; }
+
+template <Mode KIND>
+constexpr int waves_of() { return KIND == kManyRows ? 8 : 4; }
+
+// Exclusive sum over the threads of a workgroup of NW waves, and the total.
+template <int NW>
+WGKV_DEVICE int block_scan(int v, int* s_wave, int* total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int incl = wave_incl_scan(v, lane);
+  if (lane == 63) s_wave[w] = incl;
   __syncthreads();
-  total = uniform(total);
-  const int per = uniform(range_cost(total, a.slots));
-  if (wg == 0) {
-    for (int i = t; i <= E; i += kThreads) a.plan[i] = s_base[i];
-    if (t == 0) a.plan[E + 1] = per;
+  int run = incl - v, all = 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) {
+    run += i < w ? s_wave[i] : 0;
+    all += s_wave[i];
   }
-  const int lo = (int)min((int64_t)wg * per, (int64_t)total), hi = (int)min((int64_t)lo + per, (int64_t)total);
-  if (lo >= hi) return;
-  int first = 0, last = E - 1;  // the last entry that begins at or before lo
-  while (first < last) {
-    const int mid = (first + last + 1) >> 1;
-    if (uniform(s_base[mid]) <= lo) first = mid; else last = mid - 1;
+  __syncthreads();
+  *total = uniform(all);
+  return run;
+}
+
+// The greatest value of the threads before (0: none), of values of 0 or more.
+template <int NW>
+WGKV_DEVICE int block_max_before(int v, int* s_wave) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 1; i < 64; i <<= 1) {
+    const int o = __shfl_up(v, i, 64);
+    v = max(v, lane >= i ? o : 0);
   }
-  for (int e = first; e < E; ++e) {
-    const int base = uniform(s_base[e]);
-    if (base >= hi) break;
-    if (uniform(s_base[e + 1]) == base) continue;
-    Entry x = entry_of<KIND>(a, e);
-    x.tokens = uniform(x.tokens);
-    x.tiles = uniform(x.tiles);
-    x.row_tiles = uniform(x.row_tiles);
-    // the entry's tiles (row tile after row tile) that begin in [lo, hi)
-    int u0 = uniform(max(0, (lo - base + x.weight - 1) / x.weight));
-    const int u1 = uniform(min(x.tiles * x.row_tiles, (hi - base + x.weight - 1) / x.weight));
-    while (u0 < u1) {
-      const int row_tile = uniform(u0 / x.tiles), t0 = u0 - row_tile * x.tiles;
-      const int t1 = min(x.tiles, t0 + u1 - u0);
-      u0 += t1 - t0;
-      Queries q;
-      Pages p;
-      float *ml, *o;
-      const bool pre = KIND != kWindowed && e < NH;
-      constexpr int R = rows_of<KIND>();
-      if (pre) {
-        const int n = uniform(e / a.H);
-        q.h = e - n * a.H;
-        q.b0 = uniform(group_start(a, n));
-        q.first = row_tile * R;
-        q.count = uniform(group_size(a, n)) * a.G;
-        p.bt = a.pbt + n * a.pbt_sb + q.h * a.pbt_sh;
-        const int64_t id = wg + piece_of<KIND>(a, n, q.h, row_tile);
-        ml = a.pre_ml + id * (R * 2);
-        o = a.pre_o + id * (R * D);
-      } else {
-        const int bh = e - NH;
-        q.b0 = uniform(bh / a.H);
-        q.h = bh - q.b0 * a.H;
-        q.first = 0;
-        q.count = a.G;
-        p.bt = a.bt + q.b0 * a.bt_sb + q.h * a.bt_sh;
-        const int64_t id = wg + bh;
-        ml = a.own_ml + id * (a.G * 2);
-        o = a.own_o + id * (a.G * D);
-      }
-      p.seen = seen_of<KIND>(a, x.tokens);
-      const int rows = min(R, q.count - q.first);
-      if (KIND == kManyRows && pre) {
-        tile_piece<D>(a, p, t0, t1, q, rows, ml, o, s0, s1, s2, s3);
-      } else {
-        float* const part[kWaves] = {(float*)s0, (float*)s1, (float*)s2, (float*)s3};
-        stream_piece<D, KIND>(a, p, t0, t1, q, rows, ml, o, part);
-      }
+  if (lane == 63) s_wave[w] = v;
+  const int up = __shfl_up(v, 1, 64);
+  __syncthreads();
+  int before = lane ? up : 0;
+#pragma unroll
+  for (int i = 0; i < NW; ++i) before = max(before, i < w ? s_wave[i] : 0);
+  __syncthreads();
+  return before;
+}
+
+template <int D, Mode KIND>
+__global__ __launch_bounds__(64 * waves_of<KIND>()) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void stream_split_kernel(StreamArgs a) {
+  constexpr int NW = waves_of<KIND>(), NT = 64 * NW;
+  // tile buffers, as four objects: loads into one provably leave the others alone
+  constexpr int kTile = KIND == kManyRows ? attn::kKeys * D : 8;
+  __shared__ __attribute__((aligned(16))) uint16_t s_k0[kTile];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v0[kTile];
+  __shared__ __attribute__((aligned(16))) uint16_t s_k1[kTile];
+  __shared__ __attribute__((aligned(16))) uint16_t s_v1[kTile];
+  constexpr int kEntries = (KIND == kWindowed ? 1 : 2) * kMaxHeads;
+  __shared__ int s_base[kEntries + 1], s_tokens[kEntries], s_start[KIND == kWindowed ? 1 : kMaxHeads + 1];
+  __shared__ int s_wave[NW];
+  const int t = threadIdx.x, wg = blockIdx.x, wave = uniform(t >> 6);
+  const int NH = a.N * a.H, E = NH + a.B * a.H;
+  const Plan plan = {s_base, s_tokens, s_start};
+  // The plan, the same in every workgroup; each thread has some entries.
+  const int each = (E + NT - 1) / NT, e0 = min(E, t * each), e1 = min(E, e0 + each);
+  for (int e = e0; e < e1; ++e) s_tokens[e] = entry_tokens(a, e);
+  if constexpr (KIND != kWindowed) {
+    // starts, made to ascend: what the workspace holds relies on it
+    const int n1 = a.N + 1, nt = (n1 + NT - 1) / NT, b0 = min(n1, t * nt), b1 = min(n1, b0 + nt);
+    int most = 0;
+    for (int n = b0; n < b1; ++n) s_start[n] = most = max(most, clamp_to(a.starts[n], a.B));
+    const int before = block_max_before<NW>(most, s_wave);
+    for (int n = b0; n < b1; ++n) s_start[n] = max(s_start[n], before);
+    __syncthreads();
+  }
+  const auto rows_tiles = [&](int e) {
+    if (KIND == kWindowed || e >= NH) return 1;
+    const int n = e / a.H;
+    return row_tiles<KIND>(a, s_start[n + 1] - s_start[n]);
+  };
+  int chunk = 0, total;
+  if constexpr (KIND == kManyRows) {
+    int tiles = 0, rts = 0, all_tiles, all_rts;
+    for (int e = e0; e < min(e1, NH); ++e) {
+      const int x = entry_tiles<KIND>(a, true, s_tokens[e]), rt = rows_tiles(e);
+      tiles += x * rt;
+      rts += x ? rt : 0;
     }
+    block_scan<NW>(tiles, s_wave, &all_tiles);
+    block_scan<NW>(rts, s_wave, &all_rts);
+    chunk = chunk_tiles(all_tiles, all_rts, a.slots);
+  }
+  {
+    int mine = 0;
+    for (int e = e0; e < e1; ++e) {
+      int x = entry_tiles<KIND>(a, e < NH, s_tokens[e]);
+      if (KIND == kManyRows && e < NH) x = (x + chunk - 1) / chunk;
+      mine += x * rows_tiles(e);
+      s_base[e + 1] = mine;
+    }
+    const int run = block_scan<NW>(mine, s_wave, &total);
+    for (int e = e0; e < e1; ++e) s_base[e + 1] += run;
+    if (t == 0) s_base[0] = 0;
+    __syncthreads();
+  }
+  const int zero = uniform(own_zero<KIND>(s_base, NH)), line = total - zero;
+  const int per = uniform(range_tiles(line, a.slots * NW, kLeastStreamed));
+  if (wg == 0) {
+    for (int i = t; i <= E; i += NT) a.plan[i] = s_base[i];
+    if (t == 0) {
+      a.plan[E + 1] = chunk;
+      a.plan[E + 2] = per;
+    }
+    if constexpr (KIND != kWindowed)
+      for (int n = t; n <= a.N; n += NT) a.plan[E + 3 + n] = s_start[n];
+  }
+  const int range = wg * NW + wave;
+  const auto stream = [&]() __attribute__((always_inline)) {
+    if ((int64_t)range * per >= line) return;
+    const int lo = range * per, from = KIND == kManyRows ? NH : 0;
+    int first = from, last = E - 1;  // the last entry that begins at or before lo
+    while (first < last) {
+      const int mid = (first + last + 1) >> 1;
+      if (uniform(s_base[mid]) - zero <= lo) first = mid; else last = mid - 1;
+    }
+    const int lane = t & 63;
+    const Stream<D, KIND> s = {a, plan, NH, zero, min(lo + per, line), range, lane & 15, lane >> 4};
+    s.run(lo, first);
+  };
+  if constexpr (KIND != kManyRows) {
+    stream();
+  } else {
+    const bool own_first = wg >= a.slots / 2;
+    if (own_first) stream();
+    for (int unit = wg; unit < zero; unit += a.slots) {
+      int e = 0, last = NH - 1;  // the last entry that begins at or before the unit
+      while (e < last) {
+        const int mid = (e + last + 1) >> 1;
+        if (uniform(s_base[mid]) <= unit) e = mid; else last = mid - 1;
+      }
+      const int n = uniform(e / a.H), tiles = uniform(entry_tiles<KIND>(a, true, uniform(s_tokens[e])));
+      const int chunks = uniform((tiles + chunk - 1) / chunk), at = unit - uniform(s_base[e]);
+      const int row_tile = uniform(at / chunks), c = at - row_tile * chunks;
+      Queries q;
+      q.h = e - n * a.H;
+      q.b0 = uniform(s_start[n]);
+      q.first = row_tile * kMany;
+      q.count = (uniform(s_start[n + 1]) - q.b0) * a.G;
+      const Pages p = {a.pbt + n * a.pbt_sb + q.h * a.pbt_sh, seen_of<KIND>(a, uniform(s_tokens[e]))};
+      tile_piece<D>(a, p, uniform((int)((int64_t)tiles * c / chunks)), uniform((int)((int64_t)tiles * (c + 1) / chunks)), q,
+                    min(kMany, q.count - q.first), a.pre_ml + (int64_t)unit * (kMany * 2),
+                    a.pre_o + (int64_t)unit * (kMany * D), s_k0, s_v0, s_k1, s_v1);
+    }
+    if (!own_first) stream();
   }
 }
 
-// The pieces of a query row under one softmax, in the order of the line: one
-// workgroup per (sequence, KV head, query head), a thread group of D/4
-// threads per piece in turn, then the groups in order.
-template <int D, Mode KIND>
+// The pieces of a query row under one softmax, in the order of the line.  A
+// row's pieces are dealt in turn to groups of D/4 lanes, four values of d
+// each, of one wave, or (few rows, of which some may have many pieces) of the
+// four waves of a workgroup; the groups then meet in order.
+template <int D, Mode KIND, bool WIDE>
 __global__ __launch_bounds__(256) void stream_merge_kernel(StreamArgs a) {
-  constexpr int NQ = D / 4, GROUPS = 256 / NQ, kBatch = 8, R = rows_of<KIND>();
-  __shared__ f32x4_t s_a[256];
-  __shared__ float s_m[256], s_l[256];
-  const int bh = blockIdx.x, b = bh / a.H, h = bh - b * a.H, gq = blockIdx.y;
-  const int t = threadIdx.x, vq = t % NQ, grp = t / NQ;
+  constexpr int NQ = D / 4, PER_WAVE = 64 / NQ, GROUPS = WIDE ? 4 * PER_WAVE : PER_WAVE, kBatch = 8, R = rows_of<KIND>();
+  __shared__ f32x4_t s_a[WIDE ? 256 : 1];
+  __shared__ float s_m[WIDE ? 256 : 1], s_l[WIDE ? 256 : 1];
+  const int bh = blockIdx.x, b = uniform(bh / a.H), h = bh - b * a.H;
+  const int t = threadIdx.x, wave = uniform(t >> 6), vq = t % NQ;
+  const int gq = WIDE ? (int)blockIdx.y : (int)blockIdx.y * 4 + wave;
+  if (gq >= a.G) return;  // (whole waves, and no barrier follows)
+  const int grp = (WIDE ? t : t & 63) / NQ;
   const int NH = a.N * a.H;
-  const int per = a.plan[NH + a.B * a.H + 1];
+  const int E = NH + a.B * a.H, chunk = a.plan[E + 1], per = a.plan[E + 2];
   int n_pre = 0;
   const float *pre_ml = nullptr, *pre_o = nullptr;
   if constexpr (KIND != kWindowed) {
-    int lo = 0, hi = a.N;  // the last group that starts at or before b
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (group_start(a, mid) <= b) lo = mid; else hi = mid;
+    const int* starts = a.plan + E + 3;
+    int n = 0, hi = a.N;  // the last group that starts at or before b
+    while (hi - n > 1) {
+      const int mid = (n + hi) >> 1;
+      if (starts[mid] <= b) n = mid; else hi = mid;
     }
-    const int at = b - group_start(a, lo);
-    if (at >= 0 && at < group_size(a, lo)) {
-      const int e = lo * a.H + h;
-      const Entry x = entry_of<KIND>(a, e);
-      if (x.tiles) {
-        const int row = at * a.G + gq, row_tile = row / R;
-        const int64_t base = a.plan[e] + (int64_t)row_tile * x.tiles * x.weight;
-        const int w0 = (int)(base / per), w1 = (int)((base + (int64_t)(x.tiles - 1) * x.weight) / per);
-        n_pre = w1 - w0 + 1;
-        const int64_t first = (w0 + piece_of<KIND>(a, lo, h, row_tile)) * R + row - row_tile * R;
-        pre_ml = a.pre_ml + first * 2;
-        pre_o = a.pre_o + first * D;
+    const int start = starts[n], size = starts[n + 1] - start, e = n * a.H + h;
+    const int tiles = entry_tiles<KIND>(a, true, entry_tokens(a, e));
+    if (b >= start && b - start < size && tiles) {
+      const int row = (b - start) * a.G + gq, row_tile = row / R;
+      int64_t first;
+      if constexpr (KIND == kManyRows) {
+        n_pre = (tiles + chunk - 1) / chunk;
+        first = a.plan[e] + row_tile * n_pre;
+      } else {
+        const int base = a.plan[e] + row_tile * tiles, w0 = base / per;
+        n_pre = (base + tiles - 1) / per - w0 + 1;
+        first = w0 + piece_of(a, start, size, n, h, row_tile);
       }
+      first = first * R + row - row_tile * R;
+      pre_ml = a.pre_ml + first * 2;
+      pre_o = a.pre_o + first * D;
     }
   }
   int n_own = 0;
   const float *own_ml = nullptr, *own_o = nullptr;
-  const Entry x = entry_of<KIND>(a, NH + bh);
-  if (x.tiles) {
-    const int base = a.plan[NH + bh];
-    const int w0 = base / per, w1 = (base + (x.tiles - 1) * x.weight) / per;
-    n_own = w1 - w0 + 1;
+  const int tiles = entry_tiles<KIND>(a, false, entry_tokens(a, NH + bh));
+  if (tiles) {
+    const int base = a.plan[NH + bh] - own_zero<KIND>(a.plan, NH), w0 = base / per;
+    n_own = (base + tiles - 1) / per - w0 + 1;
     const int64_t first = ((int64_t)w0 + bh) * a.G + gq;
     own_ml = a.own_ml + first * 2;
     own_o = a.own_o + first * D;
   }
   const int pieces = n_pre + n_own;
-  float M = -INFINITY, L = 0.f;
-  f32x4_t A = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  f32x4_t o = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   for (int c0 = grp; c0 < pieces; c0 += GROUPS * kBatch) {
     float mc[kBatch], lc[kBatch];
-    f32x4_t ac[kBatch];
+    f32x4_t oc[kBatch];
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
       const int c = min(c0 + k * GROUPS, pieces - 1);
@@ -683,40 +850,39 @@ __global__ __launch_bounds__(256) void stream_merge_kernel(StreamArgs a) {
       const float* ml = (pre ? pre_ml : own_ml) + i * 2;
       mc[k] = ml[0];
       lc[k] = ml[1];
-      ac[k] = *(const f32x4_t*)((pre ? pre_o : own_o) + i * D + vq * 4);
+      oc[k] = *(const f32x4_t*)((pre ? pre_o : own_o) + i * D + vq * 4);
     }
 #pragma unroll
     for (int k = 0; k < kBatch; ++k) {
-      // (a row whose every score is NaN keeps its maximum at -inf and a sum of NaN)
-      if (c0 + k * GROUPS >= pieces || (mc[k] == -INFINITY && lc[k] == 0.f)) continue;
-      const float mn = fmaxf(M, mc[k]);
-      const float sa = M == -INFINITY && L == 0.f ? 0.f : fast_exp2(M - mn);
-      const float sb = fast_exp2(mc[k] - mn);
-      L = L * sa + lc[k] * sb;
-      A = A * sa + ac[k] * sb;
-      M = mn;
+      if (c0 + k * GROUPS >= pieces) continue;
+      join(m, l, o, mc[k], lc[k], oc[k]);
     }
   }
-  s_m[t] = M;
-  s_l[t] = L;
-  s_a[t] = A;
-  __syncthreads();
-  if (t >= NQ) return;
-  float Mx = -INFINITY;
-  for (int i = 0; i < GROUPS; ++i) Mx = fmaxf(Mx, s_m[i * NQ + t]);
-  float Lt = 0.f;
-  f32x4_t At = (f32x4_t){0.f, 0.f, 0.f, 0.f};
-  for (int i = 0; i < GROUPS; ++i) {
-    const float m = s_m[i * NQ + t];
-    if (m == -INFINITY && s_l[i * NQ + t] == 0.f) continue;
-    const float c = fast_exp2(m - Mx);
-    Lt += c * s_l[i * NQ + t];
-    At += c * s_a[i * NQ + t];
-  }
-  uint16_t* o = a.out + b * a.out_sb + (int64_t)(h * a.G + gq) * a.out_sh + vq * 4;
-  const float inv = 1.f / Lt;
+  if constexpr (WIDE) {
+    s_m[t] = m;
+    s_l[t] = l;
+    s_a[t] = o;
+    __syncthreads();
+    if (t >= NQ) return;
+    m = -INFINITY;
+    l = 0.f;
+    o = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < GROUPS; ++i) join(m, l, o, s_m[i * NQ + t], s_l[i * NQ + t], s_a[i * NQ + t]);
+  } else {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] = Lt == 0.f ? 0 : f32_to_bf16(At[e] * inv);
+    for (int i = NQ; i < 64; i <<= 1) {
+      const float mo = __shfl_xor(m, i, 64), lo = __shfl_xor(l, i, 64);
+      f32x4_t oo;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) oo[e] = __shfl_xor(o[e], i, 64);
+      join(m, l, o, mo, lo, oo);
+    }
+    if ((t & 63) >= NQ) return;
+  }
+  uint16_t* out = a.out + b * a.out_sb + (int64_t)(h * a.G + gq) * a.out_sh + vq * 4;
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = l == 0.f ? 0 : f32_to_bf16(o[e] * inv);
 }
 
 // Whether an even share of the batch has more rows than one operand.
@@ -729,13 +895,15 @@ struct Scratch {
 
 size_t aligned(size_t n) { return (n + 255) & ~(size_t)255; }
 
-constexpr size_t kPlanBytes = ((2 * kMaxHeads + 2) * sizeof(int) + 255) & ~(size_t)255;
+constexpr size_t kPlanBytes = ((3 * kMaxHeads + 4) * sizeof(int) + 255) & ~(size_t)255;
 
+// Pieces: one per range, and one more per entry (and row tile).
 Scratch scratch_for(int B, int N, int G, int H, int D) {
-  const int R = many_rows(B, N, G) ? kMany : kFew;
+  const bool many = N && many_rows(B, N, G);
+  const int R = many ? kMany : kFew;
   Scratch s;
-  s.pre = kMaxSlots + (int64_t)H * ((int64_t)B * G / R + N + 1);
-  s.own = kMaxSlots + (int64_t)B * H;
+  s.pre = N ? (many ? kMaxWaves / 8 : kMaxWaves) + (int64_t)H * ((int64_t)B * G / R + N + 1) : 0;
+  s.own = kMaxWaves + (int64_t)B * H;
   s.pre_ml = kPlanBytes;
   s.pre_o = s.pre_ml + aligned(s.pre * R * 2 * sizeof(float));
   s.own_ml = s.pre_o + aligned(s.pre * R * D * sizeof(float));
@@ -744,13 +912,27 @@ Scratch scratch_for(int B, int N, int G, int H, int D) {
   return s;
 }
 
+void use_scratch(StreamArgs& a, const Scratch& s, void* p) {
+  char* ws = (char*)p;
+  a.plan = (int*)ws;
+  a.pre_ml = (float*)(ws + s.pre_ml);
+  a.pre_o = (float*)(ws + s.pre_o);
+  a.own_ml = (float*)(ws + s.own_ml);
+  a.own_o = (float*)(ws + s.own_o);
+}
+
 template <int D, Mode KIND>
 hipError_t launch(StreamArgs& a, hipStream_t st) {
-  a.slots = min(kMaxSlots, cu_count() * kWgsPerCu);
-  hipLaunchKernelGGL((stream_split_kernel<D, KIND>), dim3(a.slots), dim3(kThreads), 0, st, a);
+  constexpr int NW = waves_of<KIND>();
+  a.slots = min(kMaxWaves, cu_count() * kWavesPerCu) / NW;
+  hipLaunchKernelGGL((stream_split_kernel<D, KIND>), dim3(a.slots), dim3(64 * NW), 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((stream_merge_kernel<D, KIND>), dim3(a.B * a.H, a.G), dim3(256), 0, st, a);
+  // a wave per row once there are rows for all the CUs' waves
+  if (a.B * a.H * a.G >= 4 * cu_count())
+    hipLaunchKernelGGL((stream_merge_kernel<D, KIND, false>), dim3(a.B * a.H, (a.G + 3) / 4), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((stream_merge_kernel<D, KIND, true>), dim3(a.B * a.H, a.G), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 
@@ -762,10 +944,7 @@ hipError_t launch_rows(StreamArgs& a, bool many, hipStream_t st) {
 }  // namespace
 
 // Bytes of `scratch` (any contents) for wgkv_stream_window.
-size_t wgkv_stream_window_bytes(int B, int H, int G, int D) {
-  return kPlanBytes + aligned(((size_t)kMaxSlots + (size_t)B * H) * G * 2 * sizeof(float)) +
-         aligned(((size_t)kMaxSlots + (size_t)B * H) * G * D * sizeof(float));
-}
+size_t wgkv_stream_window_bytes(int B, int H, int G, int D) { return scratch_for(B, 0, G, H, D).bytes; }
 
 // The windowed call for batches of many heads (arguments checked by the caller).
 int wgkv_stream_window(const StreamWindow& w, void* scratch, hipStream_t st) {
@@ -794,10 +973,7 @@ int wgkv_stream_window(const StreamWindow& w, void* scratch, hipStream_t st) {
   a.scale_log2 = w.scale_log2;
   a.q_and = w.q_and;
   a.q_xor = w.q_xor;
-  char* s = (char*)scratch;
-  a.plan = (int*)s;
-  a.own_ml = (float*)(s + kPlanBytes);
-  a.own_o = (float*)(s + kPlanBytes + aligned(((size_t)kMaxSlots + (size_t)w.B * w.H) * w.G * 2 * sizeof(float)));
+  use_scratch(a, scratch_for(w.B, 0, w.G, w.H, w.D), scratch);
   const hipError_t e = w.D == 128 ? launch<128, kWindowed>(a, st) : launch<64, kWindowed>(a, st);
   return e == hipSuccess ? WGKV_OK : WGKV_ERR_HIP;
 }
@@ -835,8 +1011,7 @@ extern "C" int wgkv_shared_decode_attn(
   if (cap > 0x7fffff00 || pcap > 0x7fffff00) return WGKV_ERR_UNSUPPORTED;
   const bool many = many_rows(batch, num_groups, G);
   const int64_t row_tiles = (int64_t)batch * G / (many ? kMany : kFew) + num_groups;
-  if ((cap + 31) / 32 * own * kStreamed + (pcap + 31) / 32 * row_tiles * num_kv_heads * (many ? kTiled : kStreamed) >
-      0x70000000)
+  if ((cap + 31) / 32 * own + (pcap + 31) / 32 * row_tiles * num_kv_heads > 0x70000000)
     return WGKV_ERR_UNSUPPORTED;
   if (((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) return WGKV_ERR_UNSUPPORTED;
   if ((q_stride_b | q_stride_h) & 7) return WGKV_ERR_UNSUPPORTED;
@@ -876,12 +1051,7 @@ extern "C" int wgkv_shared_decode_attn(
   a.scale_log2 = softmax_scale == 0.f ? 1.f : fabsf(softmax_scale) * attn::kLog2e;
   a.q_and = softmax_scale == 0.f ? 0u : ~0u;
   a.q_xor = softmax_scale < 0.f ? 0x80008000u : 0u;
-  char* ws = (char*)workspace;
-  a.plan = (int*)ws;
-  a.pre_ml = (float*)(ws + sc.pre_ml);
-  a.pre_o = (float*)(ws + sc.pre_o);
-  a.own_ml = (float*)(ws + sc.own_ml);
-  a.own_o = (float*)(ws + sc.own_o);
+  use_scratch(a, sc, workspace);
   hipStream_t st = (hipStream_t)stream;
   const hipError_t e = head_dim == 128 ? launch_rows<128>(a, many, st) : launch_rows<64>(a, many, st);
   return e == hipSuccess ? WGKV_OK : WGKV_ERR_HIP;
