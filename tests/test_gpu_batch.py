@@ -98,8 +98,9 @@ def test_tables_of_prompts(req, masked, H, P):
     rng = np.random.default_rng(sum(req) + H)
     lens = held_tokens(rng, len(req), H, 100)
     mask = rng.random((H, sum(req) + 9)) < rng.choice([0.02, 0.3, 0.98], (H, 1)) if masked else None
-    check_tables(lens, req, H, P, mask, free=list(range(90000, 90013)), blocks=10 ** 5, first=4, tail=5,
-                 in_place=masked)
+    for in_place in (False, True):
+        check_tables(lens, req, H, P, mask, free=list(range(90000, 90013)), blocks=10 ** 5, first=4, tail=5,
+                     in_place=in_place)
 
 
 @pytest.mark.parametrize("masked", [False, True])
@@ -110,6 +111,15 @@ def test_tables_of_many_requests_in_a_tile(masked):
     req = rng.choice([0, 1, 1, 2, 5], 900).tolist()
     mask = rng.random((8, sum(req))) < 0.5 if masked else None
     check_tables(held_tokens(rng, 900, 8, 40), req, 8, 16, mask)
+    check_tables(held_tokens(rng, 900, 8, 40), req, 8, 16, mask, in_place=True)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+def test_tables_of_many_heads(masked):
+    """More (tile, head) pairs than a workgroup sums up in LDS."""
+    rng = np.random.default_rng(4)
+    mask = rng.random((1400, 300)) < 0.5 if masked else None
+    check_tables(held_tokens(rng, 1, 1400, 40), [300], 1400, 16, mask)
 
 
 def test_tables_without_tokens():
@@ -117,6 +127,7 @@ def test_tables_without_tokens():
     check_tables([[0, 5], [16, 17]], [0, 0], 2, 16, first=3, tail=2)
     check_tables([[0]], [0], 1, 16, np.zeros((1, 0), bool))
     check_tables(np.zeros((300, 20), int), [0] * 300, 20, 16)
+    check_tables(np.zeros((300, 20), int), [0] * 300, 20, 16, np.zeros((20, 0), bool))
 
 
 @pytest.mark.parametrize("N", [40, 600])

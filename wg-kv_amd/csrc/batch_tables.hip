@@ -15,10 +15,12 @@
 // writes the page's table entry, so no launch goes over pages.
 //
 // All of it is latency: 0.5 MB of mask and 2 MB of rows of 16K tokens and 8
-// heads take under a microsecond of bandwidth.  So a step of up to 256 tokens
-// (a decode step) is one launch of one workgroup, and longer ones are cut
-// into tiles of 256 tokens: counts of the mask per tile (masked ones), the
-// plan over heads, the tiles' rows.
+// heads take under a microsecond of bandwidth.  So launches are few and loads
+// do not wait for one another: a step of up to 256 tokens (a decode step) is one
+// launch of one workgroup.  A longer one has a workgroup per 256 tokens, each
+// of which makes the whole plan in LDS for itself; its kept tokens are counted
+// by a launch before that if there is a mask.  Where the plan does not fit into
+// LDS it is a launch of one workgroup between the two.
 #include <string.h>
 
 #include "kv4.h"
@@ -28,7 +30,7 @@ namespace {
 constexpr int kTile = 256;       // tokens per tile
 constexpr int kHeadGroup = 16;   // heads whose rows are gathered in LDS for one coalesced write
 constexpr int kPlanThreads = 1024;
-constexpr int kSmallHeads = 4096;  // (request, head) pairs that one workgroup plans in LDS
+constexpr int kLdsHeads = 4096;    // (request, head) pairs that a workgroup plans in LDS, (tile, head) pairs too
 
 struct TablesArgs {
   const int32_t* len;
@@ -53,10 +55,14 @@ struct TablesArgs {
   int32_t* status;
   // scratch of the steps that take more than one launch
   int tiles;
-  int* tile_count;   // (H, tiles): kept tokens of a tile, then of the tiles before it
+  int* tile_count;   // (H, tiles): kept tokens of a tile; of the tiles before it once there is a plan
   int* start_count;  // (B + 1, H): kept tokens of cu[b]'s tile before cu[b]
   int4* plan;        // (B * H)
   int4* head;        // one entry
+  // lengths and page state as they were, for the workgroups that read them while
+  // one replaces them
+  int* len_copy;
+  int* state_copy;
 };
 
 // What the rows of a head need: tokens held, kept tokens of the whole batch
@@ -77,14 +83,14 @@ WGKV_DEVICE int clamped_len(const TablesArgs& a, int e) {
   return min(max(a.len[(int64_t)b * a.len_sb + h], 0), a.max_pages << a.page_log2);
 }
 
-// The last request that starts at or before token n, or -1 where n lies in
-// none (before the first or behind the last).
-WGKV_DEVICE int request_of(const TablesArgs& a, int n) {
-  int lo = 0, hi = a.B;  // cu[lo] <= n < cu[hi]
-  if (n < a.cu[0] || n >= a.cu[a.B]) return -1;
+// The last of B requests that starts at or before token n, or -1 where n lies
+// in none (before the first or behind the last).
+WGKV_DEVICE int request_of(const int* cu, int B, int n) {
+  int lo = 0, hi = B;  // cu[lo] <= n < cu[hi]
+  if (n < cu[0] || n >= cu[B]) return -1;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (a.cu[mid] <= n) lo = mid; else hi = mid;
+    if (cu[mid] <= n) lo = mid; else hi = mid;
   }
   return lo;
 }
@@ -146,101 +152,93 @@ WGKV_DEVICE int block_exclusive_scan(int v, int* s_wave, int* total) {
   return before + incl - v;
 }
 
-// The plan over all heads, by one workgroup: every thread takes consecutive
-// entries.  kept_before(b, h) is the batch's kept tokens before request b's
-// first; it does not change while the plan is made.  Also writes the new
-// lengths, the page state and the status.
-template <int kThreads, typename Kept, typename Put>
-WGKV_DEVICE StepPlan plan_heads(const TablesArgs& a, int* s_wave, int* s_over, Kept kept_before, Put put) {
-  const int t = threadIdx.x, BH = a.B * a.H;
-  const int per = (BH + kThreads - 1) / kThreads;
-  const int lo = min(BH, t * per), hi = min(BH, lo + per);
+// Page state as a plan starts from it.
+struct PageState {
+  int next, held, held_given;
+};
+WGKV_DEVICE PageState page_state(const TablesArgs& a) {
+  const int given = a.state[1];
+  return {max(a.state[0], 0), a.free_ids ? min(max(given, 0), a.free_cap) : 0, given};
+}
+
+// New pages of a head that keeps `kept` tokens more; *over: it outgrows its table.
+WGKV_DEVICE int pages_needed(const TablesArgs& a, int len, int kept, int* over) {
   const int up = (1 << a.page_log2) - 1;
-  const int64_t room = (int64_t)a.max_pages << a.page_log2;
-  if (t == 0) *s_over = 0;
-  __syncthreads();
-  int need = 0;
-  for (int e = lo; e < hi; ++e) {
-    const int b = e / a.H, h = e - b * a.H, len = clamped_len(a, e);
-    const int64_t now = (int64_t)len + max(kept_before(b + 1, h) - kept_before(b, h), 0);
-    if (now > room) *s_over = 1;
-    else need += (((int)now + up) >> a.page_log2) - ((len + up) >> a.page_log2);
+  if ((int64_t)len + kept > (int64_t)a.max_pages << a.page_log2) {
+    *over = 1;
+    return 0;
   }
-  int total;
-  int page = block_exclusive_scan<kThreads>(need, s_wave, &total);
+  return ((len + kept + up) >> a.page_log2) - ((len + up) >> a.page_log2);
+}
+
+// The step's plan from the pages that it needs in all.
+WGKV_DEVICE StepPlan step_plan(const TablesArgs& a, const PageState& st, int total, bool over) {
   StepPlan s;
-  const int held = a.free_ids ? a.state[1] : 0;
-  s.held = min(max(held, 0), a.free_cap);
-  s.next = max(a.state[0], 0);
+  s.held = st.held;
+  s.next = st.next;
   s.take = min(total, s.held);
-  s.fits = !*s_over && (int64_t)s.next + total - s.take <= a.num_pages;
-  const int state1 = a.free_ids ? s.held - (s.fits ? s.take : 0) : a.state[1];
-  for (int e = lo; e < hi; ++e) {
-    const int b = e / a.H, h = e - b * a.H, len = clamped_len(a, e);
-    const int before = kept_before(b, h);
-    const int kept = max(kept_before(b + 1, h) - before, 0);
-    put(e, HeadPlan{len, before, page});
-    if (s.fits) page += ((len + kept + up) >> a.page_log2) - ((len + up) >> a.page_log2);
-    // (in place: only this thread reads this length, before)
-    a.out[(int64_t)b * a.out_sb + h] = len + (s.fits ? kept : 0);
-  }
-  __syncthreads();  // the page state has been read by every thread
-  if (t == 0) {
-    a.state_out[0] = s.next + (s.fits ? total - s.take : 0);
-    a.state_out[1] = state1;
-    if (!s.fits && a.status) *a.status = WGKV_ERR_CAPACITY;
-  }
+  s.fits = !over && (int64_t)s.next + total - s.take <= a.num_pages;
   return s;
 }
 
+// New page state and status, by one thread.
+WGKV_DEVICE void put_state(const TablesArgs& a, const PageState& st, const StepPlan& s, int total) {
+  a.state_out[0] = s.next + (s.fits ? total - s.take : 0);
+  a.state_out[1] = a.free_ids ? s.held - (s.fits ? s.take : 0) : st.held_given;
+  if (!s.fits && a.status) *a.status = WGKV_ERR_CAPACITY;
+}
+
 // Rows of a tile's tokens for all heads, by a workgroup of NW waves: a wave
-// takes a head, a lane four tokens; the rows of kHeadGroup heads meet in LDS
-// and are written as they lie in memory.  tile_before(h): kept tokens of
-// the tiles before this one.
+// takes a head and 64 of the tokens, whose requests are in s_req; the rows of
+// kHeadGroup heads meet in LDS and are written as they lie in memory.
+// tile_before(h): kept tokens of the tiles before this one.
 template <int NW, typename Plan, typename Before>
-WGKV_DEVICE void tile_rows(const TablesArgs& a, int tile, const StepPlan& s, int* s_req, int* s_row, Plan plan,
+WGKV_DEVICE void tile_rows(const TablesArgs& a, int tile, const StepPlan& s, const int* s_req, int* s_row, Plan plan,
                            Before tile_before) {
   const int t = threadIdx.x, lane = t & 63, w = t >> 6;
   const int mask = (1 << a.page_log2) - 1;
   const int n_tok = min(kTile, a.N - tile * kTile);
-  if (t < kTile) s_req[t] = t < n_tok ? request_of(a, tile * kTile + t) : -1;
-  __syncthreads();
   for (int h0 = 0; h0 < a.H; h0 += kHeadGroup) {
     const int hg = min(kHeadGroup, a.H - h0);
-    for (int hh = w; hh < hg; hh += NW) {
-      const int h = h0 + hh;
-      int bits = 15, at = 0;
+    for (int u = w; u < hg * (kTile / 64); u += NW) {
+      const int hh = u / (kTile / 64), part = u % (kTile / 64), h = h0 + hh, x = part * 64 + lane;
+      bool kept = x < n_tok;
+      int before = tile * kTile + x;  // kept tokens of the batch before this one
       if (a.mask) {
-        bits = kept_bits(a, h, tile, lane);
-        const int mine = __builtin_popcount(bits);
-        at = tile_before(h) + wave_incl_scan(mine, lane) - mine;
-      }
+        const uint8_t* m = a.mask + (int64_t)h * a.mask_sh + tile * kTile;
+        uint8_t on[kTile / 64];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int x = 4 * lane + i, b = s_req[x];
-        int row = -1;
-        if (b >= 0 && (bits >> i & 1) && s.fits) {
-          const HeadPlan p = plan(b * a.H + h);
-          const int pos = p.len + (a.mask ? at : tile * kTile + x) - p.before;
-          const int j = pos >> a.page_log2, p0 = (p.len + mask) >> a.page_log2;
-          // (a negative or too large position: cu does not ascend)
-          if (pos >= p.len && j < a.max_pages) {
-            int32_t* entry = a.bt + (int64_t)b * a.bt_sb + (int64_t)h * a.bt_sh + j;
-            int id;
-            if (j < p0) {
-              id = *entry;
-            } else {
-              const int k = p.page + j - p0;
-              id = k < 0 ? -1 : k < s.take ? a.free_ids[s.held - s.take + k] : s.next + k - s.take;
-              if (k >= 0 && (pos & mask) == 0) *entry = id;
-            }
-            if (id >= 0 && id < a.num_pages) row = (id << a.page_log2) + (pos & mask);
-            else if (a.status) *a.status = WGKV_ERR_CAPACITY;
+        for (int i = 0; i < kTile / 64; ++i) on[i] = i <= part && i * 64 + lane < n_tok ? m[i * 64 + lane] : 0;
+        before = tile_before(h);
+#pragma unroll
+        for (int i = 0; i < kTile / 64; ++i) {
+          const uint64_t set = __ballot(on[i] != 0);
+          if (i < part) before += __popcll(set);
+          if (i == part) {
+            before += __popcll(set & ((1ull << lane) - 1));
+            kept = on[i] != 0;
           }
         }
-        at += bits >> i & 1;
-        s_row[x * hg + hh] = row;
       }
+      const int b = s_req[x];
+      int row = -1;
+      if (b >= 0 && kept && s.fits) {
+        const HeadPlan p = plan(b * a.H + h);
+        const int pos = p.len + before - p.before;
+        const int j = pos >> a.page_log2, p0 = (p.len + mask) >> a.page_log2;
+        // (a negative or too large position: cu does not ascend)
+        if (pos >= p.len && j < a.max_pages) {
+          int32_t* entry = a.bt + (int64_t)b * a.bt_sb + (int64_t)h * a.bt_sh + j;
+          const int k = p.page + j - p0;  // of the new pages
+          int id = k < 0 ? -1 : s.next + k - s.take;
+          const int32_t* held = j < p0 ? entry : k >= 0 && k < s.take ? a.free_ids + (s.held - s.take + k) : nullptr;
+          if (held) id = *held;
+          if (j >= p0 && k >= 0 && (pos & mask) == 0) *entry = id;
+          if (id >= 0 && id < a.num_pages) row = (id << a.page_log2) + (pos & mask);
+          else if (a.status) *a.status = WGKV_ERR_CAPACITY;
+        }
+      }
+      s_row[x * hg + hh] = row;
     }
     __syncthreads();
     for (int i = t; i < n_tok * hg; i += NW * 64) {
@@ -251,37 +249,93 @@ WGKV_DEVICE void tile_rows(const TablesArgs& a, int tile, const StepPlan& s, int
   }
 }
 
-// Steps of up to kTile tokens and kSmallHeads heads: everything in one launch
-// of one workgroup.  256 requests x 8 heads x 1 token: see the table in the
-// documentation of the host entry point.
-__global__ __launch_bounds__(kPlanThreads) void tables_small_kernel(TablesArgs a) {
-  __shared__ int s_start[kSmallHeads + kTile];  // ((B + 1) * H fits: the host checks)
-  __shared__ HeadPlan s_plan[kSmallHeads];
+// Steps whose plan fits into LDS.  ONE: of up to kTile tokens, one workgroup,
+// which counts the mask itself; otherwise a workgroup per tile, of which the
+// first writes the lengths and the state.
+template <bool ONE>
+__global__ __launch_bounds__(kPlanThreads) void tables_step_kernel(TablesArgs a) {
+  constexpr int NW = kPlanThreads / 64, PER = kLdsHeads / kPlanThreads;
+  __shared__ int s_cu[kLdsHeads], s_len[kLdsHeads], s_before[kLdsHeads], s_page[kLdsHeads];
+  __shared__ int s_kept[kLdsHeads + kTile];  // ONE: kept tokens before each start; else before each tile
   __shared__ int s_row[kTile * kHeadGroup];
-  __shared__ int s_req[kTile], s_wave[kPlanThreads / 64], s_over;
-  const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+  __shared__ int s_req[kTile], s_wave[NW], s_over;
+  const int t = threadIdx.x, lane = t & 63, w = t >> 6, tile = blockIdx.x, BH = a.B * a.H;
+  const int per = (BH + kPlanThreads - 1) / kPlanThreads;
+  const int lo = min(BH, t * per), n_mine = min(BH, lo + per) - lo;
+  // What does not depend on anything is asked for at once.
+  const PageState st = page_state(a);
+  int len[PER];
+#pragma unroll
+  for (int k = 0; k < PER; ++k) len[k] = k < n_mine ? clamped_len(a, lo + k) : 0;
+  for (int b = t; b <= a.B; b += kPlanThreads) s_cu[b] = clamped_cu(a, b);
+  if (t == 0) s_over = 0;
   if (a.mask) {
-    for (int h = w; h < a.H; h += kPlanThreads / 64) count_tile(a, h, 0, 0, a.B + 1, lane, s_start);
-    // (a start at N = kTile lies behind the tile's last lane)
-    __syncthreads();
-    for (int h = w; h < a.H; h += kPlanThreads / 64) {
-      const int all = wave_sum_int(__builtin_popcount(kept_bits(a, h, 0, lane)));
-      for (int b = lane; b <= a.B; b += 64)
-        if (clamped_cu(a, b) >= kTile) s_start[b * a.H + h] = all;
+    for (int h = w; h < a.H; h += NW) {
+      if constexpr (ONE) {
+        const int all = count_tile(a, h, 0, 0, a.B + 1, lane, s_kept);
+        // (a start at kTile lies behind the tile's last lane)
+        for (int b = lane; b <= a.B; b += 64)
+          if (clamped_cu(a, b) >= kTile) s_kept[b * a.H + h] = all;
+      } else {
+        const int* c = a.tile_count + (int64_t)h * a.tiles;
+        int run = 0;
+        for (int i0 = 0; i0 <= a.tiles; i0 += 64) {  // entry `tiles` is the total
+          const int n = i0 + lane < a.tiles ? c[i0 + lane] : 0;
+          const int incl = wave_incl_scan(n, lane);
+          if (i0 + lane <= a.tiles) s_kept[h * (a.tiles + 1) + i0 + lane] = run + incl - n;
+          run += __builtin_amdgcn_readlane(incl, 63);
+        }
+      }
     }
-    __syncthreads();
   }
-  const StepPlan s = plan_heads<kPlanThreads>(
-      a, s_wave, &s_over, [&](int b, int h) { return a.mask ? s_start[b * a.H + h] : clamped_cu(a, b); },
-      [&](int e, const HeadPlan& p) { s_plan[e] = p; });
   __syncthreads();
-  if (a.N) tile_rows<kPlanThreads / 64>(a, 0, s, s_req, s_row, [&](int e) { return s_plan[e]; }, [](int) { return 0; });
+  if (t < kTile) s_req[t] = tile * kTile + t < a.N ? request_of(s_cu, a.B, tile * kTile + t) : -1;
+  const auto kept_before = [&](int b, int h) {
+    if (!a.mask) return s_cu[b];
+    if (ONE) return s_kept[b * a.H + h];
+    const int n = s_cu[b], in_tile = n < a.N ? a.start_count[(int64_t)b * a.H + h] : 0;
+    return s_kept[h * (a.tiles + 1) + (n < a.N ? n / kTile : a.tiles)] + in_tile;
+  };
+  int need[PER], kept[PER], mine = 0, over = 0, total;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    need[k] = kept[k] = 0;
+    if (k >= n_mine) continue;
+    const int e = lo + k, b = e / a.H, h = e - b * a.H, before = kept_before(b, h);
+    kept[k] = max(kept_before(b + 1, h) - before, 0);
+    need[k] = pages_needed(a, len[k], kept[k], &over);
+    s_len[e] = len[k];
+    s_before[e] = before;
+    mine += need[k];
+  }
+  if (over) s_over = 1;
+  int page = block_exclusive_scan<kPlanThreads>(mine, s_wave, &total);
+  const StepPlan s = step_plan(a, st, total, s_over);
+#pragma unroll
+  for (int k = 0; k < PER; ++k) {
+    if (k >= n_mine) continue;
+    const int e = lo + k, b = e / a.H;
+    s_page[e] = page;
+    page += need[k];
+    // (in place, ONE only: this thread alone has read this length)
+    if (ONE || tile == 0) a.out[(int64_t)b * a.out_sb + e - b * a.H] = len[k] + (s.fits ? kept[k] : 0);
+  }
+  if ((ONE || tile == 0) && t == 0) put_state(a, st, s, total);  // (every thread has read it: it has passed barriers)
+  __syncthreads();
+  if (a.N)
+    tile_rows<NW>(a, tile, s, s_req, s_row, [&](int e) { return HeadPlan{s_len[e], s_before[e], s_page[e]}; },
+                  [&](int h) { return ONE ? 0 : s_kept[h * (a.tiles + 1) + tile]; });
 }
 
-// Kept tokens of every tile and head, and of a tile before the request
-// starts in it.
+// Kept tokens of every tile and head, and of a tile before the request starts
+// in it; copies of what is replaced in place.
 __global__ __launch_bounds__(256) void tables_count_kernel(TablesArgs a) {
   const int tile = blockIdx.x, lane = threadIdx.x & 63;
+  if (tile == 0 && a.len_copy) {
+    for (int e = threadIdx.x; e < a.B * a.H; e += 256) a.len_copy[e] = clamped_len(a, e);
+    if (threadIdx.x < 2) a.state_copy[threadIdx.x] = a.state[threadIdx.x];
+  }
+  if (!a.mask) return;
   const int b0 = first_start(a, tile * kTile), b1 = first_start(a, (tile + 1) * kTile);
   for (int h = threadIdx.x >> 6; h < a.H; h += 4) {
     const int n = count_tile(a, h, tile, b0, b1, lane, a.start_count);
@@ -289,11 +343,13 @@ __global__ __launch_bounds__(256) void tables_count_kernel(TablesArgs a) {
   }
 }
 
+// The plan over all heads, by one workgroup whose threads take consecutive
+// entries.
 __global__ __launch_bounds__(kPlanThreads) void tables_plan_kernel(TablesArgs a) {
   __shared__ int s_wave[kPlanThreads / 64], s_over;
-  const int lane = threadIdx.x & 63;
+  const int t = threadIdx.x, lane = t & 63, BH = a.B * a.H;
   if (a.mask) {  // tile counts become sums of the tiles before; entry `tiles` is the total
-    for (int h = threadIdx.x >> 6; h < a.H; h += kPlanThreads / 64) {
+    for (int h = t >> 6; h < a.H; h += kPlanThreads / 64) {
       int* c = a.tile_count + (int64_t)h * a.tiles;
       int run = 0;
       for (int i0 = 0; i0 < a.tiles; i0 += 64) {
@@ -305,18 +361,37 @@ __global__ __launch_bounds__(kPlanThreads) void tables_plan_kernel(TablesArgs a)
       if (lane == 0) a.tile_count[(int64_t)a.H * a.tiles + h] = run;
     }
     __threadfence_block();
-    __syncthreads();
   }
-  const StepPlan s = plan_heads<kPlanThreads>(
-      a, s_wave, &s_over,
-      [&](int b, int h) {
-        const int n = clamped_cu(a, b);
-        if (!a.mask) return n;
-        if (n >= a.N) return a.tile_count[(int64_t)a.H * a.tiles + h];
-        return a.tile_count[(int64_t)h * a.tiles + n / kTile] + a.start_count[(int64_t)b * a.H + h];
-      },
-      [&](int e, const HeadPlan& p) { a.plan[e] = make_int4(p.len, p.before, p.page, 0); });
-  if (threadIdx.x == 0) *a.head = make_int4(s.take, s.next, s.held, s.fits);
+  if (t == 0) s_over = 0;
+  __syncthreads();
+  const auto kept_before = [&](int b, int h) {
+    const int n = clamped_cu(a, b);
+    if (!a.mask) return n;
+    if (n >= a.N) return a.tile_count[(int64_t)a.H * a.tiles + h];
+    return a.tile_count[(int64_t)h * a.tiles + n / kTile] + a.start_count[(int64_t)b * a.H + h];
+  };
+  const PageState st = page_state(a);
+  const int per = (BH + kPlanThreads - 1) / kPlanThreads, lo = min(BH, t * per), hi = min(BH, lo + per);
+  int mine = 0, over = 0, total;
+  for (int e = lo; e < hi; ++e) {
+    const int b = e / a.H, h = e - b * a.H, before = kept_before(b, h);
+    mine += pages_needed(a, clamped_len(a, e), max(kept_before(b + 1, h) - before, 0), &over);
+  }
+  if (over) s_over = 1;
+  int page = block_exclusive_scan<kPlanThreads>(mine, s_wave, &total);
+  const StepPlan s = step_plan(a, st, total, s_over);
+  for (int e = lo; e < hi; ++e) {
+    const int b = e / a.H, h = e - b * a.H, len = clamped_len(a, e), before = kept_before(b, h);
+    const int kept = max(kept_before(b + 1, h) - before, 0);
+    a.plan[e] = make_int4(len, before, page, 0);
+    page += pages_needed(a, len, kept, &over);
+    // (in place: only this thread reads this length, before)
+    a.out[(int64_t)b * a.out_sb + h] = len + (s.fits ? kept : 0);
+  }
+  if (t == 0) {
+    put_state(a, st, s, total);  // (every thread has read it: it has passed barriers)
+    *a.head = make_int4(s.take, s.next, s.held, s.fits);
+  }
 }
 
 __global__ __launch_bounds__(256) void tables_rows_kernel(TablesArgs a) {
@@ -324,7 +399,9 @@ __global__ __launch_bounds__(256) void tables_rows_kernel(TablesArgs a) {
   __shared__ int s_req[kTile];
   const int4 hd = *a.head;
   const StepPlan s = {hd.x, hd.y, hd.z, hd.w};
-  const int tile = blockIdx.x;
+  const int t = threadIdx.x, tile = blockIdx.x;
+  s_req[t] = tile * kTile + t < a.N ? request_of(a.cu, a.B, tile * kTile + t) : -1;
+  __syncthreads();
   tile_rows<4>(a, tile, s, s_req, s_row,
                [&](int e) {
                  const int4 p = a.plan[e];
@@ -378,7 +455,11 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
 
 int page_log2_of(int page_size) { return page_size == 16 ? 4 : page_size == 32 ? 5 : page_size == 64 ? 6 : -1; }
 
-bool small_step(int B, int H, int N) { return N <= kTile && (int64_t)(B + 1) * H <= kSmallHeads; }
+// Whether the plan fits into LDS, with the sums over its tiles.
+bool lds_step(int B, int H, int N) {
+  return (int64_t)(B + 1) * H <= kLdsHeads && ((int64_t)N / kTile + 2) * H <= kLdsHeads;
+}
+bool small_step(int B, int H, int N) { return N <= kTile && (int64_t)(B + 1) * H <= kLdsHeads; }
 
 size_t aligned(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -455,7 +536,7 @@ extern "C" int wgkv_build_block_tables(
   a.status = status;
   hipStream_t st = (hipStream_t)stream;
   if (small) {
-    hipLaunchKernelGGL(tables_small_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
+    hipLaunchKernelGGL(tables_step_kernel<true>, dim3(1), dim3(kPlanThreads), 0, st, a);
     return hipGetLastError() == hipSuccess ? WGKV_OK : WGKV_ERR_HIP;
   }
   a.tiles = (num_tokens + kTile - 1) / kTile;
@@ -464,9 +545,24 @@ extern "C" int wgkv_build_block_tables(
   a.start_count = (int*)(ws + sc.start);
   a.plan = (int4*)(ws + sc.plan);
   a.head = (int4*)(ws + sc.head);
-  if (g_mask && a.tiles) {
-    hipLaunchKernelGGL(tables_count_kernel, dim3(a.tiles), dim3(256), 0, st, a);
+  const bool lds = lds_step(batch, num_kv_heads, num_tokens);
+  const bool copies = lds && (new_lengths == lengths || state_out == page_state);
+  if (copies) {
+    a.len_copy = (int*)a.plan;
+    a.state_copy = (int*)a.head;
+  }
+  if ((g_mask && a.tiles) || copies) {
+    hipLaunchKernelGGL(tables_count_kernel, dim3(g_mask ? a.tiles : 1), dim3(256), 0, st, a);
     WGKV_HIP_CHECK(hipGetLastError());
+  }
+  if (lds) {
+    if (copies) {
+      a.len = a.len_copy;
+      a.len_sb = num_kv_heads;
+      a.state = a.state_copy;
+    }
+    hipLaunchKernelGGL(tables_step_kernel<false>, dim3(a.tiles), dim3(kPlanThreads), 0, st, a);
+    return hipGetLastError() == hipSuccess ? WGKV_OK : WGKV_ERR_HIP;
   }
   hipLaunchKernelGGL(tables_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
   WGKV_HIP_CHECK(hipGetLastError());
