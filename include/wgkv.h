@@ -737,7 +737,8 @@ int wgkv_kv4_decode_attn_block(const void* args);
  * give zeros; what a row does not see has no part in it, NaN included.  Rows
  * of no sequence are left as they are, or cleared (clear_rest != 0).  window
  * >= 1; D in {64,128}; G = Hq/Hkv in 1..8; up to 2048 sequences and 2^30
- * rows.
+ * rows.  Few rows with long windows take a workspace (as sized, 0 bytes for
+ * others; any contents; calls that share one ordered) and two launches.
  *
  * wgkv_paged_decode_attn_window: wgkv_paged_decode_attn where a head of T
  * tokens shows those t with t >= T - window or t < num_sinks.  Page ids of the
@@ -769,6 +770,9 @@ int wgkv_paged_append(
     void* k_cache, void* v_cache, int64_t cache_rows, const int32_t* slots,
     int32_t num_tokens, int32_t num_kv_heads, int32_t head_dim, void* stream);
 
+size_t wgkv_sink_window_workspace_bytes(int32_t batch, int32_t num_rows, int32_t num_keys, int32_t num_q_heads,
+                                        int32_t num_kv_heads, int32_t head_dim, int32_t window, int32_t num_sinks);
+
 int wgkv_sink_window_attn(
     const void* q, int64_t q_stride_n, int64_t q_stride_h,
     const void* k, int64_t k_stride_n, int64_t k_stride_h,
@@ -776,7 +780,8 @@ int wgkv_sink_window_attn(
     void* out, int64_t out_stride_n, int64_t out_stride_h,
     const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int32_t batch, int32_t num_rows, int32_t num_keys,
     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-    int32_t window, int32_t num_sinks, float softmax_scale, int32_t clear_rest, void* stream);
+    int32_t window, int32_t num_sinks, float softmax_scale, int32_t clear_rest, void* workspace, size_t workspace_bytes,
+    void* stream);
 
 size_t wgkv_paged_decode_window_workspace_bytes(int32_t batch, int32_t num_q_heads, int32_t num_kv_heads,
                                                 int32_t head_dim);

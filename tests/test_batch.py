@@ -150,11 +150,15 @@ def test_c_entry_points_check_arguments_without_gpu():
     refused(L.wgkv_paged_append, append, [
         (0, None, ARG), (3, None, ARG), (6, None, ARG), (9, None, ARG), (10, -1, ARG), (11, 0, ARG), (12, 0, ARG),
         (12, 60, UNS), (0, p + 2, UNS), (1, 129, UNS), (8, 1 << 32, UNS), (8, -1, ARG), (7, p + 512, ARG), (7, p, ARG)])
-    prompt = [p, 256, 64, p, 128, 64, p, 128, 64, p, 256, 64, p, p, 2, 3, 3, 4, 2, 64, 4, 1, 0.1, 0, None]
+    prompt = [p, 256, 64, p, 128, 64, p, 128, 64, p, 256, 64, p, p, 2, 3, 3, 4, 2, 64, 4, 1, 0.1, 0, None, 0, None]
     refused(L.wgkv_sink_window_attn, prompt, [
         (0, None, ARG), (3, None, ARG), (9, None, ARG), (12, None, ARG), (13, None, ARG), (14, 0, ARG), (14, 2049, UNS),
         (15, -1, ARG), (16, -1, ARG), (17, 3, ARG), (17, 18, UNS), (19, 96, UNS), (20, 0, ARG), (21, -1, ARG),
         (0, p + 2, UNS), (1, 260, UNS), (10, 64, ARG), (10, 0, ARG), (11, 0, ARG), (15, (1 << 30) + 1, UNS)])
+    few = prompt[:16] + [4000] + prompt[17:20] + [4000] + prompt[21:]  # few rows, many keys: cut into parts
+    need = L.wgkv_sink_window_workspace_bytes(2, 3, 4000, 4, 2, 64, 4000, 1)
+    assert need > 0 == L.wgkv_sink_window_workspace_bytes(2, 3, 4000, 4, 2, 64, 200, 1)
+    refused(L.wgkv_sink_window_attn, few[:24] + [p, need, None], [(24, None, WS), (25, need - 1, WS), (24, p + 4, WS)])
     window = [p, 256, 64, p, p, 8, 16, p, 2, p, 8, 4, 4, p, 256, 64, 2, 4, 2, 64, 4, 1, 0.1, p, 1 << 40, None]
     refused(L.wgkv_paged_decode_attn_window, window, [
         (0, None, ARG), (3, None, ARG), (5, 0, ARG), (6, 8, UNS), (7, None, ARG), (9, None, ARG), (12, 0, ARG),
@@ -174,7 +178,7 @@ def test_block_words_that_do_not_fit():
     L = _lib.lib()
     assert L.wgkv_build_block_tables_block(batch._pack_tables(*([1] * 3), 1 << 40, *([1] * 21))) == _lib.ERR_UNSUPPORTED
     assert L.wgkv_paged_append_block(batch._pack_append(*([1] * 10), 1 << 40, 1, 1, 1)) == _lib.ERR_UNSUPPORTED
-    assert L.wgkv_sink_window_attn_block(batch._pack_prompt(*([1] * 14), 1 << 40, *([1] * 7), 1.0, 1, 1)) == \
+    assert L.wgkv_sink_window_attn_block(batch._pack_prompt(*([1] * 14), 1 << 40, *([1] * 7), 1.0, 1, 1, 1, 1)) == \
         _lib.ERR_UNSUPPORTED
     assert L.wgkv_paged_decode_attn_window_block(batch._pack_window(*([1] * 6), 1 << 40, *([1] * 15), 1.0, 1, 1, 1)) == \
         _lib.ERR_UNSUPPORTED

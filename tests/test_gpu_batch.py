@@ -316,6 +316,72 @@ def test_prompt_takes_nothing_from_what_it_does_not_see(bad, D):
     check_close(torch.where(fine, out.double(), 0), torch.where(fine, want, 0), torch.where(fine, bound, 0))
 
 
+@pytest.mark.parametrize("D,G,H", [(64, 1, 1), (64, 8, 3), (128, 4, 8), (128, 3, 2), (128, 2, 1)])
+@pytest.mark.parametrize("req,past,window,sinks", [
+    ([1], [9000], 1 << 30, 0), ([1], [9000], 4096, 64), ([5, 70, 0, 1], [4000, 0, 3, 700], 2000, 4),
+    ([64, 33], [-20, 5000], 3000, 1), ([300], [2000], 2222, 100)])
+def test_prompt_few_rows_behind_many_keys(D, G, H, req, past, window, sinks):
+    """The keys of an item are cut into parts, some of which may be empty."""
+    check_prompt(req, past, G * H, H, D, window, sinks, seed=G, first=2)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("D", [64, 128])
+def test_prompt_parts_take_nothing_from_what_is_not_seen(bad, D):
+    import wgkv
+    cu, cuk, W, S = [0, 7, 47], [0, 3007, 6047], 1500, 3
+    q, k, v = qkv(cu[-1], cuk[-1], 4, 2, D, 3)
+    for t in (k, v):
+        t[700:900] = bad           # before the windows
+        t[3007 - 3] = bad          # the first sequence's rows 4 .. see it
+    v[6047 - 1 - W - 20, 1, 9] = bad  # the second's rows .. 19, of KV head 1
+    k[3007 + 1, 0] = bad           # a first token, of KV head 0: seen by all
+    out = wgkv.sink_window_attn(q, k, v, i32(cu), W, S, None, i32(cuk))
+    torch.cuda.synchronize()
+    want, bound = ob.prompt(q, k, v, cu, cuk, W, S, D ** -0.5)
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(out), fine) and fine[:4].all()
+    check_close(torch.where(fine, out.double(), 0), torch.where(fine, want, 0), torch.where(fine, bound, 0))
+
+
+@pytest.mark.parametrize("past", [None, [150, 100]])
+def test_prompt_rows_far_apart(past):
+    """Keys more than 2^31 bytes apart, in one tile and over the call."""
+    import wgkv
+    req = [200, 100]
+    cu = starts_of(req)
+    cuk = cu if past is None else starts_of([a + b for a, b in zip(req, past)])
+    Nk, stride = cuk[-1], 1 << 22
+    q, k, v = qkv(cu[-1], Nk, 4, 2, 64, 5)
+    big = torch.empty(Nk * stride, dtype=BF16, device=DEV)
+    kf = big.as_strided((Nk, 2, 64), (stride, 64, 1), 0)
+    vf = big.as_strided((Nk, 2, 64), (stride, 64, 1), 1024)
+    kf.copy_(k)
+    vf.copy_(v)
+    out = wgkv.sink_window_attn(q, kf, vf, i32(cu), 70, 3, None, i32(cuk))
+    want, bound = ob.prompt(q, k, v, cu, cuk, 70, 3, 64 ** -0.5)
+    check_close(out, want, bound)
+    assert torch.equal(out, wgkv.sink_window_attn(q, k, v, i32(cu), 70, 3, None, i32(cuk)))
+
+
+def test_prompt_parts_captured():
+    """Replays of a call that is cut into parts, with eager work between."""
+    import wgkv
+    q, k, v = qkv(40, 5040, 8, 2, 128, 1)
+    cu, cuk = i32([0, 40]), i32([0, 5040])
+    want = wgkv.sink_window_attn(q, k, v, cu, 4000, 4, None, cuk)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = wgkv.sink_window_attn(q, k, v, cu, 4000, 4, None, cuk)
+    for i in range(4):
+        out.fill_(-1)
+        g.replay()
+        other = wgkv.sink_window_attn(q + i, k, v, cu, 4000, 4, None, cuk)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        assert i == 0 or not torch.equal(other, want)
+
+
 def test_prompt_layouts():
     import wgkv
     N, Hq, H, D = 150, 8, 2, 64

@@ -23,9 +23,13 @@
 // their sums are taken of the rounded values.  Only the tiles at the two ends
 // of a row's window are masked; a wave passes over a tile none of its rows sees.
 //
+// Few rows (a last piece of a prompt, drafted tokens behind a long one) do not
+// fill the card: the tiles of every item are then cut into equal parts, a
+// workgroup each, whose (max, sum, O) a second launch joins.
+//
 // A masked probability is 0, and 0 times a key's value that is not finite is
 // NaN: rows whose result is not finite are worked out once more, key by key
-// (exact_rows).
+// (exact_row).
 #include <string.h>
 
 #include "attn_tile.h"
@@ -35,6 +39,7 @@ namespace {
 
 constexpr int kBlk = 64;      // query rows per item
 constexpr int kMaxSeqs = 2048;
+constexpr int kLeastTiles = 4;  // of a part: less than about what the join costs
 
 struct WindowArgs {
   const uint16_t* q;
@@ -52,6 +57,9 @@ struct WindowArgs {
   float scale_log2;
   uint32_t q_and, q_xor;
   int clear_rest;  // rows of no sequence get zeros
+  int parts;       // of an item's tiles; more than 1: (max, sum) and O of (part, row, head) go to
+  float* part_ml;
+  float* part_o;
 };
 
 WGKV_DEVICE int clamp_to(int x, int hi) { return min(max(x, 0), hi); }
@@ -117,7 +125,7 @@ struct Item {
   int r_blk, p_blk;   // the item's first row in the sequence, and its position
   int h, hq0;         // KV head, first query head
   Keys keys;
-  int tiles;
+  int part, t0, tiles;  // the part's tiles begin at t0
   const uint16_t *kb, *vb;
 };
 
@@ -205,15 +213,16 @@ void window_prefill_kernel(WindowArgs a) {
   }
   const attn::Offsets<D> at(n, g);
 
-  // A round's item.  Items go from the last row block to the first -- later
+  // A round's item (part).  Items go from the last row block to the first -- later
   // blocks of a sequence see no fewer keys --, heads innermost: workgroups are
   // dealt to the XCDs in turn, so with 8 KV heads each XCD's L2 serves one
   // head's keys.  A workgroup takes items from alternate ends of its rounds.
   const auto item_at = [&](int round, Item* p) {
     const int64_t item = (int64_t)round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    if (item >= (int64_t)blocks * per_block) return false;
+    if (item >= (int64_t)blocks * a.parts * per_block) return false;
     const int of = uniform((int)(item / per_block)), rest = uniform((int)(item - (int64_t)of * per_block));
-    const int blk = blocks - 1 - of;
+    const int blk = blocks - 1 - uniform(of / a.parts);
+    p->part = uniform(of % a.parts);
     int seq, r_blk, p_blk;
     Keys k;
     find_block(a, s_blocks, blk, &seq, &r_blk, &p_blk, &k);
@@ -224,7 +233,9 @@ void window_prefill_kernel(WindowArgs a) {
     p->r_blk = uniform(r_blk);
     p->p_blk = uniform(p_blk);
     p->keys = {uniform(k.first), uniform(k.shift), uniform(k.count)};
-    p->tiles = (p->keys.count + attn::kKeys - 1) / attn::kKeys;
+    const int tiles = (p->keys.count + attn::kKeys - 1) / attn::kKeys;
+    p->t0 = uniform((int)((int64_t)tiles * p->part / a.parts));
+    p->tiles = uniform((int)((int64_t)tiles * (p->part + 1) / a.parts)) - p->t0;
     p->h = uniform(rest % a.Hkv);
     p->hq0 = p->h * a.G + uniform(rest / a.Hkv) * HPW;
     const int k0 = uniform(s.k0);
@@ -240,7 +251,7 @@ void window_prefill_kernel(WindowArgs a) {
   const auto tile_load = [&](const Item& p, int tl, bool on, uint16_t* dK, uint16_t* dV) __attribute__((always_inline)) {
     if (wid >= NL) return;
     const Keys& ks = p.keys;
-    const int x0 = tl * attn::kKeys;
+    const int x0 = (p.t0 + tl) * attn::kKeys;
     if constexpr (!FAR) {
       const int j0 = ks.key(x0);
       const int rows = p.nk - j0 - 1;  // (nothing is asked for where there is no tile)
@@ -296,7 +307,7 @@ void window_prefill_kernel(WindowArgs a) {
       // Row p sees the list's entries x <= p - shift, of them those > p -
       // window - shift or < sinks.  (Of the first tokens, below the band, all
       // rows see all.)
-      const int x0 = tile * attn::kKeys, x1 = min(x0 + attn::kKeys, ks.count) - 1;
+      const int x0 = (cur.t0 + tile) * attn::kKeys, x1 = min(x0 + attn::kKeys, ks.count) - 1;
       const int e0 = p0 - ks.shift, e1 = e0 + 31;  // the last entries of the wave's first and last row
       f32x4_t sc[4][2];
       attn::tile_scores<D>(r, sK, at, sc);
@@ -336,6 +347,19 @@ void window_prefill_kernel(WindowArgs a) {
     }
     const Item done = cur;
     const int hq = done.hq0 + (wid >> 1);
+    if (a.parts > 1) {
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt) {
+        const int s = r0 + rt * 16 + n;
+        if (s >= done.nq) continue;
+        const int64_t at_row = ((int64_t)done.part * a.N + done.q0 + s) * (a.Hkv * a.G) + hq;
+        if (g == 0) *(float2*)(a.part_ml + at_row * 2) = make_float2(r.m[rt], r.sum[rt][0]);
+#pragma unroll
+        for (int dt = 0; dt < D / 16; ++dt) *(f32x4_t*)(a.part_o + at_row * D + dt * 16 + 4 * g) = r.o[dt][rt];
+      }
+      cur = nxt;
+      continue;
+    }
     uint32_t again = 0;  // rows with a value that is not finite
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
@@ -372,6 +396,64 @@ void window_prefill_kernel(WindowArgs a) {
   }
 }
 
+// The parts of every row, in order: D/4 lanes a row, four values of d each.
+template <int D>
+__global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
+  constexpr int NQ = D / 4, kBatch = 8;
+  const int t = threadIdx.x, lane = t & 63, vq = t % NQ, Hq = a.Hkv * a.G;
+  const int64_t rows = (int64_t)a.N * Hq, rh = (int64_t)blockIdx.x * (256 / NQ) + t / NQ;
+  const int64_t x = min(rh, rows - 1);
+  const int row = (int)(x / Hq), hq = (int)(x - (int64_t)row * Hq);
+  const bool on = rh < rows && row >= a.cu_q[0] && row < a.cu_q[a.B];
+  float m = -INFINITY, l = 0.f;
+  f32x4_t o = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  for (int c0 = 0; on && c0 < a.parts; c0 += kBatch) {
+    float2 ml[kBatch];
+    f32x4_t oc[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int64_t i = min(c0 + k, a.parts - 1) * rows + x;
+      ml[k] = *(const float2*)(a.part_ml + i * 2);
+      oc[k] = *(const f32x4_t*)(a.part_o + i * D + vq * 4);
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (c0 + k >= a.parts) continue;
+      // (a part without keys that weigh has a sum of 0, one of scores that are no numbers a sum of NaN)
+      const float mn = fmaxf(m, ml[k].x);
+      const float was = m == -INFINITY && l == 0.f ? 0.f : fast_exp2(m - mn);
+      const float w = ml[k].x == -INFINITY && ml[k].y == 0.f ? 0.f : fast_exp2(ml[k].x - mn);
+      l = l * was + ml[k].y * w;
+      o = o * was + oc[k] * w;
+      m = mn;
+    }
+  }
+  const float bad = l * 0.f + o[0] * 0.f + o[1] * 0.f + o[2] * 0.f + o[3] * 0.f;
+  uint64_t again = __builtin_amdgcn_ballot_w64(on && bad != bad);
+  const uint64_t mine = ((1ull << NQ) - 1) << (lane / NQ * NQ);
+  if (on && !(again & mine)) {
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *(uint64_t*)(a.out + (int64_t)row * a.o_sn + (int64_t)hq * a.o_sh + vq * 4) =
+        (uint64_t)pack_bf16x2(o[0] * inv, o[1] * inv) | (uint64_t)pack_bf16x2(o[2] * inv, o[3] * inv) << 32;
+  }
+  while (again) {  // a wave per row that is not finite
+    const int from = __builtin_ctzll(again) / NQ * NQ;
+    again &= ~(((1ull << NQ) - 1) << from);
+    const int r = __builtin_amdgcn_readlane(row, from), h = __builtin_amdgcn_readlane(hq, from);
+    int b = 0;
+    for (int hi = a.B - 1; b < hi;) {  // the last sequence that begins at or before the row
+      const int mid = (b + hi + 1) >> 1;
+      if (a.cu_q[mid] <= r) b = mid; else hi = mid - 1;
+    }
+    const Seq s = seq_of(a, uniform(b));
+    const int p = r - s.q0 + s.nk - s.nq;
+    const int64_t kv = h / a.G;
+    if (p < 0 || p >= s.nk) continue;  // (starts that do not ascend)
+    exact_row<D>(a, a.q + (int64_t)r * a.q_sn + (int64_t)h * a.q_sh, a.k + s.k0 * a.k_sn + kv * a.k_sh,
+                 a.v + s.k0 * a.v_sn + kv * a.v_sh, p, a.out + (int64_t)r * a.o_sn + (int64_t)h * a.o_sh, lane);
+  }
+}
+
 template <int D, int HPW, bool FAR>
 int resident() {
   static int per_cu = 0;
@@ -386,11 +468,65 @@ int resident() {
   return per_cu * cu_count();
 }
 
+// How a call is cut: query heads per workgroup and parts of an item.
+struct Cut {
+  int heads, parts;
+};
+
+int64_t items_of(int64_t N, int64_t B, int Hkv, int G, int heads) { return (N / kBlk + B) * Hkv * (G / heads); }
+
+// Heads: as many of 4, 2, 1 as divide G.
+// Parts: one for each time that the items fit into the card, of kLeastTiles
+// tiles at least.
+// Below kLongTiles tiles the join of more parts costs what they save, and where
+// workgroups of four heads leave half of the CUs without one, those of two
+// do better.  Measured (D 128, 8 KV heads of 4; us for 4 heads / 2 heads / 2
+// heads in twice as many parts):
+//   1000 rows of 1000 keys, window 1024, 2 parts / 1 / 2   43.3 / 34.4 / 41.3
+//   40 rows of 1040 keys, window 700, 2 / 2 / 2            20.5 / 18.2 / 18.3
+//   1, 5, 9 rows of 3 to 5 thousand, window 2000           20.4 / 22.0 / 22.4
+//   256 rows of 6256 keys, window 4096, 6 / 3 / 6          41.8 / 55.2 / 46.8
+//   512 rows of 32512 keys, all, 3 / 1 / 3                 307 / 826 / 368
+//   64 rows of 32064 keys, all, 16 / 8 / 16                73.7 / 116 / 68.7 (955 in one part of one head)
+constexpr int kLongTiles = 32;
+
+Cut cut_of(int N, int Nk, int B, int Hkv, int G, int window, int sinks) {
+  Cut c = {4, 1};
+  while (G % c.heads) c.heads >>= 1;
+  const int64_t keys = (Nk < (int64_t)window + kBlk ? Nk : (int64_t)window + kBlk) + (Nk < sinks ? Nk : sinks);
+  const int64_t tiles = keys / attn::kKeys, cus = cu_count();
+  const bool is_long = tiles >= kLongTiles;
+  if (!is_long && c.heads == 4 && items_of(N, B, Hkv, G, 2) <= cus) c.heads = 2;
+  // (a long item's workgroups of four waves or fewer come two a CU)
+  const int64_t by_room = (is_long && c.heads < 4 ? 2 * cus : cus) / items_of(N, B, Hkv, G, c.heads);
+  const int64_t by_tiles = tiles / kLeastTiles, parts = by_room < by_tiles ? by_room : by_tiles;
+  if (parts > 1) c.parts = (int)parts;
+  return c;
+}
+
+size_t aligned(size_t n) { return (n + 255) & ~(size_t)255; }
+
+struct PartsScratch {
+  size_t o, bytes;
+};
+PartsScratch parts_scratch(int parts, int64_t rows, int D) {
+  PartsScratch s = {0, 0};
+  if (parts == 1) return s;
+  s.o = aligned((size_t)parts * rows * 2 * sizeof(float));
+  s.bytes = s.o + (size_t)parts * rows * D * sizeof(float);
+  return s;
+}
+
 // Workgroups: those resident at once, at most one per item.
 template <int D, int HPW, bool FAR>
 hipError_t launch_items(const WindowArgs& a, hipStream_t st) {
-  const int64_t items = ((int64_t)a.N / kBlk + a.B) * a.Hkv * (a.G / HPW), most = resident<D, HPW, FAR>();
+  const int64_t items = items_of(a.N, a.B, a.Hkv, a.G, HPW) * a.parts, most = resident<D, HPW, FAR>();
   hipLaunchKernelGGL((window_prefill_kernel<D, HPW, FAR>), dim3((unsigned)(items < most ? items : most)), dim3(128 * HPW),
+                     0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.parts == 1) return e;
+  const int64_t per = 256 / (D / 4);
+  hipLaunchKernelGGL((window_join_kernel<D>), dim3((unsigned)(((int64_t)a.N * a.Hkv * a.G + per - 1) / per)), dim3(256),
                      0, st, a);
   return hipGetLastError();
 }
@@ -402,23 +538,24 @@ hipError_t launch(const WindowArgs& a, hipStream_t st) {
   return far ? launch_items<D, HPW, true>(a, st) : launch_items<D, HPW, false>(a, st);
 }
 
-// Query heads per workgroup: as many of 4, 2, 1 as divide G, halved while the
-// smaller workgroups would still get a CU each (a short call's time is its
-// longest item's, and a SIMD with one wave runs a tile sooner).
-int heads_per_wg(const WindowArgs& a) {
-  int h = 4;
-  while (a.G % h) h >>= 1;
-  while (h > 1 && ((int64_t)a.N / kBlk + a.B) * a.Hkv * (a.G / h) * 2 <= cu_count()) h >>= 1;
-  return h;
+template <int D>
+hipError_t launch_heads(const WindowArgs& a, int heads, hipStream_t st) {
+  return heads == 4 ? launch<D, 4>(a, st) : heads == 2 ? launch<D, 2>(a, st) : launch<D, 1>(a, st);
 }
 
-template <int D>
-hipError_t launch_heads(const WindowArgs& a, hipStream_t st) {
-  const int h = heads_per_wg(a);
-  return h == 4 ? launch<D, 4>(a, st) : h == 2 ? launch<D, 2>(a, st) : launch<D, 1>(a, st);
+bool bad_shape(int B, int N, int Nk, int Hq, int Hkv, int window, int sinks) {
+  return B <= 0 || N < 0 || Nk < 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || window < 1 || sinks < 0;
 }
 
 }  // namespace
+
+extern "C" size_t wgkv_sink_window_workspace_bytes(int32_t batch, int32_t num_rows, int32_t num_keys, int32_t num_q_heads,
+                                                   int32_t num_kv_heads, int32_t head_dim, int32_t window,
+                                                   int32_t num_sinks) {
+  if (bad_shape(batch, num_rows, num_keys, num_q_heads, num_kv_heads, window, num_sinks) || head_dim <= 0) return 0;
+  const Cut c = cut_of(num_rows, num_keys, batch, num_kv_heads, num_q_heads / num_kv_heads, window, num_sinks);
+  return parts_scratch(c.parts, (int64_t)num_rows * num_q_heads, head_dim).bytes;
+}
 
 extern "C" int wgkv_sink_window_attn(
     const void* q, int64_t q_stride_n, int64_t q_stride_h,
@@ -427,9 +564,9 @@ extern "C" int wgkv_sink_window_attn(
     void* out, int64_t out_stride_n, int64_t out_stride_h,
     const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, int32_t batch, int32_t num_rows, int32_t num_keys,
     int32_t num_q_heads, int32_t num_kv_heads, int32_t head_dim,
-    int32_t window, int32_t num_sinks, float softmax_scale, int32_t clear_rest, void* stream) {
-  if (batch <= 0 || num_rows < 0 || num_keys < 0 || num_kv_heads <= 0 || num_q_heads <= 0) return WGKV_ERR_ARG;
-  if (num_q_heads % num_kv_heads || window < 1 || num_sinks < 0) return WGKV_ERR_ARG;
+    int32_t window, int32_t num_sinks, float softmax_scale, int32_t clear_rest, void* workspace, size_t workspace_bytes,
+    void* stream) {
+  if (bad_shape(batch, num_rows, num_keys, num_q_heads, num_kv_heads, window, num_sinks)) return WGKV_ERR_ARG;
   if (num_rows == 0) return WGKV_OK;
   if (!q || !out || !cu_seqlens_q || !cu_seqlens_k || (num_keys && (!k || !v))) return WGKV_ERR_ARG;
   const int G = num_q_heads / num_kv_heads;
@@ -439,6 +576,9 @@ extern "C" int wgkv_sink_window_attn(
   if ((q_stride_n | q_stride_h | k_stride_n | k_stride_h | v_stride_n | v_stride_h | out_stride_n | out_stride_h) & 7)
     return WGKV_ERR_UNSUPPORTED;
   if (kv4_rows_meet({num_rows, num_q_heads, 1, 1}, {out_stride_n, out_stride_h, 0, 0}, head_dim)) return WGKV_ERR_ARG;
+  const Cut cut = cut_of(num_rows, num_keys, batch, num_kv_heads, G, window, num_sinks);
+  const PartsScratch sc = parts_scratch(cut.parts, (int64_t)num_rows * num_q_heads, head_dim);
+  if (sc.bytes && (!workspace || workspace_bytes < sc.bytes || ((uintptr_t)workspace & 15))) return WGKV_ERR_WORKSPACE;
   WindowArgs a{};
   a.q = (const uint16_t*)q;
   a.q_sn = q_stride_n;
@@ -467,13 +607,16 @@ extern "C" int wgkv_sink_window_attn(
   a.q_and = softmax_scale == 0.f ? 0u : ~0u;
   a.q_xor = softmax_scale < 0.f ? 0x80008000u : 0u;
   a.clear_rest = clear_rest;
-  const hipError_t e =
-      head_dim == 128 ? launch_heads<128>(a, (hipStream_t)stream) : launch_heads<64>(a, (hipStream_t)stream);
+  a.parts = cut.parts;
+  a.part_ml = (float*)workspace;
+  a.part_o = (float*)((char*)workspace + sc.o);
+  hipStream_t st = (hipStream_t)stream;
+  const hipError_t e = head_dim == 128 ? launch_heads<128>(a, cut.heads, st) : launch_heads<64>(a, cut.heads, st);
   return e == hipSuccess ? WGKV_OK : WGKV_ERR_HIP;
 }
 
 extern "C" int wgkv_sink_window_attn_block(const void* args) {
-  int64_t a[25];
+  int64_t a[27];
   memcpy(a, args, sizeof a);
   if (!kv4_narrow(a, 14, 15, 16, 17, 18, 19, 20, 21, 23)) return WGKV_ERR_UNSUPPORTED;
   double scale;
@@ -482,5 +625,5 @@ extern "C" int wgkv_sink_window_attn_block(const void* args) {
                                a[8], (void*)a[9], a[10], a[11], (const int32_t*)a[12], (const int32_t*)a[13],
                                (int32_t)a[14], (int32_t)a[15], (int32_t)a[16], (int32_t)a[17], (int32_t)a[18],
                                (int32_t)a[19], (int32_t)a[20], (int32_t)a[21], (float)scale, (int32_t)a[23],
-                               (void*)a[24]);
+                               (void*)a[24], (size_t)a[25], (void*)a[26]);
 }

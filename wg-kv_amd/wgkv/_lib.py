@@ -242,7 +242,8 @@ SIGNATURES = {
         c_ptr, c_i64, c_i64,
         c_ptr, c_ptr, c_i32, c_i32, c_i32,
         c_i32, c_i32, c_i32,
-        c_i32, c_i32, c_f32, c_i32, c_ptr]),
+        c_i32, c_i32, c_f32, c_i32, c_ptr, c_size, c_ptr]),
+    "wgkv_sink_window_workspace_bytes": (c_size, [c_i32] * 8),
     "wgkv_paged_decode_window_workspace_bytes": (c_size, [c_i32, c_i32, c_i32, c_i32]),
     "wgkv_paged_decode_attn_window": (ctypes.c_int, [
         c_ptr, c_i64, c_i64,

@@ -31,7 +31,7 @@ _I32, _U8, _BF16 = torch.int32, torch.uint8, torch.bfloat16
 # arguments of the C calls as blocks of 8-byte words (wgkv_*_block)
 _pack_tables = struct.Struct("25q").pack
 _pack_append = struct.Struct("14q").pack
-_pack_prompt = struct.Struct("22qd2q").pack
+_pack_prompt = struct.Struct("22qd4q").pack
 _pack_window = struct.Struct("22qd3q").pack
 _pack_shared = struct.Struct("28qd3q").pack
 _MOST = 2 ** 31 - 1
@@ -248,9 +248,13 @@ def sink_window_attn(q, k, v, cu_seqlens, window, num_sinks, softmax_scale=None,
     q, qp, qs = _rows3(q)
     k, kp, ks = _rows3(k)
     v, vp, vs = _rows3(v)
-    st = _lib.lib().wgkv_sink_window_attn_block(_pack_prompt(
+    window, num_sinks = min(window, _MOST), min(num_sinks, _MOST)
+    L = _lib.lib()
+    nbytes = L.wgkv_sink_window_workspace_bytes(B, N, Nk, Hq, H, D, window, num_sinks)
+    ws = torch.empty(nbytes, dtype=_U8, device=dev) if nbytes else None
+    st = L.wgkv_sink_window_attn_block(_pack_prompt(
         qp, qs[0], qs[1], kp, ks[0], ks[1], vp, vs[0], vs[1], op, os[0], os[1], cu.data_ptr(), cuk.data_ptr(), B, N, Nk,
-        Hq, H, D, min(window, _MOST), min(num_sinks, _MOST), softmax_scale, not given, _stream(dev)))
+        Hq, H, D, window, num_sinks, softmax_scale, not given, 0 if ws is None else ws.data_ptr(), nbytes, _stream(dev)))
     if st:
         _lib.check(st, "wgkv_sink_window_attn")
     return out
