@@ -261,6 +261,11 @@ def test_prompt_behind_cached_keys(past, window, sinks):
     check_prompt([64, 70, 130], past, 8, 2, 128, window, sinks, seed=1)
 
 
+@pytest.mark.parametrize("window,sinks", [(1 << 40, 0), ((1 << 31) - 1, (1 << 31) - 1), (3, 1 << 40)])
+def test_prompt_largest_windows_with_fewer_keys_than_rows(window, sinks):
+    check_prompt([64, 70, 130, 20], [-3, -70, 5, -10], 4, 2, 64, window, sinks, seed=1)
+
+
 @pytest.mark.parametrize("scale", [-0.3, 0.0, 1.0, 1e-4])
 def test_prompt_scales(scale):
     check_prompt([150, 20], None, 4, 2, 64, 33, 4, scale=scale)

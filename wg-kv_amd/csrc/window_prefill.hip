@@ -599,8 +599,9 @@ extern "C" int wgkv_sink_window_attn(
   a.Nk = num_keys;
   a.Hkv = num_kv_heads;
   a.G = G;
-  a.window = window;
-  a.sinks = num_sinks;
+  // (positions are within 2^30: a larger window shows the same, and its difference to a position stays 32-bit)
+  a.window = window < (1 << 30) ? window : 1 << 30;
+  a.sinks = num_sinks < (1 << 30) ? num_sinks : 1 << 30;
   // a negative scale negates the queries, and a scale of 0 clears them: masked
   // scores are -inf, and -inf * 0 is not a number
   a.scale_log2 = softmax_scale == 0.f ? 1.f : fabsf(softmax_scale) * attn::kLog2e;
