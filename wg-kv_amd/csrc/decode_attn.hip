@@ -301,7 +301,7 @@ void decode_split_kernel(DecodeArgs a) {
     __shared__ int s_tmp[kPlanThreads];
     pl = a.B * a.Hkv <= kWaveBH ? plan_wave<NW, WIN>(a, w) : plan_block(a, w, s_pref, s_tmp);
   } else {
-    pl = plan_wave<NW, WIN>(a, w);  // the host takes 8 waves only for B*Hkv < 32
+    pl = plan_wave<NW, WIN>(a, w);  // the host takes 8 waves only for B*Hkv < 32, or <= 64 (windows)
   }
   if (w >= pl.n_chunks) return;
   const int bh = pl.bh;
@@ -885,12 +885,14 @@ extern "C" int wgkv_paged_decode_attn_noalloc(
 namespace {
 
 // Windows of a batch with many heads, or more than four query heads each, are
-// cut into even ranges of all heads' tokens (stream_attn.hip): chunks of one
-// size leave heads of about that size a full and a small one (64 x 8 heads of
-// 4160 tokens 303 us in chunks, 194 in ranges; 32 x 8 heads 121 / 104; 16 x 8
-// 67 / 53; 8 x 8 40.5 / 36.2, of 32772 tokens 203 / 192; 5 x 8 of 704 tokens
-// 15.2 / 16.7).  Few heads take the 8-wave chunks, which need one launch.
-bool in_ranges(int heads, int G) { return heads >= kWideBelowBH || G > 4; }
+// cut into even ranges of all heads' tokens (stream_attn.hip).  Up to 64 heads
+// take chunks by 8-wave workgroups, each wave of which plans in its registers,
+// and need one launch (us in chunks / in ranges, G 4, D 128: 1 x 8 heads of 1028
+// tokens 11.8 / 12.1, of 32772 28.8 / 34.7; 4 x 8 of 4100 20.9 / 22.9; 8 x 8 of 1004
+// 13.9 / 14.4, of 4100 29.7 / 31.8, of 32772 172 / 174).  More heads of one length
+// would have a full and a small chunk each (64 x 8 of 4160: 303 us in 4-wave
+// chunks, 180 in ranges).
+bool in_ranges(int heads, int G) { return heads > kWaveBH || G > 4; }
 
 }  // namespace
 
