@@ -8,8 +8,9 @@
 // under softmax(q . k * scale).  Rows that see nothing (p < 0) give zeros.
 // Query head hq uses KV head hq / G.
 //
-// Work item = (64 rows of a sequence, KV head, group of HPW of its G query
-// heads) for a workgroup of 2 * HPW waves; a wave serves 32 rows of one head.
+// Work item = (64 rows of a sequence, KV head, group of 4 or 2 of its G query
+// heads, or 128 rows and one head) for a workgroup of 8 or 4 waves; a wave
+// serves 32 rows of one head.
 // The item's keys are the `first` tokens below the band and the band
 // [lo, last row's position] that the rows' windows reach, counted through as
 // one list and cut into tiles of 64, so that a few first tokens cost their
@@ -21,7 +22,7 @@
 // domain, fp32, with a running maximum that moves only when a score exceeds it
 // by more than 8; probabilities are rounded to bf16 for the products, and
 // their sums are taken of the rounded values.  Only the tiles at the two ends
-// of a row's window are masked; a wave passes over a tile none of its rows sees.
+// of a row's window are masked.
 //
 // Few rows (a last piece of a prompt, drafted tokens behind a long one) do not
 // fill the card: the tiles of every item are then cut into equal parts, a
@@ -37,7 +38,9 @@
 
 namespace {
 
-constexpr int kBlk = 64;      // query rows per item
+// Query rows per item of that many heads.
+constexpr int item_rows(int heads) { return heads == 1 ? 128 : 64; }
+constexpr int item_waves(int heads) { return heads * item_rows(heads) / 32; }
 constexpr int kMaxSeqs = 2048;
 constexpr int kLeastTiles = 4;  // of a part: less than about what the join costs
 
@@ -136,6 +139,7 @@ WGKV_DEVICE Keys keys_of(const WindowArgs& a, int p_blk, int p_last) {
 }
 
 // The block's sequence, rows and keys; s_blocks: row blocks of the sequences before each.
+template <int BLK>
 WGKV_DEVICE void find_block(const WindowArgs& a, const int* s_blocks, int blk, int* seq, int* r_blk, int* p_blk,
                             Keys* keys) {
   int b = 0;
@@ -145,9 +149,9 @@ WGKV_DEVICE void find_block(const WindowArgs& a, const int* s_blocks, int blk, i
   }
   const Seq s = seq_of(a, b);
   *seq = b;
-  *r_blk = (blk - s_blocks[b]) * kBlk;
+  *r_blk = (blk - s_blocks[b]) * BLK;
   *p_blk = *r_blk + s.nk - s.nq;
-  *keys = keys_of(a, *p_blk, *p_blk + min(kBlk, s.nq - *r_blk) - 1);
+  *keys = keys_of(a, *p_blk, *p_blk + min(BLK, s.nq - *r_blk) - 1);
 }
 
 // A buffer of `bytes` at p (a scalar address), and 16 bytes of it to LDS at lds
@@ -161,9 +165,9 @@ WGKV_DEVICE void buffer_to_lds(__amdgpu_buffer_rsrc_t r, uint16_t* lds, int off)
 
 // FAR: keys that may lie 2^31 bytes or more apart.
 template <int D, int HPW, bool FAR>
-__global__ __launch_bounds__(128 * HPW) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ __launch_bounds__(64 * item_waves(HPW)) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void window_prefill_kernel(WindowArgs a) {
-  constexpr int NT = 128 * HPW, NW = 2 * HPW;
+  constexpr int NW = item_waves(HPW), NT = 64 * NW, BLK = item_rows(HPW);
   constexpr int CH = D / 8;        // 16-byte slices per row
   constexpr int RPB = 64 / CH;     // key rows of 1 KB of LDS, one load instruction of a wave
   constexpr int NBLK = attn::kKeys / RPB;
@@ -183,11 +187,12 @@ void window_prefill_kernel(WindowArgs a) {
   const int t = threadIdx.x;
   const int lane = t & 63, wid = uniform(t >> 6);
   const int n = lane & 15, g = lane >> 4;
+  const int w_row = wid % (BLK / 32) * 32, w_head = wid / (BLK / 32);  // the wave's rows and head of the item
 
   {
     const int per = (a.B + NT - 1) / NT, b0 = min(a.B, t * per), b1 = min(a.B, b0 + per);
     int mine = 0;
-    for (int b = b0; b < b1; ++b) mine += (seq_of(a, b).nq + kBlk - 1) / kBlk;
+    for (int b = b0; b < b1; ++b) mine += (seq_of(a, b).nq + BLK - 1) / BLK;
     const int incl = wave_incl_scan(mine, lane);
     if (lane == 63) s_wave[wid] = incl;
     __syncthreads();
@@ -195,7 +200,7 @@ void window_prefill_kernel(WindowArgs a) {
     for (int i = 0; i < NW; ++i) run += i < wid ? s_wave[i] : 0;
     for (int b = b0; b < b1; ++b) {
       s_blocks[b] = run;
-      run += (seq_of(a, b).nq + kBlk - 1) / kBlk;
+      run += (seq_of(a, b).nq + BLK - 1) / BLK;
       if (b == a.B - 1) s_blocks[a.B] = run;
     }
     __syncthreads();
@@ -225,7 +230,7 @@ void window_prefill_kernel(WindowArgs a) {
     p->part = uniform(of % a.parts);
     int seq, r_blk, p_blk;
     Keys k;
-    find_block(a, s_blocks, blk, &seq, &r_blk, &p_blk, &k);
+    find_block<BLK>(a, s_blocks, blk, &seq, &r_blk, &p_blk, &k);
     const Seq s = seq_of(a, uniform(seq));
     p->q0 = uniform(s.q0);
     p->nq = uniform(s.nq);
@@ -280,10 +285,10 @@ void window_prefill_kernel(WindowArgs a) {
     }
   };
   const auto load_rows = [&](const Item& p, attn::Rows32<D>& r) __attribute__((always_inline)) {
-    const int r0 = p.r_blk + (wid & 1) * 32;
+    const int r0 = p.r_blk + w_row;
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt)
-      r.load_q(rt, a.q + (int64_t)(p.q0 + min(r0 + rt * 16 + n, p.nq - 1)) * a.q_sn + (int64_t)(p.hq0 + (wid >> 1)) * a.q_sh,
+      r.load_q(rt, a.q + (int64_t)(p.q0 + min(r0 + rt * 16 + n, p.nq - 1)) * a.q_sn + (int64_t)(p.hq0 + w_head) * a.q_sh,
                g, a.q_and, a.q_xor);
   };
 
@@ -293,7 +298,7 @@ void window_prefill_kernel(WindowArgs a) {
   for (int round = 1; more; ++round) {
     more = item_at(round, &nxt);
     const Keys& ks = cur.keys;
-    const int r0 = cur.r_blk + (wid & 1) * 32, p0 = cur.p_blk + (wid & 1) * 32;  // the wave's rows
+    const int r0 = cur.r_blk + w_row, p0 = cur.p_blk + w_row;  // the wave's rows
     attn::Rows32<D> r;
     load_rows(cur, r);
     r.clear();
@@ -346,7 +351,7 @@ void window_prefill_kernel(WindowArgs a) {
       tile_load(nxt, 0, more && nxt.tiles > 0, sK0, sV0);
     }
     const Item done = cur;
-    const int hq = done.hq0 + (wid >> 1);
+    const int hq = done.hq0 + w_head;
     if (a.parts > 1) {
 #pragma unroll
       for (int rt = 0; rt < 2; ++rt) {
@@ -459,7 +464,8 @@ int resident() {
   static int per_cu = 0;
   if (per_cu == 0) {
     int nb = 0;
-    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&nb, window_prefill_kernel<D, HPW, FAR>, 128 * HPW, 0) !=
+    if (hipOccupancyMaxActiveBlocksPerMultiprocessor(&nb, window_prefill_kernel<D, HPW, FAR>,
+                                                     64 * item_waves(HPW), 0) !=
             hipSuccess ||
         nb <= 0)
       nb = 1;
@@ -473,7 +479,9 @@ struct Cut {
   int heads, parts;
 };
 
-int64_t items_of(int64_t N, int64_t B, int Hkv, int G, int heads) { return (N / kBlk + B) * Hkv * (G / heads); }
+int64_t items_of(int64_t N, int64_t B, int Hkv, int G, int heads) {
+  return (N / item_rows(heads) + B) * Hkv * (G / heads);
+}
 
 // Heads: as many of 4, 2, 1 as divide G.
 // Parts: one for each time that the items fit into the card, of kLeastTiles
@@ -493,7 +501,8 @@ constexpr int kLongTiles = 32;
 Cut cut_of(int N, int Nk, int B, int Hkv, int G, int window, int sinks) {
   Cut c = {4, 1};
   while (G % c.heads) c.heads >>= 1;
-  const int64_t keys = (Nk < (int64_t)window + kBlk ? Nk : (int64_t)window + kBlk) + (Nk < sinks ? Nk : sinks);
+  const int64_t reach = (int64_t)window + item_rows(c.heads);
+  const int64_t keys = (Nk < reach ? Nk : reach) + (Nk < sinks ? Nk : sinks);
   const int64_t tiles = keys / attn::kKeys, cus = cu_count();
   const bool is_long = tiles >= kLongTiles;
   if (!is_long && c.heads == 4 && items_of(N, B, Hkv, G, 2) <= cus) c.heads = 2;
@@ -521,8 +530,8 @@ PartsScratch parts_scratch(int parts, int64_t rows, int D) {
 template <int D, int HPW, bool FAR>
 hipError_t launch_items(const WindowArgs& a, hipStream_t st) {
   const int64_t items = items_of(a.N, a.B, a.Hkv, a.G, HPW) * a.parts, most = resident<D, HPW, FAR>();
-  hipLaunchKernelGGL((window_prefill_kernel<D, HPW, FAR>), dim3((unsigned)(items < most ? items : most)), dim3(128 * HPW),
-                     0, st, a);
+  hipLaunchKernelGGL((window_prefill_kernel<D, HPW, FAR>), dim3((unsigned)(items < most ? items : most)),
+                     dim3(64 * item_waves(HPW)), 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == 1) return e;
   const int64_t per = 256 / (D / 4);
