@@ -38,7 +38,9 @@
 
 namespace {
 
-// Query rows per item of that many heads.
+// Query rows per item of that many heads.  (Two waves of one head would load
+// each tile for 64 rows alone: 32768 rows, window 1024, three heads a KV head 975
+// us, in items of 128 rows 616.)
 constexpr int item_rows(int heads) { return heads == 1 ? 128 : 64; }
 constexpr int item_waves(int heads) { return heads * item_rows(heads) / 32; }
 constexpr int kMaxSeqs = 2048;
@@ -277,7 +279,8 @@ void window_prefill_kernel(WindowArgs a) {
     } else if (on) {
 #pragma unroll
       for (int i = 0; i < KPT; ++i) {
-        const int row = (wid + i * NL) * RPB + lane / CH;
+        int row = (wid + i * NL) * RPB + lane / CH;
+        asm volatile("" : "+v"(row));
         const int64_t j = ks.key(min(x0 + row, ks.count - 1));
         attn::lds_dma16(p.kb + j * a.k_sn + ((lane % CH) ^ attn::swz_k<D>(row)) * 8, dK + (wid + i * NL) * 512);
         attn::lds_dma16(p.vb + j * a.v_sn + ((lane % CH) ^ attn::swz_v<D>(row)) * 8, dV + (wid + i * NL) * 512);
