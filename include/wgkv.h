@@ -720,8 +720,8 @@ int wgkv_kv4_decode_attn_block(const void* args);
  * written but slots (-1), unchanged lengths and state, and *status (or NULL) =
  * WGKV_ERR_CAPACITY; a held page id outside the pool sets it too, and its
  * tokens' slots are -1.  num_pages * page_size and N*H < 2^31, (B+1)*H <=
- * 2^24.  One launch for N <= 256 and (B+1)*H <= 4096; two otherwise, three
- * with a mask, and then a workspace (as sized, any contents).
+ * 2^24.  One launch for N <= 256 and (B+1)*H <= 4096; otherwise up to three,
+ * and a workspace (as sized, any contents; calls that share one ordered).
  *
  * wgkv_paged_append copies rows of key/value bf16 (N, H, D) (element strides,
  * d contiguous; 16-byte aligned, strides multiples of 8) to rows slots[n,h]
@@ -750,7 +750,8 @@ int wgkv_kv4_decode_attn_block(const void* args);
  * group_starts[n] .. group_starts[n+1]-1 (i32 (num_groups+1), ascending) also
  * attend, under the same softmax, to the first prefix_lens[n,h] tokens of
  * prefix n, whose pages are prefix_table (num_groups, Hkv, prefix_pages).
- * Sequences of no group have none.  B*Hkv and num_groups*Hkv <= 2048.  Two
+ * Sequences of no group have none; starts that do not ascend count as the
+ * greatest so far.  B*Hkv and num_groups*Hkv <= 2048.  Two
  * launches; workspace as sized, any contents, calls that share one ordered.
  * ---------------------------------------------------------------------- */
 size_t wgkv_block_tables_workspace_bytes(int32_t batch, int32_t num_kv_heads, int32_t num_tokens);

@@ -249,7 +249,9 @@ WGKV_DEVICE void tile_rows(const TablesArgs& a, int tile, const StepPlan& s, con
   }
 }
 
-// Steps whose plan fits into LDS.  ONE: of up to kTile tokens, one workgroup,
+// Steps whose plan fits into LDS.  (256 requests x 8 heads x 1 token 6.9 us; 8
+// requests of 2 to 4 thousand gated tokens 8.7 behind 4.3 of counting; 64K tokens
+// of one request 6.9.)  ONE: of up to kTile tokens, one workgroup,
 // which counts the mask itself; otherwise a workgroup per tile, of which the
 // first writes the lengths and the state.
 template <bool ONE>
@@ -422,7 +424,8 @@ struct AppendArgs {
 
 // Rows to their places, 16 bytes per thread and step, keys and values
 // together: pure bandwidth.  Four pieces of each are asked for before the
-// first is written.
+// first is written.  64K tokens x 8 heads, D 128: 537 MB in 109 us, 4.9 TB/s (a
+// plain copy 5.0).
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   constexpr int U = 4;
   const int64_t total = a.rows * a.chunks;

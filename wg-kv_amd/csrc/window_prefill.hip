@@ -15,7 +15,7 @@
 // [lo, last row's position] that the rows' windows reach, counted through as
 // one list and cut into tiles of 64, so that a few first tokens cost their
 // share of a tile and not one of their own.  Tiles go from memory straight
-// into LDS, one tile ahead of the arithmetic (global_load_lds_dwordx4), and
+// into LDS, one tile ahead of the arithmetic (buffer loads), and
 // serve all heads of the group.  S^T = K Q^T on v_mfma_f32_16x16x32_bf16
 // leaves each lane 16 scores of a query row, which are the B operand of
 // O^T += V^T P^T; V^T comes by LDS transpose reads.  Softmax is in the log2
@@ -27,6 +27,13 @@
 // Few rows (a last piece of a prompt, drafted tokens behind a long one) do not
 // fill the card: the tiles of every item are then cut into equal parts, a
 // workgroup each, whose (max, sum, O) a second launch joins.
+//
+// Measured (32/8 heads, D 128): 32768 rows, window 1024 and 4 first tokens 665
+// us, 820 TFLOP/s of the pairs that are seen, 920 of the tiles, where a large
+// bf16 product reaches 1395; rows behind cached keys with a window of 4096 1010.
+// Matrix instructions take 39 % of the cycles and vector ones (exponentials,
+// masks, packing) 56 %, which share a SIMD's issue.  Short prompts (7 of 300 to
+// 600 rows, D 64: 17 us) are a chain of tiles' round trips to memory.
 //
 // A masked probability is 0, and 0 times a key's value that is not finite is
 // NaN: rows whose result is not finite are worked out once more, key by key
