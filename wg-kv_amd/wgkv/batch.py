@@ -143,7 +143,7 @@ def build_block_tables(lengths, cu_seqlens, num_tokens, block_table, page_state,
     if out is None:
         out = torch.empty_like(lens, memory_format=torch.contiguous_format)
     if slots is None:
-        slots = torch.empty((num_tokens, H), dtype=_I32, device=dev)
+        slots = lens.new_empty((num_tokens, H))
     if state_out is None:
         state_out = torch.empty_like(page_state)
     L = _lib.lib()
@@ -235,7 +235,7 @@ def sink_window_attn(q, k, v, cu_seqlens, window, num_sinks, softmax_scale=None,
         softmax_scale = D ** -0.5
     given = out is not None
     if not given:
-        out = torch.empty(shape, dtype=_BF16, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != shape or out.dtype is not _BF16:
         raise AssertionError("out must be (rows, num_query_heads, head_dim) bf16")
     if not N:
@@ -250,11 +250,13 @@ def sink_window_attn(q, k, v, cu_seqlens, window, num_sinks, softmax_scale=None,
     v, vp, vs = _rows3(v)
     window, num_sinks = min(window, _MOST), min(num_sinks, _MOST)
     L = _lib.lib()
-    nbytes = L.wgkv_sink_window_workspace_bytes(B, N, Nk, Hq, H, D, window, num_sinks)
-    ws = torch.empty(nbytes, dtype=_U8, device=dev) if nbytes else None
-    st = L.wgkv_sink_window_attn_block(_pack_prompt(
+    args = (
         qp, qs[0], qs[1], kp, ks[0], ks[1], vp, vs[0], vs[1], op, os[0], os[1], cu.data_ptr(), cuk.data_ptr(), B, N, Nk,
-        Hq, H, D, window, num_sinks, softmax_scale, not given, 0 if ws is None else ws.data_ptr(), nbytes, _stream(dev)))
+        Hq, H, D, window, num_sinks, softmax_scale, not given)
+    st = L.wgkv_sink_window_attn_block(_pack_prompt(*args, 0, 0, _stream(dev)))
+    if st == _lib.ERR_WORKSPACE:  # few rows behind many keys; others are spared the question (1 us)
+        ws = torch.empty(L.wgkv_sink_window_workspace_bytes(B, N, Nk, Hq, H, D, window, num_sinks), dtype=_U8, device=dev)
+        st = L.wgkv_sink_window_attn_block(_pack_prompt(*args, ws.data_ptr(), ws.numel(), _stream(dev)))
     if st:
         _lib.check(st, "wgkv_sink_window_attn")
     return out
@@ -277,7 +279,7 @@ def _check_token(q, cache_seqlens, block_table, pool):
 def _token_out(q, out):
     """The output of a call with one row per sequence, its address and strides."""
     if out is None:
-        out = torch.empty(q.shape, dtype=_BF16, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype is not _BF16:
         raise AssertionError("out must be (batch, 1, num_query_heads, head_dim) bf16")
     st = out.stride()
