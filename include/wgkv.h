@@ -736,8 +736,8 @@ int wgkv_kv4_decode_attn_block(const void* args);
  * iff j <= p and (j > p - window or j < num_sinks).  Rows that see nothing
  * give zeros; what a row does not see has no part in it, NaN included.  Rows
  * of no sequence are left as they are, or cleared (clear_rest != 0).  window
- * >= 1; D in {64,128}; G = Hq/Hkv in 1..8; up to 2048 sequences and 2^30
- * rows.  Few rows with long windows take a workspace (as sized, 0 bytes for
+ * >= 1; D in {64,128}; G = Hq/Hkv in 1..8; up to 2048 sequences, 2^30
+ * rows and 2^36 of both together (sequences times rows).  Few rows with long windows take a workspace (as sized, 0 bytes for
  * others; any contents; calls that share one ordered) and two launches.
  *
  * wgkv_paged_decode_attn_window: wgkv_paged_decode_attn where a head of T

@@ -155,6 +155,7 @@ def test_c_entry_points_check_arguments_without_gpu():
         (0, None, ARG), (3, None, ARG), (9, None, ARG), (12, None, ARG), (13, None, ARG), (14, 0, ARG), (14, 2049, UNS),
         (15, -1, ARG), (16, -1, ARG), (17, 3, ARG), (17, 18, UNS), (19, 96, UNS), (20, 0, ARG), (21, -1, ARG),
         (0, p + 2, UNS), (1, 260, UNS), (10, 64, ARG), (10, 0, ARG), (11, 0, ARG), (15, (1 << 30) + 1, UNS)])
+    refused(L.wgkv_sink_window_attn, prompt[:14] + [2048] + prompt[15:], [(15, 1 << 26, UNS)])  # rows of all sequences
     few = prompt[:16] + [4000] + prompt[17:20] + [4000] + prompt[21:]  # few rows, many keys: cut into parts
     need = L.wgkv_sink_window_workspace_bytes(2, 3, 4000, 4, 2, 64, 4000, 1)
     assert need > 0 == L.wgkv_sink_window_workspace_bytes(2, 3, 4000, 4, 2, 64, 200, 1)

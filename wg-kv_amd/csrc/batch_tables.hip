@@ -428,21 +428,21 @@ struct AppendArgs {
 // plain copy 5.0).
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   constexpr int U = 4;
-  const int64_t total = a.rows * a.chunks;
-  const int64_t e0 = (int64_t)blockIdx.x * (256 * U) + threadIdx.x;
+  // the workgroup's first piece; what is behind it stays in 32 bits
+  const int64_t e0 = (int64_t)blockIdx.x * (256 * U);
+  const uint32_t r0 = (uint32_t)(e0 / a.chunks), c0 = (uint32_t)(e0 - (int64_t)r0 * a.chunks);
   u32x4_t x[2][U];
   int64_t at[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t e = e0 + u * 256;
+    const uint32_t e = c0 + threadIdx.x + u * 256, up = e / (uint32_t)a.chunks, r = r0 + up;
+    const int c = (int)(e - up * a.chunks);
     at[u] = -1;
-    if (e >= total) continue;
-    const int64_t r = e / a.chunks;
-    const int c = (int)(e - r * a.chunks);
+    if (r >= a.rows) continue;
     const int64_t row = a.slots[r];
     if (row < 0 || row >= a.cache_rows) continue;
-    const int64_t n = r / a.H;
-    const int h = (int)(r - n * a.H);
+    const int64_t n = r / (uint32_t)a.H;
+    const int h = (int)(r - (uint32_t)n * a.H);
     at[u] = row * a.chunks + c;
 #pragma unroll
     for (int i = 0; i < 2; ++i)

@@ -782,9 +782,10 @@ void stream_split_kernel(StreamArgs a) {
       q.first = row_tile * kMany;
       q.count = (uniform(s_start[n + 1]) - q.b0) * a.G;
       const Pages p = {a.pbt + n * a.pbt_sb + q.h * a.pbt_sh, seen_of<KIND>(a, uniform(s_tokens[e]))};
-      tile_piece<D>(a, p, uniform((int)((int64_t)tiles * c / chunks)), uniform((int)((int64_t)tiles * (c + 1) / chunks)), q,
-                    min(kMany, q.count - q.first), a.pre_ml + (int64_t)unit * (kMany * 2),
-                    a.pre_o + (int64_t)unit * (kMany * D), s_k0, s_v0, s_k1, s_v1);
+      const int each = uniform(tiles / chunks), over = tiles - each * chunks, from = c * each + min(c, over);
+      tile_piece<D>(a, p, from, from + each + (c < over), q, min(kMany, q.count - q.first),
+                    a.pre_ml + (int64_t)unit * (kMany * 2), a.pre_o + (int64_t)unit * (kMany * D), s_k0, s_v0, s_k1,
+                    s_v1);
     }
     if (!own_first) stream();
   }

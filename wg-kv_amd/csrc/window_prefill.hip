@@ -147,20 +147,14 @@ WGKV_DEVICE Keys keys_of(const WindowArgs& a, int p_blk, int p_last) {
   return {first, lo - first, first + p_last - lo + 1};
 }
 
-// The block's sequence, rows and keys; s_blocks: row blocks of the sequences before each.
-template <int BLK>
-WGKV_DEVICE void find_block(const WindowArgs& a, const int* s_blocks, int blk, int* seq, int* r_blk, int* p_blk,
-                            Keys* keys) {
+// The block's sequence; s_blocks: row blocks of the sequences before each.
+WGKV_DEVICE int sequence_of(const WindowArgs& a, const int* s_blocks, int blk) {
   int b = 0;
   for (int hi = a.B - 1; b < hi;) {  // the last sequence that begins at or before the block
     const int mid = (b + hi + 1) >> 1;
-    if (s_blocks[mid] <= blk) b = mid; else hi = mid - 1;
+    if (uniform(s_blocks[mid]) <= blk) b = mid; else hi = mid - 1;
   }
-  const Seq s = seq_of(a, b);
-  *seq = b;
-  *r_blk = (blk - s_blocks[b]) * BLK;
-  *p_blk = *r_blk + s.nk - s.nq;
-  *keys = keys_of(a, *p_blk, *p_blk + min(BLK, s.nq - *r_blk) - 1);
+  return b;
 }
 
 // A buffer of `bytes` at p (a scalar address), and 16 bytes of it to LDS at lds
@@ -209,7 +203,7 @@ void window_prefill_kernel(WindowArgs a) {
     for (int i = 0; i < NW; ++i) run += i < wid ? s_wave[i] : 0;
     for (int b = b0; b < b1; ++b) {
       s_blocks[b] = run;
-      run += (seq_of(a, b).nq + BLK - 1) / BLK;
+      run += per == 1 ? mine : (seq_of(a, b).nq + BLK - 1) / BLK;
       if (b == a.B - 1) s_blocks[a.B] = run;
     }
     __syncthreads();
@@ -232,26 +226,29 @@ void window_prefill_kernel(WindowArgs a) {
   // dealt to the XCDs in turn, so with 8 KV heads each XCD's L2 serves one
   // head's keys.  A workgroup takes items from alternate ends of its rounds.
   const auto item_at = [&](int round, Item* p) {
-    const int64_t item = (int64_t)round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-    if (item >= (int64_t)blocks * a.parts * per_block) return false;
-    const int of = uniform((int)(item / per_block)), rest = uniform((int)(item - (int64_t)of * per_block));
-    const int blk = blocks - 1 - uniform(of / a.parts);
-    p->part = uniform(of % a.parts);
-    int seq, r_blk, p_blk;
-    Keys k;
-    find_block<BLK>(a, s_blocks, blk, &seq, &r_blk, &p_blk, &k);
-    const Seq s = seq_of(a, uniform(seq));
+    // (32-bit throughout: a 64-bit division is 150 instructions of a short call's start)
+    const uint32_t item = round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    if (item >= (uint32_t)(blocks * a.parts) * per_block) return false;
+    const uint32_t of = uniform(item / (uint32_t)per_block), rest = item - of * per_block;
+    const uint32_t back = uniform(of / (uint32_t)a.parts);
+    const int blk = blocks - 1 - back;
+    p->part = of - back * a.parts;
+    const int seq = uniform(sequence_of(a, s_blocks, blk));
+    const Seq s = seq_of(a, seq);
     p->q0 = uniform(s.q0);
     p->nq = uniform(s.nq);
     p->nk = uniform(s.nk);
-    p->r_blk = uniform(r_blk);
-    p->p_blk = uniform(p_blk);
+    p->r_blk = (blk - uniform(s_blocks[seq])) * BLK;
+    p->p_blk = p->r_blk + p->nk - p->nq;
+    const Keys k = keys_of(a, p->p_blk, p->p_blk + min(BLK, p->nq - p->r_blk) - 1);
     p->keys = {uniform(k.first), uniform(k.shift), uniform(k.count)};
     const int tiles = (p->keys.count + attn::kKeys - 1) / attn::kKeys;
-    p->t0 = uniform((int)((int64_t)tiles * p->part / a.parts));
-    p->tiles = uniform((int)((int64_t)tiles * (p->part + 1) / a.parts)) - p->t0;
-    p->h = uniform(rest % a.Hkv);
-    p->hq0 = p->h * a.G + uniform(rest / a.Hkv) * HPW;
+    const uint32_t each = uniform((uint32_t)tiles / (uint32_t)a.parts), over = tiles - each * a.parts;
+    p->t0 = p->part * each + min((uint32_t)p->part, over);
+    p->tiles = each + (p->part < (int)over);
+    const uint32_t group = uniform(rest / (uint32_t)a.Hkv);
+    p->h = rest - group * a.Hkv;
+    p->hq0 = p->h * a.G + group * HPW;
     const int k0 = uniform(s.k0);
     p->kb = a.k + (int64_t)k0 * a.k_sn + (int64_t)p->h * a.k_sh;
     p->vb = a.v + (int64_t)k0 * a.v_sn + (int64_t)p->h * a.v_sh;
@@ -597,6 +594,9 @@ extern "C" int wgkv_sink_window_attn(
   if (kv4_rows_meet({num_rows, num_q_heads, 1, 1}, {out_stride_n, out_stride_h, 0, 0}, head_dim)) return WGKV_ERR_ARG;
   const Cut cut = cut_of(num_rows, num_keys, batch, num_kv_heads, G, window, num_sinks);
   const PartsScratch sc = parts_scratch(cut.parts, (int64_t)num_rows * num_q_heads, head_dim);
+  // row blocks and items are counted in 32 bits, also where starts do not ascend (workgroups step over the end)
+  if ((int64_t)batch * (num_rows / 64 + 1) > (1 << 30)) return WGKV_ERR_UNSUPPORTED;
+  if (items_of(num_rows, batch, num_kv_heads, G, cut.heads) * cut.parts > 0x7f000000) return WGKV_ERR_UNSUPPORTED;
   if (sc.bytes && (!workspace || workspace_bytes < sc.bytes || ((uintptr_t)workspace & 15))) return WGKV_ERR_WORKSPACE;
   WindowArgs a{};
   a.q = (const uint16_t*)q;
