@@ -32,7 +32,7 @@
 //
 // Split: the tiles of all (prefix, head, row tile) and (sequence, head) are
 // laid end to end and the waves take equal ranges of that line, whatever the
-// lengths; a wave goes through the pieces of its range without draining its
+// lengths (short lines of half the waves); a wave goes through the pieces of its range without draining its
 // loads.  Prefixes of many rows are not on the line: they are cut into chunks
 // of equal size, one per workgroup where that can be, and the workgroups' waves
 // have their ranges of the line besides.  One half of the workgroups begins
@@ -63,7 +63,8 @@ constexpr int kMaxG = 8;
 constexpr int kWavesPerCu = 8;      // what the registers hold: two per SIMD
 constexpr int kMaxWaves = 4096;     // of the split launch
 constexpr int kFew = 16, kMany = 256;  // rows of a piece
-constexpr int kLeastStreamed = 2, kLeastTiled = 2;  // tiles of a range
+constexpr int kLeastStreamed = 2, kShortRange = 6;  // tiles of 32 tokens of a wave's range
+constexpr int kLeastTiled = 2;  // tiles of 64 tokens of a chunk
 
 struct StreamArgs {
   const uint16_t* q;
@@ -155,8 +156,18 @@ WGKV_DEVICE int entry_tiles(const StreamArgs& a, bool pre, int tokens) {
 template <Mode KIND>
 WGKV_DEVICE int row_tiles(const StreamArgs& a, int size) { return (size * a.G + rows_of<KIND>() - 1) / rows_of<KIND>(); }
 
-// Tiles of a range of a line: an equal share, but `least` at least.
-WGKV_DEVICE int range_tiles(int total, int ranges, int least) { return max((total + ranges - 1) / ranges, least); }
+// Tiles of a range of the line: an equal share of all waves, or of half of them
+// (one per SIMD) while that is short: then the pieces to join count as much as
+// the reads.  (4 sequences behind one prefix, 8 heads, us with shares of all / of
+// half: 8192 tokens 24.8 / 20.9, 16384 30.2 / 24.9, 24000 34.4 / 29.6, 32768 40.7 /
+// 46.7.)  But kLeastStreamed at least (2048 tokens: 1 15.7, 2 14.5, 3 15.7; 300
+// tokens: 11.4, 12.5, 14.6).  Beside prefixes of many rows all workgroups are
+// there anyway (32 sequences of 500 tokens behind 3000: 31.3 / 35.4).
+template <Mode KIND>
+WGKV_DEVICE int range_tiles(int total, int waves) {
+  const int of_half = (total + waves / 2 - 1) / (waves / 2);
+  return max(KIND != kManyRows && of_half <= kShortRange ? of_half : (total + waves - 1) / waves, kLeastStreamed);
+}
 
 // Prefixes of few rows: number of a (prefix, head, row tile) that only grows
 // along the line: groups before n have at most starts[n] * G / 16 + n row tiles.
@@ -738,7 +749,7 @@ void stream_split_kernel(StreamArgs a) {
     __syncthreads();
   }
   const int zero = uniform(own_zero<KIND>(s_base, NH)), line = total - zero;
-  const int per = uniform(range_tiles(line, a.slots * NW, kLeastStreamed));
+  const int per = uniform(range_tiles<KIND>(line, a.slots * NW));
   if (wg == 0) {
     for (int i = t; i <= E; i += NT) a.plan[i] = s_base[i];
     if (t == 0) {
