@@ -88,13 +88,18 @@ struct Rows32 {
       for (int dt = 0; dt < D / 16; ++dt) o[dt][rt] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
     }
   }
-  // lane's row of row tile rt at p; the bits' masks apply the scale's sign
-  WGKV_DEVICE void load_q(int rt, const uint16_t* p, int g, uint32_t q_and, uint32_t q_xor) {
+  // asks for the lane's row of row tile rt at p
+  WGKV_DEVICE void ask_q(int rt, const uint16_t* p, int g) {
 #pragma unroll
-    for (int j = 0; j < D / 32; ++j) {
-      const u32x4_t w = *(const u32x4_t*)(p + (j * 4 + g) * 8);
-      q[rt][j] = __builtin_bit_cast(bf16x8_t, (w & q_and) ^ q_xor);
-    }
+    for (int j = 0; j < D / 32; ++j) q[rt][j] = __builtin_bit_cast(bf16x8_t, *(const u32x4_t*)(p + (j * 4 + g) * 8));
+  }
+  // the rows have come: the bits' masks apply the scale's sign
+  WGKV_DEVICE void take_q(uint32_t q_and, uint32_t q_xor) {
+#pragma unroll
+    for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+        q[rt][j] = __builtin_bit_cast(bf16x8_t, (__builtin_bit_cast(u32x4_t, q[rt][j]) & q_and) ^ q_xor);
   }
 };
 

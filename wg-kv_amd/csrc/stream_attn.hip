@@ -32,14 +32,15 @@
 //
 // Split: the tiles of all (prefix, head, row tile) and (sequence, head) are
 // laid end to end and the waves take equal ranges of that line, whatever the
-// lengths (short lines of half the waves); a wave goes through the pieces of its range without draining its
-// loads.  Prefixes of many rows are not on the line: they are cut into chunks
-// of equal size, one per workgroup where that can be, and the workgroups' waves
-// have their ranges of the line besides.  One half of the workgroups begins
-// with the prefix and the other with the sequences' own tokens, so that some
-// compute while others read.  Pieces are numbered (range + position of their
-// entry, or the chunk), store (max, sum, O) there, and a second launch joins
-// the pieces of every query row in a fixed order.
+// lengths (half of the waves those of a short line); a wave goes through the
+// pieces of its range without draining its loads.  Prefixes of many rows are
+// not on the line: they are cut into chunks of equal size, one per workgroup
+// where that can be, and the workgroups' waves have their ranges of the line
+// besides.  One half of the workgroups begins with the prefix and the other
+// with the sequences' own tokens, so that some compute while others read.
+// Pieces are numbered (range + position of their entry, or the chunk), store
+// (max, sum, O) there, and a second launch joins the pieces of every query row
+// in a fixed order.
 //
 // Measured (us, split + join): 64 windows of 4160 of 8 heads, D 128, 1.09 GB:
 // 174 + 6, 6.2 TB/s, more than a copy of the same size reaches (reads only); 128
@@ -565,7 +566,7 @@ WGKV_DEVICE void tile_piece(const StreamArgs& a, const Pages& p, int t0, int t1,
   attn::Rows32<D> r;
   r.clear();
 #pragma unroll
-  for (int rt = 0; rt < 2; ++rt) r.load_q(rt, q.row(a, w * 32 + rt * 16 + n), g, a.q_and, a.q_xor);
+  for (int rt = 0; rt < 2; ++rt) r.ask_q(rt, q.row(a, w * 32 + rt * 16 + n), g);
   const int sub = w & 3;
   const bool keys = w < 4;
   const uint16_t* pool = keys ? a.kc : a.vc;
@@ -590,6 +591,7 @@ WGKV_DEVICE void tile_piece(const StreamArgs& a, const Pages& p, int t0, int t1,
   int ids = ids_from(t0), ids_next = ids_from(t0 + 16);
   const auto id_of = [&](int tile) { return __builtin_amdgcn_readlane(ids, (tile - t0) % 16 * 4 + sub); };
   load(t0, id_of(t0), sK0, sV0);
+  r.take_q(a.q_and, a.q_xor);
   const auto step = [&](int tile, const uint16_t* sK, const uint16_t* sV, uint16_t* nK, uint16_t* nV)
       __attribute__((always_inline)) {
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the tile has landed

@@ -291,23 +291,25 @@ void window_prefill_kernel(WindowArgs a) {
       }
     }
   };
-  const auto load_rows = [&](const Item& p, attn::Rows32<D>& r) __attribute__((always_inline)) {
+  const auto ask_rows = [&](const Item& p, attn::Rows32<D>& r) __attribute__((always_inline)) {
     const int r0 = p.r_blk + w_row;
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt)
-      r.load_q(rt, a.q + (int64_t)(p.q0 + min(r0 + rt * 16 + n, p.nq - 1)) * a.q_sn + (int64_t)(p.hq0 + w_head) * a.q_sh,
-               g, a.q_and, a.q_xor);
+      r.ask_q(rt, a.q + (int64_t)(p.q0 + min(r0 + rt * 16 + n, p.nq - 1)) * a.q_sn + (int64_t)(p.hq0 + w_head) * a.q_sh, g);
   };
 
   Item cur = {}, nxt = {};
   bool more = item_at(0, &cur);
-  if (more) tile_load(cur, 0, cur.tiles > 0, sK0, sV0);
+  attn::Rows32<D> r;
+  if (more) {
+    tile_load(cur, 0, cur.tiles > 0, sK0, sV0);
+    ask_rows(cur, r);
+  }
   for (int round = 1; more; ++round) {
     more = item_at(round, &nxt);
     const Keys& ks = cur.keys;
     const int r0 = cur.r_blk + w_row, p0 = cur.p_blk + w_row;  // the wave's rows
-    attn::Rows32<D> r;
-    load_rows(cur, r);
+    r.take_q(a.q_and, a.q_xor);
     r.clear();
     const auto step = [&](int tile, const uint16_t* sK, const uint16_t* sV, uint16_t* nK, uint16_t* nV,
                           bool second) __attribute__((always_inline)) {
@@ -323,6 +325,7 @@ void window_prefill_kernel(WindowArgs a) {
       const int e0 = p0 - ks.shift, e1 = e0 + 31;  // the last entries of the wave's first and last row
       f32x4_t sc[4][2];
       attn::tile_scores<D>(r, sK, at, sc);
+      if (last && more) ask_rows(nxt, r);  // the item's own queries have had their last use
       const bool full = x1 - x0 == attn::kKeys - 1 && x1 <= e0 && (e1 - x0 < a.window || x1 < a.sinks);
       if (!full) {
 #pragma unroll
@@ -356,6 +359,7 @@ void window_prefill_kernel(WindowArgs a) {
     if (cur.tiles == 0 || cur.tiles % 2 != 0) {  // the first buffers were the last in use, or none were
       __syncthreads();
       tile_load(nxt, 0, more && nxt.tiles > 0, sK0, sV0);
+      if (cur.tiles == 0 && more) ask_rows(nxt, r);
     }
     const Item done = cur;
     const int hq = done.hq0 + w_head;
