@@ -720,8 +720,10 @@ int wgkv_kv4_decode_attn_block(const void* args);
  * written but slots (-1), unchanged lengths and state, and *status (or NULL) =
  * WGKV_ERR_CAPACITY; a held page id outside the pool sets it too, and its
  * tokens' slots are -1.  num_pages * page_size and N*H < 2^31, (B+1)*H <=
- * 2^24.  One launch for N <= 256 and (B+1)*H <= 4096; otherwise up to three,
- * and a workspace (as sized, any contents; calls that share one ordered).
+ * 2^24.  One launch for N <= 256 and (B+1)*H <= 4096; otherwise up to three and
+ * a workspace (as sized, any contents; calls that share one ordered), which calls
+ * without a mask that replace nothing in place may leave out while (B+1)*H and
+ * (N/256+2)*H <= 4096.
  *
  * wgkv_paged_append copies rows of key/value bf16 (N, H, D) (element strides,
  * d contiguous; 16-byte aligned, strides multiples of 8) to rows slots[n,h]

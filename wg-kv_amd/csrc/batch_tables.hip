@@ -513,7 +513,10 @@ extern "C" int wgkv_build_block_tables(
     return WGKV_ERR_ARG;
   const TablesScratch sc = tables_scratch(batch, num_kv_heads, num_tokens);
   const bool small = small_step(batch, num_kv_heads, num_tokens);
-  if (!small && (!workspace || workspace_bytes < sc.bytes || ((uintptr_t)workspace & 15))) return WGKV_ERR_WORKSPACE;
+  const bool lds = lds_step(batch, num_kv_heads, num_tokens);
+  const bool copies = !small && lds && (new_lengths == lengths || state_out == page_state);
+  const bool scratch = !small && (g_mask || copies || !lds);
+  if (scratch && (!workspace || workspace_bytes < sc.bytes || ((uintptr_t)workspace & 15))) return WGKV_ERR_WORKSPACE;
   TablesArgs a{};
   a.len = lengths;
   a.len_sb = len_stride_b;
@@ -543,13 +546,13 @@ extern "C" int wgkv_build_block_tables(
     return hipGetLastError() == hipSuccess ? WGKV_OK : WGKV_ERR_HIP;
   }
   a.tiles = (num_tokens + kTile - 1) / kTile;
-  char* ws = (char*)workspace;
-  a.tile_count = (int*)(ws + sc.count);
-  a.start_count = (int*)(ws + sc.start);
-  a.plan = (int4*)(ws + sc.plan);
-  a.head = (int4*)(ws + sc.head);
-  const bool lds = lds_step(batch, num_kv_heads, num_tokens);
-  const bool copies = lds && (new_lengths == lengths || state_out == page_state);
+  if (scratch) {
+    char* ws = (char*)workspace;
+    a.tile_count = (int*)(ws + sc.count);
+    a.start_count = (int*)(ws + sc.start);
+    a.plan = (int4*)(ws + sc.plan);
+    a.head = (int4*)(ws + sc.head);
+  }
   if (copies) {
     a.len_copy = (int*)a.plan;
     a.state_copy = (int*)a.head;

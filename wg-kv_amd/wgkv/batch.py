@@ -147,14 +147,17 @@ def build_block_tables(lengths, cu_seqlens, num_tokens, block_table, page_state,
     if state_out is None:
         state_out = torch.empty_like(page_state)
     L = _lib.lib()
-    nbytes = 0 if num_tokens <= 256 and (B + 1) * H <= 4096 else L.wgkv_block_tables_workspace_bytes(B, H, num_tokens)
-    ws = torch.empty(nbytes, dtype=_U8, device=dev) if nbytes else None
     free, held = (free_ids.data_ptr(), free_ids.shape[0]) if free_ids is not None and free_ids.shape[0] else (0, 0)
-    st = L.wgkv_build_block_tables_block(_pack_tables(
+    args = (
         lens.data_ptr(), ls, cu.data_ptr(), num_tokens, mp, ms, table.data_ptr(), bs[0], bs[1], width,
         page_state.data_ptr(), state_out.data_ptr(), free, held, num_blocks, block_size, out.data_ptr(), out.stride(0),
-        slots.data_ptr(), B, H, 0 if status is None else status.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes,
-        _stream(dev)))
+        slots.data_ptr(), B, H, 0 if status is None else status.data_ptr())
+    st = _lib.ERR_WORKSPACE
+    if num_tokens <= 256 or not mp:  # (most of these need no scratch)
+        st = L.wgkv_build_block_tables_block(_pack_tables(*args, 0, 0, _stream(dev)))
+    if st == _lib.ERR_WORKSPACE:
+        ws = torch.empty(L.wgkv_block_tables_workspace_bytes(B, H, num_tokens), dtype=_U8, device=dev)
+        st = L.wgkv_build_block_tables_block(_pack_tables(*args, ws.data_ptr(), ws.numel(), _stream(dev)))
     if st:
         _lib.check(st, "wgkv_build_block_tables")
     return out, slots, state_out
