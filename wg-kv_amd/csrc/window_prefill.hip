@@ -394,11 +394,20 @@ void window_prefill_kernel(WindowArgs a) {
       const int s = r0 + rt * 16 + n;
       if (s >= done.nq || (again >> (rt * 16 + n) & 1)) continue;
       uint16_t* orow = a.out + (int64_t)(done.q0 + s) * a.o_sn + (int64_t)hq * a.o_sh;
+      // a lane has 4 values of d of each dt; lanes g and g ^ 1 (of one row, so both
+      // are here) trade so that one has 8 of the even dt and the other of the odd
 #pragma unroll
-      for (int dt = 0; dt < D / 16; ++dt) {
-        const uint32_t w0 = pack_bf16x2(r.o[dt][rt][0] * inv, r.o[dt][rt][1] * inv);
-        const uint32_t w1 = pack_bf16x2(r.o[dt][rt][2] * inv, r.o[dt][rt][3] * inv);
-        *(uint64_t*)(orow + dt * 16 + 4 * g) = (uint64_t)w0 | ((uint64_t)w1 << 32);
+      for (int dt = 0; dt < D / 16; dt += 2) {
+        u32x4_t w;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const auto x = __builtin_amdgcn_permlane16_swap(
+              pack_bf16x2(r.o[dt][rt][2 * i] * inv, r.o[dt][rt][2 * i + 1] * inv),
+              pack_bf16x2(r.o[dt + 1][rt][2 * i] * inv, r.o[dt + 1][rt][2 * i + 1] * inv), false, false);
+          w[i] = x[0];
+          w[2 + i] = x[1];
+        }
+        *(u32x4_t*)(orow + (dt + (g & 1)) * 16 + 8 * (g >> 1)) = w;
       }
     }
     while (again) {
