@@ -28,12 +28,13 @@
 // fill the card: the tiles of every item are then cut into equal parts, a
 // workgroup each, whose (max, sum, O) a second launch joins.
 //
-// Measured (32/8 heads, D 128): 32768 rows, window 1024 and 4 first tokens 665
-// us, 820 TFLOP/s of the pairs that are seen, 920 of the tiles, where a large
-// bf16 product reaches 1395; rows behind cached keys with a window of 4096 1010.
+// Measured (32/8 heads, D 128): 32768 rows, window 1024 and 4 first tokens 644
+// us, 840 TFLOP/s of the pairs that are seen, 940 of the tiles, where a large
+// bf16 product reaches 1395; rows behind cached keys with a window of 4096 1020.
 // Matrix instructions take 39 % of the cycles and vector ones (exponentials,
 // masks, packing) 56 %, which share a SIMD's issue.  Short prompts (7 of 300 to
-// 600 rows, D 64: 17 us) are a chain of tiles' round trips to memory.
+// 600 rows, D 64: 15.4 us, of which one row takes 6.6) are a chain of tiles' round
+// trips to memory.
 //
 // A masked probability is 0, and 0 times a key's value that is not finite is
 // NaN: rows whose result is not finite are worked out once more, key by key
@@ -394,6 +395,7 @@ void window_prefill_kernel(WindowArgs a) {
       const int s = r0 + rt * 16 + n;
       if (s >= done.nq || (again >> (rt * 16 + n) & 1)) continue;
       uint16_t* orow = a.out + (int64_t)(done.q0 + s) * a.o_sn + (int64_t)hq * a.o_sh;
+      // (16.4 -> 15.3 us for 7 prompts of 300 to 600 rows, D 64)
       // a lane has 4 values of d of each dt; lanes g and g ^ 1 (of one row, so both
       // are here) trade so that one has 8 of the even dt and the other of the odd
 #pragma unroll
