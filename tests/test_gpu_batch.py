@@ -281,6 +281,14 @@ def test_prompt_long():
     check_prompt([2500], [3000], 4, 1, 64, 1 << 30, 0)
 
 
+@pytest.mark.parametrize("D,G,H", [(128, 4, 8), (64, 4, 8), (128, 3, 8), (64, 2, 16), (128, 8, 4)])
+def test_prompt_more_items_than_workgroups(D, G, H):
+    """A workgroup goes through several items, of odd and even numbers of tiles
+    and (rows that see nothing) of none."""
+    req, past = [900, 1, 130, 700, 300, 0, 1200, 64, 400], [0, 70, -129, 100, -300, 5, 64, 0, -200]
+    check_prompt(req * 2, past * 2, G * H, H, D, 150, 3, seed=G)
+
+
 def test_prompt_many_sequences():
     rng = np.random.default_rng(0)
     check_prompt(rng.choice([0, 1, 2, 3], 2048).tolist(), None, 2, 1, 64, 2, 1)
@@ -594,6 +602,15 @@ def test_shared_nan_is_seen_by_those_who_see_it():
     kc[int(ptable[0, 0, 0]), 0] = float("nan")      # the prefix of every sequence's first head
     out = wgkv.paged_decode_attn_shared(q, kc, vc, *args, 0.1)
     assert torch.isnan(out[:, 0, :2]).all() and torch.isfinite(out[2, 0, 2:]).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_shared_more_chunks_than_workgroups(D):
+    """A workgroup takes several chunks of prefixes besides its sequences."""
+    rng = np.random.default_rng(D)
+    B, H, N = 200, 8, 40
+    check_shared(rng.integers(0, 200, (B, H)), rng.integers(0, 700, (N, H)), [B * i // N for i in range(N + 1)], 4 * H, 16,
+                 D)
 
 
 @pytest.mark.parametrize("N", [2, 64])
