@@ -357,6 +357,30 @@ def test_prompt_parts_take_nothing_from_what_is_not_seen(bad, D):
     check_close(torch.where(fine, out.double(), 0), torch.where(fine, want, 0), torch.where(fine, bound, 0))
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("D,G,H", [(64, 2, 2), (128, 4, 2), (128, 3, 1)])
+@pytest.mark.parametrize("past", [[-20, 5000], [-20, 3], [-60, 4000], [-20, 0]])
+def test_prompt_rows_that_see_nothing_give_zeros_whatever_the_values(bad, D, G, H, past):
+    """More rows than keys: the first rows share their item's tiles with rows that
+    see keys, and these hold values that are not finite.  With many keys behind
+    the second sequence the call is cut into parts."""
+    import wgkv
+    req = [64, 33]
+    cu, cuk = starts_of(req), starts_of([a + b for a, b in zip(req, past)])
+    q, k, v = qkv(cu[-1], cuk[-1], G * H, H, D, 7)
+    v[2] = bad                             # the first sequence's third key
+    v[cuk[1] + 1, H - 1, 9] = bad          # one value, of the second's
+    out = torch.full_like(q, 7.0)
+    print(f"[prompt] past={past} G={G} H={H} D={D} bad={bad}", flush=True)
+    wgkv.sink_window_attn(q, k, v, i32(cu), 3000, 1, None, i32(cuk), out=out)
+    torch.cuda.synchronize()
+    want, bound = ob.prompt(q, k, v, cu, cuk, 3000, 1, D ** -0.5)
+    assert not out[:-past[0]].any(), "a row that sees nothing"
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isfinite(out), fine) and not fine[-past[0] + 2:64].any()
+    check_close(torch.where(fine, out.double(), 0), torch.where(fine, want, 0), torch.where(fine, bound, 0))
+
+
 @pytest.mark.parametrize("past", [None, [150, 100]])
 def test_prompt_rows_far_apart(past):
     """Keys more than 2^31 bytes apart, in one tile and over the call."""

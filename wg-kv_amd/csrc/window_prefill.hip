@@ -475,7 +475,9 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
     const Seq s = seq_of(a, uniform(b));
     const int p = r - s.q0 + s.nk - s.nq;
     const int64_t kv = h / a.G;
-    if (p < 0 || p >= s.nk) continue;  // (starts that do not ascend)
+    if (p >= s.nk) continue;  // behind the sequence's rows (starts that do not ascend)
+    // (a row at p < 0 sees nothing and gets zeros here: 0 times what other rows of its
+    // item see may be NaN)
     exact_row<D>(a, a.q + (int64_t)r * a.q_sn + (int64_t)h * a.q_sh, a.k + s.k0 * a.k_sn + kv * a.k_sh,
                  a.v + s.k0 * a.v_sn + kv * a.v_sh, p, a.out + (int64_t)r * a.o_sn + (int64_t)h * a.o_sh, lane);
   }
