@@ -545,6 +545,74 @@ def test_window_masked_tokens_of_a_visible_page():
         check_close(out, *ob.token(q, kc, vc, lens, table, 0.1, 21, 3))
 
 
+@pytest.mark.parametrize("B,H,G,D", [(1, 2, 4, 128), (5, 2, 1, 64), (2, 2, 5, 128), (33, 2, 4, 64)])
+@pytest.mark.parametrize("window", [1, 70, 1 << 20])
+@pytest.mark.parametrize("what", ["key nan", "key inf", "keys nan", "all keys nan", "query nan", "query inf", "value nan",
+                                  "value inf"])
+def test_window_shows_what_is_seen_and_not_finite(B, H, G, D, window, what):
+    """In the results of the heads that see it, and of no others, however the
+    call is cut (up to 64 heads of 4 query heads in chunks, others in ranges)."""
+    import wgkv
+    P, T = 16, 2100
+    lens = torch.full((B, H), T)
+    table, _, n = paged(lens, P, D, 3)
+    kc, vc = pools(n, P, D, 4)
+    q = query(B, G * H, D, 5)
+    q[..., 0] = q[..., 0].abs() + 0.5      # (an infinite key's scores are +inf)
+    kc[..., 0] = kc[..., 0].abs() + 0.5    # (and an infinite query's)
+    b, h = B - 1, H - 1
+
+    def rows(pool, t0, t1):
+        return [pool[int(table[b, h, t // P]), t % P] for t in range(t0, t1)]
+
+    kind, bad = what.rsplit(" ", 1)[0], float(what.rsplit(" ", 1)[1])
+    if kind.startswith("query"):
+        q[b, 0, h * G, 0] = bad
+    elif kind == "keys":                   # the newest ones: every score of a wave's share
+        for r in rows(kc, T - 64, T):
+            r[:] = bad
+    elif kind == "all keys":
+        for r in rows(kc, 0, T):
+            r[:] = bad
+    else:
+        rows(kc if kind == "key" else vc, T - 1, T)[0][0] = bad
+    print(f"[window] B={B} H={H} G={G} D={D} W={window} {what}", flush=True)
+    out = wgkv.paged_decode_attn_window(q, kc, vc, lens.to(DEV, I32), table, window, 0, 0.1)
+    torch.cuda.synchronize()
+    want, bound = ob.token(q, kc, vc, lens, table, 0.1, window, 0)
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(torch.isinf(out), torch.isinf(want))
+    hit = fine.new_zeros(fine.shape)
+    mine = hit[b, 0, h * G:h * G + (1 if kind == "query" else G)]
+    (mine[:, :1] if kind == "value" else mine)[:] = True
+    assert torch.equal(~fine, hit)
+    check_close(torch.where(fine, out.double(), 0), torch.where(fine, want, 0), torch.where(fine, bound, 0))
+
+
+@pytest.mark.parametrize("B,H,G", [(1, 2, 4), (2, 2, 5)])
+@pytest.mark.parametrize("T,window", [(3, 2), (2100, 70)])
+def test_window_scores_of_minus_infinity_weigh_nothing(B, H, G, T, window):
+    """A key whose score is -inf, and a head that sees no other."""
+    import wgkv
+    P, D = 16, 64
+    lens = torch.full((B, H), T)
+    table, _, n = paged(lens, P, D, 3)
+    kc, vc = pools(n, P, D, 4)
+    q = query(B, G * H, D, 5)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    kc[int(table[0, 0, (T - 1) // P]), (T - 1) % P, 0] = -float("inf")
+    for t in range(T - window, T):
+        kc[int(table[0, 1, t // P]), t % P, 0] = -float("inf")
+    out = wgkv.paged_decode_attn_window(q, kc, vc, lens.to(DEV, I32), table, window, 0, 0.1)
+    torch.cuda.synchronize()
+    assert not out[0, 0, G:2 * G].any()
+    t = torch.arange(T - window, T - 1, device=DEV)
+    at = table[0, 0].long()[t // P] * P + t % P
+    see = torch.ones(G, len(t), dtype=torch.bool, device=DEV)
+    want, bound = ob.attend(q[0, 0, :G], kc.view(-1, D)[at], vc.view(-1, D)[at], see, 0.1)
+    check_close(out[0, 0, :G], want, bound)
+
+
 def check_shared(lens, plens, starts, Hq, P, D, scale=None, seed=0, spread=1.0, given=None):
     import wgkv
     lens, plens = torch.as_tensor(lens), torch.as_tensor(plens)

@@ -123,6 +123,13 @@ __device__ __forceinline__ Visible visible_subpages(const DecodeArgs& a, int T) 
   return v;
 }
 
+// Whether a sum of weights has a quotient: in a windowed call one of NaN does, so
+// that a score that is seen and no number shows.
+template <bool WIN>
+__device__ __forceinline__ bool has_quotient(float l) {
+  return WIN ? l != 0.f : l > 0.f;
+}
+
 template <bool WIN>
 __device__ __forceinline__ int head_subpages(const DecodeArgs& a, int bh) {
   return visible_subpages<WIN>(a, clamped_tokens(a, bh)).nsub;
@@ -461,7 +468,9 @@ void decode_split_kernel(DecodeArgs a) {
   for (int i = 0; i < G; ++i) {
     const float lw = wave_sum(l_lane[i]);
     if (lane == 0) {
-      s_ml[wid][0][i] = m_run[i];
+      // (a maximum of -inf has no part in the merges, but where every score of the
+      // wave is NaN, the sum is NaN too and has to get there)
+      s_ml[wid][0][i] = WIN && lw != lw ? 0.f : m_run[i];
       s_ml[wid][1][i] = lw;
     }
   }
@@ -495,7 +504,7 @@ void decode_split_kernel(DecodeArgs a) {
       A = fmaf(sc, sum, A);
     }
     if (single) {
-      const float o = L > 0.f ? A / L : 0.f;
+      const float o = has_quotient<WIN>(L) ? A / L : 0.f;
       a.out[(int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + d] = f32_to_bf16(o);
     } else if constexpr (kFused) {
       if (d == 0) {
@@ -568,8 +577,10 @@ void decode_split_kernel(DecodeArgs a) {
   float M = -INFINITY, L = 0.f;
   f32x4_t A = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   if (grp < GROUPS) {
-    const __amdgpu_buffer_rsrc_t acc_rsrc =
-        __builtin_amdgcn_make_buffer_rsrc(a.part_acc + (int64_t)c0 * G * D, (short)0, 0x7fffffff, 0x00020000);
+    // (a windowed call's entries of a batch behind the last chunk read as zeros: a
+    // weight of 0 times an infinite value would be NaN)
+    const __amdgpu_buffer_rsrc_t acc_rsrc = __builtin_amdgcn_make_buffer_rsrc(
+        a.part_acc + (int64_t)c0 * G * D, (short)0, WIN ? pl.n_bh * (G * D * (int)sizeof(float)) : 0x7fffffff, 0x00020000);
     for (int cb = c0 + grp; cb < c1; cb += GROUPS * kBatch) {
       float mc[kBatch], lc[kBatch];
       f32x4_t ac[kBatch];
@@ -578,7 +589,8 @@ void decode_split_kernel(DecodeArgs a) {
         const int c = min(cb + k * GROUPS, c1 - 1);
         mc[k] = load_coherent(&a.part_m[c * G + i]);
         lc[k] = load_coherent(&a.part_l[c * G + i]);
-        ac[k] = load_coherent4(acc_rsrc, ((c - c0) * G * D + vq * 4) * (int)sizeof(float));
+        const int ca = WIN ? cb + k * GROUPS : c;
+        ac[k] = load_coherent4(acc_rsrc, ((ca - c0) * G * D + vq * 4) * (int)sizeof(float));
       }
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
@@ -612,10 +624,10 @@ void decode_split_kernel(DecodeArgs a) {
       Lt += sc * s_l[gg * NQ + t];
       At += sc * s_a[gg * NQ + t];
     }
-    const float inv = Lt > 0.f ? 1.f / Lt : 0.f;
+    const float inv = has_quotient<WIN>(Lt) ? 1.f / Lt : 0.f;
     uint16_t* o = a.out + (int64_t)b * a.out_sb + (int64_t)(h * G + i) * a.out_sh + (vq * 4 - i * D);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = f32_to_bf16(Lt > 0.f ? At[e] * inv : 0.f);
+    for (int e = 0; e < 4; ++e) o[e] = f32_to_bf16(has_quotient<WIN>(Lt) ? At[e] * inv : 0.f);
   }
 }
 
