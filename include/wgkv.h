@@ -728,8 +728,9 @@ int wgkv_kv4_decode_attn_block(const void* args);
  * wgkv_paged_append copies rows of key/value bf16 (N, H, D) (element strides,
  * d contiguous; 16-byte aligned, strides multiples of 8) to rows slots[n,h]
  * of the pools (cache_rows, D); slots outside [0, cache_rows) are left out.
- * D a multiple of 8.  The pools share no byte; of two tokens with one slot
- * either may stay.
+ * D a multiple of 8.  The pools share no byte.  Slots are to differ:
+ * tokens that share one leave rows in which each 16 bytes are one token's, but
+ * not all the same token's, and not the same in every call.
  *
  * wgkv_sink_window_attn: q, out bf16 (N, Hq, D), k, v (Nk, Hkv, D) (element
  * strides, d contiguous, 16-byte aligned).  Sequence b holds rows cu_seqlens_q[b]

@@ -218,6 +218,31 @@ def test_append(N, H, D, layout):
     assert torch.equal(kc.view(-1, D), want[0]) and torch.equal(vc.view(-1, D), want[1])
 
 
+@pytest.mark.parametrize("D", [40, 64, 128])
+def test_append_of_tokens_with_one_slot(D):
+    """Each 8 values of the row are one of the tokens'; other rows stay."""
+    import wgkv
+    N, H = 3000, 2
+    k = torch.arange(N, device=DEV).to(torch.int16).view(BF16)[:, None, None].expand(N, H, D).contiguous()
+    v = (torch.arange(N, device=DEV) + N).to(torch.int16).view(BF16)[:, None, None].expand(N, H, D).contiguous()
+    kc, vc = (torch.full((4, 16, D), 7.0, dtype=BF16, device=DEV) for _ in range(2))
+    slots = torch.full((N, H), -1, dtype=I32, device=DEV)
+    slots[::3, 0] = 5
+    slots[1::3, 1] = 40
+    wgkv.paged_append(k, v, kc, vc, slots)
+    torch.cuda.synchronize()
+    for pool, base in ((kc, 0), (vc, N)):
+        rows = pool.view(-1, D)
+        bits = rows.view(torch.int16).long() - base
+        for slot, first in ((5, 0), (40, 1)):
+            pieces = bits[slot].view(-1, 8)
+            assert (pieces == pieces[:, :1]).all() and (pieces % 3 == first).all()
+            assert pieces.min() >= 0 and pieces.max() < N
+        rest = torch.ones(64, dtype=torch.bool, device=DEV)
+        rest[[5, 40]] = False
+        assert (rows[rest] == 7).all()
+
+
 # ---- prompts -------------------------------------------------------------------
 def qkv(N, Nk, Hq, H, D, seed, spread=1.0):
     gen = torch.Generator().manual_seed(seed)

@@ -424,7 +424,8 @@ struct AppendArgs {
 
 // Rows to their places, 16 bytes per thread and step, keys and values
 // together: pure bandwidth.  Four pieces of each are asked for before the
-// first is written.  64K tokens x 8 heads, D 128: 537 MB in 109 us, 4.9 TB/s (a
+// first is written.  Nothing orders two tokens with one slot: a row may come to
+// hold pieces of both.  64K tokens x 8 heads, D 128: 537 MB in 109 us, 4.9 TB/s (a
 // plain copy 5.0).
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   constexpr int U = 4;

@@ -166,7 +166,10 @@ def build_block_tables(lengths, cu_seqlens, num_tokens, block_table, page_state,
 def paged_append(k, v, k_cache, v_cache, slots):
     """Copies the rows of k, v (tokens, num_kv_heads, head_dim) bf16, in any
     layout, to rows ``slots[n, h]`` (int32) of the pools; slots outside them
-    (-1) are left out.  Of two tokens with one slot either may stay."""
+    (-1) are left out.  The slots in them are to differ, as those of
+    build_block_tables do where no page stands in the tables twice: tokens that
+    share one leave rows in which each 8 values are one token's, but not all the
+    same token's, and not the same in every call."""
     shape = k.shape
     pool = _check_pool(k_cache, v_cache)
     if len(shape) != 3 or v.shape != shape or shape[2] != pool[2]:
