@@ -168,6 +168,45 @@ def test_tables_clamp_lengths_and_starts():
             assert guard.tolist() == [5] * 4 and int(slots.max()) < 64 * 16 and int(slots.min()) >= -1
 
 
+def inside(shape, fill, margin=4096):
+    """An int32 tensor with `margin` entries of `fill` before and behind it, and the whole."""
+    n = int(np.prod(shape))
+    whole = torch.full((n + 2 * margin,), fill, dtype=I32, device=DEV)
+    return whole[margin:margin + n].view(shape), whole
+
+
+@pytest.mark.parametrize("cu", [[50, 10, 1 << 30, -4], [700, 0, 700, 0], [-9, -9, -9, -9], [0, 650, 20, 640],
+                                [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1, 5], [300, 299, 298, 297]])
+@pytest.mark.parametrize("N", [100, 256, 257, 700])
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("H,in_place", [(2, False), (2, True), (1400, False)])
+def test_tables_write_only_their_own_for_any_starts(cu, N, masked, H, in_place):
+    """Starts that do not ascend or lie outside the tokens, lengths outside the
+    table: what lies around the outputs stays, lengths and rows are in range."""
+    import wgkv
+    B, width, P, blocks = 3, 8, 16, 64
+    table, t_all = inside((B, H, width), 77)
+    out, o_all = inside((B, H), 77)
+    slots, s_all = inside((N, H), 77)
+    state, st_all = inside((2,), 77)
+    free = i32(list(range(40, 50)))
+    lens = torch.tensor([[0, 3], [9, -2 ** 31], [2 ** 31 - 1, 128]], dtype=I32, device=DEV).repeat(1, H // 2)
+    state.copy_(i32([5, 10]))
+    given = i32([5, 10])
+    if in_place:
+        out.copy_(lens)
+        lens, given = out, state
+    mask = (torch.arange(N * H, device=DEV).view(H, N) % 3 != 1) if masked else None
+    print(f"[tables] cu={cu} N={N} H={H} masked={masked} in_place={in_place}", flush=True)
+    wgkv.build_block_tables(lens, i32(cu), N, table, given, blocks, P, g_mask=mask, free_ids=free, out=out,
+                            state_out=state, slots=slots)
+    torch.cuda.synchronize()
+    for whole, n in ((t_all, table.numel()), (o_all, out.numel()), (s_all, slots.numel()), (st_all, 2)):
+        assert (whole[:4096] == 77).all() and (whole[4096 + n:] == 77).all()
+    assert out.min() >= 0 and out.max() <= width * P
+    assert slots.min() >= -1 and slots.max() < blocks * P
+
+
 def test_tables_strides_and_buffers():
     import wgkv
     rng = np.random.default_rng(5)
