@@ -737,11 +737,14 @@ int wgkv_kv4_decode_attn_block(const void* args);
  * .. cu_seqlens_q[b+1]-1 and keys cu_seqlens_k[b] .. cu_seqlens_k[b+1]-1; with
  * nq rows and nk keys its row i is at position p = i + nk - nq and sees key j
  * iff j <= p and (j > p - window or j < num_sinks).  Rows that see nothing
- * give zeros; what a row does not see has no part in it, NaN included.  Rows
- * of no sequence are left as they are, or cleared (clear_rest != 0).  window
- * >= 1; D in {64,128}; G = Hq/Hkv in 1..8; up to 2048 sequences, 2^30
- * rows and 2^36 of both together (sequences times rows).  Few rows with long windows take a workspace (as sized, 0 bytes for
- * others; any contents; calls that share one ordered) and two launches.
+ * give zeros; what a row does not see has no part in it, NaN included.  (For
+ * that, rows next to those that see a value that is not finite are worked out
+ * on their own, 0.12 ms per 1000 keys, up to 32 in turn.)  Rows of no sequence
+ * are left as they are, or cleared (clear_rest != 0).  window >= 1; D in
+ * {64,128}; G = Hq/Hkv in 1..8; up to 2048 sequences, 2^30 rows and 2^36 of both
+ * together (sequences times rows).  Few rows with long windows take a workspace
+ * (as sized, 0 bytes for others; any contents; calls that share one ordered) and
+ * two launches.
  *
  * wgkv_paged_decode_attn_window: wgkv_paged_decode_attn where a head of T
  * tokens shows those t with t >= T - window or t < num_sinks.  Page ids of the

@@ -445,6 +445,114 @@ def test_prompt_rows_that_see_nothing_give_zeros_whatever_the_values(bad, D, G, 
     check_close(torch.where(fine, out.double(), 0), torch.where(fine, want, 0), torch.where(fine, bound, 0))
 
 
+def check_not_finite(out, want, bound):
+    """NaN and infinities where the oracle has them, the rest within the bound."""
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isnan(out), torch.isnan(want))
+    assert torch.equal(out[torch.isinf(want)].double(), want[torch.isinf(want)]) and torch.isfinite(out[fine]).all()
+    check_close(torch.where(fine, out.double(), 0), torch.where(fine, want, 0), torch.where(fine, bound, 0))
+
+
+@pytest.mark.parametrize("D,G,H", [(64, 2, 1), (128, 4, 1), (128, 1, 2)])
+@pytest.mark.parametrize("req,past", [([200], [0]), ([70, 40], [30, 2500])])
+@pytest.mark.parametrize("window,sinks", [(40, 3), (65, 0), (3000, 0), (33, 100)])
+@pytest.mark.parametrize("at", [(0,), (63,), (100,), (127, 5), (-1,), (-64, -65), (-100, 0, 50)])
+def test_prompt_values_that_are_not_finite_anywhere(D, G, H, req, past, window, sinks, at):
+    """Rows that see them show them and others do not, in calls cut along the keys
+    or not."""
+    import wgkv
+    cu, cuk = starts_of(req), starts_of([a + b for a, b in zip(req, past)])
+    q, k, v = qkv(cu[-1], cuk[-1], G * H, H, D, 11)
+    for i, j in enumerate(at):
+        v[j, 0, 9 * i + 1] = (float("inf"), float("nan"), -float("inf"))[i]
+        v[j, H - 1, 40] = -float("inf") if i else float("inf")  # those of both signs: NaN
+    print(f"[prompt] at={at} req={req} past={past} G={G} H={H} D={D} W={window} S={sinks}", flush=True)
+    out = wgkv.sink_window_attn(q, k, v, i32(cu), window, sinks, None, i32(cuk))
+    torch.cuda.synchronize()
+    check_not_finite(out, *ob.prompt(q, k, v, cu, cuk, window, sinks, D ** -0.5))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("past", [0, 3000])
+@pytest.mark.parametrize("bad", [False, True])
+def test_prompt_values_next_to_the_largest(D, past, bad):
+    """Scores that grow by 7 in log2 after the first tile, for 36 keys: 36 * 2^7 *
+    2^120 passes fp32's range, under the row's own maximum the sums do not (36 +
+    2500 * 2^-7 < 2^6 weights of values of 2^120).  `bad`: among them one that is
+    not finite, which some rows see."""
+    import wgkv
+    N = 100
+    q, k, v = qkv(N, N + past, 2, 1, D, 12)
+    v = torch.sign(v.float()).mul(2.0 ** 120).to(BF16)
+    q[..., 0] = 1.0
+    k[..., 0] = 0.0
+    k[64 + past // 2:100 + past // 2, :, 0] = 7 * 0.6931 * D ** 0.5
+    k[..., 1:] *= 0.01
+    if bad:
+        v[past + 50, 0, 3] = float("inf")
+    cu, cuk = [0, N], [0, N + past]
+    out = wgkv.sink_window_attn(q, k, v, i32(cu), 2500, 0, None, i32(cuk))
+    torch.cuda.synchronize()
+    want, bound = ob.prompt(q, k, v, cu, cuk, 2500, 0, D ** -0.5)
+    assert torch.isfinite(want).all() == (not bad)
+    check_not_finite(out, want, bound)
+
+
+@pytest.mark.parametrize("past", [0, 3000])
+def test_prompt_scores_of_minus_infinity(past):
+    """Weights of 0: a finite value has no part, an infinite one makes NaN, and a
+    row without other keys gives zeros."""
+    import wgkv
+    N, D = 100, 64
+    q, k, v = qkv(N, N + past, 2, 1, D, 13)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    k[past + 10:past + 20, :, 0] = -float("inf")
+    v[past + 15, 0, 7] = float("inf")
+    k[past + 60, 0, 0] = -float("inf")
+    cu, cuk = [0, N], [0, N + past]
+    scale = D ** -0.5
+    for W in (3, 2000):
+        out = wgkv.sink_window_attn(q, k, v, i32(cu), W, 0, None, i32(cuk))
+        torch.cuda.synchronize()
+        p, j = torch.arange(N, device=DEV)[:, None] + past, torch.arange(N + past, device=DEV)[None]
+        see = (j <= p) & (j > p - W) & ~torch.isinf(k[:, 0, 0])[None]
+        sees = (j <= p) & (j > p - W)
+        for h in range(2):
+            vv = v.clone()
+            vv[past + 15, 0, 7] = 0
+            want, bound = ob.attend(q[:, h], torch.nan_to_num(k[:, 0], neginf=0.0), vv[:, 0], see, scale)
+            alone = see.sum(1) == 0
+            assert not out[alone, h].any() and bool(alone.any()) == (W == 3)
+            hit = torch.zeros_like(want, dtype=torch.bool)
+            hit[:, 7] = sees[:, past + 15] & ~alone
+            assert torch.equal(torch.isnan(out[:, h]), hit)
+            check_close(torch.where(hit, 0, out[:, h].double()), torch.where(hit, 0, want), bound)
+
+
+@pytest.mark.parametrize("D,what", [(128, "value"), (64, "row")])
+def test_prompt_time_with_a_value_that_is_not_finite(D, what):
+    """An infinite value of a first token, seen by every row, costs no row a pass
+    of its own (4096 rows took more than 100 times as long)."""
+    import wgkv
+    q, k, v = qkv(4096, 4096, 8, 2, D, 14)
+    cu = i32([0, 4096])
+    events = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+
+    def best(n=5):
+        times = []
+        for _ in range(n):
+            events[0].record()
+            wgkv.sink_window_attn(q, k, v, cu, 1024, 4)
+            events[1].record()
+            torch.cuda.synchronize()
+            times.append(events[0].elapsed_time(events[1]))
+        return min(times)
+
+    finite = best()
+    v[1, 0, 3 if what == "value" else slice(None)] = float("inf")
+    assert best() < 10 * finite
+
+
 @pytest.mark.parametrize("past", [None, [150, 100]])
 def test_prompt_rows_far_apart(past):
     """Keys more than 2^31 bytes apart, in one tile and over the call."""
@@ -463,6 +571,28 @@ def test_prompt_rows_far_apart(past):
     want, bound = ob.prompt(q, k, v, cu, cuk, 70, 3, 64 ** -0.5)
     check_close(out, want, bound)
     assert torch.equal(out, wgkv.sink_window_attn(q, k, v, i32(cu), 70, 3, None, i32(cuk)))
+
+
+@pytest.mark.parametrize("past", [None, [1500, 900]])
+def test_prompt_values_that_are_not_finite_far_apart(past):
+    """Keys more than 2^31 bytes apart: the last row of a block, and of a sequence,
+    shows its own key's value."""
+    import wgkv
+    req = [100, 70]
+    cu = starts_of(req)
+    cuk = cu if past is None else starts_of([a + b for a, b in zip(req, past)])
+    Nk, stride = cuk[-1], 1 << 21
+    q, k, v = qkv(cu[-1], Nk, 4, 2, 64, 15)
+    for i, j in enumerate((cuk[1] - 100, cuk[1] - 37, cuk[1] - 1, cuk[1] + 2, Nk - 7, Nk - 1)):
+        v[j, i % 2, 5 * i] = (float("inf"), -float("inf"), float("nan"))[i % 3]
+    big = torch.empty(Nk * stride, dtype=BF16, device=DEV)
+    kf, vf = (big.as_strided((Nk, 2, 64), (stride, 64, 1), at) for at in (0, 1024))
+    kf.copy_(k)
+    vf.copy_(v)
+    for window, sinks in ((70, 3), (2000, 0)):
+        out = wgkv.sink_window_attn(q, kf, vf, i32(cu), window, sinks, None, i32(cuk))
+        torch.cuda.synchronize()
+        check_not_finite(out, *ob.prompt(q, k, v, cu, cuk, window, sinks, 64 ** -0.5))
 
 
 def test_prompt_parts_captured():

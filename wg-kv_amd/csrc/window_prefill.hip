@@ -37,8 +37,13 @@
 // trips to memory.
 //
 // A masked probability is 0, and 0 times a key's value that is not finite is
-// NaN: rows whose result is not finite are worked out once more, key by key
-// (exact_row).
+// NaN: of the rows whose result is not finite, those whose tiles held such a value
+// that they do not see are worked out once more, one after the other (rows_to_redo,
+// exact_row).  Rows that see it keep theirs.  (4096 rows, 8/2 heads, D 128, window
+// 1024, 0.06 ms: an infinite value of a first token, which all rows see, 0.07 ms,
+// and 12.8 when every such row was redone key by key; of a middle token, which up to
+// 63 rows around its block and 63 at the windows' end do not see, 3.8, whatever
+// the number of rows; infinities throughout 3.8, and 30 for 32768 rows of 32 heads.)
 #include <string.h>
 
 #include "attn_tile.h"
@@ -70,6 +75,7 @@ struct WindowArgs {
   float scale_log2;
   uint32_t q_and, q_xor;
   int clear_rest;  // rows of no sequence get zeros
+  bool far;        // keys may lie 2^31 bytes or more apart
   int parts;       // of an item's tiles; more than 1: (max, sum) and O of (part, row, head) go to
   float* part_ml;
   float* part_o;
@@ -98,39 +104,132 @@ struct Keys {
   WGKV_DEVICE int key(int x) const { return x < first ? x : x + shift; }
 };
 
-// A row key by key, for results that are not finite: a wave, D/64 values of d
-// each lane.
+// A row on its own, by a wave: 64 keys at a time, one a lane for the scores; for
+// the values D/8 lanes a key, eight values of d each.  What the row does not see
+// is not touched.
 template <int D>
 WGKV_DEVICE void exact_row(const WindowArgs& a, const uint16_t* q, const uint16_t* k, const uint16_t* v, int p,
                            uint16_t* out, int lane) {
-  constexpr int C = D / 64;
-  float qf[C], acc[C], m = -INFINITY, l = 0.f;
+  constexpr int CH = D / 8, KPI = 64 / CH;  // 16-byte slices of a row, keys whose values one load of the wave takes
+  constexpr int kAhead = 8;                 // loads of values that are asked for together
+  const int c = lane % CH;
+  float acc[8], m = -INFINITY, l = 0.f;
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const uint32_t w = ((uint32_t)q[lane * C + c] & (a.q_and & 0xffffu)) ^ (a.q_xor & 0xffffu);
-    qf[c] = __uint_as_float(w << 16);
-    acc[c] = 0.f;
-  }
-  const int lo = max(0, p - a.window + 1), first = min(a.sinks, lo);
-  for (int x = 0; x < first + p - lo + 1; ++x) {
-    const int64_t j = x < first ? x : x - first + lo;
+  for (int e = 0; e < 8; ++e) acc[e] = 0.f;
+  const int lo = max(0, p - a.window + 1), first = min(a.sinks, lo), count = first + p - lo + 1;
+  const auto key = [&](int x) { return (int64_t)(x < first ? x : x - first + lo); };
+  for (int x0 = 0; x0 < count; x0 += 64) {
+    const uint16_t* row = k + key(min(x0 + lane, count - 1)) * a.k_sn;
     float s = 0.f;
+#pragma unroll(CH / 2)
+    for (int j = 0; j < CH; ++j) {
+      const u32x4_t kw = *((const u32x4_t*)row + j), qw = (*((const u32x4_t*)q + j) & a.q_and) ^ a.q_xor;
 #pragma unroll
-    for (int c = 0; c < C; ++c) s = fmaf(qf[c], __uint_as_float((uint32_t)k[j * a.k_sn + lane * C + c] << 16), s);
-    s = wave_sum(s) * a.scale_log2;
-    if (s == -INFINITY) continue;
-    const float mn = s > m ? s : m;
-    const float was = m == -INFINITY ? 0.f : fast_exp2(m - mn), e = fast_exp2(s - mn);
-    const float w = round_to_bf16(e);
-    l = l * was + w;
-#pragma unroll
-    for (int c = 0; c < C; ++c) acc[c] = acc[c] * was + w * __uint_as_float((uint32_t)v[j * a.v_sn + lane * C + c] << 16);
+      for (int i = 0; i < 4; ++i) {
+        s = fmaf(__uint_as_float(qw[i] << 16), __uint_as_float(kw[i] << 16), s);
+        s = fmaf(__uint_as_float(qw[i] & 0xffff0000u), __uint_as_float(kw[i] & 0xffff0000u), s);
+      }
+    }
+    s = x0 + lane < count ? s * a.scale_log2 : -INFINITY;
+    if (__builtin_amdgcn_ballot_w64(s != s || s == INFINITY) != 0) {  // so is the row's sum
+      l = NAN;
+      break;
+    }
+    const float mn = fmaxf(m, wave_max(s)), by = mn == -INFINITY ? 0.f : mn;  // (a score of -inf: a weight of 0)
+    const float was = m == -INFINITY ? 0.f : fast_exp2(m - mn), w = round_to_bf16(fast_exp2(s - by));
     m = mn;
-    if (l != l) break;  // nothing can change any more
-  }
-  const float inv = 1.f / l;
+    l = l * was + wave_sum(w);
 #pragma unroll
-  for (int c = 0; c < C; ++c) out[lane * C + c] = l == 0.f ? 0 : f32_to_bf16(acc[c] * inv);
+    for (int e = 0; e < 8; ++e) acc[e] *= was;
+    for (int y0 = lane / CH; y0 < 64; y0 += KPI * kAhead) {
+      u32x4_t vw[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+        vw[j] = *((const u32x4_t*)(v + key(min(x0 + y0 + j * KPI, count - 1)) * a.v_sn) + c);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const int y = y0 + j * KPI;
+        const float wy = __shfl(w, y, 64);
+        const bool on = x0 + y < count;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          acc[2 * i] = on ? fmaf(wy, __uint_as_float(vw[j][i] << 16), acc[2 * i]) : acc[2 * i];
+          acc[2 * i + 1] = on ? fmaf(wy, __uint_as_float(vw[j][i] & 0xffff0000u), acc[2 * i + 1]) : acc[2 * i + 1];
+        }
+      }
+    }
+    bool nan = true;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) nan = nan && acc[e] != acc[e];
+    uint64_t y = __builtin_amdgcn_ballot_w64(nan);
+#pragma unroll
+    for (int off = CH; off < 64; off <<= 1) y |= y >> off;
+    if ((~y & ((1ull << CH) - 1)) == 0 && l != 0.f) break;  // every value is NaN
+  }
+#pragma unroll
+  for (int off = CH; off < 64; off <<= 1)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor(acc[e], off, 64);
+  if (lane >= CH) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  u32x4_t o;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = l == 0.f ? 0u : pack_bf16x2(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  *((u32x4_t*)out + c) = o;
+}
+
+// Values of d as bits: word d % 4, bit d / 4.
+typedef u32x4_t Columns;
+
+// Of up to 32 rows from position p0 on, by a wave, whose sums O are not finite in
+// `need` (lane i: row i % 32's; the sum of their weights is finite): those to be
+// worked out on their own.  `ks`: the keys that their tiles held.  A row is right as
+// it is if keys that it sees have such values in all of these places and others in
+// its tiles have none.  It is not if a key that it does not see has some, since a
+// masked weight of 0 times its value is NaN, or if no key has: then large values
+// have overflowed under a maximum that lags.  A tile that every row sees in full is
+// read only while some row lacks such keys.  `twice`: a row's own key may have
+// stood in its tiles a second time, masked.
+template <int D>
+WGKV_DEVICE uint32_t rows_to_redo(const WindowArgs& a, const Keys& ks, const uint16_t* v, int nk, int p0, uint32_t rows,
+                                  Columns need, bool twice, int lane) {
+  const int p = p0 + (lane & 31);  // the lane's row
+  const bool mine = rows >> (lane & 31) & 1;
+  bool unseen = false;
+  const auto open = [&]() { return mine && !unseen && (need[0] | need[1] | need[2] | need[3]) != 0; };
+  for (int x0 = 0; x0 < ks.count; x0 += attn::kKeys) {
+    const int x1 = x0 + attn::kKeys - 1, e0 = p0 - ks.shift;
+    const bool full = x1 < ks.count && x1 <= e0 && (e0 + 31 - x0 < a.window || x1 < a.sinks);
+    if (full && __builtin_amdgcn_ballot_w64(open()) == 0) continue;
+    // a key a lane (also behind the rows' keys: the last tile holds them)
+    const int j = ks.key(x0 + lane);
+    const uint16_t* row = v + (int64_t)min(j, nk - 1) * a.v_sn;
+    Columns bad = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int i = 0; i < D / 8; ++i) {
+      const u32x4_t w = *((const u32x4_t*)row + i);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t inf = e & 1 ? 0x7f800000u : 0x7f80u;
+        bad[e % 4] |= (uint32_t)((w[e / 2] & inf) == inf) << (2 * i + e / 4);
+      }
+    }
+    const bool some = j < nk && (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
+    for (uint64_t left = __builtin_amdgcn_ballot_w64(some); left; left &= left - 1) {
+      const int at = __builtin_ctzll(left), jb = ks.key(x0 + at);
+      const bool sees = jb <= p && (jb > p - a.window || jb < a.sinks);
+      unseen = unseen || !sees || (twice && jb == p);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t has = __builtin_amdgcn_readlane(bad[e], at);
+        need[e] = sees ? need[e] & ~has : need[e];
+      }
+      if (__builtin_amdgcn_ballot_w64(mine && !unseen) == 0) return rows;
+      if (full && __builtin_amdgcn_ballot_w64(open()) == 0) break;
+    }
+  }
+  return rows & (uint32_t)__builtin_amdgcn_ballot_w64(unseen || open());
 }
 
 struct Item {
@@ -377,23 +476,41 @@ void window_prefill_kernel(WindowArgs a) {
       cur = nxt;
       continue;
     }
-    uint32_t again = 0;  // rows with a value that is not finite
+    uint32_t again = 0, none = 0;  // rows with a value that is not finite; of no weight
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
-      float bad = r.sum[rt][0] * 0.f;
+      float bad = 0.f;
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
         for (int i = 0; i < 4; ++i) bad += r.o[dt][rt][i] * 0.f;
-      const uint64_t y = __builtin_amdgcn_ballot_w64(r0 + rt * 16 + n < done.nq && bad != bad);
+      // (a sum that is NaN, as its row's scores were, makes every value NaN below)
+      const bool here = r0 + rt * 16 + n < done.nq && bad != bad && r.sum[rt][0] == r.sum[rt][0];
+      const uint64_t y = __builtin_amdgcn_ballot_w64(here), z = __builtin_amdgcn_ballot_w64(here && r.sum[rt][0] == 0.f);
       again |= (uint32_t)((y | y >> 16 | y >> 32 | y >> 48) & 0xffff) << (16 * rt);
+      none |= (uint32_t)((z | z >> 16 | z >> 32 | z >> 48) & 0xffff) << (16 * rt);
+    }
+    Columns need = {0, 0, 0, 0};
+    if (again) {
+#pragma unroll
+      for (int rt = 0; rt < 2; ++rt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w = 0;
+#pragma unroll
+          for (int dt = 0; dt < D / 16; ++dt) w |= (uint32_t)(r.o[dt][rt][i] * 0.f != 0.f) << (4 * dt);
+          w <<= g;
+          w |= __shfl_xor(w, 16, 64);
+          w |= __shfl_xor(w, 32, 64);
+          need[i] = (g & 1) == rt ? w : need[i];  // lane i: row i % 32
+        }
     }
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
       const float l = r.sum[rt][0];
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const int s = r0 + rt * 16 + n;
-      if (s >= done.nq || (again >> (rt * 16 + n) & 1)) continue;
+      if (s >= done.nq) continue;
       uint16_t* orow = a.out + (int64_t)(done.q0 + s) * a.o_sn + (int64_t)hq * a.o_sh;
       // (16.4 -> 15.3 us for 7 prompts of 300 to 600 rows, D 64)
       // a lane has 4 values of d of each dt; lanes g and g ^ 1 (of one row, so both
@@ -412,6 +529,8 @@ void window_prefill_kernel(WindowArgs a) {
         *(u32x4_t*)(orow + (dt + (g & 1)) * 16 + 8 * (g >> 1)) = w;
       }
     }
+    // (the wave's own stores to a row keep their order)
+    if (again) again = none | rows_to_redo<D>(a, done.keys, done.vb, done.nk, p0, again, need, FAR, lane);
     while (again) {
       const int row = r0 + __builtin_ctz(again);
       again &= again - 1;
@@ -421,6 +540,21 @@ void window_prefill_kernel(WindowArgs a) {
     }
     cur = nxt;
   }
+}
+
+// A row of the call, the same in the whole wave: its sequence, and its position.
+struct RowOfCall {
+  Seq s;
+  int p;
+};
+WGKV_DEVICE RowOfCall row_of_call(const WindowArgs& a, int r) {
+  int b = 0;
+  for (int hi = a.B - 1; b < hi;) {  // the last sequence that begins at or before the row
+    const int mid = (b + hi + 1) >> 1;
+    if (a.cu_q[mid] <= r) b = mid; else hi = mid - 1;
+  }
+  const Seq s = seq_of(a, uniform(b));
+  return {s, r - s.q0 + s.nk - s.nq};
 }
 
 // The parts of every row, in order: D/4 lanes a row, four values of d each.
@@ -455,31 +589,41 @@ __global__ __launch_bounds__(256) void window_join_kernel(WindowArgs a) {
       m = mn;
     }
   }
-  const float bad = l * 0.f + o[0] * 0.f + o[1] * 0.f + o[2] * 0.f + o[3] * 0.f;
-  uint64_t again = __builtin_amdgcn_ballot_w64(on && bad != bad);
-  const uint64_t mine = ((1ull << NQ) - 1) << (lane / NQ * NQ);
-  if (on && !(again & mine)) {
+  // (a sum that is NaN makes every value NaN below)
+  uint64_t again = 0, left = 0;  // the first lanes of rows to be worked out on their own; rows to be looked at
+  uint64_t wrong[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) left |= wrong[e] = __builtin_amdgcn_ballot_w64(on && l == l && o[e] * 0.f != 0.f);
+  while (left) {
+    const int from = __builtin_ctzll(left) / NQ * NQ;
+    left &= ~(((1ull << NQ) - 1) << from);
+    const RowOfCall w = row_of_call(a, __builtin_amdgcn_readlane(row, from));
+    bool redo = w.p < 0 || __builtin_amdgcn_readlane(__float_as_int(l), from) == 0;
+    if (!redo) {  // (at least the keys that its item's tiles held, wherever the item began)
+      const Keys ks = keys_of(a, w.p - 127, min(w.p + 127 + attn::kKeys - 1, w.s.nk - 1));
+      const int64_t kv = __builtin_amdgcn_readlane(hq, from) / a.G;
+      Columns need;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) need[e] = (uint32_t)(wrong[e] >> from) & (uint32_t)((1ull << NQ) - 1);
+      redo = rows_to_redo<D>(a, ks, a.v + w.s.k0 * a.v_sn + kv * a.v_sh, w.s.nk, w.p, 1u, need, a.far, lane) != 0;
+    }
+    if (redo && w.p < w.s.nk) again |= 1ull << from;  // (behind the sequence's rows: starts that do not ascend)
+  }
+  if (on && !(again >> (lane / NQ * NQ) & 1)) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     *(uint64_t*)(a.out + (int64_t)row * a.o_sn + (int64_t)hq * a.o_sh + vq * 4) =
         (uint64_t)pack_bf16x2(o[0] * inv, o[1] * inv) | (uint64_t)pack_bf16x2(o[2] * inv, o[3] * inv) << 32;
   }
-  while (again) {  // a wave per row that is not finite
-    const int from = __builtin_ctzll(again) / NQ * NQ;
-    again &= ~(((1ull << NQ) - 1) << from);
+  while (again) {  // a wave per row
+    const int from = __builtin_ctzll(again);
+    again &= again - 1;
     const int r = __builtin_amdgcn_readlane(row, from), h = __builtin_amdgcn_readlane(hq, from);
-    int b = 0;
-    for (int hi = a.B - 1; b < hi;) {  // the last sequence that begins at or before the row
-      const int mid = (b + hi + 1) >> 1;
-      if (a.cu_q[mid] <= r) b = mid; else hi = mid - 1;
-    }
-    const Seq s = seq_of(a, uniform(b));
-    const int p = r - s.q0 + s.nk - s.nq;
+    const RowOfCall w = row_of_call(a, r);
     const int64_t kv = h / a.G;
-    if (p >= s.nk) continue;  // behind the sequence's rows (starts that do not ascend)
     // (a row at p < 0 sees nothing and gets zeros here: 0 times what other rows of its
     // item see may be NaN)
-    exact_row<D>(a, a.q + (int64_t)r * a.q_sn + (int64_t)h * a.q_sh, a.k + s.k0 * a.k_sn + kv * a.k_sh,
-                 a.v + s.k0 * a.v_sn + kv * a.v_sh, p, a.out + (int64_t)r * a.o_sn + (int64_t)h * a.o_sh, lane);
+    exact_row<D>(a, a.q + (int64_t)r * a.q_sn + (int64_t)h * a.q_sh, a.k + w.s.k0 * a.k_sn + kv * a.k_sh,
+                 a.v + w.s.k0 * a.v_sn + kv * a.v_sh, w.p, a.out + (int64_t)r * a.o_sn + (int64_t)h * a.o_sh, lane);
   }
 }
 
@@ -565,14 +709,14 @@ hipError_t launch_items(const WindowArgs& a, hipStream_t st) {
 }
 
 template <int D, int HPW>
-hipError_t launch(const WindowArgs& a, hipStream_t st) {
+hipError_t launch(WindowArgs& a, hipStream_t st) {
   const int64_t bytes = ((int64_t)a.Nk + attn::kKeys) * 2 * (a.k_sn > a.v_sn ? a.k_sn : a.v_sn);
-  const bool far = a.k_sn < 0 || a.v_sn < 0 || bytes >= 0x7ffff000;
-  return far ? launch_items<D, HPW, true>(a, st) : launch_items<D, HPW, false>(a, st);
+  a.far = a.k_sn < 0 || a.v_sn < 0 || bytes >= 0x7ffff000;
+  return a.far ? launch_items<D, HPW, true>(a, st) : launch_items<D, HPW, false>(a, st);
 }
 
 template <int D>
-hipError_t launch_heads(const WindowArgs& a, int heads, hipStream_t st) {
+hipError_t launch_heads(WindowArgs& a, int heads, hipStream_t st) {
   return heads == 4 ? launch<D, 4>(a, st) : heads == 2 ? launch<D, 2>(a, st) : launch<D, 1>(a, st);
 }
 

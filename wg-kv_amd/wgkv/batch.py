@@ -212,8 +212,11 @@ def sink_window_attn(q, k, v, cu_seqlens, window, num_sinks, softmax_scale=None,
     Returns (rows, Hq, D) bf16; rows of no sequence are zeros, or left as they
     are in a given ``out``.  Probabilities are rounded to bf16 for the products;
     sums are fp32, before their division by the probabilities' sum.  What a row
-    does not see has no part in its result, whatever it holds.  Up to 2048
-    sequences.
+    does not see has no part in its result, whatever it holds; what it sees has,
+    with a weight of 0 too (0 times infinity is NaN).  Up to 2048 sequences.
+
+    Rows next to those that see a value that is not finite are worked out on their
+    own: 0.12 ms per 1000 keys, up to 32 of them one after the other.
     """
     shape, kshape = q.shape, k.shape
     if len(shape) != 3 or len(kshape) != 3 or v.shape != kshape or kshape[2] != shape[2]:
