@@ -207,7 +207,8 @@ def sink_window_attn(q, k, v, cu_seqlens, window, num_sinks, softmax_scale=None,
     keys ``cu_seqlens_k[b] ..`` (without it: the same).  With nq rows and nk
     keys its row i is at position p = i + nk - nq (the rows are the last of its
     keys) and sees key j if j <= p and (j > p - window or j < num_sinks);
-    ``window`` counts the row's own key.  Rows that see nothing give zeros.
+    ``window`` counts the row's own key.  Rows that see nothing give zeros.  Keys
+    and values are dense, those of earlier chunks too; pages are not read.
 
     Returns (rows, Hq, D) bf16; rows of no sequence are zeros, or left as they
     are in a given ``out``.  Probabilities are rounded to bf16 for the products;
@@ -304,7 +305,8 @@ def paged_decode_attn_window(q, k_cache, v_cache, cache_seqlens, block_table, wi
     """``paged_decode_attn`` over a sliding window and the first tokens: q (B,
     1, Hq, D) bf16 attends, of the T = cache_seqlens[b, h] tokens of its KV
     head, to those t with t >= T - window or t < num_sinks (the newest token
-    counts to the window); returns (B, 1, Hq, D) bf16, zeros for a head without
+    counts to the window; where a gate left tokens out, these are the head's kept
+    tokens, not the positions that sink_window_attn counts); returns (B, 1, Hq, D) bf16, zeros for a head without
     tokens.  Pages that hold none of them are not read, and their table
     entries may be anything: they can be given back.  Hq / Hkv up to 8, B * Hkv
     up to 2048.  Lengths and page ids out of range are clamped to the table
