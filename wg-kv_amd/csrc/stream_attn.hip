@@ -5,8 +5,9 @@
 // them attends to the first prefix_lens[n, h] tokens of the prefix's pages and
 // to the first lens[b, h] tokens of its own, under one softmax.
 //
-// The prefix is read once for all queries of its group, whose rows (sequence,
-// query head of the KV head) form a matrix.
+// The queries of a group are the rows (sequence, query head of the KV head) of a
+// matrix; its prefix is read once per 16 rows or once per 256, as one choice for
+// the whole call from the average group (many_rows).
 //
 // Window: KV head (b, h) of T tokens shows those t with t >= T - window or t <
 // first; the sub-pages of 16 tokens that hold some are counted through.
@@ -911,6 +912,11 @@ __global__ __launch_bounds__(256) void stream_merge_kernel(StreamArgs a) {
 // 4, own 100 tokens; us streamed / in LDS tiles: 5 sequences 15.4 / 17.6 at 2048
 // tokens of prefix, 28.9 / 20.6 at 8192, 55.4 / 41.7 at 32K; 16 sequences 23.9 /
 // 20.5, 39.5 / 21.9, 92.7 / 45.5; 4 sequences, one operand, 41.0 / 41.3 at 32K.)
+// The starts are on the device, so the average decides for all groups.  Where they
+// differ much, a large group's prefix may be streamed once per 16 rows all the
+// same: of 10 groups one of 31 sequences, 9 of one, 99 us at 8192 tokens and 355 at
+// 32K (one more sequence, and tiles: 87 and 273); of 32 groups one of 97, 31 of one,
+// 305 at 8192 (tiles: 350, since the small groups' rows then fill a tile each).
 bool many_rows(int B, int N, int G) { return (int64_t)B * G > (int64_t)kFew * N; }
 
 struct Scratch {

@@ -346,7 +346,8 @@ def _shared_bytes(B, N, Hq, H, D):
 def paged_decode_attn_shared(q, k_cache, v_cache, cache_seqlens, block_table, prefix_lens, prefix_table, group_starts,
                              softmax_scale, out=None):
     """``paged_decode_attn`` of a batch whose sequences share prefixes, each
-    prefix read once for its whole group.
+    prefix read for many rows of its group at once: for 16 (sequence, query head
+    of a KV head) where groups have up to 16 on average, otherwise for 256.
 
     Sequences ``group_starts[n] .. group_starts[n + 1] - 1`` (int32, ascending;
     N + 1 entries) share prefix n: each of their heads attends to the first
