@@ -748,7 +748,8 @@ int wgkv_kv4_decode_attn_block(const void* args);
  *
  * wgkv_paged_decode_attn_window: wgkv_paged_decode_attn where a head of T
  * tokens shows those t with t >= T - window or t < num_sinks.  Page ids of the
- * others are not read.  The workspace's first 8192 bytes (per-head arrival
+ * others are not read.  A NaN or +inf among the scores that a head sees gives
+ * NaN (wgkv_paged_decode_attn: zeros).  The workspace's first 8192 bytes (per-head arrival
  * counters) must be zero before a call; every call leaves them zero.  Calls
  * that share a workspace must be ordered.
  *

@@ -30,11 +30,15 @@
 //
 // Measured (32/8 heads, D 128): 32768 rows, window 1024 and 4 first tokens 644
 // us, 840 TFLOP/s of the pairs that are seen, 940 of the tiles, where a large
-// bf16 product reaches 1395; rows behind cached keys with a window of 4096 1020.
-// Matrix instructions take 39 % of the cycles and vector ones (exponentials,
-// masks, packing) 56 %, which share a SIMD's issue.  Short prompts (7 of 300 to
-// 600 rows, D 64: 15.4 us, of which one row takes 6.6) are a chain of tiles' round
-// trips to memory.
+// bf16 product reaches 1395; rows behind earlier keys with a window of 4096 1020;
+// the first with D 64 446 us, 609.  Neither unit is full: matrix instructions take
+// 41 % of a SIMD's cycles, and a wave, of which a SIMD has two, executes vector
+// instructions (these included) in 26 % of its own.  A wave issues 228 that are not
+// matrix ones per tile, where the prefill of one prompt (sparse_prefill.hip) takes
+// 138; among them are addresses and bounds of the coming tile's loads, which stand
+// before the first product, and moves of the 112 scalars that do not fit.  Short prompts
+// (7 of 300 to 600 rows, D 64: 15.4 us, of which one row takes 6.6) are a chain of
+// tiles' round trips to memory.
 //
 // A masked probability is 0, and 0 times a key's value that is not finite is
 // NaN: of the rows whose result is not finite, those whose tiles held such a value

@@ -308,7 +308,8 @@ def paged_decode_attn_window(q, k_cache, v_cache, cache_seqlens, block_table, wi
     counts to the window; where a gate left tokens out, these are the head's kept
     tokens, not the positions that sink_window_attn counts); returns (B, 1, Hq, D) bf16, zeros for a head without
     tokens.  Pages that hold none of them are not read, and their table
-    entries may be anything: they can be given back.  Hq / Hkv up to 8, B * Hkv
+    entries may be anything: they can be given back.  Unlike there, a NaN or +inf
+    among the scores that a head sees makes its result NaN.  Hq / Hkv up to 8, B * Hkv
     up to 2048.  Lengths and page ids out of range are clamped to the table
     and the pool."""
     pool = _check_pool(k_cache, v_cache)
