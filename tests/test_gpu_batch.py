@@ -358,6 +358,34 @@ def test_prompt_many_sequences():
     check_prompt(rng.choice([0, 1, 2, 3], 2048).tolist(), None, 2, 1, 64, 2, 1)
 
 
+def test_prompt_starts_that_do_not_ascend():
+    """They give some result, in the time of as many rows: not every stretch that
+    they name over again, 64 million rows here."""
+    import wgkv
+    N, B = 64000, 2000
+    q, k, v = qkv(N, N, 2, 1, 64, 3)
+    cu = i32([0, N] * (B // 2) + [N])
+    events = [torch.cuda.Event(enable_timing=True) for _ in range(2)]
+    times = []
+    for starts in (i32([N * b // B for b in range(B + 1)]), cu):
+        for _ in range(2):
+            events[0].record()
+            out = wgkv.sink_window_attn(q, k, v, starts, 1024, 4)
+            events[1].record()
+            torch.cuda.synchronize()
+        times.append(events[0].elapsed_time(events[1]))
+    assert out.shape == q.shape and times[1] < 20 * times[0] + 5
+    for starts in ([50, 10, 30, -4], [2 ** 31 - 1, 0, -2 ** 31, 77], [90, 80, 70, 60], [0, 100, 0, 100]):
+        for keys in (100, 5000):
+            kk, vv = (t[:keys] for t in (k, v))
+            ck = i32([0, keys // 3, keys // 2, keys])
+            whole = torch.full((300, 2, 64), 7.0, dtype=BF16, device=DEV)
+            wgkv.sink_window_attn(q[:100], kk, vv, i32(starts), 4000, 4, None, ck, out=whole[100:200])
+            wgkv.sink_window_attn(q[:100], kk, vv, ck.clamp(max=100), 4000, 4, None, i32(starts), out=whole[100:200])
+            torch.cuda.synchronize()
+            assert (whole[:100] == 7).all() and (whole[200:] == 7).all()
+
+
 def test_prompt_rows_of_no_sequence():
     import wgkv
     q, k, v = qkv(100, 100, 4, 2, 64, 0)

@@ -308,7 +308,9 @@ void window_prefill_kernel(WindowArgs a) {
     for (int b = b0; b < b1; ++b) {
       s_blocks[b] = run;
       run += per == 1 ? mine : (seq_of(a, b).nq + BLK - 1) / BLK;
-      if (b == a.B - 1) s_blocks[a.B] = run;
+      // (all of them where starts ascend; what others would make of it is cut off: items
+      // are then no more than the host has counted, within 32 bits)
+      if (b == a.B - 1) s_blocks[a.B] = min(run, a.N / BLK + a.B);
     }
     __syncthreads();
   }
@@ -759,7 +761,7 @@ extern "C" int wgkv_sink_window_attn(
   if (kv4_rows_meet({num_rows, num_q_heads, 1, 1}, {out_stride_n, out_stride_h, 0, 0}, head_dim)) return WGKV_ERR_ARG;
   const Cut cut = cut_of(num_rows, num_keys, batch, num_kv_heads, G, window, num_sinks);
   const PartsScratch sc = parts_scratch(cut.parts, (int64_t)num_rows * num_q_heads, head_dim);
-  // row blocks and items are counted in 32 bits, also where starts do not ascend (workgroups step over the end)
+  // row blocks (also where starts do not ascend) and items are counted in 32 bits; workgroups step over the end
   if ((int64_t)batch * (num_rows / 64 + 1) > (1 << 30)) return WGKV_ERR_UNSUPPORTED;
   if (items_of(num_rows, batch, num_kv_heads, G, cut.heads) * cut.parts > 0x7f000000) return WGKV_ERR_UNSUPPORTED;
   if (sc.bytes && (!workspace || workspace_bytes < sc.bytes || ((uintptr_t)workspace & 15))) return WGKV_ERR_WORKSPACE;
