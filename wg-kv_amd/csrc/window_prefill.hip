@@ -31,12 +31,12 @@
 // Measured (32/8 heads, D 128): 32768 rows, window 1024 and 4 first tokens 644
 // us, 840 TFLOP/s of the pairs that are seen, 940 of the tiles, where a large
 // bf16 product reaches 1395; rows behind earlier keys with a window of 4096 1020;
-// the first with D 64 446 us, 609.  Neither unit is full: matrix instructions take
+// the first with D 64 435 us, 624.  Neither unit is full: matrix instructions take
 // 41 % of a SIMD's cycles, and a wave, of which a SIMD has two, executes vector
 // instructions (these included) in 26 % of its own.  A wave issues 228 that are not
 // matrix ones per tile, where the prefill of one prompt (sparse_prefill.hip) takes
 // 138; among them are addresses and bounds of the coming tile's loads, which stand
-// before the first product, and moves of the 112 scalars that do not fit.  Short prompts
+// before the first product, and moves of the 111 scalars that do not fit.  Short prompts
 // (7 of 300 to 600 rows, D 64: 15.4 us, of which one row takes 6.6) are a chain of
 // tiles' round trips to memory.
 //
@@ -482,22 +482,21 @@ void window_prefill_kernel(WindowArgs a) {
       cur = nxt;
       continue;
     }
-    uint32_t again = 0, none = 0;  // rows with a value that is not finite; of no weight
+    // Rows with a value that is not finite.  (A sum that is NaN, as its row's scores
+    // were, makes every value NaN below.)
+    bool bad = false;
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
-      float bad = 0.f;
+      float x = 0.f;
 #pragma unroll
       for (int dt = 0; dt < D / 16; ++dt)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) bad += r.o[dt][rt][i] * 0.f;
-      // (a sum that is NaN, as its row's scores were, makes every value NaN below)
-      const bool here = r0 + rt * 16 + n < done.nq && bad != bad && r.sum[rt][0] == r.sum[rt][0];
-      const uint64_t y = __builtin_amdgcn_ballot_w64(here), z = __builtin_amdgcn_ballot_w64(here && r.sum[rt][0] == 0.f);
-      again |= (uint32_t)((y | y >> 16 | y >> 32 | y >> 48) & 0xffff) << (16 * rt);
-      none |= (uint32_t)((z | z >> 16 | z >> 32 | z >> 48) & 0xffff) << (16 * rt);
+        for (int i = 0; i < 4; ++i) x += r.o[dt][rt][i] * 0.f;
+      bad = bad || (r0 + rt * 16 + n < done.nq && x != x && r.sum[rt][0] == r.sum[rt][0]);
     }
-    Columns need = {0, 0, 0, 0};
-    if (again) {
+    uint32_t again = 0, none = 0;  // such rows; those of them whose weights are 0
+    Columns need = {0, 0, 0, 0};   // lane i: row i % 32's values
+    if (__builtin_amdgcn_ballot_w64(bad) != 0) {
 #pragma unroll
       for (int rt = 0; rt < 2; ++rt)
 #pragma unroll
@@ -508,8 +507,12 @@ void window_prefill_kernel(WindowArgs a) {
           w <<= g;
           w |= __shfl_xor(w, 16, 64);
           w |= __shfl_xor(w, 32, 64);
-          need[i] = (g & 1) == rt ? w : need[i];  // lane i: row i % 32
+          need[i] = (g & 1) == rt ? w : need[i];
         }
+      const float l = g & 1 ? r.sum[1][0] : r.sum[0][0];
+      const bool here = r0 + (lane & 31) < done.nq && l == l && (need[0] | need[1] | need[2] | need[3]) != 0;
+      again = (uint32_t)__builtin_amdgcn_ballot_w64(here);
+      none = (uint32_t)__builtin_amdgcn_ballot_w64(here && l == 0.f);
     }
 #pragma unroll
     for (int rt = 0; rt < 2; ++rt) {
